@@ -380,6 +380,7 @@ bool bind_gemm_swiglu_bwd(const torch::Tensor& dy, const torch::Tensor& w, const
 void register_comm(pybind11::module_& m);
 void register_attn(pybind11::module_& m);
 void register_block(pybind11::module_& m);
+void register_moe(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", [](const torch::Tensor& a, const torch::Tensor& b, torch::Tensor& out, bool a_mn, bool b_mn, int64_t out_mode,
@@ -476,4 +477,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_comm(m);
   register_attn(m);
   register_block(m);
+  register_moe(m);
 }

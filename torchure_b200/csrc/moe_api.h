@@ -1,0 +1,66 @@
+// Host-callable launchers of the mixture-of-experts kernels and of the 8-bit activation checkpoints (raw pointers, sizes, a stream).
+//
+// Rows grouped by expert: row r belongs to the expert e with offsets[e] <= r < offsets[e + 1]; offsets has E + 1 entries, starts at 0
+// and does not decrease; rows from offsets[E] on belong to none.  The kernels clamp what they read from `offsets` to [0, R], and skip
+// slots and rows outside their matrices: wrong values give wrong results, never an access outside a tensor.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tb {
+
+constexpr int kMaxExperts = 384;
+constexpr int kMaxChoices = 16;
+constexpr int kActBlock = 64;      // values of a row that share a scale in an 8-bit checkpoint
+
+// ---- router (moe_route.cu) ------------------------------------------------------------------------
+// Choices of one row of logits: the k largest, ties to the lowest index; a choice whose logit is -inf is not made.
+// weights [T, k], experts [T, k], slots [T, k] (row of the choice, -1: not made or beyond the capacity), offsets [E + 1],
+// rows [T k] (t k + j of each row, -1 behind offsets[E]), counts [E] (choices made, before the capacity), aux [1].
+// scratch: route_scratch_ints(T, E) 32-bit words.  capacity 0: no limit.
+int64_t route_scratch_ints(int T, int E);
+int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts, int* slots,
+              int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream);
+// dlogits [T, E] (the logits' type) from dweights [T, k] (nullptr: none) and daux [1] (nullptr: none)
+int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* experts, const int* counts,
+              const float* dweights, const float* daux, void* dlogits, int T, int E, int k, cudaStream_t stream);
+
+// ---- rows to expert order and back (moe_rows.cu) -----------------------------------------------------
+// out[r] = bf16(x[rows[r] / k]), zeros where rows[r] < 0
+void rows_gather(const void* x, bool x_bf16, int64_t ldx, const int* rows, __nv_bfloat16* out, int T, int k, int R, int D,
+                 cudaStream_t stream);
+// out[t] = sum_j weights[t, j] y[slots[t, j]] (weights nullptr: 1), fp32 sums in the order of the choices
+void rows_combine(const __nv_bfloat16* y, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
+                  cudaStream_t stream);
+// dy[slots[t, j]] = bf16(weights[t, j] dout[t]), zeros in rows of no choice; dweights[t, j] = <y[slot], dout[t]>, 0 without a slot
+void rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_bfloat16* y, const float* weights, const int* slots,
+                      const int* offsets, __nv_bfloat16* dy, float* dweights, int T, int k, int E, int D, cudaStream_t stream);
+
+// ---- products grouped by expert (grouped_gemm_sm100.cu) ------------------------------------------------
+// y[r] = x[r] W[e(r)]^T (w_t false, W [E, N, K]) or x[r] W[e(r)] (w_t true, W [E, K, N]); rows of no expert: zeros.  x [R, K].
+int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
+                 int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
+// dw[e] [N, K] = sum over the rows of e of dy[r]^T x[r], bf16 or fp32; zeros for an expert without rows
+int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,
+                  int R, int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
+
+// ---- 8-bit activation checkpoints (act8.cu) --------------------------------------------------------------
+// Per row and block of 64 values: a = the largest magnitude, q = sign(x) floor(127 |x| / a + 1/2), scale = a / 127 (0 for a block of
+// zeros, NaN for one that holds a value that is not finite).  q [M, N], scales [M, ceil(N / 64)].
+void quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, int64_t M, int N, cudaStream_t stream);
+void dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream);
+// act [M, F] = silu(g) u of gu [M, 2F] = g | u; q [M, 2F] and scales [M, 2 ceil(F / 64)]: both halves as quantize8 keeps them
+void swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
+                 cudaStream_t stream);
+void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M, int F,
+                 cudaStream_t stream);
+// The experts' SwiGLU backward, over choices i = t k + j with row r = slots[i] and weight w = weights[i]; s [R, F] = dout W_down.
+// Gate and up come from gu (bf16) or, where gu is nullptr, from (q, scales).  dgu[r] = d(gate) | d(up) for d(act) = w s,
+// act_w[r] = w act, dweights[i] = <act, s>; zeros in rows of no choice, and 0 for a choice without a row.
+void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,
+                       const int* slots, const int* offsets, __nv_bfloat16* dgu, __nv_bfloat16* act_w, float* dweights, int R, int E,
+                       int F, cudaStream_t stream);
+
+}  // namespace tb

@@ -1,0 +1,414 @@
+// The router of a mixture of experts: top-k choice, weights, the order of rows by expert, the load-balancing term, and the
+// gradient of weights and term.
+//
+// Per token, logits l over E experts, k of them chosen in falling order (ties to the lowest index):
+//   w_j = exp(l_j) / sum over the chosen of exp(l_i),  p = softmax(l),  aux = E sum_e share_e mean_t p[t, e]
+//   dl[t, e_j] += w_j (dw_j - sum_i w_i dw_i),  dl[t, e] += daux E / T p[t, e] (share_e - sum_i share_i p[t, i])
+// with share_e = choices made for e / (T k).
+//
+// A token belongs to a group of LANES threads (the power of two that holds E, 32 at most, VALS logits each), which finds one choice
+// per round with two warp reductions: the largest key (floats as ordered integers), then the lowest index that has it.  Rows are
+// numbered by a counting sort that keeps the order of the choices inside an expert: every CTA counts the choices of a run of
+// consecutive tokens; the second kernel adds up the counts before its own run and ranks its choices.  No float atomics: the sums of p
+// are added in a fixed order.  Few tokens take one launch of one CTA.
+#include "common.cuh"
+#include "moe_api.h"
+
+namespace tb {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxChunks = 148;
+
+__device__ __forceinline__ uint32_t to_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.f);      // -0 and 0 tie
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float from_key(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
+constexpr uint32_t kKeyMinusInf = 0x007fffffu;      // to_key(-inf); 0: taken, or past the last expert
+
+__device__ __forceinline__ float load_logit(const float* p) { return *p; }
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+template <int LANES>
+__device__ __forceinline__ uint32_t group_mask(int lane) {
+  return LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, uint32_t mask) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o, LANES);
+  return v;
+}
+
+struct RouteArgs {
+  int64_t ld;
+  int T, E, k, capacity;
+  int chunk;               // tokens of a CTA
+  float* weights;
+  int* experts;
+  int* slots;
+  int* offsets;
+  int* rows;
+  int* counts;
+  float* aux;
+  int* hist;               // [chunks][E]
+  float* psum;             // [chunks][E]
+};
+
+// Numbers the choices of CTA `c` of `chunks`.  slots holds the expert of each choice (-1: not made) and receives its row.
+__device__ void plan_rows(const RouteArgs& a, int c, int chunks, int* sm) {
+  const int E = a.E, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* total = sm;                 // [E]
+  int* before = sm + E;            // [E] in earlier CTAs; later the place of the next choice of this CTA's first warp
+  int* first = sm + 2 * E;         // [E + 1] first row of each expert
+  int* cnt = sm + 3 * E + 1;       // [kWarps][E]
+  float* aux_part = reinterpret_cast<float*>(cnt + kWarps * E);      // [kWarps]
+  for (int i = tid; i < 2 * E; i += kThreads) sm[i] = 0;
+  for (int i = tid; i < kWarps * E; i += kThreads) cnt[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < chunks * E; i += kThreads) {
+    const int e = i % E, v = a.hist[i];
+    if (v) {
+      atomicAdd(&total[e], v);
+      if (i / E < c) atomicAdd(&before[e], v);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {                 // exclusive prefix sums of the kept counts
+    int run = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      const int n = e < E ? (a.capacity > 0 ? min(total[e], a.capacity) : total[e]) : 0;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += up;
+      }
+      if (e < E) first[e] = run + s - n;
+      run += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) first[E] = run;
+  }
+  __syncthreads();
+  const int n_flat = a.T * a.k;
+  if (c == 0) {
+    for (int e = tid; e <= E; e += kThreads) {
+      a.offsets[e] = first[e];
+      if (e < E) a.counts[e] = total[e];
+    }
+    float s = 0.f;
+    for (int i = tid; i < chunks * E; i += kThreads) s += static_cast<float>(total[i % E]) * a.psum[i];
+    s = group_sum<32>(s, 0xffffffffu);
+    if (lane == 0) aux_part[warp] = s;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 1; i < kWarps; ++i) s += aux_part[i];
+      a.aux[0] = s * (static_cast<float>(E) / static_cast<float>(n_flat)) / static_cast<float>(a.T);
+    }
+  }
+  // this CTA's choices, a consecutive part for each warp: counted, then ranked
+  const int lo = c * a.chunk * a.k, hi = min(n_flat, lo + a.chunk * a.k);
+  const int part = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int wlo = min(hi, lo + warp * part), whi = min(hi, wlo + part);
+  for (int i = wlo + lane; i < whi; i += 32) {
+    const int e = a.slots[i];
+    if (e >= 0) atomicAdd(&cnt[warp * E + e], 1);
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += kThreads) {
+    int run = before[e];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = cnt[w * E + e];
+      cnt[w * E + e] = run;
+      run += n;
+    }
+  }
+  __syncthreads();
+  for (int i0 = wlo; i0 < whi; i0 += 32) {
+    const int i = i0 + lane;
+    const int e = i < whi ? a.slots[i] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    int place = 0;
+    if (e >= 0) place = cnt[warp * E + e] + rank;
+    __syncwarp();
+    if (e >= 0 && rank == 0) cnt[warp * E + e] += __popc(same);
+    __syncwarp();
+    if (i < whi) {
+      int row = -1;
+      if (e >= 0 && place < first[e + 1] - first[e]) {
+        row = first[e] + place;
+        a.rows[row] = i;
+      }
+      a.slots[i] = row;
+    }
+  }
+  for (int r = first[E] + c * kThreads + tid; r < n_flat; r += chunks * kThreads) a.rows[r] = -1;
+}
+
+constexpr int plan_smem_ints(int E) { return 3 * E + 1 + kWarps * E + kWarps; }
+
+template <class T, int LANES, int VALS>
+__global__ void __launch_bounds__(kThreads)
+route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ int sm[];
+  constexpr int GROUPS = kThreads / LANES;
+  const int E = a.E, tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1), group = tid / LANES;
+  const uint32_t mask = group_mask<LANES>(lane);
+  int* hist = sm;                                         // [E]
+  float* part = reinterpret_cast<float*>(sm + E);         // [GROUPS][E]
+  for (int e = tid; e < E; e += kThreads) hist[e] = 0;
+  __syncthreads();
+  float acc[VALS];
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) acc[v] = 0.f;
+  const int t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
+  for (int t = t0 + group; t < t1; t += GROUPS) {
+    const T* row = logits + t * a.ld;
+    float x[VALS];
+    uint32_t key[VALS];
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const int e = v * LANES + gl;
+      x[v] = e < E ? load_logit(row + e) : -INFINITY;
+      key[v] = e < E ? to_key(x[v]) : 0u;
+    }
+    uint32_t my_key = 0;
+    int my_e = 0;
+    float top = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = 0;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
+      best = __reduce_max_sync(mask, best);
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int v = VALS - 1; v >= 0; --v)
+        if (key[v] == best) at = v * LANES + gl;
+      at = __reduce_min_sync(mask, at);
+#pragma unroll
+      for (int v = 0; v < VALS; ++v)
+        if (at == v * LANES + gl) key[v] = 0;
+      if (j == 0) top = from_key(best);
+      if (gl == j) { my_key = best; my_e = at; }
+    }
+    const bool made = gl < a.k && my_key != kKeyMinusInf;
+    const float ex = made ? expf(from_key(my_key) - top) : 0.f;
+    const float sum = group_sum<LANES>(ex, mask);
+    if (gl < a.k) {
+      const int64_t i = static_cast<int64_t>(t) * a.k + gl;
+      a.weights[i] = made ? ex / sum : 0.f;
+      a.experts[i] = my_e;
+      a.slots[i] = made ? my_e : -1;
+      if (made) atomicAdd(&hist[my_e], 1);
+    }
+    if (top != -INFINITY) {
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) {
+        x[v] = expf(x[v] - top);
+        s += x[v];
+      }
+      s = group_sum<LANES>(s, mask);
+      const float r = 1.f / s;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) acc[v] += x[v] * r;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) {
+    const int e = v * LANES + gl;
+    if (e < E) part[group * E + e] = acc[v];
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += kThreads) {
+    float s = 0.f;
+    for (int g = 0; g < GROUPS; ++g) s += part[g * E + e];
+    a.psum[static_cast<int64_t>(blockIdx.x) * E + e] = s;
+    a.hist[static_cast<int64_t>(blockIdx.x) * E + e] = hist[e];
+  }
+  if (single) {
+    __syncthreads();
+    plan_rows(a, 0, 1, sm);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+route_plan_kernel(RouteArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ int sm[];
+  plan_rows(a, blockIdx.x, gridDim.x, sm);
+}
+
+template <class T, int LANES, int VALS>
+__global__ void __launch_bounds__(kThreads)
+route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ weights, const int* __restrict__ experts,
+                 const int* __restrict__ counts, const float* __restrict__ dweights, const float* __restrict__ daux,
+                 T* __restrict__ dlogits, int n_tokens, int E, int k) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int GROUPS = kThreads / LANES;
+  const int tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1);
+  const uint32_t mask = group_mask<LANES>(lane);
+  const float pull = daux ? *daux * static_cast<float>(E) / static_cast<float>(n_tokens) : 0.f;
+  const float per = 1.f / (static_cast<float>(n_tokens) * static_cast<float>(k));
+  float share[VALS];
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) share[v] = v * LANES + gl < E ? static_cast<float>(counts[v * LANES + gl]) * per : 0.f;
+  for (int t = blockIdx.x * GROUPS + tid / LANES; t < n_tokens; t += gridDim.x * GROUPS) {
+    float x[VALS], top = -INFINITY;
+    bool odd = false;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const int e = v * LANES + gl;
+      x[v] = e < E ? load_logit(logits + t * ld + e) : -INFINITY;
+      odd |= x[v] != x[v];
+      top = fmaxf(top, x[v]);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o, LANES));
+    odd = __any_sync(mask, odd);      // a NaN among the logits makes the whole row's gradient NaN
+    if (odd) top = __uint_as_float(0x7fffffffu);
+    float s = 0.f, mean = 0.f;
+    const bool none = top == -INFINITY;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      x[v] = none ? 0.f : expf(x[v] - top);
+      s += x[v];
+      mean += x[v] * share[v];
+    }
+    s = group_sum<LANES>(s, mask);
+    mean = group_sum<LANES>(mean, mask);
+    const float r = none ? 0.f : 1.f / s;
+    mean *= r;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) x[v] = odd ? top : pull == 0.f ? 0.f : pull * (x[v] * r) * (share[v] - mean);
+    if (dweights) {
+      float w = 0.f, dw = 0.f;
+      int e = -1;
+      if (gl < k) {
+        const int64_t i = static_cast<int64_t>(t) * k + gl;
+        w = weights[i];
+        e = experts[i];
+        dw = w != 0.f ? dweights[i] : 0.f;
+      }
+      const float inner = group_sum<LANES>(w * dw, mask);
+      const float g = w * (dw - inner);
+      for (int j = 0; j < k; ++j) {
+        const float gj = __shfl_sync(mask, g, j, LANES);
+        const int ej = __shfl_sync(mask, e, j, LANES);
+#pragma unroll
+        for (int v = 0; v < VALS; ++v)
+          if (ej == v * LANES + gl) x[v] += gj;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const int e = v * LANES + gl;
+      if (e < E) dlogits[static_cast<int64_t>(t) * E + e] = static_cast<T>(x[v]);
+    }
+  }
+}
+
+int lanes_for(int E) {
+  int l = 4;
+  while (l < E && l < 32) l <<= 1;
+  return l;
+}
+
+// (chunks, tokens of a chunk)
+void chunks_for(int T, int E, int& chunks, int& chunk) {
+  const int groups = kThreads / lanes_for(E);
+  if (T <= 4 * groups) {       // one CTA, four rounds of tokens
+    chunks = 1;
+    chunk = T;
+    return;
+  }
+  chunk = (T + kMaxChunks - 1) / kMaxChunks;
+  chunk = (chunk + groups - 1) / groups * groups;
+  chunks = (T + chunk - 1) / chunk;
+}
+
+#define TB_ROUTE_SIZES(CASE) CASE(4, 1) CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(32, 2) CASE(32, 4) CASE(32, 8) CASE(32, 16)
+
+int vals_for(int E) {
+  int v = 1;
+  while (v * 32 < E) v <<= 1;
+  return v;
+}
+
+template <class T>
+int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t stream) {
+  const int lanes = lanes_for(a.E), vals = vals_for(a.E);
+  const int ints = a.E + kThreads / lanes * a.E, plan = plan_smem_ints(a.E);
+  const size_t smem = 4 * static_cast<size_t>(ints > plan ? ints : plan);
+#define CASE(L, V)                                                                                                            \
+  if (lanes == L && vals == V) {                                                                                              \
+    if (launch_pdl(route_fwd_kernel<T, L, V>, dim3(chunks), dim3(kThreads), smem, stream, logits, a, chunks == 1 ? 1 : 0) !=   \
+        cudaSuccess)                                                                                                          \
+      return -21;                                                                                                             \
+    if (chunks > 1 && launch_pdl(route_plan_kernel, dim3(chunks), dim3(kThreads), 4 * static_cast<size_t>(plan), stream, a) != \
+                          cudaSuccess)                                                                                        \
+      return -21;                                                                                                             \
+    return 0;                                                                                                                 \
+  }
+  TB_ROUTE_SIZES(CASE)
+#undef CASE
+  return -2;
+}
+
+}  // namespace
+
+int64_t route_scratch_ints(int T, int E) {
+  int chunks, chunk;
+  chunks_for(T, E, chunks, chunk);
+  return 2 * static_cast<int64_t>(chunks) * E;
+}
+
+int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts, int* slots,
+              int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream) {
+  if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices || static_cast<int64_t>(T) * k > (1ll << 30)) return -1;
+  RouteArgs a{};
+  a.ld = ld; a.T = T; a.E = E; a.k = k; a.capacity = capacity;
+  a.weights = weights; a.experts = experts; a.slots = slots; a.offsets = offsets; a.rows = rows; a.counts = counts; a.aux = aux;
+  int chunks;
+  chunks_for(T, E, chunks, a.chunk);
+  a.hist = scratch;
+  a.psum = reinterpret_cast<float*>(scratch + static_cast<int64_t>(chunks) * E);
+  return bf16 ? launch_fwd(static_cast<const __nv_bfloat16*>(logits), a, chunks, stream)
+              : launch_fwd(static_cast<const float*>(logits), a, chunks, stream);
+}
+
+int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* experts, const int* counts,
+              const float* dweights, const float* daux, void* dlogits, int T, int E, int k, cudaStream_t stream) {
+  if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices) return -1;
+  const int lanes = lanes_for(E), vals = vals_for(E);
+  const int groups = kThreads / lanes;
+  const int need = (T + groups - 1) / groups;
+  const int grid = need < 148 * 8 ? need : 148 * 8;
+#define CASE(L, V)                                                                                                              \
+  if (lanes == L && vals == V) {                                                                                                \
+    const cudaError_t rc =                                                                                                      \
+        bf16 ? launch_pdl(route_bwd_kernel<__nv_bfloat16, L, V>, dim3(grid), dim3(kThreads), 0, stream,                          \
+                          static_cast<const __nv_bfloat16*>(logits), ld, weights, experts, counts, dweights, daux,               \
+                          static_cast<__nv_bfloat16*>(dlogits), T, E, k)                                                         \
+             : launch_pdl(route_bwd_kernel<float, L, V>, dim3(grid), dim3(kThreads), 0, stream,                                  \
+                          static_cast<const float*>(logits), ld, weights, experts, counts, dweights, daux,                       \
+                          static_cast<float*>(dlogits), T, E, k);                                                                \
+    return rc == cudaSuccess ? 0 : -21;                                                                                          \
+  }
+  TB_ROUTE_SIZES(CASE)
+#undef CASE
+  return -2;
+}
+
+}  // namespace tb

@@ -3,7 +3,9 @@
 Not in the reference (its registry holds the dense model only; expert parallelism is an empty file there).  It exists
 so that the expert-parallel layer (``parallel/expert_parallel.py``) has a model the config can select: every block
 keeps the dense model's attention and norms and swaps the MLP for ``MoELayer``.  The blocks run the PyTorch path
-(``impl`` is fixed to "torch"): the sm_100a engine has no grouped expert GEMM.
+(``impl`` is fixed to "torch"); ``experts: "grouped"`` runs the feed-forwards on the sm_100a operators of ``ops/moe.py``
+instead of batched library products over padded buffers, and ``act_bits: 8`` keeps their gate and up in 8 bits between the
+passes.
 
 With ``mesh: {"dp": D, "ep": E}`` the Trainer calls ``shard_experts``: rank r of an ``ep`` group keeps experts
 [r E_total / E, (r + 1) E_total / E) of every layer, tokens travel to their experts' owners and back through the
@@ -25,16 +27,16 @@ class Qwen3MoE(Qwen3):
                  capacity_factor: float = 2.0, aux_loss_coef: float = 0.01, ffn_dim: int | None = None,
                  norm_eps: float = 1e-6,
                  rope_theta: float = 1_000_000.0, qk_norm: bool = True, tie_embeddings: bool = True,
-                 impl: str = "torch"):
+                 impl: str = "torch", experts: str = "capacity", act_bits: int = 16):
         super().__init__(num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, emb_dim=emb_dim,
                          head_dim=head_dim, vocab_size=vocab_size, ffn_dim=ffn_dim, norm_eps=norm_eps,
                          rope_theta=rope_theta, qk_norm=qk_norm, tie_embeddings=tie_embeddings, impl="torch")
         width = moe_ffn_dim if moe_ffn_dim is not None else self.cfg["ffn_dim"]
         self.cfg.update(num_experts=num_experts, top_k=top_k, moe_ffn_dim=width, capacity_factor=capacity_factor,
-                        aux_loss_coef=aux_loss_coef)
+                        aux_loss_coef=aux_loss_coef, experts=experts, act_bits=act_bits)
         self.aux_loss_coef = aux_loss_coef
         for block in self.blocks:
-            block.ffn = MoELayer(emb_dim, width, num_experts, top_k, capacity_factor)
+            block.ffn = MoELayer(emb_dim, width, num_experts, top_k, capacity_factor, experts=experts, act_bits=act_bits)
 
     @torch.no_grad()
     def init_weights(self, std: float = 0.02) -> None:

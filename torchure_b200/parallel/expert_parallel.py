@@ -9,6 +9,10 @@ shuffle is the even-split ``all_to_all``.  Here:
   owning rank, processed, sent back (combine) and weighted by their gate values.  Overflowing tokens are dropped
   (contribute zero), as in capacity-factor routing.
 * both exchanges are autograd functions (the backward of an all-to-all is the inverse all-to-all).
+* ``experts="grouped"`` runs the layer on the operators of ``ops/moe.py``: rows in expert order instead of padded buffers, products
+  grouped by expert instead of batched library products, with ``act_bits=8`` gate and up kept in 8 bits for the backward pass.  The
+  capacity drops the same choices (``capacity_factor`` 0: none are dropped).  Spread over a mesh axis the exchange keeps its padded
+  buffers and the grouped products run on what arrives.
 """
 
 from __future__ import annotations
@@ -18,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from torchure_b200.core.collective import all_to_all
+from torchure_b200.ops import act8, moe
 
 
 class _AllToAll(torch.autograd.Function):
@@ -33,8 +38,13 @@ class _AllToAll(torch.autograd.Function):
 
 class MoELayer(nn.Module):
     def __init__(self, hidden: int, ffn: int, num_experts: int, top_k: int = 2, capacity_factor: float = 2.0,
-                 mesh=None, dim: str = "ep"):
+                 mesh=None, dim: str = "ep", experts: str = "capacity", act_bits: int = 16):
         super().__init__()
+        if experts not in ("capacity", "grouped"):
+            raise ValueError(f'MoELayer: experts are "capacity" or "grouped", not {experts!r}')
+        if act_bits not in (8, 16) or (act_bits == 8 and experts != "grouped"):
+            raise ValueError(f"MoELayer: activations in {act_bits} bits (8: with grouped experts only)")
+        self.experts, self.act_bits = experts, act_bits
         self.hidden, self.ffn, self.E, self.k, self.cf = hidden, ffn, num_experts, top_k, capacity_factor
         self.mesh, self.dim = mesh, dim
         self.n = mesh.size(dim) if mesh is not None else 1
@@ -72,10 +82,29 @@ class MoELayer(nn.Module):
     def capacity(self, tokens: int) -> int:
         return max(1, int(self.cf * tokens * self.k / self.E + 0.999))
 
+    def _grouped_products(self, work: torch.Tensor) -> torch.Tensor:
+        """The experts' feed-forwards on buffers [local_E, rows, hidden] of what the ranks sent."""
+        E, R, D = work.shape
+        rows = work.reshape(E * R, D)
+        if rows.is_cuda:
+            rows = rows.to(torch.bfloat16)
+        offsets = torch.arange(E + 1, device=work.device, dtype=torch.int32) * R
+        gu = moe.grouped_linear(rows, torch.cat([self.w_gate, self.w_up], dim=1), offsets)
+        if self.act_bits == 8 and gu.dtype == torch.bfloat16:
+            act = act8.swiglu_8bit(gu)
+        else:
+            g, u = gu.chunk(2, dim=-1)
+            act = F.silu(g) * u
+        return moe.grouped_linear(act, self.w_down, offsets).view(E, R, D)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         x = x.reshape(-1, self.hidden)
         T = x.shape[0]
+        if self.experts == "grouped" and self.n == 1:
+            out, self.aux_loss = moe.expert_mlp(x, self.router(x), (self.w_gate, self.w_up), self.w_down, self.k,
+                                                self.capacity(T) if self.cf > 0 else 0, self.act_bits)
+            return out.view(shape)
         C = self.capacity(T)
         probs = F.softmax(self.router(x).float(), dim=-1)
         gate, expert = probs.topk(self.k, dim=-1)                 # (T, k)
@@ -100,8 +129,11 @@ class MoELayer(nn.Module):
             work = buf.view(self.n, self.local_E, C, self.hidden).transpose(0, 1).reshape(self.local_E, self.n * C, -1)
         else:
             work = buf.view(self.local_E, C, self.hidden)
-        h = F.silu(torch.bmm(work, self.w_gate.transpose(1, 2))) * torch.bmm(work, self.w_up.transpose(1, 2))
-        y = torch.bmm(h, self.w_down.transpose(1, 2))
+        if self.experts == "grouped":
+            y = self._grouped_products(work)
+        else:
+            h = F.silu(torch.bmm(work, self.w_gate.transpose(1, 2))) * torch.bmm(work, self.w_up.transpose(1, 2))
+            y = torch.bmm(h, self.w_down.transpose(1, 2))
         if self.n > 1:
             y = y.view(self.local_E, self.n, C, self.hidden).transpose(0, 1).reshape(self.E * C, self.hidden)
             y = _AllToAll.apply(y, self.mesh, self.dim)
