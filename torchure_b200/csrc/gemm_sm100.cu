@@ -436,25 +436,24 @@ EncodeFn encode_fn() {
 namespace {
 struct TmapKey {
   const void* base; uint64_t rows, cols, ld; uint32_t box_rows, box_cols; int elem_bytes;
+  uint64_t planes = 0;      // 0: a 2-D map
   bool operator==(const TmapKey& o) const {
     return base == o.base && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows &&
-           box_cols == o.box_cols && elem_bytes == o.elem_bytes;
+           box_cols == o.box_cols && elem_bytes == o.elem_bytes && planes == o.planes;
   }
 };
 struct TmapKeyHash {
   size_t operator()(const TmapKey& k) const {
     uint64_t h = reinterpret_cast<uint64_t>(k.base) * 0x9E3779B97F4A7C15ull;
     h ^= (k.rows + 0x9E3779B97F4A7C15ull + (h << 6) + (h >> 2));
-    h ^= (k.cols * 31 + k.ld * 131 + k.box_rows * 7 + k.box_cols * 3 + k.elem_bytes + (h << 6) + (h >> 2));
+    h ^= (k.cols * 31 + k.ld * 131 + k.box_rows * 7 + k.box_cols * 3 + k.elem_bytes + k.planes * 17 + (h << 6) + (h >> 2));
     return static_cast<size_t>(h);
   }
 };
 }  // namespace
 
-int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld,
-                 uint32_t box_rows, uint32_t box_cols) {
+static int make_tmap(CUtensorMap* map, const TmapKey& key) {
   static thread_local std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
-  const TmapKey key{base, rows, cols, ld, box_rows, box_cols, elem_bytes};
   auto hit = cache.find(key);
   if (hit != cache.end()) {
     std::memcpy(map, &hit->second, sizeof(CUtensorMap));
@@ -462,20 +461,36 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t ro
   }
   EncodeFn fn = encode_fn();
   if (!fn) return -10;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return -11;
-  if ((ld * elem_bytes) % 16 != 0) return -12;
-  if (box_cols * elem_bytes != 128) return -13;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld * static_cast<uint64_t>(elem_bytes)};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  // a thread that has launched nothing yet (autograd's, where the first thing it does is a product) has no current context
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return -10;
+  if ((reinterpret_cast<uintptr_t>(key.base) & 15) != 0) return -11;
+  if ((key.ld * key.elem_bytes) % 16 != 0) return -12;
+  if (key.box_cols * key.elem_bytes != 128) return -13;
+  const uint64_t row = key.ld * static_cast<uint64_t>(key.elem_bytes);
+  cuuint64_t dims[3] = {key.cols, key.rows, key.planes};
+  cuuint64_t strides[2] = {row, row * key.rows};
+  cuuint32_t box[3] = {key.box_cols, key.box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUtensorMapDataType dt = key.elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  CUresult r = fn(map, dt, key.planes ? 3 : 2, const_cast<void*>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return -14;
   if (cache.size() > 16384) cache.clear();
   cache.emplace(key, *map);
   return 0;
+}
+
+int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld,
+                 uint32_t box_rows, uint32_t box_cols) {
+  return make_tmap(map, TmapKey{base, rows, cols, ld, box_rows, box_cols, elem_bytes});
+}
+
+// `planes` contiguous matrices [rows, cols], box [1, box_rows, box_cols]: what lies past a plane's rows or columns reads as zero and
+// is not written
+int make_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t planes, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                 uint32_t box_cols) {
+  return make_tmap(map, TmapKey{base, rows, cols, cols, box_rows, box_cols, elem_bytes, planes});
 }
 
 template <bool A_MN, bool B_MN, int OUT>

@@ -1,113 +1,550 @@
-// Matrix products of rows grouped by expert, each group with its expert's matrix, and the gradient of the matrices.
+// Matrix products of rows grouped by expert, each group with its expert's matrix, and the gradient of the matrices, on CTA pairs
+// (tcgen05.mma.cta_group::2, 256 x 256 tiles over two SMs; the pipeline is that of gemm2_sm100.cu).
 //
-// One CTA per 64 x 64 tile of one expert's output, operands staged in shared memory as fp32, 4 x 4 sums per thread.  Bound by the
-// FMA units: 32768 x 1024 x 1536 x 6 operations take 14.2 ms over 32 experts.
-#include "common.cuh"
+// Rows times matrices, y[r] = x[r] W[e(r)]^T: the tile is computed transposed.  The matrix supplies the 256 rows of the tile (the
+// instruction's M, fixed), the group's rows its columns (the instruction's N, any multiple of 32 up to 256).  Groups end anywhere, and
+// what a group's last tile costs in arithmetic goes with its rows: 2049 rows take 8.1 tiles, not 9.  Nothing is padded in memory: a
+// tile reads rows of the next group along, whose columns of the tile are not stored.  The epilogue turns the accumulator round on its
+// way out: fragments of 16 lanes x 8 columns (tcgen05.ld.16x256b) are rounded to pairs and stored transposed (stmatrix), so that rows
+// of the output leave in pieces of 64 bytes.
+//
+// The gradient of the matrices, dW[e] = sum of dy[r]^T x[r]: the group's rows are the reduction.  Blocks of 64 rows; of a last block
+// that is not full only the steps of 16 rows that hold some are multiplied, and in a step that is not full the rows of the next group
+// are overwritten with zeros in shared memory, in both operands (0 x NaN is NaN), by a warp that does nothing else.
+//
+// Groups are read from `offsets` on the device: no call waits for them.  The grid is persistent; tiles go round over the pairs.
+#include "cta_pair.cuh"
 #include "moe_api.h"
 
 namespace tb {
 
+int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
+                 uint32_t box_cols);
+int make_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t planes, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                 uint32_t box_cols);
+
 namespace {
 
-constexpr int TILE = 64, KB = 16;
+constexpr int BM = 128, BN = 256, BNH = 128, BK = 64, STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BNH * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BAR_BYTES = 256;
+constexpr int EDGE_BYTES = (kMaxExperts + 1) * 4;
+constexpr uint32_t TMEM_COLS = 512;
 
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+constexpr int PITCH = 80;                       // bytes of a staged row of 32 values: eight of them fall on all banks once
+constexpr int ROW_EPI_BYTES = 4 * 64 * PITCH;   // per epilogue warp 64 rows
+constexpr int ROW_THREADS = 192;
+constexpr int ROW_SMEM = STAGES * STAGE_BYTES + ROW_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
 
-// acc[i][j] += sum over k0 <= k < k1 of A(m0 + 4 ty + i, k) B(n0 + 4 tx + j, k), with A(m, k) = a[m * am + k * ak], zero from M / N on
-__device__ __forceinline__ void tile_product(const __nv_bfloat16* a, int64_t am, int64_t ak, int m0, int M, const __nv_bfloat16* b,
-                                             int64_t bm, int64_t bk, int n0, int N, int64_t k0, int64_t k1, float (&acc)[4][4]) {
-  __shared__ float sa[KB][TILE + 1], sb[KB][TILE + 1];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  for (int64_t k = k0; k < k1; k += KB) {
-    for (int i = tid; i < TILE * KB; i += 256) {
-      // the faster index runs along the contiguous direction
-      const int ka = ak == 1 ? i % KB : i / TILE, ma = ak == 1 ? i / KB : i % TILE;
-      sa[ka][ma] = m0 + ma < M && k + ka < k1 ? __bfloat162float(a[(m0 + ma) * am + (k + ka) * ak]) : 0.f;
-      const int kb = bk == 1 ? i % KB : i / TILE, mb = bk == 1 ? i / KB : i % TILE;
-      sb[kb][mb] = n0 + mb < N && k + kb < k1 ? __bfloat162float(b[(n0 + mb) * bm + (k + kb) * bk]) : 0.f;
+constexpr int EPI_BUF = 4096;                   // 32 rows x 128 B
+constexpr int W_EPI_BYTES = 4 * 2 * EPI_BUF;
+constexpr int W_THREADS = 224;
+constexpr int W_SMEM = STAGES * STAGE_BYTES + W_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
+static_assert(ROW_SMEM <= 232448 && W_SMEM <= 232448, "shared memory of one CTA");
+
+// edge[e] = first row of group e, edge[E] = end of the last: what `offsets` says, brought into [0, R] and made not to fall
+__device__ __forceinline__ void load_edges(const int* offsets, int* edge, int E, int R) {
+  if (threadIdx.x < 32) {
+    int run = 0;
+    for (int e0 = 0; e0 <= E; e0 += 32) {
+      const int e = e0 + static_cast<int>(threadIdx.x);
+      int v = e > 0 && e <= E ? min(max(offsets[e], 0), R) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, v, o);
+        if (threadIdx.x >= o) v = max(v, up);
+      }
+      v = max(v, run);
+      if (e <= E) edge[e] = v;
+      run = __shfl_sync(0xffffffffu, v, 31);
     }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < KB; ++kk) {
-      float x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { x[i] = sa[kk][4 * ty + i]; y[i] = sb[kk][4 * tx + i]; }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
-    }
-    __syncthreads();
   }
 }
 
-__global__ void __launch_bounds__(256)
-grouped_simple_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w, int64_t wn, int64_t wk,
-                      const int* __restrict__ offsets, __nv_bfloat16* __restrict__ y, int R, int E, int N, int K) {
-  // tile blockIdx.y of the row tiles of all groups, the rows of no expert being the last group
-  int left = blockIdx.y, lo = 0, hi = 0, e = 0;
-  for (; e <= E; ++e) {
-    lo = hi;
-    hi = e < E ? min(max(offsets[e + 1], lo), R) : R;
-    const int tiles = (hi - lo + TILE - 1) / TILE;
-    if (left < tiles) break;
-    left -= tiles;
-  }
-  if (e > E) return;
-  const int m0 = lo + left * TILE, n0 = blockIdx.x * TILE;
-  float acc[4][4] = {};
-  if (e < E)
-    tile_product(x, ldx, 1, m0, hi, w + static_cast<int64_t>(e) * N * K, wn, wk, n0, N, 0, K, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + 4 * ty + i, n = n0 + 4 * tx + j;
-      if (m < hi && n < N) y[static_cast<int64_t>(m) * N + n] = __float2bfloat16(acc[i][j]);
+// Where a unit lies; units only grow from call to call.
+struct Place {
+  const int* edge;
+  int E, e = 0, base = 0;      // base: first unit of group e
+  __device__ __forceinline__ int rows() const { return edge[e + 1] - edge[e]; }
+};
+
+// The units of group e are its tiles of 256 rows times `cols` tiles of the matrix, rows fastest.  False: past the last.
+__device__ __forceinline__ bool find_rows(Place& p, int unit, int cols, int& r0, int& live, int& col) {
+  while (p.e < p.E) {
+    const int tiles = (p.rows() + BN - 1) / BN;
+    if (unit - p.base < tiles * cols) {
+      const int at = unit - p.base;
+      r0 = p.edge[p.e] + at % tiles * BN;
+      live = min(BN, p.edge[p.e + 1] - r0);
+      col = at / tiles;
+      return true;
     }
+    p.base += tiles * cols;
+    ++p.e;
+  }
+  return false;
 }
 
-template <class O>
-__global__ void __launch_bounds__(256)
-grouped_wgrad_simple_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, const __nv_bfloat16* __restrict__ x, int64_t ldx,
-                            const int* __restrict__ offsets, O* __restrict__ dw, int R, int N, int K) {
-  const int e = blockIdx.z;
-  int lo = 0;
-  for (int i = 1; i <= e; ++i) lo = min(max(offsets[i], lo), R);
-  const int hi = min(max(offsets[e + 1], lo), R);
-  const int n0 = blockIdx.y * TILE, k0 = blockIdx.x * TILE;
-  float acc[4][4] = {};
-  tile_product(dy, 1, lddy, n0, N, x, 1, ldx, k0, K, lo, hi, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + 4 * ty + i, k = k0 + 4 * tx + j;
-      if (n < N && k < K) put(dw + (static_cast<int64_t>(e) * N + n) * K + k, acc[i][j]);
+// y [R, N] from x [R, K] and matrices [E, N, K] (W_MN false) or [E, K, N]
+template <bool W_MN>
+__global__ void __launch_bounds__(ROW_THREADS, 1)
+grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
+                    __nv_bfloat16* __restrict__ y, int R, int E, int N, int K, int* err) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* epi = smem + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + ROW_EPI_BYTES);
+  uint64_t* full = bars;                     // [STAGES]  used in the leader
+  uint64_t* empty = bars + STAGES;           // [STAGES]  one per CTA
+  uint64_t* tfull = bars + 2 * STAGES;       // [2]       one per CTA
+  uint64_t* tempty = bars + 2 * STAGES + 2;  // [2]       used in the leader
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  int* edge = reinterpret_cast<int*>(epi + ROW_EPI_BYTES + BAR_BYTES);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cluster = static_cast<int>(blockIdx.x) >> 1, num_clusters = static_cast<int>(gridDim.x) >> 1;
+  const int cols = (N + 2 * BM - 1) / (2 * BM);
+  const int num_kb = (K + BK - 1) / BK;
+
+  load_edges(offsets, edge, E, R);
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 256);
+    }
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  Place at{edge, E};
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0, r0, live, col;
+      uint32_t phase = 0;
+      bool ok = true;
+      uint32_t lead_full[STAGES];
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) lead_full[s] = map_to_cta(&full[s], 0);
+      for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+        const int n0 = col * 2 * BM + static_cast<int>(rank) * BM;
+        const int half = (live + 31) / 32 * 16;      // rows in each CTA's half of the instruction's columns
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) { ok = false; break; }
+          uint8_t* sA = smem + stage * STAGE_BYTES;
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
+          if (!W_MN) {
+            tma_load_3d_pair(sA, &tmW, lead_full[stage], kb * BK, n0, at.e);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_3d_pair(sA + j * 8192, &tmW, lead_full[stage], n0 + j * 64, kb * BK, at.e);
+          }
+          tma_load_2d_pair(sA + A_BYTES, &tmX, lead_full[stage], kb * BK, r0 + static_cast<int>(rank) * half);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t a_lbo = W_MN ? 8192u : 16u, a_step = W_MN ? (2048u >> 4) : (32u >> 4);
+      int stage = 0, it = 0, r0, live, col;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+        const uint32_t idesc = make_idesc_bf16(2 * BM, (live + 31) / 32 * 32, W_MN, false);
+        const int acc = it & 1;
+        if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, err, kErrMmaTmemEmptyWait)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, err, kErrMmaFullWait)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+          const uint64_t da = make_desc_sw128(a_addr, a_lbo, 1024);
+          const uint64_t db = make_desc_sw128(a_addr + A_BYTES, 16u, 1024);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma2_f16_ss(d_tmem, da + static_cast<uint64_t>(k * a_step), db + static_cast<uint64_t>(k * (32u >> 4)), idesc,
+                         (kb != 0 || k != 0) ? 1u : 0u);
+          umma2_commit_both(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma2_commit_both(&tfull[acc]);
+        ++it;
+      }
+    }
+  } else {
+    const int q = warp & 3;      // TMEM lane quarter this warp may read
+    const uint32_t buf = smem_u32(epi + q * 64 * PITCH);
+    const uint32_t put = buf + (lane & 7) * PITCH + (lane >> 3) * 16;      // stmatrix: this lane's row and tile
+    int it = 0, r0, live, col;
+    bool ok = true;
+    for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+      const int n0 = col * 2 * BM + static_cast<int>(rank) * BM + q * 32;
+      const int acc = it & 1;
+      if (!mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+      const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
+#pragma unroll 1
+      for (int c = 0; c < live; c += 64) {
+        uint32_t v[32], u[32];
+        __syncwarp();
+        tmem_ld_16x256b_x8(t_row + c, v);
+        tmem_ld_16x256b_x8(t_row + c + (16u << 16), u);
+        tmem_ld_wait();
+        if (c + 64 >= live) {
+          tc_fence_before();
+          remote_arrive(lead_tempty);
+        }
+        if (n0 < N) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            stmatrix_x4_trans(put + j * 8 * PITCH, pack_bf16x2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
+                              pack_bf16x2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
+                              pack_bf16x2(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1])),
+                              pack_bf16x2(__uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3])));
+          __syncwarp();
+          const int piece = lane & 3, n = n0 + piece * 8;
+          if (n < N) {
+            __nv_bfloat16* dst = y + static_cast<int64_t>(r0 + c) * N + n;
+            const uint8_t* src = epi + q * 64 * PITCH + piece * 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = i * 8 + (lane >> 2);
+              if (c + row < live)
+                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(src + row * PITCH);
+            }
+          }
+        }
+      }
+      ++it;
+    }
+    // rows of no expert
+    for (int r = edge[E] + static_cast<int>(blockIdx.x) * 4 + q; r < R; r += static_cast<int>(gridDim.x) * 4)
+      for (int n = lane * 8; n < N; n += 256) *reinterpret_cast<uint4*>(y + static_cast<int64_t>(r) * N + n) = make_uint4(0, 0, 0, 0);
+  }
+
+  if (*reinterpret_cast<volatile int*>(err) != 0) {
+    // a wait expired somewhere: give copies and MMAs in flight time to land before TMEM is released
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// dw [E, N, K], OUT 0: bf16, 1: fp32
+template <int OUT>
+__global__ void __launch_bounds__(W_THREADS, 1)
+grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmDw,
+                     const int* __restrict__ offsets, int R, int E, int N, int K, int* err) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* epi = smem + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + W_EPI_BYTES);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* tail = bars + 2 * STAGES;        // [STAGES]  one per CTA: a block that needs rows zeroed has arrived here
+  uint64_t* mended = bars + 3 * STAGES;      // [STAGES]  used in the leader: the partner has zeroed its rows
+  uint64_t* tfull = bars + 4 * STAGES;
+  uint64_t* tempty = bars + 4 * STAGES + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * STAGES + 4);
+  static_assert((4 * STAGES + 5) * 8 <= BAR_BYTES, "barriers");
+  int* edge = reinterpret_cast<int*>(epi + W_EPI_BYTES + BAR_BYTES);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cluster = static_cast<int>(blockIdx.x) >> 1, num_clusters = static_cast<int>(gridDim.x) >> 1;
+  const int num_n = (N + 2 * BM - 1) / (2 * BM), num_k = (K + BN - 1) / BN;
+  const int per = num_n * num_k, num_units = per * E;
+
+  load_edges(offsets, edge, E, R);
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmDy);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmDw);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&tail[s], 1);
+      mbar_init(&mended[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 256);
+    }
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      uint32_t lead_full[STAGES];
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) lead_full[s] = map_to_cta(&full[s], 0);
+      for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
+        const int e = unit / per, t = unit % per;
+        const int lo = edge[e], rows = edge[e + 1] - lo;
+        const int n0 = t % num_n * 2 * BM + static_cast<int>(rank) * BM, k0 = t / num_n * BN + static_cast<int>(rank) * BNH;
+        const int num_kb = (rows + BK - 1) / BK;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) { ok = false; break; }
+          uint8_t* sA = smem + stage * STAGE_BYTES;
+          uint8_t* sB = sA + A_BYTES;
+          const int r0 = lo + kb * BK;
+          if (kb == num_kb - 1 && rows % 16 != 0) {
+            mbar_expect_tx(&tail[stage], STAGE_BYTES);
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d(sA + j * 8192, &tmDy, &tail[stage], n0 + j * 64, r0);
+#pragma unroll
+            for (int j = 0; j < BNH / 64; ++j) tma_load_2d(sB + j * 8192, &tmX, &tail[stage], k0 + j * 64, r0);
+          } else {
+            if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(sA + j * 8192, &tmDy, lead_full[stage], n0 + j * 64, r0);
+#pragma unroll
+            for (int j = 0; j < BNH / 64; ++j) tma_load_2d_pair(sB + j * 8192, &tmX, lead_full[stage], k0 + j * 64, r0);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = make_idesc_bf16(2 * BM, BN, true, true);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
+        const int e = unit / per, rows = edge[e + 1] - edge[e];
+        if (rows == 0) continue;
+        const int acc = it & 1;
+        if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, err, kErrMmaTmemEmptyWait)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        const int num_kb = (rows + BK - 1) / BK;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, err, kErrMmaFullWait)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+          const uint64_t da = make_desc_sw128(a_addr, 8192u, 1024);
+          const uint64_t db = make_desc_sw128(a_addr + A_BYTES, 8192u, 1024);
+          const int steps = min(BK / 16, (rows - kb * BK + 15) / 16);
+          for (int k = 0; k < steps; ++k)
+            umma2_f16_ss(d_tmem, da + static_cast<uint64_t>(k * (2048u >> 4)), db + static_cast<uint64_t>(k * (2048u >> 4)), idesc,
+                         (kb != 0 || k != 0) ? 1u : 0u);
+          umma2_commit_both(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma2_commit_both(&tfull[acc]);
+        ++it;
+      }
+    }
+  } else if (warp == 6) {
+    // zeros into the rows of the next group in a last block
+    int blocks = 0;                    // loaded so far, of all groups
+    uint32_t tail_phase = 0, mended_phase = 0;      // a bit per stage
+    bool ok = true;
+    for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
+      const int e = unit / per, rows = edge[e + 1] - edge[e];
+      blocks += (rows + BK - 1) / BK;
+      if (rows % 16 == 0) continue;
+      const int stage = (blocks - 1) % STAGES;
+      ok = mbar_wait_warp(&tail[stage], (tail_phase >> stage) & 1, err, kErrMmaFullWait);
+      if (!ok) break;
+      tail_phase ^= 1u << stage;
+      const int first = rows % BK, count = (16 - first % 16) * 8;      // 16-byte pieces of a box of 64 columns
+      uint8_t* from = smem + stage * STAGE_BYTES + first * 128;
+      for (int i = lane; i < 4 * count; i += 32)
+        *reinterpret_cast<uint4*>(from + (i / count) * 8192 + (i % count) * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (rank != 0) {
+        if (lane == 0) remote_arrive(map_to_cta(&mended[stage], 0));
+      } else {
+        ok = mbar_wait_warp(&mended[stage], (mended_phase >> stage) & 1, err, kErrMmaFullWait);
+        mended_phase ^= 1u << stage;
+        if (ok && lane == 0) mbar_arrive(&full[stage]);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int q = warp & 3;
+    uint8_t* buf0 = epi + q * 2 * EPI_BUF;
+    constexpr int COLS = OUT == 0 ? 64 : 32;      // columns per staged slab (128 B per row)
+    int it = 0, slab = 0;
+    bool ok = true;
+    for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
+      const int e = unit / per, t = unit % per;
+      const bool some = edge[e + 1] > edge[e];
+      const int n0 = t % num_n * 2 * BM + static_cast<int>(rank) * BM + q * 32, k0 = t / num_n * BN;
+      const int acc = it & 1;
+      if (some) {
+        ok = mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait);
+        if (!ok) break;
+        ++it;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+      const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
+#pragma unroll 1
+      for (int c = 0; c < BN / COLS; ++c) {
+        uint32_t v[64];
+        __syncwarp();
+        if (some) {
+          tmem_ld_32x32b_x32(t_row + c * COLS, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+          if (OUT == 0) tmem_ld_32x32b_x32(t_row + c * COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+          tmem_ld_wait();
+          if (c == BN / COLS - 1) {
+            tc_fence_before();
+            remote_arrive(lead_tempty);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = 0u;
+        }
+        if (n0 < N && k0 + c * COLS < K) {
+          uint8_t* buf = buf0 + (slab & 1) * EPI_BUF;
+          ++slab;
+          if (lane == 0) tma_wait_group_read<1>();      // the store that last used this buffer has read it
+          __syncwarp();
+          uint8_t* row = buf + lane * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint4 pk;
+            if (OUT == 0) {
+              pk.x = pack_bf16x2(__uint_as_float(v[8 * j + 0]), __uint_as_float(v[8 * j + 1]));
+              pk.y = pack_bf16x2(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3]));
+              pk.z = pack_bf16x2(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5]));
+              pk.w = pack_bf16x2(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]));
+            } else {
+              pk.x = v[4 * j + 0]; pk.y = v[4 * j + 1]; pk.z = v[4 * j + 2]; pk.w = v[4 * j + 3];
+            }
+            *reinterpret_cast<uint4*>(row + ((j ^ (lane & 7)) << 4)) = pk;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&tmDw, buf, k0 + c * COLS, n0, e);
+            tma_commit_group();
+          }
+        }
+      }
+    }
+    if (lane == 0) tma_wait_group<0>();
+  }
+
+  if (*reinterpret_cast<volatile int*>(err) != 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// CTA pairs that the device holds at once (the two CTAs sit on the two SMs of one TPC)
+int g_pairs = 0;
+
+template <class... Params, class... Args>
+int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, int num_sms, cudaStream_t stream, Args... args) {
+  if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return -20;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  if (g_pairs == 0) {
+    int dev = 0, all_sms = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&all_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -23;
+    cfg.gridDim = dim3(2 * (all_sms / 2));
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) return -23;
+    g_pairs = n < all_sms / 2 ? n : all_sms / 2;
+  }
+  const int pairs = g_pairs < num_sms / 2 ? g_pairs : num_sms / 2;
+  cfg.gridDim = dim3(2 * static_cast<int>(units < pairs ? units : pairs));
+  cfg.stream = stream;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? 0 : -21;
 }
 
 }  // namespace
 
 int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
                  int E, int N, int K, int* err, int num_sms, cudaStream_t stream) {
-  const dim3 grid((N + TILE - 1) / TILE, (R + TILE - 1) / TILE + E + 1);
-  if (grid.y > 65535) return -3;
-  grouped_simple_kernel<<<grid, 256, 0, stream>>>(x, ldx, w, w_t ? 1 : K, w_t ? N : 1, offsets, y, R, E, N, K);
-  return cudaGetLastError() == cudaSuccess ? 0 : -21;
+  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(y) & 15) != 0) return -1;
+  CUtensorMap tw, tx;
+  int r = w_t ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64) : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
+  if (r) return r;
+  r = make_tmap_2d(&tx, x, 2, R, K, ldx, BNH, 64);
+  if (r) return r - 100;
+  // at most: every group with rows ends in a tile that is not full
+  const int64_t tiles = static_cast<int64_t>(R) / BN + (E < R ? E : R);
+  const int64_t units = tiles * ((N + 2 * BM - 1) / (2 * BM));
+  return w_t ? launch_pairs(grouped_rows_kernel<true>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, y, R, E, N, K, err)
+             : launch_pairs(grouped_rows_kernel<false>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, y, R, E, N, K, err);
 }
 
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,
                   int R, int E, int N, int K, int* err, int num_sms, cudaStream_t stream) {
-  const dim3 grid((K + TILE - 1) / TILE, (N + TILE - 1) / TILE, E);
-  if (dw_bf16)
-    grouped_wgrad_simple_kernel<<<grid, 256, 0, stream>>>(dy, lddy, x, ldx, offsets, static_cast<__nv_bfloat16*>(dw), R, N, K);
-  else
-    grouped_wgrad_simple_kernel<<<grid, 256, 0, stream>>>(dy, lddy, x, ldx, offsets, static_cast<float*>(dw), R, N, K);
-  return cudaGetLastError() == cudaSuccess ? 0 : -21;
+  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1) return -1;
+  CUtensorMap ty, tx, tw;
+  int r = make_tmap_2d(&ty, dy, 2, R, N, lddy, 64, 64);
+  if (r) return r;
+  r = make_tmap_2d(&tx, x, 2, R, K, ldx, 64, 64);
+  if (r) return r - 100;
+  r = dw_bf16 ? make_tmap_3d(&tw, dw, 2, E, N, K, 32, 64) : make_tmap_3d(&tw, dw, 4, E, N, K, 32, 32);
+  if (r) return r - 200;
+  const int64_t units = static_cast<int64_t>(E) * ((N + 2 * BM - 1) / (2 * BM)) * ((K + BN - 1) / BN);
+  if (units > (1ll << 30)) return -3;
+  return dw_bf16 ? launch_pairs(grouped_wgrad_kernel<0>, W_THREADS, W_SMEM, units, num_sms, stream, ty, tx, tw, offsets, R, E, N, K, err)
+                 : launch_pairs(grouped_wgrad_kernel<1>, W_THREADS, W_SMEM, units, num_sms, stream, ty, tx, tw, offsets, R, E, N, K, err);
 }
 
 }  // namespace tb
