@@ -1,8 +1,11 @@
-// Python bindings of the mixture-of-experts kernels and of the 8-bit activation checkpoints.  Outputs are allocated here; in the
-// poison mode (ops/debug.py) `track` gets each before its kernel runs.  Every call returns the number of kernels it launched last.
+// Python bindings of the mixture-of-experts kernels and of the 8-bit activation checkpoints, with their autograd nodes: a node in
+// Python costs the host 40 - 90 us for a forward and a backward pass, more than most of these kernels run.  Outputs are allocated
+// here; in the poison mode (ops/debug.py) each is filled and remembered before its kernel runs.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+
+#include <atomic>
 
 #include "bind_common.h"
 #include "moe_api.h"
@@ -14,14 +17,20 @@ using OptTensor = c10::optional<Tensor>;
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
+// Backward passes run in threads of autograd's, which do not hold the interpreter's lock.
 struct Outputs {
-  const pybind11::object& track;
+  bool poisoned;
   Tensor operator()(const char* name, c10::IntArrayRef size, const at::TensorOptions& options) const {
     Tensor t = torch::empty(size, options);
-    if (!track.is_none()) track(name, t);
+    if (poisoned) {
+      pybind11::gil_scoped_acquire lock;
+      pybind11::module_::import("torchure_b200.ops.debug").attr("track")(name, t);
+    }
     return t;
   }
 };
+
+std::atomic<int64_t> g_launches{0};      // kernels launched by the calls of this file
 
 const __nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
 __nv_bfloat16* bfm(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
@@ -29,21 +38,22 @@ bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
 bool bf16_or_f32(const Tensor& t, const char* what) {
   const bool b = t.scalar_type() == torch::kBFloat16;
-  TORCH_CHECK(b || t.scalar_type() == torch::kFloat32, what, ": bf16 or fp32 expected, got ", t.scalar_type());
+  TORCH_CHECK_TYPE(b || t.scalar_type() == torch::kFloat32, what, ": bf16 or fp32 expected, got ", t.scalar_type());
   return b;
 }
 // A matrix on the GPU whose rows are contiguous
 void check_rows(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what, ": a 2-D CUDA tensor with contiguous rows expected");
+  TORCH_CHECK_VALUE(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what,
+                    ": a matrix on the GPU with contiguous rows expected, got ", t.sizes());
   TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31), what, ": sizes of 2^31 and more are not supported");
 }
 void check_bf16(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.scalar_type() == torch::kBFloat16, what, ": bf16 expected, got ", t.scalar_type());
+  TORCH_CHECK_TYPE(t.scalar_type() == torch::kBFloat16, what, ": bf16 expected, got ", t.scalar_type());
 }
 void check_ints(const Tensor& t, int64_t n, const Tensor& like, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.numel() == n, what, ": contiguous int32 of ", n,
+  TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.numel() == n, what, ": contiguous int32 of ", n,
               " elements on the GPU expected");
-  TORCH_CHECK(t.device() == like.device(), what, ": on another GPU than its operand");
+  TORCH_CHECK_VALUE(t.device() == like.device(), what, ": on another GPU than its operand");
 }
 int64_t blocks_of(int64_t n) { return (n + tb::kActBlock - 1) / tb::kActBlock; }
 
@@ -55,10 +65,10 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   check_rows(logits, "route");
   const bool b16 = bf16_or_f32(logits, "route: logits");
   const int64_t T = logits.size(0), E = logits.size(1);
-  TORCH_CHECK(E >= 1 && E <= tb::kMaxExperts, "route: 1 to ", tb::kMaxExperts, " experts, got ", E);
-  TORCH_CHECK(k >= 1 && k <= E && k <= tb::kMaxChoices, "route: top_k of ", k, " among ", E, " experts (at most ", tb::kMaxChoices, ")");
-  TORCH_CHECK(capacity >= 0 && capacity < (1ll << 31), "route: capacity ", capacity);
-  TORCH_CHECK(T * k <= (1ll << 30), "route: too many choices");
+  TORCH_CHECK_VALUE(E >= 1 && E <= tb::kMaxExperts, "route: 1 to ", tb::kMaxExperts, " experts, got ", E);
+  TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= tb::kMaxChoices, "route: top_k of ", k, " among ", E, " experts (at most ", tb::kMaxChoices, ")");
+  TORCH_CHECK_VALUE(capacity >= 0 && capacity < (1ll << 31), "route: capacity ", capacity);
+  TORCH_CHECK_VALUE(T * k <= (1ll << 30), "route: too many choices");
   const auto f32 = logits.options().dtype(torch::kFloat32), i32 = logits.options().dtype(torch::kInt32);
   Routed r;
   r.weights = make("route.weights", {T, k}, f32);
@@ -80,6 +90,7 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, r.weights.data_ptr<float>(),
                                r.experts.data_ptr<int>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), r.rows.data_ptr<int>(),
                                r.counts.data_ptr<int>(), r.aux.data_ptr<float>(), ints.data_ptr<int>() + 2 * E + 1, cur_stream());
+  g_launches += 1;
   TORCH_CHECK(rc == 0, "route failed with code ", rc);
   return r;
 }
@@ -100,6 +111,7 @@ Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& e
   const int rc = tb::route_bwd(logits.data_ptr(), b16, logits.stride(0), weights.data_ptr<float>(), experts.data_ptr<int>(),
                                counts.data_ptr<int>(), has(dweights) ? dweights->data_ptr<float>() : nullptr,
                                has(daux) ? daux->data_ptr<float>() : nullptr, dl.data_ptr(), (int)T, (int)E, (int)k, cur_stream());
+  g_launches += 1;
   TORCH_CHECK(rc == 0, "route_bwd failed with code ", rc);
   return dl;
 }
@@ -111,6 +123,7 @@ Tensor do_gather(const Tensor& x, const Tensor& rows, int64_t k, const Outputs& 
   check_ints(rows, R, x, "dispatch: rows");
   Tensor out = make("dispatch", {R, D}, x.options().dtype(torch::kBFloat16));
   tb::rows_gather(x.data_ptr(), b16, x.stride(0), rows.data_ptr<int>(), bfm(out), (int)T, (int)k, (int)R, (int)D, cur_stream());
+  g_launches += 1;
   return out;
 }
 
@@ -126,12 +139,12 @@ Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots
   Tensor out = make("combine", {T, D}, y.options().dtype(type));
   tb::rows_combine(bf(y), has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
                    type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream());
+  g_launches += 1;
   return out;
 }
 
-std::tuple<Tensor, Tensor> combine_bwd(const Tensor& dout, const Tensor& y, const Tensor& weights, const Tensor& slots,
-                                       const Tensor& offsets, const pybind11::object& track) {
-  const Outputs make{track};
+std::tuple<Tensor, Tensor> do_combine_bwd(const Tensor& dout, const Tensor& y, const Tensor& weights, const Tensor& slots,
+                                          const Tensor& offsets, const Outputs& make) {
   check_rows(dout, "combine_bwd");
   const bool b16 = bf16_or_f32(dout, "combine_bwd");
   const int64_t T = slots.size(0), k = slots.size(1), D = y.size(1), E = offsets.numel() - 1;
@@ -141,11 +154,11 @@ std::tuple<Tensor, Tensor> combine_bwd(const Tensor& dout, const Tensor& y, cons
   check_ints(slots, T * k, y, "combine_bwd: slots");
   check_ints(offsets, E + 1, y, "combine_bwd: offsets");
   TORCH_CHECK(weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.numel() == T * k, "combine_bwd: weights");
-  c10::cuda::CUDAGuard guard(y.device());
   Tensor dy = make("combine_bwd.dy", {T * k, D}, y.options());
   Tensor dw = make("combine_bwd.dweights", {T, k}, weights.options());
   tb::rows_combine_bwd(dout.data_ptr(), b16, dout.stride(0), bf(y), weights.data_ptr<float>(), slots.data_ptr<int>(),
                        offsets.data_ptr<int>(), bfm(dy), dw.data_ptr<float>(), (int)T, (int)k, (int)E, (int)D, cur_stream());
+  g_launches += 1;
   return {dy, dw};
 }
 
@@ -160,7 +173,8 @@ void check_group(const Tensor& x, const Tensor& offsets, const char* what) {
 Tensor do_grouped(const Tensor& x, const Tensor& w, const Tensor& offsets, bool w_t, const Outputs& make) {
   check_group(x, offsets, "grouped_linear");
   check_bf16(w, "grouped_linear: w");
-  TORCH_CHECK(w.is_cuda() && w.dim() == 3 && w.is_contiguous() && w.size(0) == offsets.numel() - 1 && w.size(w_t ? 1 : 2) == x.size(1) &&
+  TORCH_CHECK_VALUE(offsets.numel() - 1 <= tb::kMaxExperts, "grouped_linear: at most ", tb::kMaxExperts, " experts");
+  TORCH_CHECK_VALUE(w.is_cuda() && w.dim() == 3 && w.is_contiguous() && w.size(0) == offsets.numel() - 1 && w.size(w_t ? 1 : 2) == x.size(1) &&
                   w.device() == x.device(), "grouped_linear: w ", w.sizes(), " does not fit rows of ", x.size(1), " and ",
               offsets.numel() - 1, " experts");
   const int64_t R = x.size(0), K = x.size(1), N = w.size(w_t ? 2 : 1);
@@ -169,6 +183,7 @@ Tensor do_grouped(const Tensor& x, const Tensor& w, const Tensor& offsets, bool 
   if (K == 0) return y.zero_();
   const int rc = tb::grouped_gemm(bf(x), x.stride(0), bf(w), w_t, offsets.data_ptr<int>(), bfm(y), (int)R, (int)w.size(0), (int)N, (int)K,
                                   attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+  g_launches += 1;
   TORCH_CHECK(rc == 0, "grouped_linear failed with code ", rc);
   return y;
 }
@@ -184,6 +199,7 @@ Tensor do_wgrad(const Tensor& dy, const Tensor& x, const Tensor& offsets, at::Sc
   if (R == 0) return dw.zero_();
   const int rc = tb::grouped_wgrad(bf(dy), dy.stride(0), bf(x), x.stride(0), offsets.data_ptr<int>(), dw.data_ptr(), type == torch::kBFloat16,
                                    (int)R, (int)E, (int)N, (int)K, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+  g_launches += 1;
   TORCH_CHECK(rc == 0, "grouped_wgrad failed with code ", rc);
   return dw;
 }
@@ -195,6 +211,7 @@ std::tuple<Tensor, Tensor> do_quantize(const Tensor& x) {
   Tensor q = torch::empty({M, N}, x.options().dtype(torch::kInt8));
   Tensor s = torch::empty({M, blocks_of(N)}, x.options().dtype(torch::kFloat32));
   tb::quantize8(bf(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)N, cur_stream());
+  g_launches += 1;
   return {q, s};
 }
 
@@ -209,6 +226,7 @@ Tensor do_dequantize(const Tensor& q, const Tensor& s, const Outputs& make) {
   check_kept(q, s, q.dim() == 2 ? blocks_of(q.size(1)) : 0, "dequantize8");
   Tensor x = make("dequantize8", q.sizes(), q.options().dtype(torch::kBFloat16));
   tb::dequantize8(q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(x), q.size(0), (int)q.size(1), cur_stream());
+  g_launches += 1;
   return x;
 }
 
@@ -222,6 +240,7 @@ std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, const Outputs& m
   Tensor q = torch::empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
   Tensor s = torch::empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
   tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)F, cur_stream());
+  g_launches += 1;
   return {act, q, s};
 }
 
@@ -233,139 +252,321 @@ Tensor do_swiglu8_bwd(const Tensor& dact, const Tensor& q, const Tensor& s, cons
   TORCH_CHECK(q.size(0) == M && q.size(1) == 2 * F && q.device() == dact.device(), "swiglu_8bit backward: shapes");
   Tensor dgu = make("swiglu_8bit.bwd", {M, 2 * F}, dact.options());
   tb::swiglu8_bwd(bf(dact), dact.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(dgu), M, (int)F, cur_stream());
+  g_launches += 1;
   return dgu;
 }
 
+// ---- operands as the kernels read them ---------------------------------------------------------------
+// x with contiguous rows (a copy only where it has none)
+Tensor rows_of(const Tensor& x) { return x.size(-1) <= 1 || x.stride(-1) == 1 ? x : x.contiguous(); }
+// x [R, K] with columns in eights (zeros behind), the row stride and the base on 16 bytes
+Tensor operand(const Tensor& x) {
+  if (x.size(1) % 8 == 0 && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
+      (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0)
+    return x;
+  return x.size(1) % 8 ? at::constant_pad_nd(x, {0, (8 - x.size(1) % 8) % 8}).contiguous() : x.clone(at::MemoryFormat::Contiguous);
+}
+// w [E, N, K] in bf16, both widths in eights (zeros behind)
+Tensor matrices(const Tensor& w) {
+  Tensor b = w.scalar_type() == torch::kBFloat16 ? w : w.to(torch::kBFloat16);
+  const int64_t n = (8 - w.size(1) % 8) % 8, k = (8 - w.size(2) % 8) % 8;
+  b = n || k ? at::constant_pad_nd(b, {0, k, 0, n}).contiguous() : b.contiguous();
+  return (reinterpret_cast<uintptr_t>(b.data_ptr()) & 15) == 0 ? b : b.clone();
+}
+
+// ---- autograd nodes ----------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void only_once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient itself has no gradient (create_graph is not supported)");
+}
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
+
+struct RouteNode : torch::autograd::Function<RouteNode> {
+  // weights, aux, experts, slots, offsets, rows, counts
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
+    Routed r = do_route(logits, k, capacity, Outputs{poison});
+    ctx->save_for_backward({logits, r.weights, r.experts, r.counts});
+    ctx->saved_data["poison"] = poison;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({r.experts, r.slots, r.offsets, r.rows, r.counts});
+    return {r.weights, r.aux, r.experts, r.slots, r.offsets, r.rows, r.counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("route");
+    const auto s = ctx->get_saved_variables();
+    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    c10::cuda::CUDAGuard guard(s[0].device());
+    const Tensor dw = grads[0].defined() ? grads[0].to(torch::kFloat32).contiguous() : grads[0];
+    const Tensor da = grads[1].defined() ? grads[1].to(torch::kFloat32) : grads[1];
+    return {do_route_bwd(s[0], s[1], s[2], s[3], opt(dw), opt(da), Outputs{ctx->saved_data["poison"].toBool()}), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
+  check_rows(logits, "route");
+  c10::cuda::CUDAGuard guard(logits.device());
+  return RouteNode::apply(logits, k, capacity, poison);
+}
+
+struct DispatchNode : torch::autograd::Function<DispatchNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& slots, const Tensor& rows, bool poison) {
+    ctx->save_for_backward({slots});
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["poison"] = poison;
+    return do_gather(x, rows, slots.size(1), Outputs{poison});
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("dispatch");
+    const Tensor slots = ctx->get_saved_variables()[0];
+    c10::cuda::CUDAGuard guard(slots.device());
+    return {do_combine(grads[0].contiguous(), c10::nullopt, slots, static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()),
+                       Outputs{ctx->saved_data["poison"].toBool()}), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor moe_dispatch(const Tensor& x, const Tensor& slots, const Tensor& rows, bool poison) {
+  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK_VALUE(x.dim() == 2 && slots.dim() == 2 && x.size(0) == slots.size(0), "dispatch: ", slots.size(0), " tokens were routed, got ", x.sizes());
+  check_ints(slots, rows.numel(), x, "dispatch: slots");
+  return DispatchNode::apply(rows_of(x), slots, rows, poison);
+}
+
+struct CombineNode : torch::autograd::Function<CombineNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor& slots, const Tensor& offsets, bool f32,
+                        bool poison) {
+    ctx->save_for_backward({y, weights, slots, offsets});
+    ctx->saved_data["poison"] = poison;
+    return do_combine(y, weights, slots, f32 ? torch::kFloat32 : torch::kBFloat16, Outputs{poison});
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("combine");
+    const auto s = ctx->get_saved_variables();
+    c10::cuda::CUDAGuard guard(s[0].device());
+    auto r = do_combine_bwd(rows_of(grads[0]), s[0], s[1], s[2], s[3], Outputs{ctx->saved_data["poison"].toBool()});
+    return {std::get<0>(r), std::get<1>(r), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, const Tensor& offsets, bool f32, bool poison) {
+  c10::cuda::CUDAGuard guard(y.device());
+  TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ", y.sizes());
+  check_ints(offsets, offsets.numel(), y, "combine: offsets");
+  return CombineNode::apply(y.contiguous(), weights.contiguous(), slots, offsets, f32, poison);
+}
+
+struct GroupedNode : torch::autograd::Function<GroupedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, bool poison) {
+    const Tensor xb = operand(x), wb = matrices(w);
+    const Tensor y = do_grouped(xb, wb, offsets, false, Outputs{poison});
+    ctx->save_for_backward({xb, wb, offsets});
+    ctx->saved_data["n"] = w.size(1);
+    ctx->saved_data["k"] = w.size(2);
+    ctx->saved_data["type"] = static_cast<int64_t>(w.scalar_type());
+    ctx->saved_data["poison"] = poison;
+    return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("grouped_linear");
+    const auto s = ctx->get_saved_variables();
+    const int64_t n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
+    const Outputs make{ctx->saved_data["poison"].toBool()};
+    c10::cuda::CUDAGuard guard(s[0].device());
+    const Tensor dy = operand(grads[0]);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      dx = do_grouped(dy, s[1], s[2], true, make);
+      if (dx.size(1) != k) dx = dx.narrow(1, 0, k);
+    }
+    if (ctx->needs_input_grad(1)) {
+      dw = do_wgrad(dy, s[0], s[2], static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), make);
+      if (dw.size(1) != n || dw.size(2) != k) dw = dw.narrow(1, 0, n).narrow(2, 0, k);
+    }
+    return {dx, dw, Tensor(), Tensor()};
+  }
+};
+
+Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, bool poison) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3 && x.size(1) == w.size(2), "grouped_linear: rows ", x.sizes(), " and matrices ", w.sizes(),
+                    " do not fit");
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() == w.size(0) + 1, "grouped_linear: ", w.size(0) + 1, " offsets expected, got ",
+                    offsets.sizes());
+  TORCH_CHECK_TYPE(x.scalar_type() == torch::kBFloat16 && (w.scalar_type() == torch::kBFloat16 || w.scalar_type() == torch::kFloat32),
+                   "grouped_linear: bf16 rows and bf16 or fp32 matrices expected, got ", x.scalar_type(), " and ", w.scalar_type());
+  TORCH_CHECK_VALUE(offsets.scalar_type() == torch::kInt32 && offsets.device() == x.device() && w.device() == x.device(),
+                    "grouped_linear: int32 offsets and matrices on the GPU of the rows expected");
+  c10::cuda::CUDAGuard guard(x.device());
+  return GroupedNode::apply(x, w, offsets.contiguous(), poison);
+}
+
+struct Swiglu8Node : torch::autograd::Function<Swiglu8Node> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& gu, bool poison) {
+    auto r = do_swiglu8(gu, Outputs{poison});
+    ctx->save_for_backward({std::get<1>(r), std::get<2>(r)});
+    ctx->saved_data["poison"] = poison;
+    return std::get<0>(r);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("swiglu_8bit");
+    const auto s = ctx->get_saved_variables();
+    c10::cuda::CUDAGuard guard(s[0].device());
+    return {do_swiglu8_bwd(rows_of(grads[0]), s[0], s[1], Outputs{ctx->saved_data["poison"].toBool()}), Tensor()};
+  }
+};
+
+Tensor swiglu_8bit(const Tensor& gu, bool poison) {
+  check_bf16(gu, "swiglu_8bit");
+  TORCH_CHECK_VALUE(gu.dim() >= 1 && gu.size(-1) % 2 == 0, "swiglu_8bit: gate and up columns expected, got ", gu.sizes());
+  c10::cuda::CUDAGuard guard(gu.device());
+  if (gu.dim() == 2) return Swiglu8Node::apply(rows_of(gu), poison);
+  auto shape = gu.sizes().vec();
+  const Tensor act = Swiglu8Node::apply(rows_of(gu.reshape({-1, shape.back()})), poison);
+  shape.back() /= 2;
+  return act.view(shape);
+}
+
 // ---- the whole feed-forward -------------------------------------------------------------------------
-void check_experts(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd) {
-  check_rows(x, "expert_mlp: x");
-  check_bf16(wgu, "expert_mlp: w_gate_up");
-  check_bf16(wd, "expert_mlp: w_down");
-  const int64_t E = logits.size(1), D = x.size(1);
-  TORCH_CHECK(logits.dim() == 2 && logits.size(0) == x.size(0), "expert_mlp: ", x.size(0), " tokens and logits ", logits.sizes());
-  TORCH_CHECK(wd.dim() == 3 && wd.size(0) == E && wd.size(1) == D && wd.is_contiguous(), "expert_mlp: w_down ", wd.sizes(),
-              " is not [", E, ", ", D, ", units]");
-  TORCH_CHECK(wgu.dim() == 3 && wgu.size(0) == E && wgu.size(1) == 2 * wd.size(2) && wgu.size(2) == D && wgu.is_contiguous(),
-              "expert_mlp: w_gate_up ", wgu.sizes(), " is not [", E, ", ", 2 * wd.size(2), ", ", D, "]");
-  TORCH_CHECK(x.device() == logits.device() && x.device() == wgu.device() && x.device() == wd.device(), "expert_mlp: tensors on several GPUs");
-}
+struct Mlp {
+  Tensor out;
+  Routed r;
+  Tensor gu, q, scales;      // what the backward pass reads: gate | up in bf16, or in 8 bits
+};
 
-// out, aux, weights, experts, slots, offsets, rows, counts, gu (bf16, or q and scales), launches
-std::tuple<std::vector<OptTensor>, int64_t> expert_mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
-                                                           int64_t k, int64_t capacity, int64_t bits, bool keep,
-                                                           const pybind11::object& track) {
-  check_experts(x, logits, wgu, wd);
-  TORCH_CHECK(bits == 8 || bits == 16, "expert_mlp: activations are kept in 8 or 16 bits, not ", bits);
-  const Outputs make{track};
-  c10::cuda::CUDAGuard guard(x.device());
-  Routed r = do_route(logits, k, capacity, make);
-  Tensor xg = do_gather(x, r.rows, k, make);
-  Tensor gu = do_grouped(xg, wgu, r.offsets, false, make);
-  Tensor act;
-  OptTensor q, s;
+Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool keep,
+            const Outputs& make) {
+  Mlp m;
+  m.r = do_route(logits, k, capacity, make);
+  const Tensor xg = do_gather(x, m.r.rows, k, make);
+  const Tensor gu = do_grouped(xg, wgu, m.r.offsets, false, make);
+  auto t = do_swiglu8(gu, make);
+  if (keep && bits == 16) m.gu = gu;
   if (keep && bits == 8) {
-    auto t = do_swiglu8(gu, make);
-    act = std::get<0>(t);
-    q = std::get<1>(t);
-    s = std::get<2>(t);
-  } else {
-    auto t = do_swiglu8(gu, make);
-    act = std::get<0>(t);
+    m.q = std::get<1>(t);
+    m.scales = std::get<2>(t);
   }
-  Tensor y = do_grouped(act, wd, r.offsets, false, make);
-  Tensor out = do_combine(y, r.weights, r.slots, x.scalar_type(), make);
-  OptTensor kept;
-  if (keep && bits == 16) kept = gu;
-  return {{out, r.aux, r.weights, r.experts, r.slots, r.offsets, r.rows, r.counts, kept, q, s}, 7};
+  const Tensor y = do_grouped(std::get<0>(t), wd, m.r.offsets, false, make);
+  m.out = do_combine(y, m.r.weights, m.r.slots, x.scalar_type(), make);
+  return m;
 }
 
-// dx, dlogits, dw_gate_up, dw_down, launches
-std::tuple<std::vector<OptTensor>, int64_t> expert_mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits,
-                                                           const Tensor& wgu, const Tensor& wd, const Tensor& weights,
-                                                           const Tensor& experts, const Tensor& slots, const Tensor& offsets,
-                                                           const Tensor& rows, const Tensor& counts, const OptTensor& gu,
-                                                           const OptTensor& q, const OptTensor& scales, bool dw_f32,
-                                                           const pybind11::object& track) {
-  check_experts(x, logits, wgu, wd);
-  const Outputs make{track};
-  c10::cuda::CUDAGuard guard(x.device());
-  const int64_t T = x.size(0), k = slots.size(1), R = T * k, E = logits.size(1), F = wd.size(2);
-  check_ints(slots, R, x, "expert_mlp backward: slots");
-  check_ints(offsets, E + 1, x, "expert_mlp backward: offsets");
-  TORCH_CHECK(dout.dim() == 2 && dout.size(0) == T && dout.size(1) == x.size(1), "expert_mlp backward: dout");
-  if (has(gu)) {
-    TORCH_CHECK(gu->is_contiguous() && gu->scalar_type() == torch::kBFloat16 && gu->size(0) == R && gu->size(1) == 2 * F,
-                "expert_mlp backward: gu");
-  } else {
-    TORCH_CHECK(has(q) && has(scales), "expert_mlp backward: no activations were kept");
-    check_kept(*q, *scales, 2 * blocks_of(F), "expert_mlp backward");
-    TORCH_CHECK(q->size(0) == R && q->size(1) == 2 * F, "expert_mlp backward: kept activations");
-  }
-  const auto wtype = dw_f32 ? torch::kFloat32 : torch::kBFloat16;
-  Tensor dg = do_gather(dout, rows, k, make);
-  Tensor s = do_grouped(dg, wd, offsets, true, make);
+// dx, dlogits, dw_gate_up, dw_down
+variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
+                      const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Outputs& make) {
+  const int64_t T = x.size(0), k = r.slots.size(1), R = T * k, E = logits.size(1), F = wd.size(2);
+  const Tensor dg = do_gather(dout, r.rows, k, make);
+  const Tensor s = do_grouped(dg, wd, r.offsets, true, make);
   Tensor dgu = make("expert_mlp.dgu", {R, 2 * F}, wgu.options());
   Tensor act_w = make("expert_mlp.act", {R, F}, wgu.options());
-  Tensor dweights = make("expert_mlp.dweights", {T, k}, weights.options());
-  tb::expert_swiglu_bwd(bf(s), has(gu) ? bf(*gu) : nullptr, has(gu) ? nullptr : q->data_ptr<int8_t>(),
-                        has(gu) ? nullptr : scales->data_ptr<float>(), weights.data_ptr<float>(), slots.data_ptr<int>(),
-                        offsets.data_ptr<int>(), bfm(dgu), bfm(act_w), dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream());
-  Tensor dwd = do_wgrad(dg, act_w, offsets, wtype, make);
-  Tensor dxg = do_grouped(dgu, wgu, offsets, true, make);
-  Tensor dx = do_combine(dxg, c10::nullopt, slots, x.scalar_type(), make);
-  Tensor xg = do_gather(x, rows, k, make);
-  Tensor dwgu = do_wgrad(dgu, xg, offsets, wtype, make);
-  Tensor dl = do_route_bwd(logits, weights, experts, counts, dweights, daux, make);
-  return {{dx, dl, dwgu, dwd}, 9};
+  Tensor dweights = make("expert_mlp.dweights", {T, k}, r.weights.options());
+  const bool kept16 = gu.defined();
+  tb::expert_swiglu_bwd(bf(s), kept16 ? bf(gu) : nullptr, kept16 ? nullptr : q.data_ptr<int8_t>(), kept16 ? nullptr : scales.data_ptr<float>(),
+                        r.weights.data_ptr<float>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), bfm(dgu), bfm(act_w),
+                        dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream());
+  g_launches += 1;
+  const Tensor dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
+  const Tensor dxg = do_grouped(dgu, wgu, r.offsets, true, make);
+  const Tensor dx = do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make);
+  const Tensor xg = do_gather(x, r.rows, k, make);
+  const Tensor dwgu = do_wgrad(dgu, xg, r.offsets, wtype, make);
+  const Tensor dl = do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make);
+  return {dx, dl, dwgu, dwd};
+}
+
+// gate and up matrices as one bf16 stack [E, 2F, D]: given as one, or as a pair
+Tensor stack_of(const Tensor& first, const OptTensor& second) {
+  if (!has(second)) return matrices(first);
+  const int64_t E = first.size(0), F = first.size(1), D = first.size(2);
+  Tensor w = torch::empty({E, 2 * F, D}, first.options().dtype(torch::kBFloat16));
+  w.narrow(1, 0, F).copy_(first);
+  w.narrow(1, F, F).copy_(*second);
+  return w;
+}
+
+struct MlpNode : torch::autograd::Function<MlpNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second,
+                               const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool poison) {
+    const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
+    Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, bits, true, Outputs{poison});
+    ctx->save_for_backward({x, logits, wgu, wdb, m.r.weights, m.r.experts, m.r.slots, m.r.offsets, m.r.rows, m.r.counts, m.gu, m.q, m.scales});
+    ctx->saved_data["type"] = static_cast<int64_t>(wd.scalar_type());
+    ctx->saved_data["pair"] = has(second);
+    ctx->saved_data["poison"] = poison;
+    ctx->set_materialize_grads(false);
+    return {m.out, m.r.aux};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("expert_mlp");
+    const auto s = ctx->get_saved_variables();
+    const Outputs make{ctx->saved_data["poison"].toBool()};
+    variable_list out(9);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    c10::cuda::CUDAGuard guard(s[0].device());
+    const Tensor daux = grads[1].defined() ? grads[1].to(torch::kFloat32) : grads[1];
+    if (!grads[0].defined()) {
+      out[1] = do_route_bwd(s[1], s[4], s[5], s[9], c10::nullopt, opt(daux), make);
+      return out;
+    }
+    Routed r{s[4], s[5], s[6], s[7], s[8], s[9], Tensor()};
+    auto g = mlp_bwd(rows_of(grads[0]), opt(daux), s[0], s[1], s[2], s[3], r, s[10], s[11], s[12],
+                     static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), make);
+    const int64_t F = s[3].size(2);
+    out[0] = g[0];
+    out[1] = g[1];
+    out[2] = ctx->saved_data["pair"].toBool() ? g[2].narrow(1, 0, F) : g[2];
+    if (ctx->saved_data["pair"].toBool()) out[3] = g[2].narrow(1, F, F);
+    out[4] = g[3];
+    return out;
+  }
+};
+
+variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
+                         int64_t capacity, int64_t bits, bool poison) {
+  check_rows(x, "expert_mlp: x");
+  check_rows(logits, "expert_mlp: logits");
+  bf16_or_f32(x, "expert_mlp: x");
+  bf16_or_f32(first, "expert_mlp: w_gate_up");
+  TORCH_CHECK_TYPE(first.scalar_type() == wd.scalar_type(), "expert_mlp: matrices of one type expected, got ", first.scalar_type(), " and ",
+                   wd.scalar_type());
+  TORCH_CHECK_VALUE(bits == 8 || bits == 16, "expert_mlp: activations are kept in 8 or 16 bits, not ", bits);
+  const bool pair = has(second);
+  TORCH_CHECK_VALUE(!pair || (second->sizes() == first.sizes() && second->scalar_type() == first.scalar_type() && second->device() == first.device()),
+                    "expert_mlp: w_gate and w_up differ");
+  TORCH_CHECK_VALUE(wd.dim() == 3 && first.dim() == 3, "expert_mlp: matrices [E, 2F, D] and [E, D, F] expected");
+  const int64_t E = wd.size(0), D = wd.size(1), F = wd.size(2);
+  TORCH_CHECK_VALUE(first.size(0) == E && first.size(1) == (pair ? F : 2 * F) && first.size(2) == D && x.size(1) == D &&
+                        logits.size(0) == x.size(0) && logits.size(1) == E, "expert_mlp: x ", x.sizes(), ", logits ", logits.sizes(),
+                    ", w_gate_up ", first.sizes(), ", w_down ", wd.sizes(), " do not fit");
+  TORCH_CHECK_VALUE(D % 8 == 0 && F % 8 == 0 && D > 0 && F > 0, "expert_mlp: widths in multiples of 8 expected, got D ", D, " and F ", F);
+  TORCH_CHECK_VALUE(x.device() == logits.device() && x.device() == first.device() && x.device() == wd.device(),
+                    "expert_mlp: tensors on several GPUs");
+  c10::cuda::CUDAGuard guard(x.device());
+  const bool keep = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() || (pair && second->requires_grad()));
+  if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, bits, poison);
+  Mlp m = mlp_fwd(x, logits, stack_of(first, second), matrices(wd), k, capacity, bits, false, Outputs{poison});
+  return {m.out, m.r.aux};
 }
 
 }  // namespace
 
 void register_moe(pybind11::module_& m) {
-  namespace py = pybind11;
-  m.def("moe_route", [](const Tensor& logits, int64_t k, int64_t capacity, const py::object& track) {
-    c10::cuda::CUDAGuard guard(logits.device());
-    Routed r = do_route(logits, k, capacity, Outputs{track});
-    return std::make_tuple(r.weights, r.aux, r.experts, r.slots, r.offsets, r.rows, r.counts);
-  });
-  m.def("moe_route_bwd", [](const Tensor& logits, const Tensor& weights, const Tensor& experts, const Tensor& counts,
-                            const OptTensor& dweights, const OptTensor& daux, const py::object& track) {
-    c10::cuda::CUDAGuard guard(logits.device());
-    return do_route_bwd(logits, weights, experts, counts, dweights, daux, Outputs{track});
-  });
-  m.def("moe_gather", [](const Tensor& x, const Tensor& rows, int64_t k, const py::object& track) {
-    c10::cuda::CUDAGuard guard(x.device());
-    return do_gather(x, rows, k, Outputs{track});
-  });
-  m.def("moe_combine", [](const Tensor& y, const OptTensor& weights, const Tensor& slots, bool f32, const py::object& track) {
-    c10::cuda::CUDAGuard guard(y.device());
-    return do_combine(y, weights, slots, f32 ? torch::kFloat32 : torch::kBFloat16, Outputs{track});
-  });
-  m.def("moe_combine_bwd", &combine_bwd);
-  m.def("grouped_gemm", [](const Tensor& x, const Tensor& w, const Tensor& offsets, bool w_t, const py::object& track) {
-    c10::cuda::CUDAGuard guard(x.device());
-    return do_grouped(x, w, offsets, w_t, Outputs{track});
-  });
-  m.def("grouped_wgrad", [](const Tensor& dy, const Tensor& x, const Tensor& offsets, bool f32, const py::object& track) {
-    c10::cuda::CUDAGuard guard(x.device());
-    return do_wgrad(dy, x, offsets, f32 ? torch::kFloat32 : torch::kBFloat16, Outputs{track});
-  });
+  m.def("moe_route", &moe_route, "(weights, aux, experts, slots, offsets, rows, counts)");
+  m.def("moe_dispatch", &moe_dispatch);
+  m.def("moe_combine", &moe_combine);
+  m.def("grouped_linear", &grouped_linear);
+  m.def("expert_mlp", &expert_mlp, "(out, aux)");
   m.def("quantize8", [](const Tensor& x) {
+    check_rows(x, "quantize8");
     c10::cuda::CUDAGuard guard(x.device());
     return do_quantize(x);
   });
-  m.def("dequantize8", [](const Tensor& q, const Tensor& s, const py::object& track) {
+  m.def("dequantize8", [](const Tensor& q, const Tensor& s, bool poison) {
+    TORCH_CHECK_VALUE(q.is_cuda(), "dequantize8: a tensor on the GPU expected");
     c10::cuda::CUDAGuard guard(q.device());
-    return do_dequantize(q, s, Outputs{track});
+    return do_dequantize(q, s, Outputs{poison});
   });
-  m.def("swiglu8_fwd", [](const Tensor& gu, const py::object& track) {
-    c10::cuda::CUDAGuard guard(gu.device());
-    return do_swiglu8(gu, Outputs{track});
-  });
-  m.def("swiglu8_bwd", [](const Tensor& dact, const Tensor& q, const Tensor& s, const py::object& track) {
-    c10::cuda::CUDAGuard guard(dact.device());
-    return do_swiglu8_bwd(dact, q, s, Outputs{track});
-  });
-  m.def("expert_mlp_fwd", &expert_mlp_fwd);
-  m.def("expert_mlp_bwd", &expert_mlp_bwd);
+  m.def("swiglu_8bit", &swiglu_8bit);
+  m.def("moe_launches", [](bool reset) { return reset ? g_launches.exchange(0) : g_launches.load(); },
+        "kernels launched by the operators of this file since the last reset");
 }

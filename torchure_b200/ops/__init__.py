@@ -36,6 +36,7 @@ def ext():
 
 
 _FORCED_OFF = False
+_FOUND = False      # the extension and a GPU that runs it were there once; they stay
 
 
 def force_fallback(flag: bool = True) -> None:
@@ -45,15 +46,15 @@ def force_fallback(flag: bool = True) -> None:
 
 
 def available() -> bool:
-    if _FORCED_OFF or not torch.cuda.is_available():
+    global _FOUND
+    if _FORCED_OFF:
         return False
-    if ext() is None:
-        return False
-    major, _ = torch.cuda.get_device_capability()
-    return major == 10
+    if not _FOUND:
+        _FOUND = torch.cuda.is_available() and ext() is not None and torch.cuda.get_device_capability()[0] == 10
+    return _FOUND
 
 
-# launch counter: every Python wrapper that launches one of OUR kernels adds to it
+# launch counter: every Python wrapper that launches one of OUR kernels adds to it; the mixture-of-experts operators count in C++
 _LAUNCHES = 0
 
 
@@ -63,12 +64,14 @@ def count_launch(n: int = 1) -> None:
 
 
 def launches() -> int:
-    return _LAUNCHES
+    return _LAUNCHES + (_EXT.moe_launches(False) if _EXT is not None else 0)
 
 
 def reset_launches() -> None:
     global _LAUNCHES
     _LAUNCHES = 0
+    if _EXT is not None:
+        _EXT.moe_launches(True)
 
 
 def set_compute_sm_reserve(n: int) -> None:

@@ -46,9 +46,7 @@ def quantize8(x: torch.Tensor) -> Act8:
     x = _rows(x.detach(), "quantize8")
     if not ops.available() or not x.is_cuda:
         return Act8(*oracle.quantize8(x))
-    out = Act8(*_C().quantize8(x))
-    ops.count_launch()
-    return out
+    return Act8(*_C().quantize8(x))
 
 
 def dequantize8(kept: Act8) -> torch.Tensor:
@@ -56,36 +54,15 @@ def dequantize8(kept: Act8) -> torch.Tensor:
     values, scales = kept
     if not ops.available() or not values.is_cuda:
         return oracle.dequantize8(values, scales).bfloat16()
-    x = _C().dequantize8(values, scales, debug.tracker())
-    ops.count_launch()
-    return x
-
-
-class _Swiglu8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gu):
-        act, values, scales = _C().swiglu8_fwd(gu, debug.tracker())
-        ops.count_launch()
-        ctx.save_for_backward(values, scales)
-        return act
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dact):
-        values, scales = ctx.saved_tensors
-        dgu = _C().swiglu8_bwd(_rows(dact, "swiglu_8bit backward"), values, scales, debug.tracker())
-        ops.count_launch()
-        return dgu
+    return _C().dequantize8(values, scales, debug.enabled())
 
 
 def swiglu_8bit(gu: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of ``gu`` [..., 2F] = gate | up (bf16), [..., F].  Until the backward pass ``gu`` is kept in 8 bits, gate and
     up in blocks of their own; the gradient is the formula's at the values read back."""
+    if ops.available() and gu.is_cuda:
+        return _C().swiglu_8bit(gu, debug.enabled())
     if gu.dim() < 1 or gu.shape[-1] % 2:
         raise ValueError(f"swiglu_8bit: gate and up columns expected, got {tuple(gu.shape)}")
-    flat = _rows(gu, "swiglu_8bit")
-    if not ops.available() or not gu.is_cuda:
-        act = oracle.swiglu_8bit(flat).to(gu.dtype)
-    else:
-        act = _Swiglu8.apply(flat)
+    act = oracle.swiglu_8bit(_rows(gu, "swiglu_8bit")).to(gu.dtype)
     return act.view(*gu.shape[:-1], gu.shape[-1] // 2)
