@@ -6,10 +6,16 @@
 //
 // x has 8 significant bits, so 127 |x| / a is either exactly half-way between two whole numbers or at least 2^-17 (relative) away
 // from it.  The product with 127 / a, raised by 2^-20, therefore rounds to the nearest whole number as the quotient does, and
-// half-way cases away from zero, without a division per value.
+// half-way cases away from zero, without a division per value; 127 / a itself may be off by 2^-21.
 //
-// Bound by memory.  Eight lanes have a block, eight values each (16 bytes of bf16, 8 bytes of int8); widths that are no multiple of
-// 8, or rows off a 16-byte boundary, are read value by value.
+// The arithmetic has to stay below the memory's time: the largest magnitude is found on packed bf16 pairs, whole numbers are taken
+// from the low byte of x (127 / a) + 1.5 2^23 and put together by byte permutations, and read back the other way (conversion
+// instructions run at a quarter of the rate).
+//
+// Bound by memory.  Eight lanes have a block, eight values each (16 bytes of bf16, 8 bytes of int8), four blocks at a time (SwiGLU:
+// two of gate and two of up) so that as many loads are on their way; with one block at a time 16384 x 2560 took 43 us to quantise and
+// 32 to read back, and SwiGLU of 16384 x 1536 54 and 42.  Widths that are no multiple of 8, or rows off a 16-byte boundary, are read
+// value by value.
 #include "common.cuh"
 #include "moe_api.h"
 
@@ -26,22 +32,26 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// 8 bf16 values as they lie, `left` of them inside the row, zeros behind
 template <bool VEC>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, float (&v)[8]) {
-  if (VEC) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (left > 0) u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ uint4 load_raw(const __nv_bfloat16* p, int left) {
+  if (VEC) return left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
+  for (int i = 0; i < 8; ++i)
+    if (i < left) u[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ void spread(uint4 raw, float (&v)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? __bfloat162float(p[i]) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+template <bool VEC>
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, float (&v)[8]) { spread(load_raw<VEC>(p, left), v); }
 template <bool VEC>
 __device__ __forceinline__ void store8(__nv_bfloat16* p, int left, const float (&v)[8]) {
   if (VEC) {
@@ -54,123 +64,167 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, int left, const float (
       if (i < left) p[i] = __float2bfloat16(v[i]);
   }
 }
+// 8 kept values as they lie
 template <bool VEC>
-__device__ __forceinline__ void load_q(const int8_t* p, int left, float scale, float (&v)[8]) {
-  if (VEC) {
-    int2 u = make_int2(0, 0);
-    if (left > 0) u = *reinterpret_cast<const int2*>(p);
+__device__ __forceinline__ uint2 load_q(const int8_t* p, int left) {
+  if (VEC) return left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+  uint32_t u[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = static_cast<float>(static_cast<int8_t>(u.x >> (8 * i))) * scale;
-      v[4 + i] = static_cast<float>(static_cast<int8_t>(u.y >> (8 * i))) * scale;
-    }
-  } else {
+  for (int i = 0; i < 8; ++i)
+    if (i < left) u[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[i])) << (8 * (i & 3));
+  return make_uint2(u[0], u[1]);
+}
+// what they stand for: byte b ^ 128 under the exponent of 2^23 is 2^23 + 128 + b
+__device__ __forceinline__ void read_q(uint2 raw, float scale, float (&v)[8]) {
+  const uint32_t w[2] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? static_cast<float>(p[i]) * scale : 0.f;
+  for (int i = 0; i < 2; ++i) {
+    v[4 * i] = (__uint_as_float(__byte_perm(w[i], 0x4b000000u, 0x7650)) - 8388736.f) * scale;
+    v[4 * i + 1] = (__uint_as_float(__byte_perm(w[i], 0x4b000000u, 0x7651)) - 8388736.f) * scale;
+    v[4 * i + 2] = (__uint_as_float(__byte_perm(w[i], 0x4b000000u, 0x7652)) - 8388736.f) * scale;
+    v[4 * i + 3] = (__uint_as_float(__byte_perm(w[i], 0x4b000000u, 0x7653)) - 8388736.f) * scale;
   }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {      // of bf16 pairs, NaN where either is
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
 // The block of this thread's group of eight lanes: 8 values each, `left` of them inside the row.
 template <bool VEC>
-__device__ __forceinline__ void keep8(const float (&v)[8], int left, int8_t* q, float* scale, bool first) {
-  float a = 0.f;
+__device__ __forceinline__ void keep8(uint4 raw, int left, int8_t* q, float* scale, bool first) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  uint32_t top = max2_nan(max2_nan(raw.x & kAbs, raw.y & kAbs), max2_nan(raw.z & kAbs, raw.w & kAbs));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+  for (int o = 4; o > 0; o >>= 1) top = max2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = max2_nan(top, top >> 16);
+  const float a = __uint_as_float(top << 16);
   const bool finite = a <= 3.4028235e38f;
   // 127 / a is no float for the smallest a: such blocks count as zeros, off by less than 2^-120
   const bool some = finite && a >= 7.52316385e-37f;
-  const float inv = some ? __fdiv_rn(127.f, a) * 1.00000095367431640625f : 0.f;
-  if (first) *scale = finite ? (some ? __fdiv_rn(a, 127.f) : 0.f) : __uint_as_float(0x7fffffffu);
-  int w[8];
+  // a / 127: the product with the rounded reciprocal, and what it leaves given back (Markstein's correction)
+  constexpr float kPart = 1.f / 127.f;
+  const float near = a * kPart;
+  if (first) *scale = finite ? (some ? fmaf(fmaf(-127.f, near, a), kPart, near) : 0.f) : __uint_as_float(0x7fffffffu);
+  // (the fast division is good for divisors up to 2^126: both sides a quarter)
+  const float inv = some ? __fdividef(31.75f, 0.25f * a) * 1.00000095367431640625f : 0.f;
+  float v[8];
+  spread(raw, v);
+  uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = some ? __float2int_rn(v[i] * inv) : 0;
+  for (int i = 0; i < 8; ++i) w[i] = some ? __float_as_uint(fmaf(v[i], inv, 12582912.f)) : 0u;      // + 1.5 2^23: whole numbers in the low byte
+  const uint2 u = make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                             __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
   if (VEC) {
-    if (left > 0) {
-      int2 u = make_int2(0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u.x |= (w[i] & 0xff) << (8 * i);
-        u.y |= (w[4 + i] & 0xff) << (8 * i);
-      }
-      *reinterpret_cast<int2*>(q) = u;
-    }
+    if (left > 0) *reinterpret_cast<uint2*>(q) = u;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < left) q[i] = static_cast<int8_t>(w[i]);
+      if (i < left) q[i] = static_cast<int8_t>((i < 4 ? u.x : u.y) >> (8 * (i & 3)));
   }
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
-// units: blocks of a matrix; a block is worked on by eight lanes
-template <bool VEC>
-__global__ void __launch_bounds__(kThreads)
-quantize8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, float* __restrict__ scales, int64_t M, int N,
-                 int nb) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int g = threadIdx.x & 7;
-  const int64_t units = M * nb, step = static_cast<int64_t>(gridDim.x) * (kThreads / 8);
-  for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kThreads / 8) + (threadIdx.x >> 5) * 4; u0 < units; u0 += step) {
-    const int64_t u = u0 + ((threadIdx.x & 31) >> 3);      // whole warps stay: the lanes of a block shuffle
+constexpr int kGroups = kThreads / 8;      // blocks that a CTA works on at once
+
+// A unit is a block of 64 columns of one row; a CTA takes UNROLL x kGroups neighbours at a time, each thread group every kGroups-th.
+// Where a unit lies: row, first column of this lane, columns from there to the end of the row (0 or less: nothing).
+struct Unit {
+  int64_t row;
+  int b, c, left;
+  __device__ __forceinline__ Unit(uint32_t u, uint32_t units, const FastDiv& per_row, int width) {
     const bool in = u < units;
-    const int64_t row = in ? u / nb : 0;
-    const int b = in ? static_cast<int>(u - row * nb) : 0, c = b * kActBlock + g * 8;
-    const int left = in ? N - c : 0;
-    float v[8];
-    load8<VEC>(x + row * ldx + c, left, v);
-    keep8<VEC>(v, left, q + row * N + c, scales + row * nb + b, in && g == 0);
+    const uint32_t r = in ? per_row(u) : 0u;
+    row = r;
+    b = in ? static_cast<int>(u - r * per_row.d) : 0;
+    c = b * kActBlock + (threadIdx.x & 7) * 8;
+    left = in ? width - c : 0;
   }
-}
+};
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads)
-dequantize8_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x, int64_t M, int N,
-                   int nb) {
+__global__ void __launch_bounds__(kThreads, 6)
+quantize8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t units, int N,
+                 FastDiv nb) {
   pdl_wait();
   pdl_launch_dependents();
-  const int g = threadIdx.x & 7;
-  const int64_t units = M * nb, step = static_cast<int64_t>(gridDim.x) * (kThreads / 8);
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kThreads / 8) + (threadIdx.x >> 3); u < units; u += step) {
-    const int64_t row = u / nb;
-    const int b = static_cast<int>(u - row * nb), c = b * kActBlock + g * 8;
-    float v[8];
-    load_q<VEC>(q + row * N + c, N - c, scales[u], v);
-    store8<VEC>(x + row * N + c, N - c, v);
-  }
-}
-
-template <bool VEC>
-__global__ void __launch_bounds__(kThreads)
-swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
-                   float* __restrict__ scales, int64_t M, int F, int nb) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lg = threadIdx.x & 7;
-  const int64_t units = M * nb, step = static_cast<int64_t>(gridDim.x) * (kThreads / 8);
-  for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kThreads / 8) + (threadIdx.x >> 5) * 4; u0 < units; u0 += step) {
-    const int64_t u = u0 + ((threadIdx.x & 31) >> 3);
-    const bool in = u < units;
-    const int64_t row = in ? u / nb : 0;
-    const int b = in ? static_cast<int>(u - row * nb) : 0, c = b * kActBlock + lg * 8;
-    const int left = in ? F - c : 0;
-    float gate[8], up[8], out[8];
-    load8<VEC>(gu + row * ldgu + c, left, gate);
-    load8<VEC>(gu + row * ldgu + F + c, left, up);
+  constexpr int U = 4;
+  for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 - (threadIdx.x >> 3) < units; u0 += gridDim.x * (U * kGroups)) {
+    uint4 v[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = gate[i] * sigmoid(gate[i]) * up[i];
-    store8<VEC>(act + row * F + c, left, out);
-    keep8<VEC>(gate, left, q + row * 2 * F + c, scales + row * 2 * nb + b, in && lg == 0);
-    keep8<VEC>(up, left, q + row * 2 * F + F + c, scales + row * 2 * nb + nb + b, in && lg == 0);
+    for (int i = 0; i < U; ++i) {
+      const Unit at(u0 + i * kGroups, units, nb, N);
+      v[i] = load_raw<VEC>(x + at.row * ldx + at.c, at.left);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t u = u0 + i * kGroups;
+      const Unit at(u, units, nb, N);
+      keep8<VEC>(v[i], at.left, q + at.row * N + at.c, scales + u, u < units && (threadIdx.x & 7) == 0);
+    }
+  }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads)
+dequantize8_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x, uint32_t units, int N,
+                   FastDiv nb) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int U = 4;
+  for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 < units; u0 += gridDim.x * (U * kGroups)) {
+    uint2 raw[U];
+    float scale[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t u = u0 + i * kGroups;
+      const Unit at(u, units, nb, N);
+      raw[i] = load_q<VEC>(q + at.row * N + at.c, at.left);
+      scale[i] = u < units ? scales[u] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const Unit at(u0 + i * kGroups, units, nb, N);
+      float v[8];
+      read_q(raw[i], scale[i], v);
+      store8<VEC>(x + at.row * N + at.c, at.left, v);
+    }
+  }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads, 5)
+swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
+                   float* __restrict__ scales, uint32_t units, int F, FastDiv nb) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int U = 2;
+  for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 - (threadIdx.x >> 3) < units; u0 += gridDim.x * (U * kGroups)) {
+    uint4 gate[U], up[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const Unit at(u0 + i * kGroups, units, nb, F);
+      gate[i] = load_raw<VEC>(gu + at.row * ldgu + at.c, at.left);
+      up[i] = load_raw<VEC>(gu + at.row * ldgu + F + at.c, at.left);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t u = u0 + i * kGroups;
+      const Unit at(u, units, nb, F);
+      float g[8], v[8], out[8];
+      spread(gate[i], g);
+      spread(up[i], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] = g[j] * sigmoid(g[j]) * v[j];
+      store8<VEC>(act + at.row * F + at.c, at.left, out);
+      const bool first = u < units && (threadIdx.x & 7) == 0;
+      float* scale = scales + at.row * 2 * static_cast<int>(nb.d) + at.b;
+      keep8<VEC>(gate[i], at.left, q + at.row * 2 * F + at.c, scale, first);
+      keep8<VEC>(up[i], at.left, q + at.row * 2 * F + F + at.c, scale + nb.d, first);
+    }
   }
 }
 
@@ -185,23 +239,38 @@ __device__ __forceinline__ void swiglu_grad(const float (&g)[8], const float (&u
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 swiglu8_bwd_kernel(const __nv_bfloat16* __restrict__ dact, int64_t ldd, const int8_t* __restrict__ q, const float* __restrict__ scales,
-                   __nv_bfloat16* __restrict__ dgu, int64_t M, int F, int nb) {
+                   __nv_bfloat16* __restrict__ dgu, uint32_t units, int F, FastDiv nb) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lg = threadIdx.x & 7;
-  const int64_t units = M * nb, step = static_cast<int64_t>(gridDim.x) * (kThreads / 8);
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kThreads / 8) + (threadIdx.x >> 3); u < units; u += step) {
-    const int64_t row = u / nb;
-    const int b = static_cast<int>(u - row * nb), c = b * kActBlock + lg * 8, left = F - c;
-    float gate[8], up[8], d[8], dg[8], du[8];
-    load_q<VEC>(q + row * 2 * F + c, left, scales[row * 2 * nb + b], gate);
-    load_q<VEC>(q + row * 2 * F + F + c, left, scales[row * 2 * nb + nb + b], up);
-    load8<VEC>(dact + row * ldd + c, left, d);
-    swiglu_grad(gate, up, d, dg, du);
-    store8<VEC>(dgu + row * 2 * F + c, left, dg);
-    store8<VEC>(dgu + row * 2 * F + F + c, left, du);
+  constexpr int U = 2;
+  for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 < units; u0 += gridDim.x * (U * kGroups)) {
+    uint2 gate[U], up[U];
+    uint4 d[U];
+    float sg[U], su[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const Unit at(u0 + i * kGroups, units, nb, F);
+      const float* scale = scales + at.row * 2 * static_cast<int>(nb.d) + at.b;
+      const bool in = u0 + i * kGroups < units;
+      gate[i] = load_q<VEC>(q + at.row * 2 * F + at.c, at.left);
+      up[i] = load_q<VEC>(q + at.row * 2 * F + F + at.c, at.left);
+      sg[i] = in ? scale[0] : 0.f;
+      su[i] = in ? scale[nb.d] : 0.f;
+      d[i] = load_raw<VEC>(dact + at.row * ldd + at.c, at.left);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const Unit at(u0 + i * kGroups, units, nb, F);
+      float g[8], u[8], da[8], dg[8], du[8];
+      read_q(gate[i], sg[i], g);
+      read_q(up[i], su[i], u);
+      spread(d[i], da);
+      swiglu_grad(g, u, da, dg, du);
+      store8<VEC>(dgu + at.row * 2 * F + at.c, at.left, dg);
+      store8<VEC>(dgu + at.row * 2 * F + F + at.c, at.left, du);
+    }
   }
 }
 
@@ -222,12 +291,13 @@ expert_swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ s, const __nv_bfloat1
     if (r >= 0 && r < R) {
       const float w = weights[i];
       const int64_t row = r;
+#pragma unroll 2
       for (int c = lane * 8; c < F; c += 256) {
         const int left = F - c;
         float gate[8], up[8], d[8], dg[8], du[8], a[8];
         if (Q8) {
-          load_q<VEC>(q + row * 2 * F + c, left, scales[row * 2 * nb + c / kActBlock], gate);
-          load_q<VEC>(q + row * 2 * F + F + c, left, scales[row * 2 * nb + nb + c / kActBlock], up);
+          read_q(load_q<VEC>(q + row * 2 * F + c, left), scales[row * 2 * nb + c / kActBlock], gate);
+          read_q(load_q<VEC>(q + row * 2 * F + F + c, left), scales[row * 2 * nb + nb + c / kActBlock], up);
         } else {
           load8<VEC>(gu + row * 2 * F + c, left, gate);
           load8<VEC>(gu + row * 2 * F + F + c, left, up);
@@ -271,37 +341,41 @@ bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 void quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, int64_t M, int N, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return;
   const int nb = blocks_of(N);
-  const dim3 grid(grid_for(M * nb, kThreads / 8)), block(kThreads);
-  if (N % 8 == 0 && ldx % 8 == 0 && at16(x) && at16(q)) launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, M, N, nb);
-  else launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, M, N, nb);
+  const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
+  const uint32_t units = static_cast<uint32_t>(M * nb);
+  if (N % 8 == 0 && ldx % 8 == 0 && at16(x) && at16(q)) launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+  else launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
 }
 
 void dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return;
   const int nb = blocks_of(N);
-  const dim3 grid(grid_for(M * nb, kThreads / 8)), block(kThreads);
-  if (N % 8 == 0 && at16(x) && at16(q)) launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, M, N, nb);
-  else launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, M, N, nb);
+  const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
+  const uint32_t units = static_cast<uint32_t>(M * nb);
+  if (N % 8 == 0 && at16(x) && at16(q)) launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+  else launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
 }
 
 void swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
                  cudaStream_t stream) {
   if (M <= 0 || F <= 0) return;
   const int nb = blocks_of(F);
-  const dim3 grid(grid_for(M * nb, kThreads / 8)), block(kThreads);
+  const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
+  const uint32_t units = static_cast<uint32_t>(M * nb);
   if (F % 8 == 0 && ldgu % 8 == 0 && at16(gu) && at16(act) && at16(q))
-    launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, M, F, nb);
-  else launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, M, F, nb);
+    launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+  else launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
 }
 
 void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M, int F,
                  cudaStream_t stream) {
   if (M <= 0 || F <= 0) return;
   const int nb = blocks_of(F);
-  const dim3 grid(grid_for(M * nb, kThreads / 8)), block(kThreads);
+  const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
+  const uint32_t units = static_cast<uint32_t>(M * nb);
   if (F % 8 == 0 && ldd % 8 == 0 && at16(dact) && at16(dgu) && at16(q))
-    launch_pdl(swiglu8_bwd_kernel<true>, grid, block, 0, stream, dact, ldd, q, scales, dgu, M, F, nb);
-  else launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, M, F, nb);
+    launch_pdl(swiglu8_bwd_kernel<true>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
+  else launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
 }
 
 void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,

@@ -343,6 +343,16 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int m, int n, bool a_mn_m
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// n / d for n < 2^31 (multiplication by a rounded reciprocal of 33 bits)
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {
+    while ((1ull << shift) < divisor) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - divisor)) / divisor + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

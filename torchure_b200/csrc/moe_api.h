@@ -19,8 +19,8 @@ constexpr int kActBlock = 64;      // values of a row that share a scale in an 8
 // Choices of one row of logits: the k largest, ties to the lowest index; a choice whose logit is -inf is not made.
 // weights [T, k], experts [T, k], slots [T, k] (row of the choice, -1: not made or beyond the capacity), offsets [E + 1],
 // rows [T k] (t k + j of each row, -1 behind offsets[E]), counts [E] (choices made, before the capacity), aux [1].
-// scratch: route_scratch_ints(T, E) 32-bit words.  capacity 0: no limit.
-int64_t route_scratch_ints(int T, int E);
+// scratch: route_scratch_ints(T, E, k) 32-bit words.  capacity 0: no limit.
+int64_t route_scratch_ints(int T, int E, int k);
 int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts, int* slots,
               int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream);
 // dlogits [T, E] (the logits' type) from dweights [T, k] (nullptr: none) and daux [1] (nullptr: none)

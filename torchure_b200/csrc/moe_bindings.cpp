@@ -83,7 +83,7 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
     return r;
   }
   // offsets, counts and scratch of one allocation
-  const int64_t scratch = tb::route_scratch_ints((int)T, (int)E);
+  const int64_t scratch = tb::route_scratch_ints((int)T, (int)E, (int)k);
   Tensor ints = torch::empty({2 * E + 1 + scratch}, i32);
   r.offsets = ints.narrow(0, 0, E + 1);
   r.counts = ints.narrow(0, E + 1, E);
@@ -136,6 +136,7 @@ Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots
   TORCH_CHECK(!has(weights) || (weights->scalar_type() == torch::kFloat32 && weights->is_contiguous() && weights->numel() == T * k &&
                                 weights->device() == y.device()), "combine: weights must be contiguous fp32 [tokens, choices]");
   TORCH_CHECK(type == torch::kBFloat16 || type == torch::kFloat32, "combine: bf16 or fp32 output");
+  TORCH_CHECK_VALUE(T * ((D + 7) / 8) < (1ll << 31), "combine: 2^34 values and more are not supported");
   Tensor out = make("combine", {T, D}, y.options().dtype(type));
   tb::rows_combine(bf(y), has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
                    type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream());
@@ -204,10 +205,15 @@ Tensor do_wgrad(const Tensor& dy, const Tensor& x, const Tensor& offsets, at::Sc
   return dw;
 }
 
+void check_blocks(int64_t rows, int64_t cols, const char* what) {
+  TORCH_CHECK_VALUE(rows * blocks_of(cols) < (1ll << 31), what, ": 2^31 blocks of ", tb::kActBlock, " values and more are not supported");
+}
+
 std::tuple<Tensor, Tensor> do_quantize(const Tensor& x) {
   check_rows(x, "quantize8");
   check_bf16(x, "quantize8");
   const int64_t M = x.size(0), N = x.size(1);
+  check_blocks(M, N, "quantize8");
   Tensor q = torch::empty({M, N}, x.options().dtype(torch::kInt8));
   Tensor s = torch::empty({M, blocks_of(N)}, x.options().dtype(torch::kFloat32));
   tb::quantize8(bf(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)N, cur_stream());
@@ -224,6 +230,7 @@ void check_kept(const Tensor& q, const Tensor& s, int64_t blocks, const char* wh
 
 Tensor do_dequantize(const Tensor& q, const Tensor& s, const Outputs& make) {
   check_kept(q, s, q.dim() == 2 ? blocks_of(q.size(1)) : 0, "dequantize8");
+  check_blocks(q.size(0), q.size(1), "dequantize8");
   Tensor x = make("dequantize8", q.sizes(), q.options().dtype(torch::kBFloat16));
   tb::dequantize8(q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(x), q.size(0), (int)q.size(1), cur_stream());
   g_launches += 1;
@@ -236,6 +243,7 @@ std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, const Outputs& m
   check_bf16(gu, "swiglu_8bit");
   TORCH_CHECK(gu.size(1) % 2 == 0, "swiglu_8bit: gate and up columns expected, got an odd number: ", gu.size(1));
   const int64_t M = gu.size(0), F = gu.size(1) / 2;
+  check_blocks(M, F, "swiglu_8bit");
   Tensor act = make("swiglu_8bit", {M, F}, gu.options());
   Tensor q = torch::empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
   Tensor s = torch::empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));

@@ -18,7 +18,8 @@ namespace tb {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 1024;      // of the forward kernels: one CTA per SM, and its latencies have 32 warps to hide behind
+constexpr int kBwdThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxChunks = 148;
 
@@ -59,23 +60,39 @@ struct RouteArgs {
   float* psum;             // [chunks][E]
 };
 
-// Numbers the choices of CTA `c` of `chunks`.  slots holds the expert of each choice (-1: not made) and receives its row.
-__device__ void plan_rows(const RouteArgs& a, int c, int chunks, int* sm) {
+// Numbers the choices of CTA `c` of `chunks`.  codes: the expert of each of its choices (-1: not made), from its first on.
+__device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_hist, const float* all_psum, int c, int chunks, int* sm) {
   const int E = a.E, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* total = sm;                 // [E]
-  int* before = sm + E;            // [E] in earlier CTAs; later the place of the next choice of this CTA's first warp
+  int* before = sm + E;            // [E] in earlier CTAs
   int* first = sm + 2 * E;         // [E + 1] first row of each expert
   int* cnt = sm + 3 * E + 1;       // [kWarps][E]
   float* aux_part = reinterpret_cast<float*>(cnt + kWarps * E);      // [kWarps]
   for (int i = tid; i < 2 * E; i += kThreads) sm[i] = 0;
   for (int i = tid; i < kWarps * E; i += kThreads) cnt[i] = 0;
   __syncthreads();
-  for (int i = tid; i < chunks * E; i += kThreads) {
-    const int e = i % E, v = a.hist[i];
-    if (v) {
-      atomicAdd(&total[e], v);
-      if (i / E < c) atomicAdd(&before[e], v);
+  // this CTA's choices, a consecutive part for each warp: counted here, ranked below
+  const int n_flat = a.T * a.k;
+  const int lo = c * a.chunk * a.k, count = min(n_flat - lo, a.chunk * a.k);
+  const int part = ((count + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int wlo = min(count, warp * part), whi = min(count, wlo + part);
+  for (int i = wlo + lane; i < whi; i += 32) {
+    const int e = codes[i];
+    if (e >= 0) atomicAdd(&cnt[warp * E + e], 1);
+  }
+  // the counts of all CTAs: a thread has one expert and every `rows`-th CTA, its loads independent
+  const int rows = max(1, kThreads / E);
+  if (tid < rows * E) {
+    const int e = tid % E;
+    int all = 0, mine = 0;
+#pragma unroll 8
+    for (int i = tid / E; i < chunks; i += rows) {
+      const int v = all_hist[i * E + e];
+      all += v;
+      mine += i < c ? v : 0;
     }
+    if (all) atomicAdd(&total[e], all);
+    if (mine) atomicAdd(&before[e], mine);
   }
   __syncthreads();
   if (warp == 0) {                 // exclusive prefix sums of the kept counts
@@ -94,35 +111,9 @@ __device__ void plan_rows(const RouteArgs& a, int c, int chunks, int* sm) {
     }
     if (lane == 0) first[E] = run;
   }
-  __syncthreads();
-  const int n_flat = a.T * a.k;
-  if (c == 0) {
-    for (int e = tid; e <= E; e += kThreads) {
-      a.offsets[e] = first[e];
-      if (e < E) a.counts[e] = total[e];
-    }
-    float s = 0.f;
-    for (int i = tid; i < chunks * E; i += kThreads) s += static_cast<float>(total[i % E]) * a.psum[i];
-    s = group_sum<32>(s, 0xffffffffu);
-    if (lane == 0) aux_part[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < kWarps; ++i) s += aux_part[i];
-      a.aux[0] = s * (static_cast<float>(E) / static_cast<float>(n_flat)) / static_cast<float>(a.T);
-    }
-  }
-  // this CTA's choices, a consecutive part for each warp: counted, then ranked
-  const int lo = c * a.chunk * a.k, hi = min(n_flat, lo + a.chunk * a.k);
-  const int part = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int wlo = min(hi, lo + warp * part), whi = min(hi, wlo + part);
-  for (int i = wlo + lane; i < whi; i += 32) {
-    const int e = a.slots[i];
-    if (e >= 0) atomicAdd(&cnt[warp * E + e], 1);
-  }
-  __syncthreads();
-  for (int e = tid; e < E; e += kThreads) {
+  for (int e = kThreads - 1 - tid; e < E; e += kThreads) {      // (from the last warp on: the first one is busy)
     int run = before[e];
-#pragma unroll
+#pragma unroll 8
     for (int w = 0; w < kWarps; ++w) {
       const int n = cnt[w * E + e];
       cnt[w * E + e] = run;
@@ -132,7 +123,7 @@ __device__ void plan_rows(const RouteArgs& a, int c, int chunks, int* sm) {
   __syncthreads();
   for (int i0 = wlo; i0 < whi; i0 += 32) {
     const int i = i0 + lane;
-    const int e = i < whi ? a.slots[i] : -1;
+    const int e = i < whi ? codes[i] : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     const int rank = __popc(same & ((1u << lane) - 1u));
     int place = 0;
@@ -144,12 +135,28 @@ __device__ void plan_rows(const RouteArgs& a, int c, int chunks, int* sm) {
       int row = -1;
       if (e >= 0 && place < first[e + 1] - first[e]) {
         row = first[e] + place;
-        a.rows[row] = i;
+        a.rows[row] = lo + i;
       }
-      a.slots[i] = row;
+      a.slots[lo + i] = row;
     }
   }
   for (int r = first[E] + c * kThreads + tid; r < n_flat; r += chunks * kThreads) a.rows[r] = -1;
+  if (c == chunks - 1) {
+    for (int e = tid; e <= E; e += kThreads) {
+      a.offsets[e] = first[e];
+      if (e < E) a.counts[e] = total[e];
+    }
+    float s = 0.f;
+#pragma unroll 4
+    for (int i = tid; i < chunks * E; i += kThreads) s += static_cast<float>(total[i % E]) * all_psum[i];
+    s = group_sum<32>(s, 0xffffffffu);
+    if (lane == 0) aux_part[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+      s = group_sum<32>(lane < kWarps ? aux_part[lane] : 0.f, 0xffffffffu);
+      if (lane == 0) a.aux[0] = s * (static_cast<float>(E) / static_cast<float>(n_flat)) / static_cast<float>(a.T);
+    }
+  }
 }
 
 constexpr int plan_smem_ints(int E) { return 3 * E + 1 + kWarps * E + kWarps; }
@@ -164,7 +171,10 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
   const int E = a.E, tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1), group = tid / LANES;
   const uint32_t mask = group_mask<LANES>(lane);
   int* hist = sm;                                         // [E]
-  float* part = reinterpret_cast<float*>(sm + E);         // [GROUPS][E]
+  float* psum = reinterpret_cast<float*>(sm + E);         // [E]
+  int* codes = sm + 2 * E;                                // [T k] with one CTA
+  int* rest = codes + (single ? a.T * a.k : 0);
+  float* part = reinterpret_cast<float*>(rest);           // [GROUPS][E]
   for (int e = tid; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
   float acc[VALS];
@@ -184,21 +194,39 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
     uint32_t my_key = 0;
     int my_e = 0;
     float top = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = 0;
+    if constexpr (sizeof(T) == 2) {      // 16 bits of key and, falling, 16 of index: one reduction finds both
 #pragma unroll
-      for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
-      best = __reduce_max_sync(mask, best);
-      int at = 0x7fffffff;
+      for (int v = 0; v < VALS; ++v) key[v] = key[v] ? (key[v] & 0xffff0000u) | (0xffffu - (v * LANES + gl)) : 0u;
+      for (int j = 0; j < a.k; ++j) {
+        uint32_t best = 0;
 #pragma unroll
-      for (int v = VALS - 1; v >= 0; --v)
-        if (key[v] == best) at = v * LANES + gl;
-      at = __reduce_min_sync(mask, at);
+        for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
+        best = __reduce_max_sync(mask, best);
 #pragma unroll
-      for (int v = 0; v < VALS; ++v)
-        if (at == v * LANES + gl) key[v] = 0;
-      if (j == 0) top = from_key(best);
-      if (gl == j) { my_key = best; my_e = at; }
+        for (int v = 0; v < VALS; ++v)
+          if (key[v] == best) key[v] = 0;
+        const uint32_t whole = best | 0xffffu;      // the key of a bf16 value, its low bits as to_key leaves them
+        const uint32_t value = (best >> 31) ? best & 0xffff0000u : whole;
+        if (j == 0) top = from_key(value);
+        if (gl == j) { my_key = value; my_e = 0xffff - static_cast<int>(best & 0xffffu); }
+      }
+    } else {
+      for (int j = 0; j < a.k; ++j) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
+        best = __reduce_max_sync(mask, best);
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int v = VALS - 1; v >= 0; --v)
+          if (key[v] == best) at = v * LANES + gl;
+        at = __reduce_min_sync(mask, at);
+#pragma unroll
+        for (int v = 0; v < VALS; ++v)
+          if (at == v * LANES + gl) key[v] = 0;
+        if (j == 0) top = from_key(best);
+        if (gl == j) { my_key = best; my_e = at; }
+      }
     }
     const bool made = gl < a.k && my_key != kKeyMinusInf;
     const float ex = made ? expf(from_key(my_key) - top) : 0.f;
@@ -207,7 +235,9 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
       const int64_t i = static_cast<int64_t>(t) * a.k + gl;
       a.weights[i] = made ? ex / sum : 0.f;
       a.experts[i] = my_e;
-      a.slots[i] = made ? my_e : -1;
+      const int code = made ? my_e : -1;
+      if (single) codes[i] = code;
+      else a.slots[i] = code;
       if (made) atomicAdd(&hist[my_e], 1);
     }
     if (top != -INFINITY) {
@@ -232,12 +262,16 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
   for (int e = tid; e < E; e += kThreads) {
     float s = 0.f;
     for (int g = 0; g < GROUPS; ++g) s += part[g * E + e];
-    a.psum[static_cast<int64_t>(blockIdx.x) * E + e] = s;
-    a.hist[static_cast<int64_t>(blockIdx.x) * E + e] = hist[e];
+    if (single) {
+      psum[e] = s;
+    } else {
+      a.psum[static_cast<int64_t>(blockIdx.x) * E + e] = s;
+      a.hist[static_cast<int64_t>(blockIdx.x) * E + e] = hist[e];
+    }
   }
   if (single) {
     __syncthreads();
-    plan_rows(a, 0, 1, sm);
+    plan_rows(a, codes, hist, psum, 0, 1, rest);
   }
 }
 
@@ -246,17 +280,17 @@ route_plan_kernel(RouteArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ int sm[];
-  plan_rows(a, blockIdx.x, gridDim.x, sm);
+  plan_rows(a, a.slots + static_cast<int64_t>(blockIdx.x) * a.chunk * a.k, a.hist, a.psum, blockIdx.x, gridDim.x, sm);
 }
 
 template <class T, int LANES, int VALS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kBwdThreads)
 route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ weights, const int* __restrict__ experts,
                  const int* __restrict__ counts, const float* __restrict__ dweights, const float* __restrict__ daux,
                  T* __restrict__ dlogits, int n_tokens, int E, int k) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int GROUPS = kThreads / LANES;
+  constexpr int GROUPS = kBwdThreads / LANES;
   const int tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1);
   const uint32_t mask = group_mask<LANES>(lane);
   const float pull = daux ? *daux * static_cast<float>(E) / static_cast<float>(n_tokens) : 0.f;
@@ -326,9 +360,9 @@ int lanes_for(int E) {
 }
 
 // (chunks, tokens of a chunk)
-void chunks_for(int T, int E, int& chunks, int& chunk) {
+void chunks_for(int T, int E, int k, int& chunks, int& chunk) {
   const int groups = kThreads / lanes_for(E);
-  if (T <= 4 * groups) {       // one CTA, four rounds of tokens
+  if (T <= 4 * groups && T * k <= 4096) {       // one CTA, four rounds of tokens, the choices in shared memory
     chunks = 1;
     chunk = T;
     return;
@@ -349,10 +383,13 @@ int vals_for(int E) {
 template <class T>
 int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t stream) {
   const int lanes = lanes_for(a.E), vals = vals_for(a.E);
-  const int ints = a.E + kThreads / lanes * a.E, plan = plan_smem_ints(a.E);
-  const size_t smem = 4 * static_cast<size_t>(ints > plan ? ints : plan);
+  const int plan = plan_smem_ints(a.E), sums = kThreads / lanes * a.E;
+  const int smem = 4 * (chunks == 1 ? 2 * a.E + a.T * a.k + (sums > plan ? sums : plan) : 2 * a.E + sums);
 #define CASE(L, V)                                                                                                            \
   if (lanes == L && vals == V) {                                                                                              \
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(route_fwd_kernel<T, L, V>), smem) ||                                \
+        !ensure_dynamic_smem(reinterpret_cast<const void*>(route_plan_kernel), 4 * plan))                                      \
+      return -20;                                                                                                             \
     if (launch_pdl(route_fwd_kernel<T, L, V>, dim3(chunks), dim3(kThreads), smem, stream, logits, a, chunks == 1 ? 1 : 0) !=   \
         cudaSuccess)                                                                                                          \
       return -21;                                                                                                             \
@@ -368,9 +405,9 @@ int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t str
 
 }  // namespace
 
-int64_t route_scratch_ints(int T, int E) {
+int64_t route_scratch_ints(int T, int E, int k) {
   int chunks, chunk;
-  chunks_for(T, E, chunks, chunk);
+  chunks_for(T, E, k, chunks, chunk);
   return 2 * static_cast<int64_t>(chunks) * E;
 }
 
@@ -381,7 +418,7 @@ int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, in
   a.ld = ld; a.T = T; a.E = E; a.k = k; a.capacity = capacity;
   a.weights = weights; a.experts = experts; a.slots = slots; a.offsets = offsets; a.rows = rows; a.counts = counts; a.aux = aux;
   int chunks;
-  chunks_for(T, E, chunks, a.chunk);
+  chunks_for(T, E, k, chunks, a.chunk);
   a.hist = scratch;
   a.psum = reinterpret_cast<float*>(scratch + static_cast<int64_t>(chunks) * E);
   return bf16 ? launch_fwd(static_cast<const __nv_bfloat16*>(logits), a, chunks, stream)
@@ -392,16 +429,16 @@ int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, c
               const float* dweights, const float* daux, void* dlogits, int T, int E, int k, cudaStream_t stream) {
   if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices) return -1;
   const int lanes = lanes_for(E), vals = vals_for(E);
-  const int groups = kThreads / lanes;
+  const int groups = kBwdThreads / lanes;
   const int need = (T + groups - 1) / groups;
   const int grid = need < 148 * 8 ? need : 148 * 8;
 #define CASE(L, V)                                                                                                              \
   if (lanes == L && vals == V) {                                                                                                \
     const cudaError_t rc =                                                                                                      \
-        bf16 ? launch_pdl(route_bwd_kernel<__nv_bfloat16, L, V>, dim3(grid), dim3(kThreads), 0, stream,                          \
+        bf16 ? launch_pdl(route_bwd_kernel<__nv_bfloat16, L, V>, dim3(grid), dim3(kBwdThreads), 0, stream,                          \
                           static_cast<const __nv_bfloat16*>(logits), ld, weights, experts, counts, dweights, daux,               \
                           static_cast<__nv_bfloat16*>(dlogits), T, E, k)                                                         \
-             : launch_pdl(route_bwd_kernel<float, L, V>, dim3(grid), dim3(kThreads), 0, stream,                                  \
+             : launch_pdl(route_bwd_kernel<float, L, V>, dim3(grid), dim3(kBwdThreads), 0, stream,                                  \
                           static_cast<const float*>(logits), ld, weights, experts, counts, dweights, daux,                       \
                           static_cast<float*>(dlogits), T, E, k);                                                                \
     return rc == cudaSuccess ? 0 : -21;                                                                                          \
