@@ -16,7 +16,7 @@
 // two of gate and two of up) so that as many loads are on their way; with one block at a time 16384 x 2560 took 43 us to quantise and
 // 32 to read back, and SwiGLU of 16384 x 1536 54 and 42.  Widths that are no multiple of 8, or rows off a 16-byte boundary, are read
 // value by value.
-#include "common.cuh"
+#include "act8.cuh"
 #include "moe_api.h"
 
 namespace tb {
@@ -100,21 +100,13 @@ __device__ __forceinline__ void keep8(uint4 raw, int left, int8_t* q, float* sca
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   top = max2_nan(top, top >> 16);
-  const float a = __uint_as_float(top << 16);
-  const bool finite = a <= 3.4028235e38f;
-  // 127 / a is no float for the smallest a: such blocks count as zeros, off by less than 2^-120
-  const bool some = finite && a >= 7.52316385e-37f;
-  // a / 127: the product with the rounded reciprocal, and what it leaves given back (Markstein's correction)
-  constexpr float kPart = 1.f / 127.f;
-  const float near = a * kPart;
-  if (first) *scale = finite ? (some ? fmaf(fmaf(-127.f, near, a), kPart, near) : 0.f) : __uint_as_float(0x7fffffffu);
-  // (the fast division is good for divisors up to 2^126: both sides a quarter)
-  const float inv = some ? __fdividef(31.75f, 0.25f * a) * 1.00000095367431640625f : 0.f;
+  const ActScale k = act_scale(__uint_as_float(top << 16));
+  if (first) *scale = k.scale;
   float v[8];
   spread(raw, v);
   uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = some ? __float_as_uint(fmaf(v[i], inv, 12582912.f)) : 0u;      // + 1.5 2^23: whole numbers in the low byte
+  for (int i = 0; i < 8; ++i) w[i] = k.inv != 0.f ? act_word(v[i], k.inv) : 0u;
   const uint2 u = make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
                              __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
   if (VEC) {

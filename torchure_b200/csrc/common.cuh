@@ -293,6 +293,9 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t smem_addr, uint32_t a
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
+__device__ __forceinline__ void stmatrix_x2_trans(uint32_t smem_addr, uint32_t a, uint32_t b) {      // addresses of threads 0 to 15
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(smem_addr), "r"(a), "r"(b) : "memory");
+}
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "

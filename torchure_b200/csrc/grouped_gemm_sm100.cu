@@ -13,6 +13,15 @@
 // are overwritten with zeros in shared memory, in both operands (0 x NaN is NaN), by a warp that does nothing else.
 //
 // Groups are read from `offsets` on the device: no call waits for them.  The grid is persistent; tiles go round over the pairs.
+//
+// With SwiGLU in the epilogue the matrix is gate over up, and a CTA's 128 tile rows are four times 16 gate rows and the 16 up rows of
+// the same units: a warp, which reads 32 lanes of the accumulator, has both factors of its 16 units, in the same place of two
+// fragments.  The activation is taken from the fp32 sums; gate and up are stored beside it in bf16, or in 8 bits with a scale for the
+// CTA's 64 units (act8.cu has the format), or not at all.
+//
+// Few rows per group: grouped_few_kernel, single CTAs on 128 tile rows and at most 64 group rows, two of them on an SM.  The matrices
+// are then all the traffic there is, and what counts is how evenly it is spread and how many copies are on their way.
+#include "act8.cuh"
 #include "cta_pair.cuh"
 #include "moe_api.h"
 
@@ -31,10 +40,18 @@ constexpr int BAR_BYTES = 256;
 constexpr int EDGE_BYTES = (kMaxExperts + 1) * 4;
 constexpr uint32_t TMEM_COLS = 512;
 
-constexpr int PITCH = 80;                       // bytes of a staged row of 32 values: eight of them fall on all banks once
-constexpr int ROW_EPI_BYTES = 4 * 64 * PITCH;   // per epilogue warp 64 rows
+// Staged rows of an epilogue warp, 64 at a time.  Eight rows of 80 or of 112 bytes fall on every bank once.
+//   kStore    32 columns in bf16                                      (64 bytes used)
+//   kSwiglu   16 units: activation | gate | up in bf16                (96)
+//   kSwiglu8  16 units: activation in bf16 | gate | up in 8 bits      (64)
+enum { kStore = 0, kSwiglu = 1, kSwiglu8 = 2 };
+constexpr int PITCH = 80, WIDE_PITCH = 112;
+constexpr int ROW_EPI_BYTES = 4 * 64 * WIDE_PITCH;
+constexpr int MAX_BYTES = 4 * 2 * 64 * 2, INV_BYTES = 2 * 64 * 4;      // kSwiglu8: largest magnitudes of the warps, reciprocals
 constexpr int ROW_THREADS = 192;
 constexpr int ROW_SMEM = STAGES * STAGE_BYTES + ROW_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
+constexpr int ROW8_STAGES_EPI = 4 * 64 * PITCH + MAX_BYTES + INV_BYTES;
+static_assert(ROW8_STAGES_EPI <= ROW_EPI_BYTES, "the 8-bit epilogue stages narrower rows");
 
 constexpr int EPI_BUF = 4096;                   // 32 rows x 128 B
 constexpr int W_EPI_BYTES = 4 * 2 * EPI_BUF;
@@ -85,11 +102,206 @@ __device__ __forceinline__ bool find_rows(Place& p, int unit, int cols, int& r0,
   return false;
 }
 
+// Where the rows of a product go.  width: columns of the output (units for SwiGLU); gu, q: one of them or neither
+struct RowsOut {
+  __nv_bfloat16* y;      // the product, or the activation
+  __nv_bfloat16* gu;     // [R, 2 width]
+  int8_t* q;             // [R, 2 width]
+  float* scales;         // [R, 2 ceil(width / 64)]
+  int width;
+};
+
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {      // of bf16 pairs, NaN where either is
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The epilogue of one warp: 32 accumulator lanes from t_row on, columns 0 .. live - 1 of the tile, which are rows r0 .. of the output.
+// n0: first output column (first unit) of these lanes; buf: this warp's staging rows, shared: MAX_BYTES + INV_BYTES for all four warps.
+// release() once the accumulator has been read.
+template <int EPI, class Release>
+__device__ __forceinline__ void rows_epilogue(const RowsOut& out, uint32_t t_row, int q4, uint8_t* buf, uint8_t* shared, int r0, int live,
+                                              int n0, Release release) {
+  const int lane = threadIdx.x & 31;
+  const int N = out.width;
+  constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
+  const uint32_t put = smem_u32(buf) + (lane & 7) * P + (lane >> 3) * 16;      // stmatrix: this lane's row and tile
+#pragma unroll 1
+  for (int c = 0; c < live; c += 64) {
+    uint32_t v[32], u[32];
+    __syncwarp();
+    tmem_ld_16x256b_x8(t_row + c, v);
+    tmem_ld_16x256b_x8(t_row + c + (16u << 16), u);
+    tmem_ld_wait();
+    if (c + 64 >= live) release();
+    if constexpr (EPI == kStore) {
+      if (n0 >= N) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        stmatrix_x4_trans(put + j * 8 * P, pack_bf16x2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
+                          pack_bf16x2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
+                          pack_bf16x2(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1])),
+                          pack_bf16x2(__uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3])));
+      __syncwarp();
+      const int piece = lane & 3, n = n0 + piece * 8;
+      if (n < N) {
+        __nv_bfloat16* dst = out.y + static_cast<int64_t>(r0 + c) * N + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * 8 + (lane >> 2);
+          if (c + row < live)
+            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(buf + row * P + piece * 16);
+        }
+      }
+    } else {
+      const bool in0 = n0 < N, in1 = n0 + 8 < N;      // units of a fragment's two halves
+      uint32_t act[8][2], gate[8][2], up[8][2];       // pairs of neighbouring output rows
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float g0 = __uint_as_float(v[4 * j + 2 * h]), g1 = __uint_as_float(v[4 * j + 2 * h + 1]);
+          const float u0 = __uint_as_float(u[4 * j + 2 * h]), u1 = __uint_as_float(u[4 * j + 2 * h + 1]);
+          act[j][h] = pack_bf16x2(silu(g0) * u0, silu(g1) * u1);
+          const bool in = h ? in1 : in0;
+          gate[j][h] = in ? pack_bf16x2(g0, g1) : 0u;
+          up[j][h] = in ? pack_bf16x2(u0, u1) : 0u;
+        }
+      if constexpr (EPI == kSwiglu8) {
+        uint32_t* tops = reinterpret_cast<uint32_t*>(shared);                  // [warp][gate, up][64 rows] bf16
+        float* inv = reinterpret_cast<float*>(shared + MAX_BYTES);             // [gate, up][64 rows]
+        const int nb = (N + kActBlock - 1) / kActBlock;
+        // the largest magnitude of every row's 16 units: sixteen values over eight lanes, half of what is left handed on in each step
+        uint32_t m[16];
+        constexpr uint32_t kAbs = 0x7fff7fffu;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          m[2 * j] = max2_nan(gate[j][0] & kAbs, gate[j][1] & kAbs);
+          m[2 * j + 1] = max2_nan(up[j][0] & kAbs, up[j][1] & kAbs);
+        }
+#pragma unroll
+        for (int step = 16, n = 8; step >= 4; step >>= 1, n >>= 1)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < n) {
+              const uint32_t give = (lane & step) ? m[i] : m[i + n], keep = (lane & step) ? m[i + n] : m[i];
+              m[i] = max2_nan(keep, __shfl_xor_sync(0xffffffffu, give, step));
+            }
+        const int j = (lane >> 4) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
+        tops[q4 * 64 + j * 4 + (lane & 3)] = m[0];
+        tops[q4 * 64 + 32 + j * 4 + (lane & 3)] = m[1];
+        named_bar_sync(1, 128);
+        {
+          const int row = (q4 & 1) * 32 + lane, half = q4 >> 1;      // a thread has the gates or the ups of one row
+          float a = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float t = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(tops)[w * 128 + half * 64 + row]) << 16);
+            a = t != t ? t : (a != a ? a : fmaxf(a, t));
+          }
+          const ActScale k = act_scale(a);
+          inv[half * 64 + row] = k.inv;
+          const int blk = n0 / kActBlock;
+          if (c + row < live && blk < nb) out.scales[static_cast<int64_t>(r0 + c + row) * 2 * nb + half * nb + blk] = k.scale;
+        }
+        named_bar_sync(1, 128);
+#pragma unroll
+        for (int j2 = 0; j2 < 8; ++j2) {
+          const float2 ig = *reinterpret_cast<const float2*>(inv + 8 * j2 + 2 * (lane & 3));
+          const float2 iu = *reinterpret_cast<const float2*>(inv + 64 + 8 * j2 + 2 * (lane & 3));
+          uint8_t* to = buf + (8 * j2 + 2 * (lane & 3)) * P + 32 + (lane >> 2);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            to[8 * h] = act_byte(__uint_as_float(gate[j2][h] << 16), ig.x);
+            to[P + 8 * h] = act_byte(__uint_as_float(gate[j2][h] & 0xffff0000u), ig.y);
+            to[16 + 8 * h] = act_byte(__uint_as_float(up[j2][h] << 16), iu.x);
+            to[P + 16 + 8 * h] = act_byte(__uint_as_float(up[j2][h] & 0xffff0000u), iu.y);
+          }
+        }
+      }
+      if (n0 >= N) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (EPI == kSwiglu) {
+          stmatrix_x4_trans(put + j * 8 * P, act[j][0], act[j][1], gate[j][0], gate[j][1]);
+          stmatrix_x2_trans(put + j * 8 * P + 64, up[j][0], up[j][1]);
+        } else {
+          stmatrix_x2_trans(put + j * 8 * P, act[j][0], act[j][1]);
+        }
+      }
+      __syncwarp();
+      const int piece = lane & 1, n = n0 + piece * 8;
+      if (n < N) {
+        const int64_t at = static_cast<int64_t>(r0 + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = i * 16 + (lane >> 1);
+          if (c + row < live) {
+            const uint8_t* src = buf + row * P;
+            *reinterpret_cast<uint4*>(out.y + (at + row) * N + n) = *reinterpret_cast<const uint4*>(src + piece * 16);
+            if constexpr (EPI == kSwiglu) {
+              if (out.gu) {
+                __nv_bfloat16* gu = out.gu + (at + row) * 2 * N + n;
+                *reinterpret_cast<uint4*>(gu) = *reinterpret_cast<const uint4*>(src + 32 + piece * 16);
+                *reinterpret_cast<uint4*>(gu + N) = *reinterpret_cast<const uint4*>(src + 64 + piece * 16);
+              }
+            } else {
+              int8_t* q = out.q + (at + row) * 2 * N + n;
+              *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(src + 32 + piece * 8);
+              *reinterpret_cast<uint2*>(q + N) = *reinterpret_cast<const uint2*>(src + 48 + piece * 8);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// Zeros into the rows of no expert, by `warps` warps of which this is number `w`
+template <int EPI>
+__device__ __forceinline__ void rows_of_none(const RowsOut& out, int first, int R, int w, int warps) {
+  const int lane = threadIdx.x & 31, N = out.width;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int r = first + w; r < R; r += warps) {
+    const int64_t row = r;
+    for (int n = lane * 8; n < N; n += 256) *reinterpret_cast<uint4*>(out.y + row * N + n) = zero;
+    if (EPI == kSwiglu && out.gu)
+      for (int n = lane * 8; n < 2 * N; n += 256) *reinterpret_cast<uint4*>(out.gu + row * 2 * N + n) = zero;
+    if (EPI == kSwiglu8) {
+      const int nb = (N + kActBlock - 1) / kActBlock;
+      for (int n = lane * 8; n < 2 * N; n += 256) *reinterpret_cast<uint2*>(out.q + row * 2 * N + n) = make_uint2(0, 0);
+      for (int b = lane; b < 2 * nb; b += 32) out.scales[row * 2 * nb + b] = 0.f;
+    }
+  }
+}
+
+// The matrix's part of one k-block: 128 tile rows.  For SwiGLU n0 counts units and up rows stand F further down; `load` copies one
+// box [64 or 16 rows or k, 64] from (column, row, expert).
+template <bool W_MN, int EPI, class Load>
+__device__ __forceinline__ void load_matrix(uint8_t* sA, int k0, int n0, int F, int e, Load load) {
+  if constexpr (EPI != kStore) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      load(sA + g * 4096, k0, n0 + g * 16, e);
+      load(sA + g * 4096 + 2048, k0, F + n0 + g * 16, e);
+    }
+  } else if constexpr (W_MN) {
+#pragma unroll
+    for (int j = 0; j < BM / 64; ++j) load(sA + j * 8192, n0 + j * 64, k0, e);
+  } else {
+    load(sA, k0, n0, e);
+  }
+}
+
 // y [R, N] from x [R, K] and matrices [E, N, K] (W_MN false) or [E, K, N]
-template <bool W_MN>
+template <bool W_MN, int EPI>
 __global__ void __launch_bounds__(ROW_THREADS, 1)
 grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
-                    __nv_bfloat16* __restrict__ y, int R, int E, int N, int K, int* err) {
+                    const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
+  constexpr int UNIT = EPI == kStore ? 2 * BM : BM;      // output columns of a tile
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -106,7 +318,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cluster = static_cast<int>(blockIdx.x) >> 1, num_clusters = static_cast<int>(gridDim.x) >> 1;
-  const int cols = (N + 2 * BM - 1) / (2 * BM);
+  const int cols = (out.width + UNIT - 1) / UNIT;
   const int num_kb = (K + BK - 1) / BK;
 
   load_edges(offsets, edge, E, R);
@@ -143,18 +355,15 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 #pragma unroll
       for (int s = 0; s < STAGES; ++s) lead_full[s] = map_to_cta(&full[s], 0);
       for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
-        const int n0 = col * 2 * BM + static_cast<int>(rank) * BM;
+        const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2);
         const int half = (live + 31) / 32 * 16;      // rows in each CTA's half of the instruction's columns
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) { ok = false; break; }
           uint8_t* sA = smem + stage * STAGE_BYTES;
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
-          if (!W_MN) {
-            tma_load_3d_pair(sA, &tmW, lead_full[stage], kb * BK, n0, at.e);
-          } else {
-#pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load_3d_pair(sA + j * 8192, &tmW, lead_full[stage], n0 + j * 64, kb * BK, at.e);
-          }
+          load_matrix<W_MN, EPI>(sA, kb * BK, n0, out.width, at.e, [&](uint8_t* to, int c0, int c1, int c2) {
+            tma_load_3d_pair(to, &tmW, lead_full[stage], c0, c1, c2);
+          });
           tma_load_2d_pair(sA + A_BYTES, &tmX, lead_full[stage], kb * BK, r0 + static_cast<int>(rank) * half);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -191,54 +400,23 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     }
   } else {
     const int q = warp & 3;      // TMEM lane quarter this warp may read
-    const uint32_t buf = smem_u32(epi + q * 64 * PITCH);
-    const uint32_t put = buf + (lane & 7) * PITCH + (lane >> 3) * 16;      // stmatrix: this lane's row and tile
     int it = 0, r0, live, col;
     bool ok = true;
     for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
-      const int n0 = col * 2 * BM + static_cast<int>(rank) * BM + q * 32;
+      const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2) + q * (UNIT / 8);
       const int acc = it & 1;
       if (!mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
       const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
-#pragma unroll 1
-      for (int c = 0; c < live; c += 64) {
-        uint32_t v[32], u[32];
-        __syncwarp();
-        tmem_ld_16x256b_x8(t_row + c, v);
-        tmem_ld_16x256b_x8(t_row + c + (16u << 16), u);
-        tmem_ld_wait();
-        if (c + 64 >= live) {
-          tc_fence_before();
-          remote_arrive(lead_tempty);
-        }
-        if (n0 < N) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            stmatrix_x4_trans(put + j * 8 * PITCH, pack_bf16x2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
-                              pack_bf16x2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
-                              pack_bf16x2(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1])),
-                              pack_bf16x2(__uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3])));
-          __syncwarp();
-          const int piece = lane & 3, n = n0 + piece * 8;
-          if (n < N) {
-            __nv_bfloat16* dst = y + static_cast<int64_t>(r0 + c) * N + n;
-            const uint8_t* src = epi + q * 64 * PITCH + piece * 16;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = i * 8 + (lane >> 2);
-              if (c + row < live)
-                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(src + row * PITCH);
-            }
-          }
-        }
-      }
+      constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
+      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, q, epi + q * 64 * P, epi + 4 * 64 * P, r0, live,
+                         n0, [&] {
+                           tc_fence_before();
+                           remote_arrive(lead_tempty);
+                         });
       ++it;
     }
-    // rows of no expert
-    for (int r = edge[E] + static_cast<int>(blockIdx.x) * 4 + q; r < R; r += static_cast<int>(gridDim.x) * 4)
-      for (int n = lane * 8; n < N; n += 256) *reinterpret_cast<uint4*>(y + static_cast<int64_t>(r) * N + n) = make_uint4(0, 0, 0, 0);
+    rows_of_none<EPI>(out, edge[E], R, static_cast<int>(blockIdx.x) * 4 + q, static_cast<int>(gridDim.x) * 4);
   }
 
   if (*reinterpret_cast<volatile int*>(err) != 0) {
@@ -252,6 +430,147 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// Few rows per group: one CTA has 128 tile rows (64 units of SwiGLU) of one group and up to 64 of its rows; grid (tiles of the matrix,
+// an upper bound of the groups' tiles of rows).  The operand stages hold the epilogue's staging rows once the products are done.
+constexpr int FEW_ROWS = 64, FEW_STAGES = 4, FEW_STAGE = A_BYTES + FEW_ROWS * BK * 2;
+constexpr int FEW_SMEM = FEW_STAGES * FEW_STAGE + BAR_BYTES + 1024;
+static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE, "staging rows");
+static_assert(2 * (FEW_SMEM + 1024) <= 233472, "two CTAs on an SM");
+
+template <bool W_MN, int EPI>
+__global__ void __launch_bounds__(ROW_THREADS, 2)
+grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
+                   const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + FEW_STAGES * FEW_STAGE);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + FEW_STAGES;
+  uint64_t* tfull = bars + 2 * FEW_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FEW_STAGES + 1);
+  int* where = reinterpret_cast<int*>(bars + 2 * FEW_STAGES + 2);      // group, first row, rows, first row of no expert
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    for (int s = 0; s < FEW_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, FEW_ROWS);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 0) {
+    // the group that tile blockIdx.y of the groups' row tiles belongs to: edges as load_edges has them, 32 groups at a time
+    int run = 0, tiles_before = 0;
+    if (lane == 0) where[2] = 0;
+    __syncwarp();
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int hi = e < E ? min(max(offsets[e + 1], 0), R) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, hi, o);
+        if (lane >= o) hi = max(hi, up);
+      }
+      hi = max(hi, run);
+      int lo = __shfl_up_sync(0xffffffffu, hi, 1);
+      if (lane == 0) lo = run;
+      const int tiles = (hi - lo + FEW_ROWS - 1) / FEW_ROWS;
+      int sum = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const int at = static_cast<int>(blockIdx.y) - (tiles_before + sum - tiles);
+      if (at >= 0 && at < tiles) {
+        where[0] = e;
+        where[1] = lo + at * FEW_ROWS;
+        where[2] = min(FEW_ROWS, hi - lo - at * FEW_ROWS);
+      }
+      run = __shfl_sync(0xffffffffu, hi, 31);
+      tiles_before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) where[3] = run;
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const int e = where[0], r0 = where[1], live = where[2];
+  constexpr int UNIT = EPI == kStore ? BM : BM / 2;
+  const int n0 = static_cast<int>(blockIdx.x) * UNIT;
+  const int num_kb = live > 0 ? (K + BK - 1) / BK : 0;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) break;
+        uint8_t* sA = smem + stage * FEW_STAGE;
+        mbar_expect_tx(&full[stage], FEW_STAGE);
+        load_matrix<W_MN, EPI>(sA, kb * BK, n0, out.width, e,
+                               [&](uint8_t* to, int c0, int c1, int c2) { tma_load_3d(to, &tmW, &full[stage], c0, c1, c2); });
+        tma_load_2d(sA + A_BYTES, &tmX, &full[stage], kb * BK, r0);
+        if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t a_lbo = W_MN ? 8192u : 16u, a_step = W_MN ? (2048u >> 4) : (32u >> 4);
+      const uint32_t idesc = make_idesc_bf16(BM, (live + 15) / 16 * 16, W_MN, false);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&full[stage], phase, err, kErrMmaFullWait)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t a_addr = smem_u32(smem + stage * FEW_STAGE);
+        const uint64_t da = make_desc_sw128(a_addr, a_lbo, 1024);
+        const uint64_t db = make_desc_sw128(a_addr + A_BYTES, 16u, 1024);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          umma_f16_ss(tmem_base, da + static_cast<uint64_t>(k * a_step), db + static_cast<uint64_t>(k * (32u >> 4)), idesc,
+                      (kb != 0 || k != 0) ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
+      }
+      if (ok && num_kb > 0) umma_commit(tfull);
+    }
+  } else {
+    const int q = warp & 3;
+    if (num_kb > 0 && mbar_wait_warp(tfull, 0, err, kErrEpilogueTmemFullWait)) {
+      tc_fence_after();
+      constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
+      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16), q, smem + q * 64 * P, smem + 4 * 64 * P, r0, live,
+                         n0 + q * (UNIT / 4), [] {});
+    }
+    rows_of_none<EPI>(out, where[3], R, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x) * 4 + q,
+                      static_cast<int>(gridDim.x * gridDim.y) * 4);
+  }
+
+  if (*reinterpret_cast<volatile int*>(err) != 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, FEW_ROWS);
   }
 }
 
@@ -516,19 +835,57 @@ int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, 
 
 }  // namespace
 
-int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
-                 int E, int N, int K, int* err, int num_sms, cudaStream_t stream) {
-  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(y) & 15) != 0) return -1;
+namespace {
+
+// Up to this many rows per group, on average, the small tiles.
+constexpr int FEW_AVERAGE = 96;
+
+template <bool W_MN, int EPI>
+int launch_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R, int E, int K,
+                int* err, int num_sms, cudaStream_t stream) {
+  const int N = out.width;
+  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(out.y) & 15) != 0) return -1;
+  const bool few = R <= static_cast<int64_t>(FEW_AVERAGE) * E;
   CUtensorMap tw, tx;
-  int r = w_t ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64) : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
+  int r = EPI != kStore ? make_tmap_3d(&tw, w, 2, E, 2 * static_cast<uint64_t>(N), K, 16, 64)
+          : W_MN        ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64)
+                        : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
   if (r) return r;
-  r = make_tmap_2d(&tx, x, 2, R, K, ldx, BNH, 64);
+  r = make_tmap_2d(&tx, x, 2, R, K, ldx, few ? FEW_ROWS : BNH, 64);
   if (r) return r - 100;
   // at most: every group with rows ends in a tile that is not full
-  const int64_t tiles = static_cast<int64_t>(R) / BN + (E < R ? E : R);
-  const int64_t units = tiles * ((N + 2 * BM - 1) / (2 * BM));
-  return w_t ? launch_pairs(grouped_rows_kernel<true>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, y, R, E, N, K, err)
-             : launch_pairs(grouped_rows_kernel<false>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, y, R, E, N, K, err);
+  const int groups = E < R ? E : R;
+  if (few) {
+    constexpr int UNIT = EPI == kStore ? BM : BM / 2;
+    auto kern = grouped_few_kernel<W_MN, EPI>;
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
+    return launch_pdl(kern, dim3((N + UNIT - 1) / UNIT, R / FEW_ROWS + groups), dim3(ROW_THREADS), FEW_SMEM, stream, tw, tx, offsets, out, R,
+                      E, K, err) == cudaSuccess
+               ? 0
+               : -21;
+  }
+  constexpr int UNIT = EPI == kStore ? 2 * BM : BM;
+  const int64_t units = (static_cast<int64_t>(R) / BN + groups) * ((N + UNIT - 1) / UNIT);
+  return launch_pairs(grouped_rows_kernel<W_MN, EPI>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, out, R, E, K, err);
+}
+
+}  // namespace
+
+int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
+                 int E, int N, int K, int* err, int num_sms, cudaStream_t stream) {
+  RowsOut out{};
+  out.y = y;
+  out.width = N;
+  return w_t ? launch_rows<true, kStore>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream)
+             : launch_rows<false, kStore>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream);
+}
+
+int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, __nv_bfloat16* act, __nv_bfloat16* gu,
+                   int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms, cudaStream_t stream) {
+  if (F % 8 != 0 || (gu && q) || ((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) return -1;
+  RowsOut out{act, gu, q, scales, F};
+  return q ? launch_rows<false, kSwiglu8>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream)
+           : launch_rows<false, kSwiglu>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream);
 }
 
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,

@@ -2,6 +2,7 @@
 // Python costs the host 40 - 90 us for a forward and a backward pass, more than most of these kernels run.  Outputs are allocated
 // here; in the poison mode (ops/debug.py) each is filled and remembered before its kernel runs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -17,11 +18,14 @@ using OptTensor = c10::optional<Tensor>;
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
+// torch::empty for GPU tensors without the dispatcher (0.6 us instead of 1.8)
+Tensor empty(c10::IntArrayRef size, const at::TensorOptions& options) { return at::detail::empty_cuda(size, options); }
+
 // Backward passes run in threads of autograd's, which do not hold the interpreter's lock.
 struct Outputs {
   bool poisoned;
   Tensor operator()(const char* name, c10::IntArrayRef size, const at::TensorOptions& options) const {
-    Tensor t = torch::empty(size, options);
+    Tensor t = empty(size, options);
     if (poisoned) {
       pybind11::gil_scoped_acquire lock;
       pybind11::module_::import("torchure_b200.ops.debug").attr("track")(name, t);
@@ -73,9 +77,9 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   Routed r;
   r.weights = make("route.weights", {T, k}, f32);
   r.aux = make("route.aux", {}, f32);
-  r.experts = torch::empty({T, k}, i32);
-  r.slots = torch::empty({T, k}, i32);
-  r.rows = torch::empty({T * k}, i32);
+  r.experts = empty({T, k}, i32);
+  r.slots = empty({T, k}, i32);
+  r.rows = empty({T * k}, i32);
   if (T == 0) {
     r.offsets = torch::zeros({E + 1}, i32);
     r.counts = torch::zeros({E}, i32);
@@ -84,7 +88,7 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   }
   // offsets, counts and scratch of one allocation
   const int64_t scratch = tb::route_scratch_ints((int)T, (int)E, (int)k);
-  Tensor ints = torch::empty({2 * E + 1 + scratch}, i32);
+  Tensor ints = empty({2 * E + 1 + scratch}, i32);
   r.offsets = ints.narrow(0, 0, E + 1);
   r.counts = ints.narrow(0, E + 1, E);
   const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, r.weights.data_ptr<float>(),
@@ -214,8 +218,8 @@ std::tuple<Tensor, Tensor> do_quantize(const Tensor& x) {
   check_bf16(x, "quantize8");
   const int64_t M = x.size(0), N = x.size(1);
   check_blocks(M, N, "quantize8");
-  Tensor q = torch::empty({M, N}, x.options().dtype(torch::kInt8));
-  Tensor s = torch::empty({M, blocks_of(N)}, x.options().dtype(torch::kFloat32));
+  Tensor q = empty({M, N}, x.options().dtype(torch::kInt8));
+  Tensor s = empty({M, blocks_of(N)}, x.options().dtype(torch::kFloat32));
   tb::quantize8(bf(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)N, cur_stream());
   g_launches += 1;
   return {q, s};
@@ -245,8 +249,8 @@ std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, const Outputs& m
   const int64_t M = gu.size(0), F = gu.size(1) / 2;
   check_blocks(M, F, "swiglu_8bit");
   Tensor act = make("swiglu_8bit", {M, F}, gu.options());
-  Tensor q = torch::empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
-  Tensor s = torch::empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
+  Tensor q = empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
+  Tensor s = empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
   tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)F, cur_stream());
   g_launches += 1;
   return {act, q, s};
@@ -446,14 +450,21 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
   Mlp m;
   m.r = do_route(logits, k, capacity, make);
   const Tensor xg = do_gather(x, m.r.rows, k, make);
-  const Tensor gu = do_grouped(xg, wgu, m.r.offsets, false, make);
-  auto t = do_swiglu8(gu, make);
-  if (keep && bits == 16) m.gu = gu;
+  const int64_t R = xg.size(0), F = wd.size(2), E = wd.size(0), D = x.size(1);
+  const Tensor act = make("expert_mlp.act", {R, F}, wgu.options());
+  if (keep && bits == 16) m.gu = make("expert_mlp.gu", {R, 2 * F}, wgu.options());
   if (keep && bits == 8) {
-    m.q = std::get<1>(t);
-    m.scales = std::get<2>(t);
+    m.q = empty({R, 2 * F}, wgu.options().dtype(torch::kInt8));
+    m.scales = make("expert_mlp.scales", {R, 2 * blocks_of(F)}, wgu.options().dtype(torch::kFloat32));
   }
-  const Tensor y = do_grouped(std::get<0>(t), wd, m.r.offsets, false, make);
+  if (R > 0) {
+    const int rc = tb::grouped_swiglu(bf(xg), D, bf(wgu), m.r.offsets.data_ptr<int>(), bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr,
+                                      m.q.defined() ? m.q.data_ptr<int8_t>() : nullptr, m.q.defined() ? m.scales.data_ptr<float>() : nullptr,
+                                      (int)R, (int)E, (int)F, (int)D, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+    TORCH_CHECK(rc == 0, "expert_mlp: gate / up product failed with code ", rc);
+    g_launches += 1;
+  }
+  const Tensor y = do_grouped(act, wd, m.r.offsets, false, make);
   m.out = do_combine(y, m.r.weights, m.r.slots, x.scalar_type(), make);
   return m;
 }
@@ -485,7 +496,7 @@ variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x
 Tensor stack_of(const Tensor& first, const OptTensor& second) {
   if (!has(second)) return matrices(first);
   const int64_t E = first.size(0), F = first.size(1), D = first.size(2);
-  Tensor w = torch::empty({E, 2 * F, D}, first.options().dtype(torch::kBFloat16));
+  Tensor w = empty({E, 2 * F, D}, first.options().dtype(torch::kBFloat16));
   w.narrow(1, 0, F).copy_(first);
   w.narrow(1, F, F).copy_(*second);
   return w;
