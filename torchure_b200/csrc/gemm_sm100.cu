@@ -437,16 +437,17 @@ namespace {
 struct TmapKey {
   const void* base; uint64_t rows, cols, ld; uint32_t box_rows, box_cols; int elem_bytes;
   uint64_t planes = 0;      // 0: a 2-D map
+  int pair_groups = 0;      // make_tmap_gate_up
   bool operator==(const TmapKey& o) const {
     return base == o.base && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows &&
-           box_cols == o.box_cols && elem_bytes == o.elem_bytes && planes == o.planes;
+           box_cols == o.box_cols && elem_bytes == o.elem_bytes && planes == o.planes && pair_groups == o.pair_groups;
   }
 };
 struct TmapKeyHash {
   size_t operator()(const TmapKey& k) const {
     uint64_t h = reinterpret_cast<uint64_t>(k.base) * 0x9E3779B97F4A7C15ull;
     h ^= (k.rows + 0x9E3779B97F4A7C15ull + (h << 6) + (h >> 2));
-    h ^= (k.cols * 31 + k.ld * 131 + k.box_rows * 7 + k.box_cols * 3 + k.elem_bytes + k.planes * 17 + (h << 6) + (h >> 2));
+    h ^= (k.cols * 31 + k.ld * 131 + k.box_rows * 7 + k.box_cols * 3 + k.elem_bytes + k.planes * 17 + k.pair_groups * 101 + (h << 6) + (h >> 2));
     return static_cast<size_t>(h);
   }
 };
@@ -468,12 +469,24 @@ static int make_tmap(CUtensorMap* map, const TmapKey& key) {
   if ((key.ld * key.elem_bytes) % 16 != 0) return -12;
   if (key.box_cols * key.elem_bytes != 128) return -13;
   const uint64_t row = key.ld * static_cast<uint64_t>(key.elem_bytes);
-  cuuint64_t dims[3] = {key.cols, key.rows, key.planes};
-  cuuint64_t strides[2] = {row, row * key.rows};
-  cuuint32_t box[3] = {key.box_cols, key.box_rows, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
+  cuuint64_t dims[5] = {key.cols, key.rows, key.planes, 1, 1};
+  cuuint64_t strides[4] = {row, row * key.rows, 0, 0};
+  cuuint32_t box[5] = {key.box_cols, key.box_rows, 1, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  int rank = key.planes ? 3 : 2;
+  if (key.pair_groups > 1) {
+    rank = 5;
+    dims[1] = 16; dims[2] = 2; dims[3] = key.rows / 16; dims[4] = key.planes;
+    strides[0] = row; strides[1] = row * key.rows; strides[2] = row * 16; strides[3] = row * 2 * key.rows;
+    box[1] = 16; box[2] = 2; box[3] = key.pair_groups;
+  } else if (key.pair_groups == 1) {
+    rank = 4;
+    dims[1] = key.rows; dims[2] = 2; dims[3] = key.planes;
+    strides[0] = row; strides[1] = row * key.rows; strides[2] = row * 2 * key.rows;
+    box[1] = 16; box[2] = 2;
+  }
   CUtensorMapDataType dt = key.elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  CUresult r = fn(map, dt, key.planes ? 3 : 2, const_cast<void*>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = fn(map, dt, rank, const_cast<void*>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return -14;
   if (cache.size() > 16384) cache.clear();
@@ -491,6 +504,14 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t ro
 int make_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t planes, uint64_t rows, uint64_t cols, uint32_t box_rows,
                  uint32_t box_cols) {
   return make_tmap(map, TmapKey{base, rows, cols, cols, box_rows, box_cols, elem_bytes, planes});
+}
+
+// `planes` matrices [2 rows, cols], gate over up: a box is 64 columns of `groups` times 16 gate rows and the 16 up rows of the same
+// units.  With rows a multiple of 16 a box takes all groups, at coordinates (column, 0, 0, unit / 16, plane); otherwise (groups 1)
+// one, at (column, unit, 0, plane).  Units past the last read as zero.
+int make_tmap_gate_up(CUtensorMap* map, const void* base, uint64_t planes, uint64_t rows, uint64_t cols, int groups) {
+  if (groups > 1 && rows % 16 != 0) return -15;
+  return make_tmap(map, TmapKey{base, rows, cols, cols, 16, 64, 2, planes, groups});
 }
 
 template <bool A_MN, bool B_MN, int OUT>

@@ -31,6 +31,7 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t ro
                  uint32_t box_cols);
 int make_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t planes, uint64_t rows, uint64_t cols, uint32_t box_rows,
                  uint32_t box_cols);
+int make_tmap_gate_up(CUtensorMap* map, const void* base, uint64_t planes, uint64_t rows, uint64_t cols, int groups);
 
 namespace {
 
@@ -40,18 +41,25 @@ constexpr int BAR_BYTES = 256;
 constexpr int EDGE_BYTES = (kMaxExperts + 1) * 4;
 constexpr uint32_t TMEM_COLS = 512;
 
-// Staged rows of an epilogue warp, 64 at a time.  Eight rows of 80 or of 112 bytes fall on every bank once.
-//   kStore    32 columns in bf16                                      (64 bytes used)
-//   kSwiglu   16 units: activation | gate | up in bf16                (96)
-//   kSwiglu8  16 units: activation in bf16 | gate | up in 8 bits      (64)
+// Staged rows of the four epilogue warps that have a CTA's 128 accumulator lanes, 32 at a time, so that the output is written in whole
+// lines of 128 bytes (in pieces of 32 bytes, a warp's own units, gate and up beside the activation took 103 us instead of 78 without
+// them).  Eight rows of 272 or of 400 bytes fall on every bank once.
+//   kStore    128 columns in bf16
+//   kSwiglu   64 units: activation | gate | up in bf16
+//   kSwiglu8  64 units: activation in bf16 | gate | up in 8 bits
 enum { kStore = 0, kSwiglu = 1, kSwiglu8 = 2 };
-constexpr int PITCH = 80, WIDE_PITCH = 112;
-constexpr int ROW_EPI_BYTES = 4 * 64 * WIDE_PITCH;
-constexpr int MAX_BYTES = 4 * 2 * 64 * 2, INV_BYTES = 2 * 64 * 4;      // kSwiglu8: largest magnitudes of the warps, reciprocals
-constexpr int ROW_THREADS = 192;
+constexpr int EPI_ROWS = 32;
+template <int EPI>
+constexpr int kPitch = EPI == kSwiglu ? 400 : 272;
+// kSwiglu8, for the four warps: their largest magnitudes, and the reciprocals
+constexpr int MAX_BYTES = 4 * 2 * EPI_ROWS * 2, INV_BYTES = 2 * EPI_ROWS * 4;
+template <int EPI>
+constexpr int kPartBytes = EPI_ROWS * kPitch<EPI> + (EPI == kSwiglu8 ? MAX_BYTES + INV_BYTES : 0);
+constexpr int ROW_EPI_BYTES = 2 * kPartBytes<kSwiglu>;
+static_assert(kPartBytes<kSwiglu8> <= kPartBytes<kSwiglu> && kPartBytes<kStore> <= kPartBytes<kSwiglu>, "staging rows");
+constexpr int ROW_THREADS = 320;      // warp 0 copies, warp 1 issues the products, warps 2 - 9 are the epilogue
+constexpr int FEW_THREADS = 192;
 constexpr int ROW_SMEM = STAGES * STAGE_BYTES + ROW_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
-constexpr int ROW8_STAGES_EPI = 4 * 64 * PITCH + MAX_BYTES + INV_BYTES;
-static_assert(ROW8_STAGES_EPI <= ROW_EPI_BYTES, "the 8-bit epilogue stages narrower rows");
 
 constexpr int EPI_BUF = 4096;                   // 32 rows x 128 B
 constexpr int W_EPI_BYTES = 4 * 2 * EPI_BUF;
@@ -119,48 +127,55 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {      // o
   return r;
 }
 
-// The epilogue of one warp: 32 accumulator lanes from t_row on, columns 0 .. live - 1 of the tile, which are rows r0 .. of the output.
-// n0: first output column (first unit) of these lanes; buf: this warp's staging rows, shared: MAX_BYTES + INV_BYTES for all four warps.
-// release() once the accumulator has been read.
+// The epilogue of four warps, of which this is number q4 with 32 accumulator lanes from t_row on: columns 0 .. live - 1 of the tile, which
+// are rows r0 .. of the output; 32 of them at a time, from `from` on in steps of `step`.  n0: first output column (first unit) of the
+// CTA's lanes; buf: kPartBytes of the four, bar: their named barrier.  release() once this warp has read the accumulator.
 template <int EPI, class Release>
-__device__ __forceinline__ void rows_epilogue(const RowsOut& out, uint32_t t_row, int q4, uint8_t* buf, uint8_t* shared, int r0, int live,
-                                              int n0, Release release) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void rows_epilogue(const RowsOut& out, uint32_t t_row, int q4, uint8_t* buf, int bar, int r0, int live, int from,
+                                              int step, int n0, Release release) {
+  const int lane = threadIdx.x & 31, tid = q4 * 32 + lane;
   const int N = out.width;
-  constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
-  const uint32_t put = smem_u32(buf) + (lane & 7) * P + (lane >> 3) * 16;      // stmatrix: this lane's row and tile
+  constexpr int P = kPitch<EPI>;
+  // stmatrix: this lane's row and tile
+  const uint32_t put = smem_u32(buf) + (lane & 7) * P + q4 * (EPI == kStore ? 64 : 32) + (lane >> 3) * 16;
+  if (from >= live) release();
 #pragma unroll 1
-  for (int c = 0; c < live; c += 64) {
-    uint32_t v[32], u[32];
+  for (int c = from; c < live; c += step) {
+    uint32_t v[16], u[16];
     __syncwarp();
-    tmem_ld_16x256b_x8(t_row + c, v);
-    tmem_ld_16x256b_x8(t_row + c + (16u << 16), u);
+    tmem_ld_16x256b_x4(t_row + c, v);
+    tmem_ld_16x256b_x4(t_row + c + (16u << 16), u);
     tmem_ld_wait();
-    if (c + 64 >= live) release();
+    if (c + step >= live) release();
     if constexpr (EPI == kStore) {
-      if (n0 >= N) continue;
+      uint32_t w[4][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        stmatrix_x4_trans(put + j * 8 * P, pack_bf16x2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
-                          pack_bf16x2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
-                          pack_bf16x2(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1])),
-                          pack_bf16x2(__uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3])));
-      __syncwarp();
-      const int piece = lane & 3, n = n0 + piece * 8;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[j][h] = pack_bf16x2(__uint_as_float(v[4 * j + 2 * h]), __uint_as_float(v[4 * j + 2 * h + 1]));
+          w[j][2 + h] = pack_bf16x2(__uint_as_float(u[4 * j + 2 * h]), __uint_as_float(u[4 * j + 2 * h + 1]));
+        }
+      named_bar_sync(bar, 128);      // the rows staged before have been read
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stmatrix_x4_trans(put + j * 8 * P, w[j][0], w[j][1], w[j][2], w[j][3]);
+      named_bar_sync(bar, 128);
+      const int n = n0 + (tid & 15) * 8;
       if (n < N) {
         __nv_bfloat16* dst = out.y + static_cast<int64_t>(r0 + c) * N + n;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = i * 8 + (lane >> 2);
+        for (int i = 0; i < 4; ++i) {
+          const int row = i * 8 + (tid >> 4);
           if (c + row < live)
-            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(buf + row * P + piece * 16);
+            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(buf + row * P + (tid & 15) * 16);
         }
       }
     } else {
-      const bool in0 = n0 < N, in1 = n0 + 8 < N;      // units of a fragment's two halves
-      uint32_t act[8][2], gate[8][2], up[8][2];       // pairs of neighbouring output rows
+      const int f0 = n0 + q4 * 16;
+      const bool in0 = f0 < N, in1 = f0 + 8 < N;      // units of a fragment's two halves
+      uint32_t act[4][2], gate[4][2], up[4][2];       // pairs of neighbouring output rows
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float g0 = __uint_as_float(v[4 * j + 2 * h]), g1 = __uint_as_float(v[4 * j + 2 * h + 1]);
@@ -171,87 +186,85 @@ __device__ __forceinline__ void rows_epilogue(const RowsOut& out, uint32_t t_row
           up[j][h] = in ? pack_bf16x2(u0, u1) : 0u;
         }
       if constexpr (EPI == kSwiglu8) {
-        uint32_t* tops = reinterpret_cast<uint32_t*>(shared);                  // [warp][gate, up][64 rows] bf16
-        float* inv = reinterpret_cast<float*>(shared + MAX_BYTES);             // [gate, up][64 rows]
+        uint32_t* tops = reinterpret_cast<uint32_t*>(buf + EPI_ROWS * P);                   // [warp][gate, up][32 rows] bf16
+        float* inv = reinterpret_cast<float*>(buf + EPI_ROWS * P + MAX_BYTES);              // [gate, up][32 rows]
         const int nb = (N + kActBlock - 1) / kActBlock;
-        // the largest magnitude of every row's 16 units: sixteen values over eight lanes, half of what is left handed on in each step
-        uint32_t m[16];
+        // the largest magnitude of every row's 16 units: eight values over eight lanes, half of what is left handed on in each step
+        uint32_t m[8];
         constexpr uint32_t kAbs = 0x7fff7fffu;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           m[2 * j] = max2_nan(gate[j][0] & kAbs, gate[j][1] & kAbs);
           m[2 * j + 1] = max2_nan(up[j][0] & kAbs, up[j][1] & kAbs);
         }
 #pragma unroll
-        for (int step = 16, n = 8; step >= 4; step >>= 1, n >>= 1)
+        for (int bit = 16, n = 4; bit >= 4; bit >>= 1, n >>= 1)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 4; ++i)
             if (i < n) {
-              const uint32_t give = (lane & step) ? m[i] : m[i + n], keep = (lane & step) ? m[i + n] : m[i];
-              m[i] = max2_nan(keep, __shfl_xor_sync(0xffffffffu, give, step));
+              const uint32_t give = (lane & bit) ? m[i] : m[i + n], keep = (lane & bit) ? m[i + n] : m[i];
+              m[i] = max2_nan(keep, __shfl_xor_sync(0xffffffffu, give, bit));
             }
-        const int j = (lane >> 4) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
-        tops[q4 * 64 + j * 4 + (lane & 3)] = m[0];
-        tops[q4 * 64 + 32 + j * 4 + (lane & 3)] = m[1];
-        named_bar_sync(1, 128);
-        {
-          const int row = (q4 & 1) * 32 + lane, half = q4 >> 1;      // a thread has the gates or the ups of one row
+        const int j0 = (lane >> 4) * 2 + ((lane >> 3) & 1), half0 = (lane >> 2) & 1;
+        tops[q4 * 32 + half0 * 16 + j0 * 4 + (lane & 3)] = m[0];
+        named_bar_sync(bar, 128);      // (also: the rows staged before have been read)
+        if (q4 < 2) {      // a thread has the gates or the ups of one row
           float a = 0.f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const float t = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(tops)[w * 128 + half * 64 + row]) << 16);
+            const float t = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(tops)[w * 64 + q4 * 32 + lane]) << 16);
             a = t != t ? t : (a != a ? a : fmaxf(a, t));
           }
           const ActScale k = act_scale(a);
-          inv[half * 64 + row] = k.inv;
+          inv[q4 * 32 + lane] = k.inv;
           const int blk = n0 / kActBlock;
-          if (c + row < live && blk < nb) out.scales[static_cast<int64_t>(r0 + c + row) * 2 * nb + half * nb + blk] = k.scale;
+          if (c + lane < live && blk < nb) out.scales[static_cast<int64_t>(r0 + c + lane) * 2 * nb + q4 * nb + blk] = k.scale;
         }
-        named_bar_sync(1, 128);
+        named_bar_sync(bar, 128);
 #pragma unroll
-        for (int j2 = 0; j2 < 8; ++j2) {
-          const float2 ig = *reinterpret_cast<const float2*>(inv + 8 * j2 + 2 * (lane & 3));
-          const float2 iu = *reinterpret_cast<const float2*>(inv + 64 + 8 * j2 + 2 * (lane & 3));
-          uint8_t* to = buf + (8 * j2 + 2 * (lane & 3)) * P + 32 + (lane >> 2);
+        for (int j = 0; j < 4; ++j) {
+          const float2 ig = *reinterpret_cast<const float2*>(inv + 8 * j + 2 * (lane & 3));
+          const float2 iu = *reinterpret_cast<const float2*>(inv + 32 + 8 * j + 2 * (lane & 3));
+          uint8_t* to = buf + (8 * j + 2 * (lane & 3)) * P + 128 + q4 * 16 + (lane >> 2);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            to[8 * h] = act_byte(__uint_as_float(gate[j2][h] << 16), ig.x);
-            to[P + 8 * h] = act_byte(__uint_as_float(gate[j2][h] & 0xffff0000u), ig.y);
-            to[16 + 8 * h] = act_byte(__uint_as_float(up[j2][h] << 16), iu.x);
-            to[P + 16 + 8 * h] = act_byte(__uint_as_float(up[j2][h] & 0xffff0000u), iu.y);
+            to[8 * h] = act_byte(__uint_as_float(gate[j][h] << 16), ig.x);
+            to[P + 8 * h] = act_byte(__uint_as_float(gate[j][h] & 0xffff0000u), ig.y);
+            to[64 + 8 * h] = act_byte(__uint_as_float(up[j][h] << 16), iu.x);
+            to[P + 64 + 8 * h] = act_byte(__uint_as_float(up[j][h] & 0xffff0000u), iu.y);
           }
         }
+      } else {
+        named_bar_sync(bar, 128);      // the rows staged before have been read
       }
-      if (n0 >= N) continue;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
+        stmatrix_x2_trans(put + j * 8 * P, act[j][0], act[j][1]);
         if constexpr (EPI == kSwiglu) {
-          stmatrix_x4_trans(put + j * 8 * P, act[j][0], act[j][1], gate[j][0], gate[j][1]);
-          stmatrix_x2_trans(put + j * 8 * P + 64, up[j][0], up[j][1]);
-        } else {
-          stmatrix_x2_trans(put + j * 8 * P, act[j][0], act[j][1]);
+          stmatrix_x2_trans(put + j * 8 * P + 128, gate[j][0], gate[j][1]);
+          stmatrix_x2_trans(put + j * 8 * P + 256, up[j][0], up[j][1]);
         }
       }
-      __syncwarp();
-      const int piece = lane & 1, n = n0 + piece * 8;
+      named_bar_sync(bar, 128);
+      const int piece = tid & 7, n = n0 + piece * 8;
       if (n < N) {
         const int64_t at = static_cast<int64_t>(r0 + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = i * 16 + (lane >> 1);
+        for (int i = 0; i < 2; ++i) {
+          const int row = i * 16 + (tid >> 3);
           if (c + row < live) {
             const uint8_t* src = buf + row * P;
             *reinterpret_cast<uint4*>(out.y + (at + row) * N + n) = *reinterpret_cast<const uint4*>(src + piece * 16);
             if constexpr (EPI == kSwiglu) {
               if (out.gu) {
                 __nv_bfloat16* gu = out.gu + (at + row) * 2 * N + n;
-                *reinterpret_cast<uint4*>(gu) = *reinterpret_cast<const uint4*>(src + 32 + piece * 16);
-                *reinterpret_cast<uint4*>(gu + N) = *reinterpret_cast<const uint4*>(src + 64 + piece * 16);
+                *reinterpret_cast<uint4*>(gu) = *reinterpret_cast<const uint4*>(src + 128 + piece * 16);
+                *reinterpret_cast<uint4*>(gu + N) = *reinterpret_cast<const uint4*>(src + 256 + piece * 16);
               }
             } else {
               int8_t* q = out.q + (at + row) * 2 * N + n;
-              *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(src + 32 + piece * 8);
-              *reinterpret_cast<uint2*>(q + N) = *reinterpret_cast<const uint2*>(src + 48 + piece * 8);
+              *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(src + 128 + piece * 8);
+              *reinterpret_cast<uint2*>(q + N) = *reinterpret_cast<const uint2*>(src + 192 + piece * 8);
             }
           }
         }
@@ -278,21 +291,40 @@ __device__ __forceinline__ void rows_of_none(const RowsOut& out, int first, int 
   }
 }
 
-// The matrix's part of one k-block: 128 tile rows.  For SwiGLU n0 counts units and up rows stand F further down; `load` copies one
-// box [64 or 16 rows or k, 64] from (column, row, expert).
-template <bool W_MN, int EPI, class Load>
-__device__ __forceinline__ void load_matrix(uint8_t* sA, int k0, int n0, int F, int e, Load load) {
+// The matrix's part of one k-block: 128 tile rows, from row (unit) n0 of expert e on.  Loads is FewLoads or PairLoads: where a copy
+// is counted.
+struct FewLoads {
+  uint64_t* bar;
+  __device__ __forceinline__ void d3(void* to, const CUtensorMap* m, int a, int b, int c) const { tma_load_3d(to, m, bar, a, b, c); }
+  __device__ __forceinline__ void d4(void* to, const CUtensorMap* m, int a, int b, int c, int d) const { tma_load_4d(to, m, bar, a, b, c, d); }
+  __device__ __forceinline__ void d5(void* to, const CUtensorMap* m, int a, int b, int c, int d, int e) const {
+    tma_load_5d(to, m, bar, a, b, c, d, e);
+  }
+};
+struct PairLoads {
+  uint32_t bar;
+  __device__ __forceinline__ void d3(void* to, const CUtensorMap* m, int a, int b, int c) const { tma_load_3d_pair(to, m, bar, a, b, c); }
+  __device__ __forceinline__ void d4(void* to, const CUtensorMap* m, int a, int b, int c, int d) const {
+    tma_load_4d_pair(to, m, bar, a, b, c, d);
+  }
+  __device__ __forceinline__ void d5(void* to, const CUtensorMap* m, int a, int b, int c, int d, int e) const {
+    tma_load_5d_pair(to, m, bar, a, b, c, d, e);
+  }
+};
+template <bool W_MN, int EPI, class Loads>
+__device__ __forceinline__ void load_matrix(uint8_t* sA, const CUtensorMap* m, const RowsOut& out, int k0, int n0, int e, const Loads& loads) {
   if constexpr (EPI != kStore) {
+    if (out.width % 16 == 0) {
+      loads.d5(sA, m, k0, 0, 0, n0 / 16, e);
+    } else {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      load(sA + g * 4096, k0, n0 + g * 16, e);
-      load(sA + g * 4096 + 2048, k0, F + n0 + g * 16, e);
+      for (int g = 0; g < 4; ++g) loads.d4(sA + g * 4096, m, k0, n0 + g * 16, 0, e);
     }
   } else if constexpr (W_MN) {
 #pragma unroll
-    for (int j = 0; j < BM / 64; ++j) load(sA + j * 8192, n0 + j * 64, k0, e);
+    for (int j = 0; j < BM / 64; ++j) loads.d3(sA + j * 8192, m, n0 + j * 64, k0, e);
   } else {
-    load(sA, k0, n0, e);
+    loads.d3(sA, m, k0, n0, e);
   }
 }
 
@@ -331,7 +363,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 256);
+      mbar_init(&tempty[a], 512);      // the epilogue threads of both CTAs
     }
     fence_barrier_init();
   }
@@ -361,9 +393,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
           if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) { ok = false; break; }
           uint8_t* sA = smem + stage * STAGE_BYTES;
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
-          load_matrix<W_MN, EPI>(sA, kb * BK, n0, out.width, at.e, [&](uint8_t* to, int c0, int c1, int c2) {
-            tma_load_3d_pair(to, &tmW, lead_full[stage], c0, c1, c2);
-          });
+          load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, at.e, PairLoads{lead_full[stage]});
           tma_load_2d_pair(sA + A_BYTES, &tmX, lead_full[stage], kb * BK, r0 + static_cast<int>(rank) * half);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -399,24 +429,24 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
       }
     }
   } else {
-    const int q = warp & 3;      // TMEM lane quarter this warp may read
+    const int q = warp & 3;                // TMEM lane quarter this warp may read
+    const int part = (warp - 2) >> 2;      // two warps to a quarter, every other 32 columns each
     int it = 0, r0, live, col;
     bool ok = true;
     for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
-      const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2) + q * (UNIT / 8);
+      const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2);
       const int acc = it & 1;
       if (!mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait)) { ok = false; break; }
       tc_fence_after();
       const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
-      constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
-      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, q, epi + q * 64 * P, epi + 4 * 64 * P, r0, live,
-                         n0, [&] {
+      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, q, epi + part * kPartBytes<EPI>, 1 + part, r0,
+                         live, part * EPI_ROWS, 2 * EPI_ROWS, n0, [&] {
                            tc_fence_before();
                            remote_arrive(lead_tempty);
                          });
       ++it;
     }
-    rows_of_none<EPI>(out, edge[E], R, static_cast<int>(blockIdx.x) * 4 + q, static_cast<int>(gridDim.x) * 4);
+    rows_of_none<EPI>(out, edge[E], R, static_cast<int>(blockIdx.x) * 8 + warp - 2, static_cast<int>(gridDim.x) * 8);
   }
 
   if (*reinterpret_cast<volatile int*>(err) != 0) {
@@ -441,7 +471,7 @@ static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE, "staging rows");
 static_assert(2 * (FEW_SMEM + 1024) <= 233472, "two CTAs on an SM");
 
 template <bool W_MN, int EPI>
-__global__ void __launch_bounds__(ROW_THREADS, 2)
+__global__ void __launch_bounds__(FEW_THREADS, 2)
 grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
                    const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -522,8 +552,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) break;
         uint8_t* sA = smem + stage * FEW_STAGE;
         mbar_expect_tx(&full[stage], FEW_STAGE);
-        load_matrix<W_MN, EPI>(sA, kb * BK, n0, out.width, e,
-                               [&](uint8_t* to, int c0, int c1, int c2) { tma_load_3d(to, &tmW, &full[stage], c0, c1, c2); });
+        load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, e, FewLoads{&full[stage]});
         tma_load_2d(sA + A_BYTES, &tmX, &full[stage], kb * BK, r0);
         if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
       }
@@ -554,9 +583,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     const int q = warp & 3;
     if (num_kb > 0 && mbar_wait_warp(tfull, 0, err, kErrEpilogueTmemFullWait)) {
       tc_fence_after();
-      constexpr int P = EPI == kSwiglu ? WIDE_PITCH : PITCH;
-      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16), q, smem + q * 64 * P, smem + 4 * 64 * P, r0, live,
-                         n0 + q * (UNIT / 4), [] {});
+      rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16), q, smem, 1, r0, live, 0, EPI_ROWS, n0, [] {});
     }
     rows_of_none<EPI>(out, where[3], R, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x) * 4 + q,
                       static_cast<int>(gridDim.x * gridDim.y) * 4);
@@ -847,7 +874,7 @@ int launch_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, con
   if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(out.y) & 15) != 0) return -1;
   const bool few = R <= static_cast<int64_t>(FEW_AVERAGE) * E;
   CUtensorMap tw, tx;
-  int r = EPI != kStore ? make_tmap_3d(&tw, w, 2, E, 2 * static_cast<uint64_t>(N), K, 16, 64)
+  int r = EPI != kStore ? make_tmap_gate_up(&tw, w, E, N, K, N % 16 == 0 ? 4 : 1)
           : W_MN        ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64)
                         : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
   if (r) return r;
@@ -859,7 +886,7 @@ int launch_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, con
     constexpr int UNIT = EPI == kStore ? BM : BM / 2;
     auto kern = grouped_few_kernel<W_MN, EPI>;
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
-    return launch_pdl(kern, dim3((N + UNIT - 1) / UNIT, R / FEW_ROWS + groups), dim3(ROW_THREADS), FEW_SMEM, stream, tw, tx, offsets, out, R,
+    return launch_pdl(kern, dim3((N + UNIT - 1) / UNIT, R / FEW_ROWS + groups), dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, out, R,
                       E, K, err) == cudaSuccess
                ? 0
                : -21;
