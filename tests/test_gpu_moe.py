@@ -392,6 +392,28 @@ def test_expert_mlp_forms(kw):
     check_mlp(400, 6, 2, 256, 200, **kw)
 
 
+@pytest.mark.parametrize("T,E,k,D,F,capacity", [(1, 8, 2, 1024, 264, 0), (2, 1, 1, 8, 8, 0), (3, 40, 7, 520, 136, 0), (4, 300, 8, 264, 72, 0),
+                                                (4, 4, 2, 64, 64, 1), (2, 16, 16, 128, 32, 0)])
+@pytest.mark.parametrize("dtype,logit", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+def test_expert_mlp_of_a_few_tokens(T, E, k, D, F, capacity, dtype, logit):
+    """Without gradients up to four tokens take kernels of their own: no rounding but the result's."""
+    x, logits, wgu, wd = mlp_inputs(T, E, D, F, dtype=dtype)
+    logits = logits.to(logit)
+    if E > 4:
+        logits[0, :E - k + 1] = NINF          # the last choice of the first token is not made
+    for closed in (False, True):
+        if closed:
+            logits[T - 1] = NINF
+        with torch.no_grad():
+            out, aux = moe.expert_mlp(x, logits, wgu, wd, k, capacity)
+        want, waux = oracle.expert_mlp(*(t.cpu().double() for t in (x, logits, wgu, wd)), k, capacity)
+        assert out.dtype == dtype and aux.dtype == torch.float32
+        size = want.abs().max(1, keepdim=True).values
+        assert ((out.cpu().double() - want).abs() <= (U if dtype == torch.bfloat16 else 2.0 ** -16) * size).all()
+        assert abs(aux.item() - waux.item()) <= 2.0 ** -20 * waux.item()
+        assert not closed or (out[T - 1] == 0).all()
+
+
 def test_expert_mlp_gradient_of_aux_alone_and_no_tokens():
     x, logits, wgu, wd = mlp_inputs(32, 4, 64, 64)
     logits.requires_grad_()

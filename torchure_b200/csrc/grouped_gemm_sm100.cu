@@ -37,7 +37,7 @@ namespace {
 
 constexpr int BM = 128, BN = 256, BNH = 128, BK = 64, STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = BNH * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int BAR_BYTES = 256;
+constexpr int BAR_BYTES = 240;
 constexpr int EDGE_BYTES = (kMaxExperts + 1) * 4;
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -63,8 +63,9 @@ constexpr int ROW_SMEM = STAGES * STAGE_BYTES + ROW_EPI_BYTES + BAR_BYTES + EDGE
 
 constexpr int EPI_BUF = 4096;                   // 32 rows x 128 B
 constexpr int W_EPI_BYTES = 4 * 2 * EPI_BUF;
+constexpr int ORDERED = 256;                    // up to this many groups are taken in falling order of their rows
 constexpr int W_THREADS = 224;
-constexpr int W_SMEM = STAGES * STAGE_BYTES + W_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
+constexpr int W_SMEM = STAGES * STAGE_BYTES + W_EPI_BYTES + BAR_BYTES + EDGE_BYTES + ORDERED + 1024;
 static_assert(ROW_SMEM <= 232448 && W_SMEM <= 232448, "shared memory of one CTA");
 
 // edge[e] = first row of group e, edge[E] = end of the last: what `offsets` says, brought into [0, R] and made not to fall
@@ -86,29 +87,30 @@ __device__ __forceinline__ void load_edges(const int* offsets, int* edge, int E,
   }
 }
 
-// Where a unit lies; units only grow from call to call.
+// The units of group e are its tiles of 256 rows times `cols` tiles of the matrix, rows fastest; a pair takes every num_clusters-th.
+// (With the units of the last, not full wave cut into pieces by rows, 3.46 waves as 3.6, nothing got faster: the clocks give what the
+// idle SMs leave.)
 struct Place {
   const int* edge;
-  int E, e = 0, base = 0;      // base: first unit of group e
-  __device__ __forceinline__ int rows() const { return edge[e + 1] - edge[e]; }
-};
-
-// The units of group e are its tiles of 256 rows times `cols` tiles of the matrix, rows fastest.  False: past the last.
-__device__ __forceinline__ bool find_rows(Place& p, int unit, int cols, int& r0, int& live, int& col) {
-  while (p.e < p.E) {
-    const int tiles = (p.rows() + BN - 1) / BN;
-    if (unit - p.base < tiles * cols) {
-      const int at = unit - p.base;
-      r0 = p.edge[p.e] + at % tiles * BN;
-      live = min(BN, p.edge[p.e + 1] - r0);
-      col = at / tiles;
-      return true;
+  int E, cols;
+  int e = 0, base = 0;      // base: first unit of group e
+  // Where unit `unit` lies (it only grows from call to call): rows and column.  False: past the last.
+  __device__ __forceinline__ bool find(int unit, int& r0, int& live, int& col) {
+    while (e < E) {
+      const int tiles = (edge[e + 1] - edge[e] + BN - 1) / BN;
+      if (unit - base < tiles * cols) {
+        const int at = unit - base;
+        r0 = edge[e] + at % tiles * BN;
+        live = min(BN, edge[e + 1] - r0);
+        col = at / tiles;
+        return true;
+      }
+      base += tiles * cols;
+      ++e;
     }
-    p.base += tiles * cols;
-    ++p.e;
+    return false;
   }
-  return false;
-}
+};
 
 // Where the rows of a product go.  width: columns of the output (units for SwiGLU); gu, q: one of them or neither
 struct RowsOut {
@@ -376,7 +378,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  Place at{edge, E};
+  Place at{edge, E, cols};
 
   if (warp == 0) {
     if (elect_one()) {
@@ -386,7 +388,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
       uint32_t lead_full[STAGES];
 #pragma unroll
       for (int s = 0; s < STAGES; ++s) lead_full[s] = map_to_cta(&full[s], 0);
-      for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+      for (int n = cluster; ok && at.find(n, r0, live, col); n += num_clusters) {
         const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2);
         const int half = (live + 31) / 32 * 16;      // rows in each CTA's half of the instruction's columns
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -405,7 +407,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
       int stage = 0, it = 0, r0, live, col;
       uint32_t phase = 0;
       bool ok = true;
-      for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+      for (int n = cluster; ok && at.find(n, r0, live, col); n += num_clusters) {
         const uint32_t idesc = make_idesc_bf16(2 * BM, (live + 31) / 32 * 32, W_MN, false);
         const int acc = it & 1;
         if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, err, kErrMmaTmemEmptyWait)) { ok = false; break; }
@@ -433,7 +435,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     const int part = (warp - 2) >> 2;      // two warps to a quarter, every other 32 columns each
     int it = 0, r0, live, col;
     bool ok = true;
-    for (int unit = cluster; ok && find_rows(at, unit, cols, r0, live, col); unit += num_clusters) {
+    for (int n = cluster; ok && at.find(n, r0, live, col); n += num_clusters) {
       const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2);
       const int acc = it & 1;
       if (!mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait)) { ok = false; break; }
@@ -601,6 +603,19 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   }
 }
 
+// Which tile of dw unit n is: the groups in falling order of their rows, so that what a pair takes last is short.  Eight groups of 16384
+// rows, the largest five times the smallest: 51 instead of 57 us.
+struct Tiles {
+  const uint8_t* order;      // nullptr: as they come
+  int per, num_n;
+  __device__ __forceinline__ void at(int n, int& e, int& n0, int& k0) const {
+    const int t = n % per;
+    e = order ? order[n / per] : n / per;
+    n0 = t % num_n * 2 * BM;
+    k0 = t / num_n * BN;
+  }
+};
+
 // dw [E, N, K], OUT 0: bf16, 1: fp32
 template <int OUT>
 __global__ void __launch_bounds__(W_THREADS, 1)
@@ -621,12 +636,14 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * STAGES + 4);
   static_assert((4 * STAGES + 5) * 8 <= BAR_BYTES, "barriers");
   int* edge = reinterpret_cast<int*>(epi + W_EPI_BYTES + BAR_BYTES);
+  uint8_t* order = reinterpret_cast<uint8_t*>(edge + kMaxExperts + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cluster = static_cast<int>(blockIdx.x) >> 1, num_clusters = static_cast<int>(gridDim.x) >> 1;
-  const int num_n = (N + 2 * BM - 1) / (2 * BM), num_k = (K + BN - 1) / BN;
-  const int per = num_n * num_k, num_units = per * E;
+  const int num_n = (N + 2 * BM - 1) / (2 * BM), per = num_n * ((K + BN - 1) / BN), num_units = per * E;
+  const Tiles tiles{E <= ORDERED ? order : nullptr, per, num_n};
+  int e, n0, k0;
 
   load_edges(offsets, edge, E, R);
   if (threadIdx.x == 32) {
@@ -651,6 +668,16 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
     tc_fence_before();
   }
   __syncthreads();
+  for (int a = threadIdx.x; a < E && E <= ORDERED; a += W_THREADS) {
+    const int rows = edge[a + 1] - edge[a];
+    int before = 0;
+    for (int b = 0; b < E; ++b) {
+      const int other = edge[b + 1] - edge[b];
+      before += other > rows || (other == rows && b < a) ? 1 : 0;
+    }
+    order[before] = static_cast<uint8_t>(a);
+  }
+  __syncthreads();
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
@@ -663,10 +690,11 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
       uint32_t lead_full[STAGES];
 #pragma unroll
       for (int s = 0; s < STAGES; ++s) lead_full[s] = map_to_cta(&full[s], 0);
-      for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
-        const int e = unit / per, t = unit % per;
+      for (int n = cluster; n < num_units && ok; n += num_clusters) {
+        tiles.at(n, e, n0, k0);
         const int lo = edge[e], rows = edge[e + 1] - lo;
-        const int n0 = t % num_n * 2 * BM + static_cast<int>(rank) * BM, k0 = t / num_n * BN + static_cast<int>(rank) * BNH;
+        n0 += static_cast<int>(rank) * BM;
+        k0 += static_cast<int>(rank) * BNH;
         const int num_kb = (rows + BK - 1) / BK;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) { ok = false; break; }
@@ -692,13 +720,14 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = make_idesc_bf16(2 * BM, BN, true, true);
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
-        const int e = unit / per, rows = edge[e + 1] - edge[e];
+      for (int n = cluster; n < num_units && ok; n += num_clusters) {
+        tiles.at(n, e, n0, k0);
+        const int rows = edge[e + 1] - edge[e];
         if (rows == 0) continue;
+        constexpr uint32_t idesc = make_idesc_bf16(2 * BM, BN, true, true);
         const int acc = it & 1;
         if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, err, kErrMmaTmemEmptyWait)) { ok = false; break; }
         tc_fence_after();
@@ -726,8 +755,9 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
     int blocks = 0;                    // loaded so far, of all groups
     uint32_t tail_phase = 0, mended_phase = 0;      // a bit per stage
     bool ok = true;
-    for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
-      const int e = unit / per, rows = edge[e + 1] - edge[e];
+    for (int n = cluster; n < num_units && ok; n += num_clusters) {
+      tiles.at(n, e, n0, k0);
+      const int rows = edge[e + 1] - edge[e];
       blocks += (rows + BK - 1) / BK;
       if (rows % 16 == 0) continue;
       const int stage = (blocks - 1) % STAGES;
@@ -755,10 +785,10 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
     constexpr int COLS = OUT == 0 ? 64 : 32;      // columns per staged slab (128 B per row)
     int it = 0, slab = 0;
     bool ok = true;
-    for (int unit = cluster; unit < num_units && ok; unit += num_clusters) {
-      const int e = unit / per, t = unit % per;
+    for (int n = cluster; n < num_units && ok; n += num_clusters) {
+      tiles.at(n, e, n0, k0);
+      n0 += static_cast<int>(rank) * BM + q * 32;
       const bool some = edge[e + 1] > edge[e];
-      const int n0 = t % num_n * 2 * BM + static_cast<int>(rank) * BM + q * 32, k0 = t / num_n * BN;
       const int acc = it & 1;
       if (some) {
         ok = mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait);

@@ -50,6 +50,14 @@ int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, 
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,
                   int R, int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
 
+// ---- the whole feed-forward of a few tokens, without gradients (moe_token.cu) ---------------------------
+constexpr int kTokenTokens = 4, kTokenChoices = 32;      // at most
+int64_t token_scratch_bytes(int T, int k, int F);
+// out [T, D] (x's type) and aux [1] from logits [T, E] and x [T, D]; scratch: token_scratch_bytes, on 16 bytes
+int token_mlp(const void* logits, bool logits_bf16, int64_t ldl, const void* x, bool x_bf16, int64_t ldx, const __nv_bfloat16* w_gate_up,
+              const __nv_bfloat16* w_down, void* out, float* aux, void* scratch, int T, int E, int k, int capacity, int D, int F,
+              cudaStream_t stream);
+
 // ---- 8-bit activation checkpoints (act8.cu) --------------------------------------------------------------
 // Per row and block of 64 values: a = the largest magnitude, q = sign(x) floor(127 |x| / a + 1/2), scale = a / 127 (0 for a block of
 // zeros, NaN for one that holds a value that is not finite).  q [M, N], scales [M, ceil(N / 64)].

@@ -2,6 +2,7 @@
 // Python costs the host 40 - 90 us for a forward and a backward pass, more than most of these kernels run.  Outputs are allocated
 // here; in the poison mode (ops/debug.py) each is filled and remembered before its kernel runs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -10,6 +11,7 @@
 
 #include "bind_common.h"
 #include "moe_api.h"
+#include "pdl.h"
 
 namespace {
 
@@ -445,9 +447,41 @@ struct Mlp {
   Tensor gu, q, scales;      // what the backward pass reads: gate | up in bf16, or in 8 bits
 };
 
+// A pass without gradients of up to four tokens runs in the two kernels of moe_token.cu, which read an expert once for every token that
+// chose it, unless that is more than 80 MB: the general path reads it once.  Measured on B200, us, general path, token kernels: experts x
+// choices x width x units 8 x 2 x 1024 x 1536, one token 36, 17, four (75 MB) 30, 24; 64 x 4 x 1024 x 768, four (75 MB) 30, 26; 64 x 8 x
+// 2048 x 1024, one (100 MB) 38, 43, two 53, 57, four 71, 107.
+constexpr int64_t TOKEN_MAX = 4, TOKEN_BYTES = 80 << 20;
+// Up to this many rows the launches of the forward pass overlap (pdl.h): every kernel is short then.
+constexpr int64_t PDL_MAX_ROWS = 2048;
+
+bool runs_by_token(const Tensor& x, int64_t k, const Tensor& wgu, const Tensor& wd) {
+  return x.size(0) >= 1 && x.size(0) <= TOKEN_MAX && x.size(0) * k <= tb::kTokenChoices && x.stride(0) % 8 == 0 &&
+         x.size(0) * k * wd.size(1) * wd.size(2) * 6 <= TOKEN_BYTES &&
+         ((reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(wgu.data_ptr()) | reinterpret_cast<uintptr_t>(wd.data_ptr())) & 15) == 0;
+}
+
+// out, aux
+variable_list mlp_by_token(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, const Outputs& make) {
+  const int64_t T = x.size(0), D = x.size(1), E = wd.size(0), F = wd.size(2);
+  TORCH_CHECK_VALUE(E <= tb::kMaxExperts, "expert_mlp: 1 to ", tb::kMaxExperts, " experts, got ", E);
+  TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= tb::kMaxChoices, "expert_mlp: top_k of ", k, " among ", E, " experts (at most ", tb::kMaxChoices, ")");
+  TORCH_CHECK_VALUE(capacity >= 0 && capacity < (1ll << 31), "expert_mlp: capacity ", capacity);
+  const Tensor out = make("expert_mlp.out", {T, D}, x.options()), aux = make("expert_mlp.aux", {}, x.options().dtype(torch::kFloat32));
+  const Tensor scratch = empty({tb::token_scratch_bytes((int)T, (int)k, (int)F)}, x.options().dtype(torch::kUInt8));
+  const int rc = tb::token_mlp(logits.data_ptr(), bf16_or_f32(logits, "expert_mlp: logits"), logits.stride(0), x.data_ptr(),
+                               x.scalar_type() == torch::kBFloat16, x.stride(0), bf(wgu), bf(wd), out.data_ptr(), aux.data_ptr<float>(),
+                               scratch.data_ptr(), (int)T, (int)E, (int)k, (int)capacity, (int)D, (int)F, cur_stream());
+  TORCH_CHECK(rc == 0, "expert_mlp failed with code ", rc);
+  g_launches += 2;
+  return {out, aux};
+}
+
 Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool keep,
             const Outputs& make) {
   Mlp m;
+  const bool eager = at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;      // a graph keeps plain edges
+  tb::PdlScope overlap(eager && x.size(0) * k <= PDL_MAX_ROWS);
   m.r = do_route(logits, k, capacity, make);
   const Tensor xg = do_gather(x, m.r.rows, k, make);
   const int64_t R = xg.size(0), F = wd.size(2), E = wd.size(0), D = x.size(1);
@@ -563,7 +597,13 @@ variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& fi
   const bool keep = at::GradMode::is_enabled() &&
                     (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() || (pair && second->requires_grad()));
   if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, bits, poison);
-  Mlp m = mlp_fwd(x, logits, stack_of(first, second), matrices(wd), k, capacity, bits, false, Outputs{poison});
+  const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
+  if (runs_by_token(x, k, wgu, wdb)) {
+    const bool eager = at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;
+    tb::PdlScope overlap(eager);
+    return mlp_by_token(x, logits, wgu, wdb, k, capacity, Outputs{poison});
+  }
+  Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, bits, false, Outputs{poison});
   return {m.out, m.r.aux};
 }
 
