@@ -424,6 +424,10 @@ def test_expert_mlp_gradient_of_aux_alone_and_no_tokens():
     assert rel(logits.grad.cpu(), ref.grad) < 1e-5
     out, aux = moe.expert_mlp(x[:0], logits[:0], wgu.clone().requires_grad_(), wd, 2)
     assert out.shape == (0, 64) and aux.item() == 0
+    leaves = [t.detach().clone().requires_grad_() for t in (x[:0], logits[:0], wgu, wd)]
+    out, aux = moe.expert_mlp(*leaves, 2)
+    (out.sum() + aux).backward()
+    assert all(t.grad.shape == t.shape and t.grad.abs().sum() == 0 for t in leaves)
 
 
 def test_operators_on_another_stream():

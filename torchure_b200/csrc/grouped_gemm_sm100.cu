@@ -20,7 +20,10 @@
 // CTA's 64 units (act8.cu has the format), or not at all.
 //
 // Few rows per group: grouped_few_kernel, single CTAs on 128 tile rows and at most 64 group rows, two of them on an SM.  The matrices
-// are then all the traffic there is, and what counts is how evenly it is spread and how many copies are on their way.
+// are then all the traffic there is, and what counts is how evenly it is spread and how many copies are on their way.  There the
+// group's rows may be listed (places of token rows in expert order) and are gathered four to a copy (tile::gather4), which spares a
+// launch.  A copy of four rows costs about 72 cycles, so that tiles of many rows do better with the rows put in order first (the pair
+// kernels with listed rows took 270 us instead of 88 + 9.6).
 #include "act8.cuh"
 #include "cta_pair.cuh"
 #include "moe_api.h"
@@ -119,6 +122,17 @@ struct RowsOut {
   int8_t* q;             // [R, 2 width]
   float* scales;         // [R, 2 ceil(width / 64)]
   int width;
+};
+
+// Where the rows of x lie: row r is row list[r] / k of `count` rows; what the list calls none (-1) is row 0, whose results are not used.
+struct Rows {
+  const int* list;
+  FastDiv k;
+  int count;
+  __device__ __forceinline__ int at(int r, int end) const {
+    const int i = r < end ? list[r] : 0;
+    return min(static_cast<int>(k(static_cast<uint32_t>(max(i, 0)))), count - 1);
+  }
 };
 
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
@@ -472,10 +486,10 @@ constexpr int FEW_SMEM = FEW_STAGES * FEW_STAGE + BAR_BYTES + 1024;
 static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE, "staging rows");
 static_assert(2 * (FEW_SMEM + 1024) <= 233472, "two CTAs on an SM");
 
-template <bool W_MN, int EPI>
+template <bool W_MN, int EPI, bool LISTED>
 __global__ void __launch_bounds__(FEW_THREADS, 2)
 grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
-                   const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
+                   const __grid_constant__ Rows rows, const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + FEW_STAGES * FEW_STAGE);
@@ -546,7 +560,25 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   const int n0 = static_cast<int>(blockIdx.x) * UNIT;
   const int num_kb = live > 0 ? (K + BK - 1) / BK : 0;
 
-  if (warp == 0) {
+  if (LISTED && warp == 0) {
+    // all lanes: each has four of the rows
+    int stage = 0;
+    uint32_t phase = 0;
+    const int used = (live + 15) / 16 * 16;
+    int from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = num_kb > 0 ? rows.at(r0 + 4 * lane + i, r0 + live) : 0;
+    for (int kb = 0; kb < num_kb; ++kb) {
+      if (!mbar_wait_warp(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) break;
+      uint8_t* sA = smem + stage * FEW_STAGE;
+      if (lane == 0) {
+        mbar_expect_tx(&full[stage], A_BYTES + used * 128);
+        load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, e, FewLoads{&full[stage]});
+      }
+      if (4 * lane < used) tma_gather4(sA + A_BYTES + lane * 512, &tmX, &full[stage], kb * BK, from);
+      if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
@@ -897,32 +929,36 @@ namespace {
 // Up to this many rows per group, on average, the small tiles.
 constexpr int FEW_AVERAGE = 96;
 
+template <bool W_MN, int EPI, bool LISTED>
+int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Rows& rows, const int* offsets, const RowsOut& out, int R, int E, int K,
+               int* err, cudaStream_t stream) {
+  constexpr int UNIT = EPI == kStore ? BM : BM / 2;
+  auto kern = grouped_few_kernel<W_MN, EPI, LISTED>;
+  if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
+  // at most: every group with rows ends in a tile that is not full
+  const dim3 grid((out.width + UNIT - 1) / UNIT, R / FEW_ROWS + (E < R ? E : R));
+  return launch_pdl(kern, grid, dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, rows, out, R, E, K, err) == cudaSuccess ? 0 : -21;
+}
+
 template <bool W_MN, int EPI>
-int launch_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R, int E, int K,
-                int* err, int num_sms, cudaStream_t stream) {
+int launch_rows(const __nv_bfloat16* x, int64_t ldx, const Rows& rows, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R,
+                int E, int K, int* err, int num_sms, cudaStream_t stream) {
   const int N = out.width;
   if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(out.y) & 15) != 0) return -1;
   const bool few = R <= static_cast<int64_t>(FEW_AVERAGE) * E;
+  if (rows.list && !(few && EPI == kSwiglu)) return -2;
   CUtensorMap tw, tx;
   int r = EPI != kStore ? make_tmap_gate_up(&tw, w, E, N, K, N % 16 == 0 ? 4 : 1)
           : W_MN        ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64)
                         : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
   if (r) return r;
-  r = make_tmap_2d(&tx, x, 2, R, K, ldx, few ? FEW_ROWS : BNH, 64);
+  r = rows.list ? make_tmap_2d(&tx, x, 2, rows.count, K, ldx, 1, 64) : make_tmap_2d(&tx, x, 2, R, K, ldx, few ? FEW_ROWS : BNH, 64);
   if (r) return r - 100;
-  // at most: every group with rows ends in a tile that is not full
-  const int groups = E < R ? E : R;
-  if (few) {
-    constexpr int UNIT = EPI == kStore ? BM : BM / 2;
-    auto kern = grouped_few_kernel<W_MN, EPI>;
-    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
-    return launch_pdl(kern, dim3((N + UNIT - 1) / UNIT, R / FEW_ROWS + groups), dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, out, R,
-                      E, K, err) == cudaSuccess
-               ? 0
-               : -21;
-  }
+  if constexpr (EPI == kSwiglu)
+    if (rows.list) return launch_few<W_MN, EPI, true>(tw, tx, rows, offsets, out, R, E, K, err, stream);
+  if (few) return launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream);
   constexpr int UNIT = EPI == kStore ? 2 * BM : BM;
-  const int64_t units = (static_cast<int64_t>(R) / BN + groups) * ((N + UNIT - 1) / UNIT);
+  const int64_t units = (static_cast<int64_t>(R) / BN + (E < R ? E : R)) * ((N + UNIT - 1) / UNIT);
   return launch_pairs(grouped_rows_kernel<W_MN, EPI>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, out, R, E, K, err);
 }
 
@@ -933,16 +969,21 @@ int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bo
   RowsOut out{};
   out.y = y;
   out.width = N;
-  return w_t ? launch_rows<true, kStore>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream)
-             : launch_rows<false, kStore>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream);
+  const Rows rows{nullptr, FastDiv(1), 0};
+  return w_t ? launch_rows<true, kStore>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream)
+             : launch_rows<false, kStore>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);
 }
 
-int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, __nv_bfloat16* act, __nv_bfloat16* gu,
-                   int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms, cudaStream_t stream) {
+bool grouped_swiglu_listed(int R, int E) { return R <= 32 * static_cast<int64_t>(E); }
+
+int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
+                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms,
+                   cudaStream_t stream) {
   if (F % 8 != 0 || (gu && q) || ((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) return -1;
   RowsOut out{act, gu, q, scales, F};
-  return q ? launch_rows<false, kSwiglu8>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream)
-           : launch_rows<false, kSwiglu>(x, ldx, w, offsets, out, R, E, K, err, num_sms, stream);
+  const Rows rows{list, FastDiv(list ? k : 1), count};
+  return q ? launch_rows<false, kSwiglu8>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream)
+           : launch_rows<false, kSwiglu>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);
 }
 
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,

@@ -44,8 +44,12 @@ int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bo
                  int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
 // act [R, F] = silu(g) u of g | u = x W[e]^T, W [E, 2F, K] = gate rows over up rows.  Gate and up go to gu [R, 2F] in bf16, or to q
 // [R, 2F] and scales [R, 2 ceil(F / 64)] in 8 bits, or nowhere; rows of no expert: zeros.
-int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, __nv_bfloat16* act, __nv_bfloat16* gu,
-                   int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms, cudaStream_t stream);
+// list (nullptr: the R rows of x are in expert order): row r is row list[r] / k of the `count` rows of x, what `rows` of route_fwd says.
+// Only where grouped_swiglu_listed, and not with q.
+bool grouped_swiglu_listed(int R, int E);
+int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
+                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms,
+                   cudaStream_t stream);
 // dw[e] [N, K] = sum over the rows of e of dy[r]^T x[r], bf16 or fp32; zeros for an expert without rows
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,
                   int R, int E, int N, int K, int* err, int num_sms, cudaStream_t stream);

@@ -477,14 +477,20 @@ variable_list mlp_by_token(const Tensor& x, const Tensor& logits, const Tensor& 
   return {out, aux};
 }
 
+// Whether the gate / up product reads token rows where they lie: few rows per expert, bf16, on 16 bytes.  Others are put in expert order
+// first, rounded where they are fp32.
+bool rows_stay(const Tensor& x, int64_t R, int64_t E, bool in8) {
+  return tb::grouped_swiglu_listed((int)R, (int)E) && !in8 && x.scalar_type() == torch::kBFloat16 && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
+         (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0;
+}
+
 Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool keep,
             const Outputs& make) {
   Mlp m;
   const bool eager = at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;      // a graph keeps plain edges
   tb::PdlScope overlap(eager && x.size(0) * k <= PDL_MAX_ROWS);
   m.r = do_route(logits, k, capacity, make);
-  const Tensor xg = do_gather(x, m.r.rows, k, make);
-  const int64_t R = xg.size(0), F = wd.size(2), E = wd.size(0), D = x.size(1);
+  const int64_t R = x.size(0) * k, F = wd.size(2), E = wd.size(0), D = x.size(1);
   const Tensor act = make("expert_mlp.act", {R, F}, wgu.options());
   if (keep && bits == 16) m.gu = make("expert_mlp.gu", {R, 2 * F}, wgu.options());
   if (keep && bits == 8) {
@@ -492,7 +498,9 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
     m.scales = make("expert_mlp.scales", {R, 2 * blocks_of(F)}, wgu.options().dtype(torch::kFloat32));
   }
   if (R > 0) {
-    const int rc = tb::grouped_swiglu(bf(xg), D, bf(wgu), m.r.offsets.data_ptr<int>(), bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr,
+    const bool listed = rows_stay(x, R, E, m.q.defined());
+    const Tensor xg = listed ? x : do_gather(x, m.r.rows, k, make);
+    const int rc = tb::grouped_swiglu(bf(xg), xg.stride(0), listed ? m.r.rows.data_ptr<int>() : nullptr, (int)k, (int)x.size(0), bf(wgu), m.r.offsets.data_ptr<int>(), bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr,
                                       m.q.defined() ? m.q.data_ptr<int8_t>() : nullptr, m.q.defined() ? m.scales.data_ptr<float>() : nullptr,
                                       (int)R, (int)E, (int)F, (int)D, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
     TORCH_CHECK(rc == 0, "expert_mlp: gate / up product failed with code ", rc);
@@ -507,6 +515,9 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
 variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
                       const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Outputs& make) {
   const int64_t T = x.size(0), k = r.slots.size(1), R = T * k, E = logits.size(1), F = wd.size(2);
+  if (R == 0)
+    return {at::zeros_like(x), at::zeros_like(logits), at::zeros(wgu.sizes(), wgu.options().dtype(wtype)),
+            at::zeros(wd.sizes(), wd.options().dtype(wtype))};
   const Tensor dg = do_gather(dout, r.rows, k, make);
   const Tensor s = do_grouped(dg, wd, r.offsets, true, make);
   Tensor dgu = make("expert_mlp.dgu", {R, 2 * F}, wgu.options());
