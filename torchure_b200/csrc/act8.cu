@@ -106,7 +106,7 @@ __device__ __forceinline__ void keep8(uint4 raw, int left, int8_t* q, float* sca
   spread(raw, v);
   uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = k.inv != 0.f ? act_word(v[i], k.inv) : 0u;
+  for (int i = 0; i < 8; ++i) w[i] = act_word(v[i], k.inv);      // (of a block that is not finite anything: its scale is NaN)
   const uint2 u = make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
                              __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
   if (VEC) {
@@ -138,7 +138,7 @@ struct Unit {
 };
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 6)
+__global__ void __launch_bounds__(kThreads, 5)
 quantize8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t units, int N,
                  FastDiv nb) {
   pdl_wait();
@@ -146,16 +146,19 @@ quantize8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int8_t* __res
   constexpr int U = 4;
   for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 - (threadIdx.x >> 3) < units; u0 += gridDim.x * (U * kGroups)) {
     uint4 v[U];
+    int64_t to[U];
+    int left[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const Unit at(u0 + i * kGroups, units, nb, N);
       v[i] = load_raw<VEC>(x + at.row * ldx + at.c, at.left);
+      to[i] = at.row * N + at.c;
+      left[i] = at.left;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t u = u0 + i * kGroups;
-      const Unit at(u, units, nb, N);
-      keep8<VEC>(v[i], at.left, q + at.row * N + at.c, scales + u, u < units && (threadIdx.x & 7) == 0);
+      keep8<VEC>(v[i], left[i], q + to[i], scales + u, u < units && (threadIdx.x & 7) == 0);
     }
   }
 }
@@ -170,25 +173,28 @@ dequantize8_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale
   for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 < units; u0 += gridDim.x * (U * kGroups)) {
     uint2 raw[U];
     float scale[U];
+    int64_t to[U];
+    int left[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t u = u0 + i * kGroups;
       const Unit at(u, units, nb, N);
-      raw[i] = load_q<VEC>(q + at.row * N + at.c, at.left);
+      to[i] = at.row * N + at.c;
+      left[i] = at.left;
+      raw[i] = load_q<VEC>(q + to[i], at.left);
       scale[i] = u < units ? scales[u] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const Unit at(u0 + i * kGroups, units, nb, N);
       float v[8];
       read_q(raw[i], scale[i], v);
-      store8<VEC>(x + at.row * N + at.c, at.left, v);
+      store8<VEC>(x + to[i], left[i], v);
     }
   }
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 5)
+__global__ void __launch_bounds__(kThreads, 4)
 swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
                    float* __restrict__ scales, uint32_t units, int F, FastDiv nb) {
   pdl_wait();
@@ -196,26 +202,32 @@ swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bflo
   constexpr int U = 2;
   for (uint32_t u0 = blockIdx.x * (U * kGroups) + (threadIdx.x >> 3); u0 - (threadIdx.x >> 3) < units; u0 += gridDim.x * (U * kGroups)) {
     uint4 gate[U], up[U];
+    int64_t row[U];
+    int c[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const Unit at(u0 + i * kGroups, units, nb, F);
       gate[i] = load_raw<VEC>(gu + at.row * ldgu + at.c, at.left);
       up[i] = load_raw<VEC>(gu + at.row * ldgu + F + at.c, at.left);
+      row[i] = at.row;
+      c[i] = at.left > 0 ? at.c : F;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t u = u0 + i * kGroups;
-      const Unit at(u, units, nb, F);
+      const int left = F - c[i];
       float g[8], v[8], out[8];
       spread(gate[i], g);
       spread(up[i], v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) out[j] = g[j] * sigmoid(g[j]) * v[j];
-      store8<VEC>(act + at.row * F + at.c, at.left, out);
+      const int64_t at = row[i] * F + c[i];
+      store8<VEC>(act + at, left, out);
       const bool first = u < units && (threadIdx.x & 7) == 0;
-      float* scale = scales + at.row * 2 * static_cast<int>(nb.d) + at.b;
-      keep8<VEC>(gate[i], at.left, q + at.row * 2 * F + at.c, scale, first);
-      keep8<VEC>(up[i], at.left, q + at.row * 2 * F + F + at.c, scale + nb.d, first);
+      float* scale = scales + (u + row[i] * static_cast<int>(nb.d));
+      int8_t* to = q + (at + row[i] * F);
+      keep8<VEC>(gate[i], left, to, scale, first);
+      keep8<VEC>(up[i], left, to + F, scale + nb.d, first);
     }
   }
 }
@@ -241,27 +253,30 @@ swiglu8_bwd_kernel(const __nv_bfloat16* __restrict__ dact, int64_t ldd, const in
     uint2 gate[U], up[U];
     uint4 d[U];
     float sg[U], su[U];
+    int64_t to[U];
+    int left[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const Unit at(u0 + i * kGroups, units, nb, F);
-      const float* scale = scales + at.row * 2 * static_cast<int>(nb.d) + at.b;
-      const bool in = u0 + i * kGroups < units;
-      gate[i] = load_q<VEC>(q + at.row * 2 * F + at.c, at.left);
-      up[i] = load_q<VEC>(q + at.row * 2 * F + F + at.c, at.left);
-      sg[i] = in ? scale[0] : 0.f;
-      su[i] = in ? scale[nb.d] : 0.f;
+      const uint32_t u = u0 + i * kGroups;
+      const Unit at(u, units, nb, F);
+      const float* scale = scales + (u + at.row * static_cast<int>(nb.d));
+      to[i] = at.row * 2 * F + at.c;
+      left[i] = at.left;
+      gate[i] = load_q<VEC>(q + to[i], at.left);
+      up[i] = load_q<VEC>(q + to[i] + F, at.left);
+      sg[i] = u < units ? scale[0] : 0.f;
+      su[i] = u < units ? scale[nb.d] : 0.f;
       d[i] = load_raw<VEC>(dact + at.row * ldd + at.c, at.left);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const Unit at(u0 + i * kGroups, units, nb, F);
       float g[8], u[8], da[8], dg[8], du[8];
       read_q(gate[i], sg[i], g);
       read_q(up[i], su[i], u);
       spread(d[i], da);
       swiglu_grad(g, u, da, dg, du);
-      store8<VEC>(dgu + at.row * 2 * F + at.c, at.left, dg);
-      store8<VEC>(dgu + at.row * 2 * F + F + at.c, at.left, du);
+      store8<VEC>(dgu + to[i], left[i], dg);
+      store8<VEC>(dgu + to[i] + F, left[i], du);
     }
   }
 }

@@ -21,6 +21,7 @@ namespace {
 constexpr int kThreads = 1024;      // of the forward kernels: one CTA per SM, and its latencies have 32 warps to hide behind
 constexpr int kBwdThreads = 256;
 constexpr int kWarps = kThreads / 32;
+static_assert(kWarps == 32, "a lane per warp");
 constexpr int kMaxChunks = 148;
 
 __device__ __forceinline__ uint32_t to_key(float x) {
@@ -66,10 +67,11 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
   int* total = sm;                 // [E]
   int* before = sm + E;            // [E] in earlier CTAs
   int* first = sm + 2 * E;         // [E + 1] first row of each expert
-  int* cnt = sm + 3 * E + 1;       // [kWarps][E]
-  float* aux_part = reinterpret_cast<float*>(cnt + kWarps * E);      // [kWarps]
+  const int S = E | 1;             // an odd stride: the counts of an expert lie in different banks
+  int* cnt = sm + 3 * E + 1;       // [kWarps][S]
+  float* aux_part = reinterpret_cast<float*>(cnt + kWarps * S);      // [kWarps]
   for (int i = tid; i < 2 * E; i += kThreads) sm[i] = 0;
-  for (int i = tid; i < kWarps * E; i += kThreads) cnt[i] = 0;
+  for (int i = tid; i < kWarps * S; i += kThreads) cnt[i] = 0;
   __syncthreads();
   // this CTA's choices, a consecutive part for each warp: counted here, ranked below
   const int n_flat = a.T * a.k;
@@ -78,7 +80,7 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
   const int wlo = min(count, warp * part), whi = min(count, wlo + part);
   for (int i = wlo + lane; i < whi; i += 32) {
     const int e = codes[i];
-    if (e >= 0) atomicAdd(&cnt[warp * E + e], 1);
+    if (e >= 0) atomicAdd(&cnt[warp * S + e], 1);
   }
   // the counts of all CTAs: a thread has one expert and every `rows`-th CTA, its loads independent
   const int rows = max(1, kThreads / E);
@@ -111,14 +113,15 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
     }
     if (lane == 0) first[E] = run;
   }
-  for (int e = kThreads - 1 - tid; e < E; e += kThreads) {      // (from the last warp on: the first one is busy)
-    int run = before[e];
-#pragma unroll 8
-    for (int w = 0; w < kWarps; ++w) {
-      const int n = cnt[w * E + e];
-      cnt[w * E + e] = run;
-      run += n;
+  for (int e = kWarps - 1 - warp; e < E; e += kWarps) {      // (from the last warp on: the first one is busy); a lane per warp's count
+    const int n = cnt[lane * S + e];
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
     }
+    cnt[lane * S + e] = before[e] + sum - n;
   }
   __syncthreads();
   for (int i0 = wlo; i0 < whi; i0 += 32) {
@@ -127,9 +130,9 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     const int rank = __popc(same & ((1u << lane) - 1u));
     int place = 0;
-    if (e >= 0) place = cnt[warp * E + e] + rank;
+    if (e >= 0) place = cnt[warp * S + e] + rank;
     __syncwarp();
-    if (e >= 0 && rank == 0) cnt[warp * E + e] += __popc(same);
+    if (e >= 0 && rank == 0) cnt[warp * S + e] += __popc(same);
     __syncwarp();
     if (i < whi) {
       int row = -1;
@@ -159,7 +162,7 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
   }
 }
 
-constexpr int plan_smem_ints(int E) { return 3 * E + 1 + kWarps * E + kWarps; }
+constexpr int plan_smem_ints(int E) { return 3 * E + 1 + kWarps * (E | 1) + kWarps; }
 
 template <class T, int LANES, int VALS>
 __global__ void __launch_bounds__(kThreads)
@@ -174,7 +177,7 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
   float* psum = reinterpret_cast<float*>(sm + E);         // [E]
   int* codes = sm + 2 * E;                                // [T k] with one CTA
   int* rest = codes + (single ? a.T * a.k : 0);
-  float* part = reinterpret_cast<float*>(rest);           // [GROUPS][E]
+  float* part = reinterpret_cast<float*>(rest);           // [kWarps][E | 1]
   for (int e = tid; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
   float acc[VALS];
@@ -256,12 +259,14 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
 #pragma unroll
   for (int v = 0; v < VALS; ++v) {
     const int e = v * LANES + gl;
-    if (e < E) part[group * E + e] = acc[v];
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
+    if (lane < LANES && e < E) part[(tid >> 5) * (E | 1) + e] = acc[v];
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kThreads) {
-    float s = 0.f;
-    for (int g = 0; g < GROUPS; ++g) s += part[g * E + e];
+  for (int e = tid >> 5; e < E; e += kWarps) {      // a warp adds up the warps' sums of one expert
+    const float s = group_sum<32>(part[lane * (E | 1) + e], 0xffffffffu);
+    if (lane != 0) continue;
     if (single) {
       psum[e] = s;
     } else {
@@ -383,7 +388,7 @@ int vals_for(int E) {
 template <class T>
 int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t stream) {
   const int lanes = lanes_for(a.E), vals = vals_for(a.E);
-  const int plan = plan_smem_ints(a.E), sums = kThreads / lanes * a.E;
+  const int plan = plan_smem_ints(a.E), sums = kWarps * (a.E | 1);
   const int smem = 4 * (chunks == 1 ? 2 * a.E + a.T * a.k + (sums > plan ? sums : plan) : 2 * a.E + sums);
 #define CASE(L, V)                                                                                                            \
   if (lanes == L && vals == V) {                                                                                              \
