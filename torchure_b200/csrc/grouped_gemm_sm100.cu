@@ -458,7 +458,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
       rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, q, epi + part * kPartBytes<EPI>, 1 + part, r0,
                          live, part * EPI_ROWS, 2 * EPI_ROWS, n0, [&] {
                            tc_fence_before();
-                           remote_arrive(lead_tempty);
+                           pair_arrive(lead_tempty);      // (a release at cluster scope would wait for the rows sent to memory before)
                          });
       ++it;
     }
