@@ -561,17 +561,23 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   const int num_kb = live > 0 ? (K + BK - 1) / BK : 0;
 
   if (LISTED && warp == 0) {
-    // all lanes: each has four of the rows
+    // all lanes: each has four of the rows; the first matrix tiles are on their way before the list is looked at
     int stage = 0;
     uint32_t phase = 0;
-    const int used = (live + 15) / 16 * 16;
+    const int used = (live + 15) / 16 * 16, ahead = min(num_kb, FEW_STAGES);
+    if (lane == 0)
+      for (int kb = 0; kb < ahead; ++kb) {
+        mbar_expect_tx(&full[kb], A_BYTES + used * 128);
+        load_matrix<W_MN, EPI>(smem + kb * FEW_STAGE, &tmW, out, kb * BK, n0, e, FewLoads{&full[kb]});
+      }
+    __syncwarp();
     int from[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) from[i] = num_kb > 0 ? rows.at(r0 + 4 * lane + i, r0 + live) : 0;
     for (int kb = 0; kb < num_kb; ++kb) {
       if (!mbar_wait_warp(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) break;
       uint8_t* sA = smem + stage * FEW_STAGE;
-      if (lane == 0) {
+      if (lane == 0 && kb >= ahead) {
         mbar_expect_tx(&full[stage], A_BYTES + used * 128);
         load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, e, FewLoads{&full[stage]});
       }

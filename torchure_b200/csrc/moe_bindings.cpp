@@ -88,14 +88,12 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
     r.aux.zero_();
     return r;
   }
-  // offsets, counts and scratch of one allocation
-  const int64_t scratch = tb::route_scratch_ints((int)T, (int)E, (int)k);
-  Tensor ints = empty({2 * E + 1 + scratch}, i32);
-  r.offsets = ints.narrow(0, 0, E + 1);
-  r.counts = ints.narrow(0, E + 1, E);
+  r.offsets = empty({E + 1}, i32);
+  r.counts = empty({E}, i32);
+  const Tensor scratch = empty({tb::route_scratch_ints((int)T, (int)E, (int)k)}, i32);
   const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, r.weights.data_ptr<float>(),
                                r.experts.data_ptr<int>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), r.rows.data_ptr<int>(),
-                               r.counts.data_ptr<int>(), r.aux.data_ptr<float>(), ints.data_ptr<int>() + 2 * E + 1, cur_stream());
+                               r.counts.data_ptr<int>(), r.aux.data_ptr<float>(), scratch.data_ptr<int>(), cur_stream());
   g_launches += 1;
   TORCH_CHECK(rc == 0, "route failed with code ", rc);
   return r;
@@ -319,9 +317,16 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
 };
 
 variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
-  check_rows(logits, "route");
+  TORCH_CHECK_VALUE(logits.dim() == 2 && logits.is_floating_point(), "route: logits [tokens, experts] expected, got ", logits.scalar_type(),
+                    " ", logits.sizes());
   c10::cuda::CUDAGuard guard(logits.device());
-  return RouteNode::apply(logits, k, capacity, poison);
+  const bool as_is = logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16;
+  const Tensor rows = rows_of(as_is ? logits : logits.to(torch::kFloat32));
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    Routed r = do_route(rows, k, capacity, Outputs{poison});
+    return {r.weights, r.aux, r.experts, r.slots, r.offsets, r.rows, r.counts};
+  }
+  return RouteNode::apply(rows, k, capacity, poison);
 }
 
 struct DispatchNode : torch::autograd::Function<DispatchNode> {
@@ -411,6 +416,10 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, b
   TORCH_CHECK_VALUE(offsets.scalar_type() == torch::kInt32 && offsets.device() == x.device() && w.device() == x.device(),
                     "grouped_linear: int32 offsets and matrices on the GPU of the rows expected");
   c10::cuda::CUDAGuard guard(x.device());
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad())) {
+    const Tensor y = do_grouped(operand(x), matrices(w), offsets.contiguous(), false, Outputs{poison});
+    return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1));
+  }
   return GroupedNode::apply(x, w, offsets.contiguous(), poison);
 }
 
@@ -627,9 +636,9 @@ void register_moe(pybind11::module_& m) {
   m.def("grouped_linear", &grouped_linear);
   m.def("expert_mlp", &expert_mlp, "(out, aux)");
   m.def("quantize8", [](const Tensor& x) {
-    check_rows(x, "quantize8");
+    TORCH_CHECK_VALUE(x.dim() == 2, "quantize8: a matrix expected, got ", x.dim(), " dimensions");
     c10::cuda::CUDAGuard guard(x.device());
-    return do_quantize(x);
+    return do_quantize(rows_of(x));
   });
   m.def("dequantize8", [](const Tensor& q, const Tensor& s, bool poison) {
     TORCH_CHECK_VALUE(q.is_cuda(), "dequantize8: a tensor on the GPU expected");

@@ -41,20 +41,19 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
 
 def quantize8(x: torch.Tensor) -> Act8:
     """A bf16 matrix [rows, columns] (any row stride) in 8 bits."""
+    if ops.available() and x.is_cuda:
+        return Act8(*_C().quantize8(x))
     if x.dim() != 2:
         raise ValueError(f"quantize8: a matrix expected, got {x.dim()} dimensions")
-    x = _rows(x.detach(), "quantize8")
-    if not ops.available() or not x.is_cuda:
-        return Act8(*oracle.quantize8(x))
-    return Act8(*_C().quantize8(x))
+    return Act8(*oracle.quantize8(_rows(x.detach(), "quantize8")))
 
 
 def dequantize8(kept: Act8) -> torch.Tensor:
     """bf16 [rows, columns] of what ``quantize8`` kept."""
     values, scales = kept
-    if not ops.available() or not values.is_cuda:
-        return oracle.dequantize8(values, scales).bfloat16()
-    return _C().dequantize8(values, scales, debug.enabled())
+    if ops.available() and values.is_cuda:
+        return _C().dequantize8(values, scales, debug.enabled())
+    return oracle.dequantize8(values, scales).bfloat16()
 
 
 def swiglu_8bit(gu: torch.Tensor) -> torch.Tensor:

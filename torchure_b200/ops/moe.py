@@ -39,7 +39,12 @@ class Routing(NamedTuple):
 
 def _plain(*tensors: torch.Tensor) -> bool:
     """Whether the plain statements run: off the GPU, or with the kernels switched off."""
-    return not (ops.available() and all(t.is_cuda for t in tensors))
+    if not ops.available():
+        return True
+    for t in tensors:
+        if not t.is_cuda:
+            return True
+    return False
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -53,18 +58,16 @@ def route(logits: torch.Tensor, top_k: int, capacity: int = 0) -> Routing:
     expert whose logit is -inf is closed to the token: such a choice is not made (weight 0, no row), so a padding token can be kept
     out of every expert.  ``capacity``: rows an expert takes at most, the first in token order; 0: no limit.  ``aux_loss`` is
     E * sum_e (share of the choices, before the capacity, that went to e) * (mean probability of e)."""
+    if not _plain(logits):
+        return Routing(*_C().moe_route(logits, top_k, capacity, debug.enabled()))
     if logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError(f"route: logits [tokens, experts] expected, got {logits.dtype} {tuple(logits.shape)}")
     if not 1 <= top_k <= logits.shape[1]:
         raise ValueError(f"route: top_k of {top_k} among {logits.shape[1]} experts")
     if capacity < 0:
         raise ValueError(f"route: capacity {capacity}")
-    if _plain(logits):
-        weights, experts, slots, offsets, rows, counts, aux = oracle.route(logits, top_k, capacity)
-        return Routing(weights, aux, experts, slots, offsets, rows, counts)
-    if logits.dtype not in (BF16, torch.float32):
-        logits = logits.float()
-    return Routing(*_C().moe_route(_rows(logits), top_k, capacity, debug.enabled()))
+    weights, experts, slots, offsets, rows, counts, aux = oracle.route(logits, top_k, capacity)
+    return Routing(weights, aux, experts, slots, offsets, rows, counts)
 
 
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
