@@ -544,3 +544,27 @@ def test_refusals_on_the_gpu():
         act8.dequantize8(act8.Act8(kept.values, kept.scales[:2]))
     with pytest.raises(ValueError, match="int32"):
         moe.combine(rand(8, 64), moe.route(logits, 2)._replace(slots=torch.zeros(4, 2, dtype=torch.int64, device="cuda")))
+
+
+def test_expert_mlp_backward_on_another_stream_under_allocation_pressure():
+    """The backward pass of many rows uses a second stream inside; to the caller and the allocator there is one.  Blocks that are freed
+    right behind it and overwritten on the caller's stream must not reach what the pass still reads or has returned."""
+    x, logits, wgu, wd = (t.requires_grad_() for t in mlp_inputs(2500, 8, 256, 256))
+    dout = rand(2500, 256, seed=9)
+
+    def once():
+        out, aux = moe.expert_mlp(x, logits, wgu, wd, 2)
+        return torch.autograd.grad((out, aux), (x, logits, wgu, wd), (dout, torch.ones_like(aux)))
+
+    want = [g.clone() for g in once()]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            for _ in range(6):
+                got = once()
+                junk = [torch.full((5000, n), float("nan"), device="cuda", dtype=torch.bfloat16) for n in (256, 512, 256, 1024)]
+                for g, w in zip(got, want):
+                    assert torch.equal(g, w)
+                del got, junk

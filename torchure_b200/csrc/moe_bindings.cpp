@@ -2,6 +2,7 @@
 // Python costs the host 40 - 90 us for a forward and a backward pass, more than most of these kernels run.  Outputs are allocated
 // here; in the poison mode (ops/debug.py) each is filled and remembered before its kernel runs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -100,7 +101,7 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
 }
 
 Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& experts, const Tensor& counts, const OptTensor& dweights,
-                    const OptTensor& daux, const Outputs& make) {
+                    const OptTensor& daux, const Outputs& make, Tensor dl = {}) {
   check_rows(logits, "route_bwd");
   const bool b16 = bf16_or_f32(logits, "route_bwd: logits");
   const int64_t T = logits.size(0), E = logits.size(1), k = weights.size(1);
@@ -110,7 +111,7 @@ Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& e
   TORCH_CHECK(!has(dweights) || (dweights->scalar_type() == torch::kFloat32 && dweights->is_contiguous() && dweights->numel() == T * k),
               "route_bwd: dweights");
   TORCH_CHECK(!has(daux) || (daux->is_cuda() && daux->scalar_type() == torch::kFloat32 && daux->numel() == 1), "route_bwd: daux");
-  Tensor dl = make("route_bwd", {T, E}, logits.options());
+  if (!dl.defined()) dl = make("route_bwd", {T, E}, logits.options());
   if (T == 0) return dl;
   const int rc = tb::route_bwd(logits.data_ptr(), b16, logits.stride(0), weights.data_ptr<float>(), experts.data_ptr<int>(),
                                counts.data_ptr<int>(), has(dweights) ? dweights->data_ptr<float>() : nullptr,
@@ -120,18 +121,19 @@ Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& e
   return dl;
 }
 
-Tensor do_gather(const Tensor& x, const Tensor& rows, int64_t k, const Outputs& make) {
+// The last argument of the next three: an output that the caller has allocated (on the stream that owns it), or an empty tensor
+Tensor do_gather(const Tensor& x, const Tensor& rows, int64_t k, const Outputs& make, Tensor out = {}) {
   check_rows(x, "dispatch");
   const bool b16 = bf16_or_f32(x, "dispatch");
   const int64_t T = x.size(0), D = x.size(1), R = rows.numel();
   check_ints(rows, R, x, "dispatch: rows");
-  Tensor out = make("dispatch", {R, D}, x.options().dtype(torch::kBFloat16));
+  if (!out.defined()) out = make("dispatch", {R, D}, x.options().dtype(torch::kBFloat16));
   tb::rows_gather(x.data_ptr(), b16, x.stride(0), rows.data_ptr<int>(), bfm(out), (int)T, (int)k, (int)R, (int)D, cur_stream());
   g_launches += 1;
   return out;
 }
 
-Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots, at::ScalarType type, const Outputs& make) {
+Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots, at::ScalarType type, const Outputs& make, Tensor out = {}) {
   check_rows(y, "combine");
   check_bf16(y, "combine");
   TORCH_CHECK(y.is_contiguous(), "combine: contiguous rows expected");
@@ -141,7 +143,7 @@ Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots
                                 weights->device() == y.device()), "combine: weights must be contiguous fp32 [tokens, choices]");
   TORCH_CHECK(type == torch::kBFloat16 || type == torch::kFloat32, "combine: bf16 or fp32 output");
   TORCH_CHECK_VALUE(T * ((D + 7) / 8) < (1ll << 31), "combine: 2^34 values and more are not supported");
-  Tensor out = make("combine", {T, D}, y.options().dtype(type));
+  if (!out.defined()) out = make("combine", {T, D}, y.options().dtype(type));
   tb::rows_combine(bf(y), has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
                    type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream());
   g_launches += 1;
@@ -463,6 +465,8 @@ struct Mlp {
 constexpr int64_t TOKEN_MAX = 4, TOKEN_BYTES = 80 << 20;
 // Up to this many rows the launches of the forward pass overlap (pdl.h): every kernel is short then.
 constexpr int64_t PDL_MAX_ROWS = 2048;
+// From here on the backward pass runs gather, sum and the router's gradient beside the products.
+constexpr int64_t BESIDE_MIN_ROWS = 4096;
 
 bool runs_by_token(const Tensor& x, int64_t k, const Tensor& wgu, const Tensor& wd) {
   return x.size(0) >= 1 && x.size(0) <= TOKEN_MAX && x.size(0) * k <= tb::kTokenChoices && x.stride(0) % 8 == 0 &&
@@ -520,6 +524,45 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
   return m;
 }
 
+// A second stream for row kernels that have nothing to do with the product on the current one: they are bound by memory and fit beside its
+// CTAs.  What they read and write is allocated on the current stream before and outlives this object, and the current stream waits for the
+// second one before it goes: to the allocator there is one stream.
+class Beside {
+ public:
+  explicit Beside(bool on) : main_(at::cuda::getCurrentCUDAStream()), on_(on) {
+    if (on_) side_ = at::cuda::getStreamFromPool(false, main_.device_index());
+  }
+  // runs f on the second stream, behind everything on the current one so far
+  template <class F>
+  void run(F f) {
+    if (!on_) return f();
+    from_.record(main_);
+    from_.block(*side_);
+    c10::cuda::CUDAStreamGuard guard(*side_);
+    f();
+    busy_ = true;
+  }
+  // the current stream waits for what was run
+  void join() {
+    if (!busy_) return;
+    back_.record(*side_);
+    back_.block(main_);
+    busy_ = false;
+  }
+  ~Beside() {
+    try {
+      join();
+    } catch (...) {      // (behind an error that is on its way already)
+    }
+  }
+
+ private:
+  c10::cuda::CUDAStream main_;
+  c10::optional<c10::cuda::CUDAStream> side_;
+  at::cuda::CUDAEvent from_, back_;
+  bool on_, busy_ = false;
+};
+
 // dx, dlogits, dw_gate_up, dw_down
 variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
                       const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Outputs& make) {
@@ -527,22 +570,29 @@ variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x
   if (R == 0)
     return {at::zeros_like(x), at::zeros_like(logits), at::zeros(wgu.sizes(), wgu.options().dtype(wtype)),
             at::zeros(wd.sizes(), wd.options().dtype(wtype))};
-  const Tensor dg = do_gather(dout, r.rows, k, make);
-  const Tensor s = do_grouped(dg, wd, r.offsets, true, make);
   Tensor dgu = make("expert_mlp.dgu", {R, 2 * F}, wgu.options());
   Tensor act_w = make("expert_mlp.act", {R, F}, wgu.options());
   Tensor dweights = make("expert_mlp.dweights", {T, k}, r.weights.options());
+  const Tensor xg = make("expert_mlp.xg", {R, x.size(1)}, wgu.options()), dx = make("expert_mlp.dx", {T, x.size(1)}, x.options());
+  const Tensor dl = make("expert_mlp.dlogits", {T, E}, logits.options());
+  Tensor dg, s, dxg, dwd, dwgu;
+  Beside beside(R >= BESIDE_MIN_ROWS);
+  dg = do_gather(dout, r.rows, k, make);
+  beside.run([&] { do_gather(x, r.rows, k, make, xg); });
+  s = do_grouped(dg, wd, r.offsets, true, make);
   const bool kept16 = gu.defined();
   tb::expert_swiglu_bwd(bf(s), kept16 ? bf(gu) : nullptr, kept16 ? nullptr : q.data_ptr<int8_t>(), kept16 ? nullptr : scales.data_ptr<float>(),
                         r.weights.data_ptr<float>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), bfm(dgu), bfm(act_w),
                         dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream());
   g_launches += 1;
-  const Tensor dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
-  const Tensor dxg = do_grouped(dgu, wgu, r.offsets, true, make);
-  const Tensor dx = do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make);
-  const Tensor xg = do_gather(x, r.rows, k, make);
-  const Tensor dwgu = do_wgrad(dgu, xg, r.offsets, wtype, make);
-  const Tensor dl = do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make);
+  dxg = do_grouped(dgu, wgu, r.offsets, true, make);
+  beside.run([&] {
+    do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make, dx);
+    do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make, dl);
+  });
+  dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
+  beside.join();
+  dwgu = do_wgrad(dgu, xg, r.offsets, wtype, make);
   return {dx, dl, dwgu, dwd};
 }
 
