@@ -65,9 +65,9 @@ constexpr int FEW_THREADS = 192;
 constexpr int ROW_SMEM = STAGES * STAGE_BYTES + ROW_EPI_BYTES + BAR_BYTES + EDGE_BYTES + 1024;
 
 constexpr int EPI_BUF = 4096;                   // 32 rows x 128 B
-constexpr int W_EPI_BYTES = 4 * 2 * EPI_BUF;
+constexpr int W_EPI_BYTES = 8 * EPI_BUF;        // a buffer for each of eight epilogue warps
 constexpr int ORDERED = 256;                    // up to this many groups are taken in falling order of their rows
-constexpr int W_THREADS = 224;
+constexpr int W_THREADS = 352;                  // warp 0 copies, 1 issues the products, 2 - 9 are the epilogue, 10 zeroes rows
 constexpr int W_SMEM = STAGES * STAGE_BYTES + W_EPI_BYTES + BAR_BYTES + EDGE_BYTES + ORDERED + 1024;
 static_assert(ROW_SMEM <= 232448 && W_SMEM <= 232448, "shared memory of one CTA");
 
@@ -696,7 +696,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 256);
+      mbar_init(&tempty[a], 512);
     }
     fence_barrier_init();
   }
@@ -788,7 +788,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
         ++it;
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == 10) {
     // zeros into the rows of the next group in a last block
     int blocks = 0;                    // loaded so far, of all groups
     uint32_t tail_phase = 0, mended_phase = 0;      // a bit per stage
@@ -818,10 +818,10 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
       __syncwarp();
     }
   } else {
-    const int q = warp & 3;
-    uint8_t* buf0 = epi + q * 2 * EPI_BUF;
-    constexpr int COLS = OUT == 0 ? 64 : 32;      // columns per staged slab (128 B per row)
-    int it = 0, slab = 0;
+    const int q = warp & 3, part = (warp - 2) >> 2;      // two warps to a quarter of the lanes, every other slab each
+    uint8_t* buf = epi + (warp - 2) * EPI_BUF;
+    constexpr int COLS = OUT == 0 ? 64 : 32;             // columns per staged slab (128 B per row)
+    int it = 0;
     bool ok = true;
     for (int n = cluster; n < num_units && ok; n += num_clusters) {
       tiles.at(n, e, n0, k0);
@@ -837,25 +837,23 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
       const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
 #pragma unroll 1
-      for (int c = 0; c < BN / COLS; ++c) {
+      for (int c = part; c < BN / COLS; c += 2) {
         uint32_t v[64];
         __syncwarp();
         if (some) {
           tmem_ld_32x32b_x32(t_row + c * COLS, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
           if (OUT == 0) tmem_ld_32x32b_x32(t_row + c * COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
           tmem_ld_wait();
-          if (c == BN / COLS - 1) {
+          if (c == BN / COLS - 2 + part) {
             tc_fence_before();
-            remote_arrive(lead_tempty);
+            pair_arrive(lead_tempty);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 64; ++i) v[i] = 0u;
         }
         if (n0 < N && k0 + c * COLS < K) {
-          uint8_t* buf = buf0 + (slab & 1) * EPI_BUF;
-          ++slab;
-          if (lane == 0) tma_wait_group_read<1>();      // the store that last used this buffer has read it
+          if (lane == 0) tma_wait_group_read<0>();      // the store that last used this buffer has read it
           __syncwarp();
           uint8_t* row = buf + lane * 128;
 #pragma unroll
