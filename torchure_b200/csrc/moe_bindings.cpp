@@ -169,6 +169,12 @@ std::tuple<Tensor, Tensor> do_combine_bwd(const Tensor& dout, const Tensor& y, c
   return {dy, dw};
 }
 
+// Up to this many rows launches overlap (pdl.h): every kernel is short then.  (A graph keeps plain edges.)
+constexpr int64_t PDL_MAX_ROWS = 2048;
+bool launches_overlap(int64_t rows) {
+  return rows <= PDL_MAX_ROWS && at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;
+}
+
 void check_group(const Tensor& x, const Tensor& offsets, const char* what) {
   check_rows(x, what);
   check_bf16(x, what);
@@ -188,6 +194,7 @@ Tensor do_grouped(const Tensor& x, const Tensor& w, const Tensor& offsets, bool 
   Tensor y = make("grouped_linear", {R, N}, x.options());
   if (R == 0 || N == 0) return y;
   if (K == 0) return y.zero_();
+  tb::PdlScope overlap(launches_overlap(R));
   const int rc = tb::grouped_gemm(bf(x), x.stride(0), bf(w), w_t, offsets.data_ptr<int>(), bfm(y), (int)R, (int)w.size(0), (int)N, (int)K,
                                   attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
   g_launches += 1;
@@ -204,6 +211,7 @@ Tensor do_wgrad(const Tensor& dy, const Tensor& x, const Tensor& offsets, at::Sc
   Tensor dw = make("grouped_wgrad", {E, N, K}, x.options().dtype(type));
   if (N == 0 || K == 0) return dw;
   if (R == 0) return dw.zero_();
+  tb::PdlScope overlap(launches_overlap(R));
   const int rc = tb::grouped_wgrad(bf(dy), dy.stride(0), bf(x), x.stride(0), offsets.data_ptr<int>(), dw.data_ptr(), type == torch::kBFloat16,
                                    (int)R, (int)E, (int)N, (int)K, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
   g_launches += 1;
@@ -463,8 +471,6 @@ struct Mlp {
 // choices x width x units 8 x 2 x 1024 x 1536, one token 36, 17, four (75 MB) 30, 24; 64 x 4 x 1024 x 768, four (75 MB) 30, 26; 64 x 8 x
 // 2048 x 1024, one (100 MB) 38, 43, two 53, 57, four 71, 107.
 constexpr int64_t TOKEN_MAX = 4, TOKEN_BYTES = 80 << 20;
-// Up to this many rows the launches of the forward pass overlap (pdl.h): every kernel is short then.
-constexpr int64_t PDL_MAX_ROWS = 2048;
 // From here on the backward pass runs gather, sum and the router's gradient beside the products.
 constexpr int64_t BESIDE_MIN_ROWS = 4096;
 
@@ -500,8 +506,7 @@ bool rows_stay(const Tensor& x, int64_t R, int64_t E, bool in8) {
 Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool keep,
             const Outputs& make) {
   Mlp m;
-  const bool eager = at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;      // a graph keeps plain edges
-  tb::PdlScope overlap(eager && x.size(0) * k <= PDL_MAX_ROWS);
+  tb::PdlScope overlap(launches_overlap(x.size(0) * k));
   m.r = do_route(logits, k, capacity, make);
   const int64_t R = x.size(0) * k, F = wd.size(2), E = wd.size(0), D = x.size(1);
   const Tensor act = make("expert_mlp.act", {R, F}, wgu.options());
@@ -669,8 +674,7 @@ variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& fi
   if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, bits, poison);
   const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
   if (runs_by_token(x, k, wgu, wdb)) {
-    const bool eager = at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None;
-    tb::PdlScope overlap(eager);
+    tb::PdlScope overlap(launches_overlap(0));
     return mlp_by_token(x, logits, wgu, wdb, k, capacity, Outputs{poison});
   }
   Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, bits, false, Outputs{poison});

@@ -7,7 +7,8 @@
 // with share_e = choices made for e / (T k).
 //
 // A token belongs to a group of LANES threads (the power of two that holds E, 32 at most, VALS logits each), which finds one choice
-// per round with two warp reductions: the largest key (floats as ordered integers), then the lowest index that has it.  Rows are
+// per round with two warp reductions: the largest key (floats as ordered integers), then the lowest index that has it (bf16 keys carry
+// their index: one reduction).  Up to four logits of a lane are sorted once, so that a round looks at its first only.  Rows are
 // numbered by a counting sort that keeps the order of the choices inside an expert: every CTA counts the choices of a run of
 // consecutive tokens; the second kernel adds up the counts before its own run and ranks its choices.  No float atomics: the sums of p
 // are added in a fixed order.  Few tokens take one launch of one CTA.
@@ -84,12 +85,15 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
   }
   // the counts of all CTAs: a thread has one expert and every `rows`-th CTA, its loads independent
   const int rows = max(1, kThreads / E);
+  const bool last = c == chunks - 1;
+  float p_sum = 0.f;               // (the last CTA) of its expert's probabilities, over every `rows`-th CTA
   if (tid < rows * E) {
     const int e = tid % E;
     int all = 0, mine = 0;
 #pragma unroll 8
     for (int i = tid / E; i < chunks; i += rows) {
       const int v = all_hist[i * E + e];
+      if (last) p_sum += all_psum[i * E + e];
       all += v;
       mine += i < c ? v : 0;
     }
@@ -144,14 +148,12 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
     }
   }
   for (int r = first[E] + c * kThreads + tid; r < n_flat; r += chunks * kThreads) a.rows[r] = -1;
-  if (c == chunks - 1) {
+  if (last) {
     for (int e = tid; e <= E; e += kThreads) {
       a.offsets[e] = first[e];
       if (e < E) a.counts[e] = total[e];
     }
-    float s = 0.f;
-#pragma unroll 4
-    for (int i = tid; i < chunks * E; i += kThreads) s += static_cast<float>(total[i % E]) * all_psum[i];
+    float s = tid < rows * E ? static_cast<float>(total[tid % E]) * p_sum : 0.f;
     s = group_sum<32>(s, 0xffffffffu);
     if (lane == 0) aux_part[warp] = s;
     __syncthreads();
@@ -184,53 +186,84 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
 #pragma unroll
   for (int v = 0; v < VALS; ++v) acc[v] = 0.f;
   const int t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
+  float next[VALS];      // the logits of the token after the one that is worked on
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) next[v] = t < t1 && v * LANES + gl < E ? load_logit(logits + t * a.ld + v * LANES + gl) : -INFINITY;
+  };
+  fetch(t0 + group);
   for (int t = t0 + group; t < t1; t += GROUPS) {
-    const T* row = logits + t * a.ld;
     float x[VALS];
     uint32_t key[VALS];
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {
-      const int e = v * LANES + gl;
-      x[v] = e < E ? load_logit(row + e) : -INFINITY;
-      key[v] = e < E ? to_key(x[v]) : 0u;
+      x[v] = next[v];
+      key[v] = v * LANES + gl < E ? to_key(x[v]) : 0u;
     }
+    fetch(t + GROUPS);
     uint32_t my_key = 0;
     int my_e = 0;
-    float top = 0.f;
-    if constexpr (sizeof(T) == 2) {      // 16 bits of key and, falling, 16 of index: one reduction finds both
+    if constexpr (sizeof(T) == 2) {      // 16 bits of key and, falling, 16 of index
 #pragma unroll
       for (int v = 0; v < VALS; ++v) key[v] = key[v] ? (key[v] & 0xffff0000u) | (0xffffu - (v * LANES + gl)) : 0u;
-      for (int j = 0; j < a.k; ++j) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
-        best = __reduce_max_sync(mask, best);
-#pragma unroll
-        for (int v = 0; v < VALS; ++v)
-          if (key[v] == best) key[v] = 0;
-        const uint32_t whole = best | 0xffffu;      // the key of a bf16 value, its low bits as to_key leaves them
-        const uint32_t value = (best >> 31) ? best & 0xffff0000u : whole;
-        if (j == 0) top = from_key(value);
-        if (gl == j) { my_key = value; my_e = 0xffff - static_cast<int>(best & 0xffffu); }
-      }
-    } else {
-      for (int j = 0; j < a.k; ++j) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int v = 0; v < VALS; ++v) best = max(best, key[v]);
-        best = __reduce_max_sync(mask, best);
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int v = VALS - 1; v >= 0; --v)
-          if (key[v] == best) at = v * LANES + gl;
-        at = __reduce_min_sync(mask, at);
-#pragma unroll
-        for (int v = 0; v < VALS; ++v)
-          if (at == v * LANES + gl) key[v] = 0;
-        if (j == 0) top = from_key(best);
-        if (gl == j) { my_key = best; my_e = at; }
-      }
     }
+    int index[VALS];
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) index[v] = v * LANES + gl;
+    if constexpr (VALS <= 4) {           // falling keys; equal ones stay in the order of their indices
+#pragma unroll
+      for (int i = 1; i < VALS; ++i)
+#pragma unroll
+        for (int v = VALS - 1; v >= i; --v) {
+          const bool swap = key[v] > key[v - 1];
+          const uint32_t lo = swap ? key[v - 1] : key[v], hi = swap ? key[v] : key[v - 1];
+          const int ilo = swap ? index[v - 1] : index[v], ihi = swap ? index[v] : index[v - 1];
+          key[v] = lo;
+          key[v - 1] = hi;
+          index[v] = ilo;
+          index[v - 1] = ihi;
+        }
+    }
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = key[0];
+      if constexpr (VALS > 4) {
+#pragma unroll
+        for (int v = 1; v < VALS; ++v) best = max(best, key[v]);
+      }
+      best = __reduce_max_sync(mask, best);
+      int at = 0x7fffffff;
+      if constexpr (sizeof(T) == 4) {
+        if constexpr (VALS <= 4) {
+          if (key[0] == best) at = index[0];
+        } else {
+#pragma unroll
+          for (int v = VALS - 1; v >= 0; --v)
+            if (key[v] == best) at = index[v];
+        }
+        at = __reduce_min_sync(mask, at);
+      } else {
+        at = 0xffff - static_cast<int>(best & 0xffffu);
+      }
+      if constexpr (VALS <= 4) {
+        if (index[0] == at) {
+#pragma unroll
+          for (int v = 0; v + 1 < VALS; ++v) {
+            key[v] = key[v + 1];
+            index[v] = index[v + 1];
+          }
+          key[VALS - 1] = 0;
+          index[VALS - 1] = -1;
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VALS; ++v)
+          if (index[v] == at) key[v] = 0;
+      }
+      if (gl == j) { my_key = best; my_e = at; }
+    }
+    // the key of a bf16 value: its low bits as to_key leaves them
+    if constexpr (sizeof(T) == 2) my_key = (my_key >> 31) ? my_key & 0xffff0000u : my_key | 0xffffu;
+    const float top = from_key(__shfl_sync(mask, my_key, 0, LANES));
     const bool made = gl < a.k && my_key != kKeyMinusInf;
     const float ex = made ? expf(from_key(my_key) - top) : 0.f;
     const float sum = group_sum<LANES>(ex, mask);
