@@ -50,10 +50,13 @@ constexpr uint32_t TMEM_COLS = 512;
 //   kStore    128 columns in bf16
 //   kSwiglu   64 units: activation | gate | up in bf16
 //   kSwiglu8  64 units: activation in bf16 | gate | up in 8 bits
-enum { kStore = 0, kSwiglu = 1, kSwiglu8 = 2 };
+//   kStore32  128 columns in fp32 (a few rows' products that are added up afterwards)
+enum { kStore = 0, kSwiglu = 1, kSwiglu8 = 2, kStore32 = 3 };
+template <int EPI>
+constexpr bool kGateUp = EPI == kSwiglu || EPI == kSwiglu8;      // the matrix is gate over up
 constexpr int EPI_ROWS = 32;
 template <int EPI>
-constexpr int kPitch = EPI == kSwiglu ? 400 : 272;
+constexpr int kPitch = EPI == kStore32 ? 528 : EPI == kSwiglu ? 400 : 272;
 // kSwiglu8, for the four warps: their largest magnitudes, and the reciprocals
 constexpr int MAX_BYTES = 4 * 2 * EPI_ROWS * 2, INV_BYTES = 2 * EPI_ROWS * 4;
 template <int EPI>
@@ -117,11 +120,12 @@ struct Place {
 
 // Where the rows of a product go.  width: columns of the output (units for SwiGLU); gu, q: one of them or neither
 struct RowsOut {
-  __nv_bfloat16* y;      // the product, or the activation
+  __nv_bfloat16* y;      // the product, or the activation; kStore32: nullptr
   __nv_bfloat16* gu;     // [R, 2 width]
   int8_t* q;             // [R, 2 width]
   float* scales;         // [R, 2 ceil(width / 64)]
   int width;
+  float* y32;            // kStore32: the product
 };
 
 // Where the rows of x lie: row r is row list[r] / k of `count` rows; what the list calls none (-1) is row 0, whose results are not used.
@@ -163,7 +167,29 @@ __device__ __forceinline__ void rows_epilogue(const RowsOut& out, uint32_t t_row
     tmem_ld_16x256b_x4(t_row + c + (16u << 16), u);
     tmem_ld_wait();
     if (c + step >= live) release();
-    if constexpr (EPI == kStore) {
+    if constexpr (EPI == kStore32) {
+      named_bar_sync(bar, 128);      // the rows staged before have been read
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {      // sixteen lanes of the accumulator in v, sixteen in u, eight apart
+          const uint32_t* from = h < 2 ? v : u;
+          uint8_t* to = buf + (8 * j + 2 * (lane & 3)) * P + (q4 * 32 + 8 * h + (lane >> 2)) * 4;
+          *reinterpret_cast<uint32_t*>(to) = from[4 * j + 2 * (h & 1)];
+          *reinterpret_cast<uint32_t*>(to + P) = from[4 * j + 2 * (h & 1) + 1];
+        }
+      named_bar_sync(bar, 128);
+      const int n = n0 + lane * 4;
+      if (n < N) {
+        float* dst = out.y32 + static_cast<int64_t>(r0 + c) * N + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * 4 + q4;
+          if (c + row < live)
+            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * N) = *reinterpret_cast<const uint4*>(buf + row * P + lane * 16);
+        }
+      }
+    } else if constexpr (EPI == kStore) {
       uint32_t w[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -296,6 +322,10 @@ __device__ __forceinline__ void rows_of_none(const RowsOut& out, int first, int 
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int r = first + w; r < R; r += warps) {
     const int64_t row = r;
+    if (EPI == kStore32) {
+      for (int n = lane * 4; n < N; n += 128) *reinterpret_cast<uint4*>(out.y32 + row * N + n) = zero;
+      continue;
+    }
     for (int n = lane * 8; n < N; n += 256) *reinterpret_cast<uint4*>(out.y + row * N + n) = zero;
     if (EPI == kSwiglu && out.gu)
       for (int n = lane * 8; n < 2 * N; n += 256) *reinterpret_cast<uint4*>(out.gu + row * 2 * N + n) = zero;
@@ -329,7 +359,7 @@ struct PairLoads {
 };
 template <bool W_MN, int EPI, class Loads>
 __device__ __forceinline__ void load_matrix(uint8_t* sA, const CUtensorMap* m, const RowsOut& out, int k0, int n0, int e, const Loads& loads) {
-  if constexpr (EPI != kStore) {
+  if constexpr (kGateUp<EPI>) {
     if (out.width % 16 == 0) {
       loads.d5(sA, m, k0, 0, 0, n0 / 16, e);
     } else {
@@ -349,7 +379,7 @@ template <bool W_MN, int EPI>
 __global__ void __launch_bounds__(ROW_THREADS, 1)
 grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
                     const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
-  constexpr int UNIT = EPI == kStore ? 2 * BM : BM;      // output columns of a tile
+  constexpr int UNIT = kGateUp<EPI> ? BM : 2 * BM;      // output columns of a tile
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -483,7 +513,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 // an upper bound of the groups' tiles of rows).  The operand stages hold the epilogue's staging rows once the products are done.
 constexpr int FEW_ROWS = 64, FEW_STAGES = 4, FEW_STAGE = A_BYTES + FEW_ROWS * BK * 2;
 constexpr int FEW_SMEM = FEW_STAGES * FEW_STAGE + BAR_BYTES + 1024;
-static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE, "staging rows");
+static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE && kPartBytes<kStore32> <= FEW_STAGES * FEW_STAGE, "staging rows");
 static_assert(2 * (FEW_SMEM + 1024) <= 233472, "two CTAs on an SM");
 
 template <bool W_MN, int EPI, bool LISTED>
@@ -556,7 +586,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int e = where[0], r0 = where[1], live = where[2];
-  constexpr int UNIT = EPI == kStore ? BM : BM / 2;
+  constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
   const int n0 = static_cast<int>(blockIdx.x) * UNIT;
   const int num_kb = live > 0 ? (K + BK - 1) / BK : 0;
 
@@ -936,7 +966,7 @@ constexpr int FEW_AVERAGE = 96;
 template <bool W_MN, int EPI, bool LISTED>
 int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Rows& rows, const int* offsets, const RowsOut& out, int R, int E, int K,
                int* err, cudaStream_t stream) {
-  constexpr int UNIT = EPI == kStore ? BM : BM / 2;
+  constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
   auto kern = grouped_few_kernel<W_MN, EPI, LISTED>;
   if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
   // at most: every group with rows ends in a tile that is not full
@@ -948,22 +978,27 @@ template <bool W_MN, int EPI>
 int launch_rows(const __nv_bfloat16* x, int64_t ldx, const Rows& rows, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R,
                 int E, int K, int* err, int num_sms, cudaStream_t stream) {
   const int N = out.width;
-  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || (reinterpret_cast<uintptr_t>(out.y) & 15) != 0) return -1;
+  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || ((reinterpret_cast<uintptr_t>(out.y) | reinterpret_cast<uintptr_t>(out.y32)) & 15) != 0)
+    return -1;
   const bool few = R <= static_cast<int64_t>(FEW_AVERAGE) * E;
   if (rows.list && !(few && EPI == kSwiglu)) return -2;
   CUtensorMap tw, tx;
-  int r = EPI != kStore ? make_tmap_gate_up(&tw, w, E, N, K, N % 16 == 0 ? 4 : 1)
-          : W_MN        ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64)
-                        : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
+  int r = kGateUp<EPI> ? make_tmap_gate_up(&tw, w, E, N, K, N % 16 == 0 ? 4 : 1)
+          : W_MN       ? make_tmap_3d(&tw, w, 2, E, K, N, 64, 64)
+                       : make_tmap_3d(&tw, w, 2, E, N, K, BM, 64);
   if (r) return r;
   r = rows.list ? make_tmap_2d(&tx, x, 2, rows.count, K, ldx, 1, 64) : make_tmap_2d(&tx, x, 2, R, K, ldx, few ? FEW_ROWS : BNH, 64);
   if (r) return r - 100;
   if constexpr (EPI == kSwiglu)
     if (rows.list) return launch_few<W_MN, EPI, true>(tw, tx, rows, offsets, out, R, E, K, err, stream);
-  if (few) return launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream);
-  constexpr int UNIT = EPI == kStore ? 2 * BM : BM;
-  const int64_t units = (static_cast<int64_t>(R) / BN + (E < R ? E : R)) * ((N + UNIT - 1) / UNIT);
-  return launch_pairs(grouped_rows_kernel<W_MN, EPI>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, out, R, E, K, err);
+  if constexpr (EPI == kStore32) {
+    return few ? launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream) : -2;
+  } else {
+    if (few) return launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream);
+    constexpr int UNIT = kGateUp<EPI> ? BM : 2 * BM;
+    const int64_t units = (static_cast<int64_t>(R) / BN + (E < R ? E : R)) * ((N + UNIT - 1) / UNIT);
+    return launch_pairs(grouped_rows_kernel<W_MN, EPI>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, out, R, E, K, err);
+  }
 }
 
 }  // namespace
@@ -978,13 +1013,23 @@ int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bo
              : launch_rows<false, kStore>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);
 }
 
+bool grouped_gemm_few(int R, int E) { return R <= static_cast<int64_t>(FEW_AVERAGE) * E; }
+
+int grouped_gemm_f32(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, float* y, int R, int E, int N, int K,
+                     int* err, int num_sms, cudaStream_t stream) {
+  RowsOut out{};
+  out.y32 = y;
+  out.width = N;
+  return launch_rows<false, kStore32>(x, ldx, Rows{nullptr, FastDiv(1), 0}, w, offsets, out, R, E, K, err, num_sms, stream);
+}
+
 bool grouped_swiglu_listed(int R, int E) { return R <= 32 * static_cast<int64_t>(E); }
 
 int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
                    __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms,
                    cudaStream_t stream) {
   if (F % 8 != 0 || (gu && q) || ((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) return -1;
-  RowsOut out{act, gu, q, scales, F};
+  RowsOut out{act, gu, q, scales, F, nullptr};
   const Rows rows{list, FastDiv(list ? k : 1), count};
   return q ? launch_rows<false, kSwiglu8>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream)
            : launch_rows<false, kSwiglu>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);

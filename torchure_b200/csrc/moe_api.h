@@ -32,7 +32,7 @@ int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, c
 void rows_gather(const void* x, bool x_bf16, int64_t ldx, const int* rows, __nv_bfloat16* out, int T, int k, int R, int D,
                  cudaStream_t stream);
 // out[t] = sum_j weights[t, j] y[slots[t, j]] (weights nullptr: 1), fp32 sums in the order of the choices
-void rows_combine(const __nv_bfloat16* y, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
+void rows_combine(const void* y, bool y_bf16, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
                   cudaStream_t stream);
 // dy[slots[t, j]] = bf16(weights[t, j] dout[t]), zeros in rows of no choice; dweights[t, j] = <y[slot], dout[t]>, 0 without a slot
 void rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_bfloat16* y, const float* weights, const int* slots,
@@ -42,6 +42,11 @@ void rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_b
 // y[r] = x[r] W[e(r)]^T (w_t false, W [E, N, K]) or x[r] W[e(r)] (w_t true, W [E, K, N]); rows of no expert: zeros.  x [R, K].
 int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
                  int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
+// The same with w_t false and y in fp32, for few rows per expert only (grouped_gemm_few): y is added up over a token's choices afterwards,
+// and costs next to nothing there.
+bool grouped_gemm_few(int R, int E);
+int grouped_gemm_f32(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, float* y, int R, int E, int N, int K,
+                     int* err, int num_sms, cudaStream_t stream);
 // act [R, F] = silu(g) u of g | u = x W[e]^T, W [E, 2F, K] = gate rows over up rows.  Gate and up go to gu [R, 2F] in bf16, or to q
 // [R, 2F] and scales [R, 2 ceil(F / 64)] in 8 bits, or nowhere; rows of no expert: zeros.
 // list (nullptr: the R rows of x are in expert order): row r is row list[r] / k of the `count` rows of x, what `rows` of route_fwd says.

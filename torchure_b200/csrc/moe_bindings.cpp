@@ -135,7 +135,7 @@ Tensor do_gather(const Tensor& x, const Tensor& rows, int64_t k, const Outputs& 
 
 Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots, at::ScalarType type, const Outputs& make, Tensor out = {}) {
   check_rows(y, "combine");
-  check_bf16(y, "combine");
+  const bool y16 = bf16_or_f32(y, "combine");
   TORCH_CHECK(y.is_contiguous(), "combine: contiguous rows expected");
   const int64_t T = slots.size(0), k = slots.size(1), R = y.size(0), D = y.size(1);
   check_ints(slots, T * k, y, "combine: slots");
@@ -144,7 +144,7 @@ Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots
   TORCH_CHECK(type == torch::kBFloat16 || type == torch::kFloat32, "combine: bf16 or fp32 output");
   TORCH_CHECK_VALUE(T * ((D + 7) / 8) < (1ll << 31), "combine: 2^34 values and more are not supported");
   if (!out.defined()) out = make("combine", {T, D}, y.options().dtype(type));
-  tb::rows_combine(bf(y), has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
+  tb::rows_combine(y.data_ptr(), y16, has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
                    type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream());
   g_launches += 1;
   return out;
@@ -379,6 +379,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
 };
 
 Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, const Tensor& offsets, bool f32, bool poison) {
+  check_bf16(y, "combine");
   c10::cuda::CUDAGuard guard(y.device());
   TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ", y.sizes());
   check_ints(offsets, offsets.numel(), y, "combine: offsets");
@@ -524,7 +525,16 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
     TORCH_CHECK(rc == 0, "expert_mlp: gate / up product failed with code ", rc);
     g_launches += 1;
   }
-  const Tensor y = do_grouped(act, wd, m.r.offsets, false, make);
+  Tensor y;
+  if (R > 0 && tb::grouped_gemm_few((int)R, (int)E)) {
+    y = make("expert_mlp.y", {R, D}, wgu.options().dtype(torch::kFloat32));
+    const int rc = tb::grouped_gemm_f32(bf(act), F, bf(wd), m.r.offsets.data_ptr<int>(), y.data_ptr<float>(), (int)R, (int)E, (int)D, (int)F,
+                                        attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+    TORCH_CHECK(rc == 0, "expert_mlp: down product failed with code ", rc);
+    g_launches += 1;
+  } else {
+    y = do_grouped(act, wd, m.r.offsets, false, make);
+  }
   m.out = do_combine(y, m.r.weights, m.r.slots, x.scalar_type(), make);
   return m;
 }

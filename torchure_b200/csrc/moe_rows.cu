@@ -21,16 +21,51 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// 8 bf16 values as they lie, `left` of them inside the row
-template <bool VEC>
-__device__ __forceinline__ uint4 load_raw(const __nv_bfloat16* p, int left) {
-  if (VEC) return *reinterpret_cast<const uint4*>(p);
-  uint32_t u[4] = {0, 0, 0, 0};
+// 8 values as they lie in memory, `left` of them inside the row, zeros behind
+template <class T>
+struct Packed;
+template <>
+struct Packed<__nv_bfloat16> {
+  uint4 raw;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int left) {
+    if (VEC) {
+      raw = left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+      return;
+    }
+    uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < left) u[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
-  return make_uint4(u[0], u[1], u[2], u[3]);
-}
+    for (int i = 0; i < 8; ++i)
+      if (i < left) u[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+    raw = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  __device__ __forceinline__ void add(float w, float (&sum)[8]) const {
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      sum[2 * n] = fmaf(w, __uint_as_float(u[n] << 16), sum[2 * n]);
+      sum[2 * n + 1] = fmaf(w, __uint_as_float(u[n] & 0xffff0000u), sum[2 * n + 1]);
+    }
+  }
+};
+template <>
+struct Packed<float> {
+  float v[8];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* p, int left) {
+    if (VEC && left > 0) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ void add(float w, float (&sum)[8]) const {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) sum[n] = fmaf(w, v[n], sum[n]);
+  }
+};
 
 // 8 values from column c of a row of D
 template <bool VEC>
@@ -110,10 +145,10 @@ rows_gather_kernel(const X* __restrict__ x, int64_t ldx, const int* __restrict__
 }
 
 // One thread per 8 columns of a token.  chunks: of 8 columns in a row.
-template <class O, bool VEC>
+template <class Y, class O, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-rows_combine_kernel(const __nv_bfloat16* __restrict__ y, const float* __restrict__ weights, const int* __restrict__ slots,
-                    O* __restrict__ out, int64_t total, int k, int R, int D, FastDiv chunks) {
+rows_combine_kernel(const Y* __restrict__ y, const float* __restrict__ weights, const int* __restrict__ slots, O* __restrict__ out,
+                    int64_t total, int k, int R, int D, FastDiv chunks) {
   pdl_wait();
   pdl_launch_dependents();
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -122,24 +157,17 @@ rows_combine_kernel(const __nv_bfloat16* __restrict__ y, const float* __restrict
     const int64_t i0 = static_cast<int64_t>(t) * k;
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < k; j0 += 4) {
-      uint4 raw[4];
+      Packed<Y> raw[4];
       float w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = j0 + j < k ? slots[i0 + j0 + j] : -1;
         const bool in = r >= 0 && r < R;
         w[j] = in ? (weights ? weights[i0 + j0 + j] : 1.f) : 0.f;
-        raw[j] = in ? load_raw<VEC>(y + static_cast<int64_t>(r) * D + c, D - c) : make_uint4(0, 0, 0, 0);
+        raw[j].template load<VEC>(y + static_cast<int64_t>(in ? r : 0) * D + c, in ? D - c : 0);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          sum[2 * n] = fmaf(w[j], __uint_as_float(u[n] << 16), sum[2 * n]);
-          sum[2 * n + 1] = fmaf(w[j], __uint_as_float(u[n] & 0xffff0000u), sum[2 * n + 1]);
-        }
-      }
+      for (int j = 0; j < 4; ++j) raw[j].add(w[j], sum);
     }
     store8<VEC>(out + static_cast<int64_t>(t) * D, c, D, sum);
   }
@@ -203,17 +231,21 @@ void rows_gather(const void* x, bool x_bf16, int64_t ldx, const int* rows, __nv_
 #undef TB_GATHER
 }
 
-void rows_combine(const __nv_bfloat16* y, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
+void rows_combine(const void* y, bool y_bf16, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
                   cudaStream_t stream) {
   if (T <= 0 || D <= 0) return;
   const int chunks = (D + 7) / 8;
   const int64_t total = static_cast<int64_t>(T) * chunks, need = (total + kThreads - 1) / kThreads;
   const dim3 grid(static_cast<int>(need < 148 * 16 ? need : 148 * 16)), block(kThreads);
   const bool vec = whole(y, D, D) && whole(out, D, D);
-#define TB_COMBINE(O, V) \
-  launch_pdl(rows_combine_kernel<O, V>, grid, block, 0, stream, y, weights, slots, static_cast<O*>(out), total, k, R, D, FastDiv(chunks))
-  if (out_bf16) { if (vec) TB_COMBINE(__nv_bfloat16, true); else TB_COMBINE(__nv_bfloat16, false); }
-  else { if (vec) TB_COMBINE(float, true); else TB_COMBINE(float, false); }
+#define TB_COMBINE(Y, O, V)                                                                                                                  \
+  launch_pdl(rows_combine_kernel<Y, O, V>, grid, block, 0, stream, static_cast<const Y*>(y), weights, slots, static_cast<O*>(out), total, k, \
+             R, D, FastDiv(chunks))
+#define TB_COMBINE_OF(Y)                                                                                                 \
+  if (out_bf16) { if (vec) TB_COMBINE(Y, __nv_bfloat16, true); else TB_COMBINE(Y, __nv_bfloat16, false); }               \
+  else { if (vec) TB_COMBINE(Y, float, true); else TB_COMBINE(Y, float, false); }
+  if (y_bf16) { TB_COMBINE_OF(__nv_bfloat16) } else { TB_COMBINE_OF(float) }
+#undef TB_COMBINE_OF
 #undef TB_COMBINE
 }
 
