@@ -568,3 +568,58 @@ def test_expert_mlp_backward_on_another_stream_under_allocation_pressure():
                 for g, w in zip(got, want):
                     assert torch.equal(g, w)
                 del got, junk
+
+
+def test_offsets_beyond_31_bits():
+    """Matrices of more than 2^31 elements: the last rows are those of a small call."""
+    R, K, N = 1_100_000, 64, 2048
+    x, w = rand(R, K, seed=1), rand(3, N, K, seed=2)
+    edges = [0, 500_000, 1_099_000, R]
+    y = moe.grouped_linear(x, w, torch.tensor(edges, dtype=torch.int32, device="cuda"))
+    tail = moe.grouped_linear(x[-1000:], w[2:], torch.tensor([0, 1000], dtype=torch.int32, device="cuda"))
+    assert y.numel() > 2 ** 31 and torch.equal(y[-1000:], tail)
+    act = act8.swiglu_8bit(y)
+    assert torch.equal(act[-1000:], act8.swiglu_8bit(tail))
+    kept = act8.quantize8(y)
+    small = act8.quantize8(tail)
+    assert torch.equal(kept.values[-1000:], small.values) and torch.equal(kept.scales[-1000:], small.scales)
+    assert torch.equal(act8.dequantize8(kept)[-1000:], act8.dequantize8(small))
+    r = moe.route(torch.randn(R, 2, device="cuda", generator=gen(3)), 1)
+    rows = moe.dispatch(y, r)
+    out = moe.combine(rows, r)          # one choice of weight 1: what went in comes out
+    assert torch.equal(out[-1000:], y[-1000:]) and torch.equal(out[:1000], y[:1000])
+
+
+def test_gradients_against_differences():
+    """The operators' own gradients against differences of their own outputs along random directions, where a step is large against
+    the rounding: grouped products are linear, so that a step of any size gives the slope."""
+    offsets = torch.tensor([0, 300, 300, 1000], dtype=torch.int32, device="cuda")
+    x, w, dy = rand(1000, 256, seed=1), rand(3, 128, 256, seed=2), rand(1000, 128, seed=3)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(moe.grouped_linear(xl, wl, offsets), (xl, wl), dy)
+    loss = lambda a, b: (moe.grouped_linear(a, b, offsets).double() * dy.double()).sum().item()
+    vx, vw = rand(1000, 256, seed=4), rand(3, 128, 256, seed=5)
+    for slope, g, v, scale in ((loss(vx, w), gx, vx, (vx.double() @ w[0].double().t()).norm()),
+                               (loss(x, vw), gw, vw, (x.double() @ vw[0].double().t()).norm())):
+        want = (g.double() * v.double()).sum().item()
+        assert abs(slope - want) <= 4 * RMS * scale.item() * dy.double().norm().item() / 10
+    logits = torch.randn(300, 12, device="cuda", generator=gen(6)).requires_grad_()
+    dw = torch.randn(300, 3, device="cuda", generator=gen(7))
+    r = moe.route(logits, 3)
+    g, = torch.autograd.grad((r.weights, r.aux_loss), (logits,), (dw, torch.tensor(2.0, device="cuda")))
+    v = torch.randn(300, 12, device="cuda", generator=gen(8))
+    h = 2.0 ** -8           # smaller than the gaps between chosen and unchosen logits of the rows compared below
+
+    def value(t):
+        q = moe.route(t, 3)
+        return q, (q.weights.double() * dw.double()).sum(1)
+
+    (qp, up), (qm, down) = value(logits.detach() + h * v), value(logits.detach() - h * v)
+    same = ((qp.experts == r.experts) & (qm.experts == r.experts)).all(1)
+    aux = 2.0 * (qp.aux_loss.double() - qm.aux_loss.double()) / (2 * h)
+    slope = ((up - down) / (2 * h))[same].sum().item() + (aux.item() if same.all() else 0.0)
+    only = torch.autograd.grad(moe.route(logits, 3).weights, (logits,), dw)[0]
+    want = (only.double() * v.double())[same].sum().item()
+    # second-order term h^2 / 6 of functions bounded by |dw| with |v| of a few, and 2^-22 / h from the weights' rounding, over 900 terms
+    assert same.sum() > 200 and abs(slope - (aux.item() if same.all() else 0.0) - want) <= 900 * (h * h * 4 + 2.0 ** -22 / h)
+    assert torch.isfinite(g).all()
