@@ -3,7 +3,8 @@
     python -m benchmarks.profile_case <case> [--iters N]
 
 Cases: gemm_fwd, gemm_dgrad, gemm_wgrad, gemm_small, gemm_swiglu, gemm_swiglu_bwd, gemm_ce, attn_fwd, attn_bwd (single pass), attn_bwd_split, attn_prep, rmsnorm, rmsnorm_bwd, qknorm_rope,
-qknorm_rope_bwd, qknorm_rope_bwd_acc, swiglu, swiglu_bwd, ce, adamw.  Each case builds inputs
+qknorm_rope_bwd, qknorm_rope_bwd_acc, swiglu, swiglu_bwd, ce, adamw, moe_train, moe_few, moe_token (all kernels of a pass of the
+experts' feed-forward), route, swiglu8, store8.  Each case builds inputs
 larger than the 126 MB L2 but well under a few GB, launches the kernel `iters` times (default 4) and prints the
 CUDA-event time of the last launch with the achieved FLOP/s or bytes/s, so the same command serves a plain timing run
 and an `ncu -k regex:<kernel> -s 2 -c 1` capture.
@@ -147,6 +148,40 @@ def main(argv=None) -> None:
         sh = torch.empty(n, dtype=torch.bfloat16, device=dev)
         fn = lambda: multi_tensor.adamw_step([p], [g], [m], [v], [sh], 1e-3, 0.9, 0.95, 1e-8, 0.1, 3)
         bytes_ = n * (16 + 14)
+    elif args.case in ("moe_train", "moe_few", "moe_token"):
+        from torchure_b200.ops import moe
+
+        T, E, k, units = {"moe_train": (M, 8, 2, 1536), "moe_few": (61, 16, 4, 768), "moe_token": (1, 8, 2, 1536)}[args.case]
+        x, dout = (torch.randn(T, D, device=dev).bfloat16() for _ in range(2))
+        logits = (torch.randn(T, E, device=dev) + 0.3 * torch.randn(E, device=dev)).bfloat16()
+        wgu, wd = torch.randn(E, 2 * units, D, device=dev).bfloat16() / 32, torch.randn(E, D, units, device=dev).bfloat16() / 32
+        leaves = [t.requires_grad_(args.case == "moe_train") for t in (x, logits, wgu, wd)]
+        capacity = int(1.25 * T * k / E) if args.case == "moe_train" else 0
+
+        def fn():
+            out, aux = moe.expert_mlp(*leaves, k, capacity)
+            if args.case == "moe_train":
+                torch.autograd.grad((out, aux), leaves, (dout, torch.ones_like(aux)))
+        flops = (18.0 if args.case == "moe_train" else 6.0) * T * k * D * units
+    elif args.case == "route":
+        from torchure_b200.ops import moe
+
+        logits = torch.randn(16389, 128, device=dev).bfloat16().requires_grad_()
+        dw = torch.randn(16389, 8, device=dev)
+        fn = lambda: torch.autograd.grad(moe.route(logits, 8).weights, logits, dw)
+        bytes_ = 16389 * (128 * 4 + 8 * 20)
+    elif args.case == "swiglu8":
+        from torchure_b200.ops import act8
+
+        gu, dact = torch.randn(2 * M, F_, device=dev).bfloat16().requires_grad_(), torch.randn(2 * M, F_ // 2, device=dev).bfloat16()
+        fn = lambda: torch.autograd.grad(act8.swiglu_8bit(gu), gu, dact)
+        bytes_ = 2 * M * F_ // 2 * 2 * 8.125
+    elif args.case == "store8":
+        from torchure_b200.ops import act8
+
+        x = torch.randn(2 * M, 2560, device=dev).bfloat16()
+        fn = lambda: act8.dequantize8(act8.quantize8(x))
+        bytes_ = 2 * M * 2560 * 2 * 3.0625
     else:
         raise SystemExit(f"unknown case {args.case}")
     start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)

@@ -623,3 +623,35 @@ def test_gradients_against_differences():
     # second-order term h^2 / 6 of functions bounded by |dw| with |v| of a few, and 2^-22 / h from the weights' rounding, over 900 terms
     assert same.sum() > 200 and abs(slope - (aux.item() if same.all() else 0.0) - want) <= 900 * (h * h * 4 + 2.0 ** -22 / h)
     assert torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("T", [40, 2100])
+@pytest.mark.parametrize("pair", [False, True])
+def test_expert_mlp_gradients_one_at_a_time(T, pair):
+    """What is asked for alone has the bits it has among all; what is not asked for is not computed."""
+    from torchure_b200 import ops
+
+    x, logits, wgu, wd = (t.requires_grad_() for t in mlp_inputs(T, 6, 128, 72))
+    gate, up = (wgu.detach()[:, i:i + 72].clone().requires_grad_() for i in (0, 72))
+    leaves = [x, logits, gate, up, wd] if pair else [x, logits, wgu, wd]
+    dout = rand(T, 128, seed=9)
+
+    def grads(of):
+        out, aux = moe.expert_mlp(x, logits, (gate, up) if pair else wgu, wd, 2)
+        before = ops.launches()
+        got = torch.autograd.grad((out, aux), of, (dout, torch.ones_like(aux)))
+        return got, ops.launches() - before
+
+    want, launches = grads(leaves)
+    for leaf, w in zip(leaves, want):
+        (got,), fewer = grads([leaf])
+        assert torch.equal(got, w) and fewer < launches
+
+
+def test_gradients_have_no_gradient():
+    x, w = rand(8, 64).requires_grad_(), rand(2, 64, 64).requires_grad_()
+    offsets = torch.tensor([0, 4, 8], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(moe.grouped_linear(x, w, offsets).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(act8.swiglu_8bit(x).sum(), x, create_graph=True)

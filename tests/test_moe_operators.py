@@ -230,3 +230,32 @@ def test_refusals():
         MoELayer(8, 8, 2, experts="dense")
     with pytest.raises(ValueError, match="grouped experts"):
         MoELayer(8, 8, 2, act_bits=8)
+
+
+def _spread(rank, world):
+    from torchure_b200.core.mesh import Mesh
+    from torchure_b200.parallel.expert_parallel import MoELayer
+
+    mesh = Mesh({"ep": world})
+    torch.manual_seed(0)
+    full = MoELayer(16, 32, num_experts=4, top_k=2, capacity_factor=8.0, experts="grouped")
+    spread = MoELayer(16, 32, num_experts=4, top_k=2, capacity_factor=8.0, experts="grouped")
+    spread.load_state_dict(full.state_dict())
+    spread.shard_(mesh, "ep")
+    x = torch.randn(6, 16, generator=torch.Generator().manual_seed(rank))
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    out, want = spread(a), full(b)
+    torch.testing.assert_close(out, want, rtol=1e-4, atol=1e-5)
+    out.square().sum().backward()
+    want.square().sum().backward()
+    torch.testing.assert_close(a.grad, b.grad, rtol=1e-4, atol=1e-5)
+    # this rank's experts saw the tokens of all ranks
+    grads = [torch.zeros_like(full.w_down) for _ in range(world)]
+    torch.distributed.all_gather(grads, full.w_down.grad)
+    torch.testing.assert_close(spread.w_down.grad, sum(grads)[rank * 2:rank * 2 + 2], rtol=1e-4, atol=1e-5)
+
+
+def test_grouped_layer_spread_over_ranks():
+    from dist_utils import run_distributed
+
+    run_distributed(_spread, 2, timeout_s=120)

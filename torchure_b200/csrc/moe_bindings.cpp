@@ -578,9 +578,14 @@ class Beside {
   bool on_, busy_ = false;
 };
 
-// dx, dlogits, dw_gate_up, dw_down
+struct Wanted {
+  bool x, logits, gate_up, down;
+};
+
+// dx, dlogits, dw_gate_up, dw_down, undefined where not wanted
 variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
-                      const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Outputs& make) {
+                      const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Wanted& wanted,
+                      const Outputs& make) {
   const int64_t T = x.size(0), k = r.slots.size(1), R = T * k, E = logits.size(1), F = wd.size(2);
   if (R == 0)
     return {at::zeros_like(x), at::zeros_like(logits), at::zeros(wgu.sizes(), wgu.options().dtype(wtype)),
@@ -588,26 +593,28 @@ variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x
   Tensor dgu = make("expert_mlp.dgu", {R, 2 * F}, wgu.options());
   Tensor act_w = make("expert_mlp.act", {R, F}, wgu.options());
   Tensor dweights = make("expert_mlp.dweights", {T, k}, r.weights.options());
-  const Tensor xg = make("expert_mlp.xg", {R, x.size(1)}, wgu.options()), dx = make("expert_mlp.dx", {T, x.size(1)}, x.options());
-  const Tensor dl = make("expert_mlp.dlogits", {T, E}, logits.options());
-  Tensor dg, s, dxg, dwd, dwgu;
+  Tensor dg, s, dxg, dwd, dwgu, xg, dx, dl;
+  if (wanted.gate_up) xg = make("expert_mlp.xg", {R, x.size(1)}, wgu.options());
+  if (wanted.x) dx = make("expert_mlp.dx", {T, x.size(1)}, x.options());
+  if (wanted.logits) dl = make("expert_mlp.dlogits", {T, E}, logits.options());
   Beside beside(R >= BESIDE_MIN_ROWS);
   dg = do_gather(dout, r.rows, k, make);
-  beside.run([&] { do_gather(x, r.rows, k, make, xg); });
+  if (wanted.gate_up) beside.run([&] { do_gather(x, r.rows, k, make, xg); });
   s = do_grouped(dg, wd, r.offsets, true, make);
   const bool kept16 = gu.defined();
   tb::expert_swiglu_bwd(bf(s), kept16 ? bf(gu) : nullptr, kept16 ? nullptr : q.data_ptr<int8_t>(), kept16 ? nullptr : scales.data_ptr<float>(),
                         r.weights.data_ptr<float>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), bfm(dgu), bfm(act_w),
                         dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream());
   g_launches += 1;
-  dxg = do_grouped(dgu, wgu, r.offsets, true, make);
-  beside.run([&] {
-    do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make, dx);
-    do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make, dl);
-  });
-  dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
+  if (wanted.x) dxg = do_grouped(dgu, wgu, r.offsets, true, make);
+  if (wanted.x || wanted.logits)
+    beside.run([&] {
+      if (wanted.x) do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make, dx);
+      if (wanted.logits) do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make, dl);
+    });
+  if (wanted.down) dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
   beside.join();
-  dwgu = do_wgrad(dgu, xg, r.offsets, wtype, make);
+  if (wanted.gate_up) dwgu = do_wgrad(dgu, xg, r.offsets, wtype, make);
   return {dx, dl, dwgu, dwd};
 }
 
@@ -646,13 +653,17 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
       return out;
     }
     Routed r{s[4], s[5], s[6], s[7], s[8], s[9], Tensor()};
+    // edges are those of the tensors that were given: x, logits, gate (and up), down
+    const bool pair = ctx->saved_data["pair"].toBool();
+    const Wanted wanted{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2) || (pair && ctx->needs_input_grad(3)),
+                        ctx->needs_input_grad(pair ? 4 : 3)};
     auto g = mlp_bwd(rows_of(grads[0]), opt(daux), s[0], s[1], s[2], s[3], r, s[10], s[11], s[12],
-                     static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), make);
+                     static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), wanted, make);
     const int64_t F = s[3].size(2);
     out[0] = g[0];
     out[1] = g[1];
-    out[2] = ctx->saved_data["pair"].toBool() ? g[2].narrow(1, 0, F) : g[2];
-    if (ctx->saved_data["pair"].toBool()) out[3] = g[2].narrow(1, F, F);
+    if (wanted.gate_up) out[2] = pair ? g[2].narrow(1, 0, F) : g[2];
+    if (wanted.gate_up && pair) out[3] = g[2].narrow(1, F, F);
     out[4] = g[3];
     return out;
   }
