@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from tests.dist_utils import run_distributed
 from torchure_b200.ops import act8, moe, oracle
 
 NINF = float("-inf")
@@ -256,6 +257,4 @@ def _spread(rank, world):
 
 
 def test_grouped_layer_spread_over_ranks():
-    from dist_utils import run_distributed
-
     run_distributed(_spread, 2, timeout_s=120)
