@@ -14,8 +14,13 @@
 //
 // Bound by memory.  Eight lanes have a block, eight values each (16 bytes of bf16, 8 bytes of int8), four blocks at a time (SwiGLU:
 // two of gate and two of up) so that as many loads are on their way; with one block at a time 16384 x 2560 took 43 us to quantise and
-// 32 to read back, and SwiGLU of 16384 x 1536 54 and 42.  Widths that are no multiple of 8, or rows off a 16-byte boundary, are read
-// value by value.
+// 32 to read back, and SwiGLU of 16384 x 1536 54 and 42; now 22, 18, 34 and 33 (128 and 204 MB).
+//
+// Widths that are no multiple of 8: a CTA takes whole rows, which lie one behind the other, brings them into shared memory as they lie (16
+// bytes at a time, the ends value by value), works on them there and sends its results out the same way: 16384 x 2557 in 55 us to quantise
+// and 42 to read back (value by value from memory 71 and 118), SwiGLU of 16384 x 1533 in 90 forward and 91 backward.  What bounds it are the
+// 2-byte accesses to shared memory; rows shifted onto 16 bytes there instead, so that eight values go at once, took 68 and 56, 139 and 144:
+// each 16 bytes are then read twice.  Rows that do not follow one another, or do not fit, go value by value from memory.
 #include "act8.cuh"
 #include "moe_api.h"
 
@@ -86,6 +91,11 @@ __device__ __forceinline__ void read_q(uint2 raw, float scale, float (&v)[8]) {
   }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {      // of bf16 pairs, NaN where either is
   uint32_t r;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -281,8 +291,189 @@ swiglu8_bwd_kernel(const __nv_bfloat16* __restrict__ dact, int64_t ldd, const in
   }
 }
 
+// ---- rows of any width, through shared memory --------------------------------------------------------
+// `bytes` from global memory to shared memory, `to` with the source's remainder by 16 (stage_at); by all threads of the CTA.
+__device__ __forceinline__ uint8_t* stage_at(uint8_t* area, const void* p) { return area + (reinterpret_cast<uintptr_t>(p) & 15); }
+__device__ __forceinline__ void stage_in(uint8_t* to, const void* from, int bytes) {
+  const uint8_t* src = static_cast<const uint8_t*>(from);
+  const int head = min(bytes, static_cast<int>(-reinterpret_cast<uintptr_t>(from) & 15)), body = (bytes - head) / 16;
+  for (int i = threadIdx.x; i < head; i += kThreads) to[i] = src[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < body; i += kThreads)
+    *reinterpret_cast<uint4*>(to + head + i * 16) = *reinterpret_cast<const uint4*>(src + head + i * 16);
+  for (int i = head + body * 16 + threadIdx.x; i < bytes; i += kThreads) to[i] = src[i];
+}
+__device__ __forceinline__ void stage_out(void* to, const uint8_t* from, int bytes) {
+  uint8_t* dst = static_cast<uint8_t*>(to);
+  const int head = min(bytes, static_cast<int>(-reinterpret_cast<uintptr_t>(to) & 15)), body = (bytes - head) / 16;
+  for (int i = threadIdx.x; i < head; i += kThreads) dst[i] = from[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < body; i += kThreads)
+    *reinterpret_cast<uint4*>(dst + head + i * 16) = *reinterpret_cast<const uint4*>(from + head + i * 16);
+  for (int i = head + body * 16 + threadIdx.x; i < bytes; i += kThreads) dst[i] = from[i];
+}
+// Value i of this lane's eight of a block: eight apart, so that eight lanes read neighbours, and turned by the warp's other blocks, which
+// lie 128 bytes (64 as bytes) further on.
+__device__ __forceinline__ int odd_place(int i) { return ((i + 2 * ((threadIdx.x >> 3) & 3)) & 7) * 8 + (threadIdx.x & 7); }
+__device__ __forceinline__ float odd_load(const uint8_t* row, int c, int width) {
+  return c < width ? __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c]) << 16) : 0.f;
+}
+__device__ __forceinline__ void odd_store(uint8_t* row, int c, int width, float v) {
+  if (c < width) reinterpret_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16(v);
+}
+// keep8 for a block in shared memory
+__device__ __forceinline__ void odd_keep(const float (&v)[8], uint8_t* q, int c0, int width, float* scale, bool in) {
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const ActScale k = act_scale(a);
+  if (in && (threadIdx.x & 7) == 0) *scale = k.scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = c0 + odd_place(i);
+    if (in && c < width) q[c] = act_byte(v[i], k.inv);
+  }
+}
+// What a staged byte stands for
+__device__ __forceinline__ float odd_read(const uint8_t* q, int c, int width, float scale) {
+  return c < width ? static_cast<float>(static_cast<int8_t>(q[c])) * scale : 0.f;
+}
+
+constexpr int kOddValues = 8192;      // values of the widest tensor of a tile; wider rows are read from memory
+
+// rows: of a tile.  Shared memory: the areas of what comes in and goes out, 16 bytes longer than they are and on 16 bytes.
+__global__ void __launch_bounds__(kThreads)
+quantize8_rows_kernel(const __nv_bfloat16* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scales, int64_t M, int N, int nb,
+                      int rows) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(16) uint8_t area[];
+  const int x_area = (rows * N * 2 + 31) / 16 * 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < M; r0 += static_cast<int64_t>(gridDim.x) * rows) {
+    const int n = static_cast<int>(M - r0 < rows ? M - r0 : rows);
+    uint8_t* sx = stage_at(area, x + r0 * N);
+    uint8_t* sq = stage_at(area + x_area, q + r0 * N);
+    stage_in(sx, x + r0 * N, n * N * 2);
+    __syncthreads();
+    for (int u0 = threadIdx.x >> 5 << 2; u0 < n * nb; u0 += kGroups) {      // whole warps: four blocks
+      const int u = u0 + ((threadIdx.x & 31) >> 3), row = u / nb, c0 = (u - row * nb) * kActBlock;
+      const bool in = u < n * nb;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = in ? odd_load(sx + row * N * 2, c0 + odd_place(i), N) : 0.f;
+      odd_keep(v, sq + row * N, c0, N, scales + r0 * nb + u, in);
+    }
+    __syncthreads();
+    stage_out(q + r0 * N, sq, n * N);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+dequantize8_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x, int64_t M, int N, int nb,
+                        int rows) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(16) uint8_t area[];
+  const int x_area = (rows * N * 2 + 31) / 16 * 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < M; r0 += static_cast<int64_t>(gridDim.x) * rows) {
+    const int n = static_cast<int>(M - r0 < rows ? M - r0 : rows);
+    uint8_t* sx = stage_at(area, x + r0 * N);
+    uint8_t* sq = stage_at(area + x_area, q + r0 * N);
+    stage_in(sq, q + r0 * N, n * N);
+    __syncthreads();
+    for (int u = threadIdx.x >> 3; u < n * nb; u += kGroups) {
+      const int row = u / nb, c0 = (u - row * nb) * kActBlock;
+      const float scale = scales[r0 * nb + u];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + odd_place(i);
+        odd_store(sx + row * N * 2, c, N, odd_read(sq + row * N, c, N, scale));
+      }
+    }
+    __syncthreads();
+    stage_out(x + r0 * N, sx, n * N * 2);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+swiglu8_fwd_rows_kernel(const __nv_bfloat16* __restrict__ gu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
+                        float* __restrict__ scales, int64_t M, int F, int nb, int rows) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(16) uint8_t area[];
+  const int gu_area = (rows * F * 4 + 31) / 16 * 16, act_area = (rows * F * 2 + 31) / 16 * 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < M; r0 += static_cast<int64_t>(gridDim.x) * rows) {
+    const int n = static_cast<int>(M - r0 < rows ? M - r0 : rows);
+    uint8_t* sg = stage_at(area, gu + r0 * 2 * F);
+    uint8_t* sa = stage_at(area + gu_area, act + r0 * F);
+    uint8_t* sq = stage_at(area + gu_area + act_area, q + r0 * 2 * F);
+    stage_in(sg, gu + r0 * 2 * F, n * F * 4);
+    __syncthreads();
+    for (int u0 = threadIdx.x >> 5 << 2; u0 < n * nb; u0 += kGroups) {
+      const int u = u0 + ((threadIdx.x & 31) >> 3), row = u / nb, b = u - row * nb, c0 = b * kActBlock;
+      const bool in = u < n * nb;
+      float gate[8], up[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + odd_place(i);
+        gate[i] = in ? odd_load(sg + row * F * 4, c, F) : 0.f;
+        up[i] = in ? odd_load(sg + row * F * 4 + F * 2, c, F) : 0.f;
+        if (in) odd_store(sa + row * F * 2, c, F, gate[i] * sigmoid(gate[i]) * up[i]);
+      }
+      float* scale = scales + (r0 + row) * 2 * nb + b;
+      odd_keep(gate, sq + row * 2 * F, c0, F, scale, in);
+      odd_keep(up, sq + row * 2 * F + F, c0, F, scale + nb, in);
+    }
+    __syncthreads();
+    stage_out(act + r0 * F, sa, n * F * 2);
+    stage_out(q + r0 * 2 * F, sq, n * F * 2);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+swiglu8_bwd_rows_kernel(const __nv_bfloat16* __restrict__ dact, const int8_t* __restrict__ q, const float* __restrict__ scales,
+                        __nv_bfloat16* __restrict__ dgu, int64_t M, int F, int nb, int rows) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ __align__(16) uint8_t area[];
+  const int gu_area = (rows * F * 4 + 31) / 16 * 16, act_area = (rows * F * 2 + 31) / 16 * 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < M; r0 += static_cast<int64_t>(gridDim.x) * rows) {
+    const int n = static_cast<int>(M - r0 < rows ? M - r0 : rows);
+    uint8_t* sg = stage_at(area, dgu + r0 * 2 * F);
+    uint8_t* sa = stage_at(area + gu_area, dact + r0 * F);
+    uint8_t* sq = stage_at(area + gu_area + act_area, q + r0 * 2 * F);
+    stage_in(sa, dact + r0 * F, n * F * 2);
+    stage_in(sq, q + r0 * 2 * F, n * F * 2);
+    __syncthreads();
+    for (int u = threadIdx.x >> 3; u < n * nb; u += kGroups) {
+      const int row = u / nb, b = u - row * nb, c0 = b * kActBlock;
+      const float* scale = scales + (r0 + row) * 2 * nb + b;
+      const float sgate = scale[0], sup = scale[nb];
+      float g[8], v[8], d[8], dg[8], du[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + odd_place(i);
+        g[i] = odd_read(sq + row * 2 * F, c, F, sgate);
+        v[i] = odd_read(sq + row * 2 * F + F, c, F, sup);
+        d[i] = odd_load(sa + row * F * 2, c, F);
+      }
+      swiglu_grad(g, v, d, dg, du);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + odd_place(i);
+        odd_store(sg + row * F * 4, c, F, dg[i]);
+        odd_store(sg + row * F * 4 + F * 2, c, F, du[i]);
+      }
+    }
+    __syncthreads();
+    stage_out(dgu + r0 * 2 * F, sg, n * F * 4);
+  }
+}
+
 // One warp per choice: the row of its gradient and the dot product that is its weight's.
-template <bool Q8, bool VEC>
+template <bool Q8>
 __global__ void __launch_bounds__(kThreads)
 expert_swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ s, const __nv_bfloat16* __restrict__ gu, const int8_t* __restrict__ q,
                          const float* __restrict__ scales, const float* __restrict__ weights, const int* __restrict__ slots,
@@ -303,13 +494,13 @@ expert_swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ s, const __nv_bfloat1
         const int left = F - c;
         float gate[8], up[8], d[8], dg[8], du[8], a[8];
         if (Q8) {
-          read_q(load_q<VEC>(q + row * 2 * F + c, left), scales[row * 2 * nb + c / kActBlock], gate);
-          read_q(load_q<VEC>(q + row * 2 * F + F + c, left), scales[row * 2 * nb + nb + c / kActBlock], up);
+          read_q(load_q<true>(q + row * 2 * F + c, left), scales[row * 2 * nb + c / kActBlock], gate);
+          read_q(load_q<true>(q + row * 2 * F + F + c, left), scales[row * 2 * nb + nb + c / kActBlock], up);
         } else {
-          load8<VEC>(gu + row * 2 * F + c, left, gate);
-          load8<VEC>(gu + row * 2 * F + F + c, left, up);
+          load8<true>(gu + row * 2 * F + c, left, gate);
+          load8<true>(gu + row * 2 * F + F + c, left, up);
         }
-        load8<VEC>(s + row * F + c, left, d);
+        load8<true>(s + row * F + c, left, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           a[j] = gate[j] * sigmoid(gate[j]) * up[j];
@@ -318,9 +509,9 @@ expert_swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ s, const __nv_bfloat1
           d[j] *= w;
         }
         swiglu_grad(gate, up, d, dg, du);
-        store8<VEC>(act_w + row * F + c, left, a);
-        store8<VEC>(dgu + row * 2 * F + c, left, dg);
-        store8<VEC>(dgu + row * 2 * F + F + c, left, du);
+        store8<true>(act_w + row * F + c, left, a);
+        store8<true>(dgu + row * 2 * F + c, left, dg);
+        store8<true>(dgu + row * 2 * F + F + c, left, du);
       }
       dot = warp_sum(dot);
     }
@@ -328,9 +519,9 @@ expert_swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ s, const __nv_bfloat1
     if (i >= live) {      // row i is no choice's
       const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int c = lane * 8; c < F; c += 256) {
-        store8<VEC>(act_w + static_cast<int64_t>(i) * F + c, F - c, zero);
-        store8<VEC>(dgu + static_cast<int64_t>(i) * 2 * F + c, F - c, zero);
-        store8<VEC>(dgu + static_cast<int64_t>(i) * 2 * F + F + c, F - c, zero);
+        store8<true>(act_w + static_cast<int64_t>(i) * F + c, F - c, zero);
+        store8<true>(dgu + static_cast<int64_t>(i) * 2 * F + c, F - c, zero);
+        store8<true>(dgu + static_cast<int64_t>(i) * 2 * F + F + c, F - c, zero);
       }
     }
   }
@@ -341,6 +532,16 @@ int grid_for(int64_t units, int per_cta) {
   const int64_t need = (units + per_cta - 1) / per_cta;
   return static_cast<int>(need < 148 * 16 ? need : 148 * 16);
 }
+// Rows of a tile that go through shared memory, and its bytes; a value of the widest tensor costs `bytes` of all areas.
+int tile_rows(int64_t M, int width) {
+  const int fit = kOddValues / width;
+  const int64_t spread = (M + 148 * 6 - 1) / (148 * 6);      // small matrices: over all SMs
+  return static_cast<int>(spread < 1 ? 1 : spread < fit ? spread : fit);
+}
+int tile_grid(int64_t M, int rows) {
+  const int64_t need = (M + rows - 1) / rows;
+  return static_cast<int>(need < 148 * 8 ? need : 148 * 8);
+}
 bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -350,8 +551,14 @@ void quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, in
   const int nb = blocks_of(N);
   const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
-  if (N % 8 == 0 && ldx % 8 == 0 && at16(x) && at16(q)) launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
-  else launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+  if (N % 8 == 0 && ldx % 8 == 0 && at16(x) && at16(q)) {
+    launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+  } else if (ldx == N && N <= kOddValues) {
+    const int rows = tile_rows(M, N);
+    launch_pdl(quantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, x, q, scales, M, N, nb, rows);
+  } else {
+    launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+  }
 }
 
 void dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream) {
@@ -359,8 +566,14 @@ void dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t
   const int nb = blocks_of(N);
   const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
-  if (N % 8 == 0 && at16(x) && at16(q)) launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
-  else launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+  if (N % 8 == 0 && at16(x) && at16(q)) {
+    launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+  } else if (N <= kOddValues) {
+    const int rows = tile_rows(M, N);
+    launch_pdl(dequantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, q, scales, x, M, N, nb, rows);
+  } else {
+    launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+  }
 }
 
 void swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
@@ -369,9 +582,14 @@ void swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
-  if (F % 8 == 0 && ldgu % 8 == 0 && at16(gu) && at16(act) && at16(q))
+  if (F % 8 == 0 && ldgu % 8 == 0 && at16(gu) && at16(act) && at16(q)) {
     launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
-  else launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+  } else if (ldgu == 2 * static_cast<int64_t>(F) && 2 * F <= kOddValues) {
+    const int rows = tile_rows(M, 2 * F);
+    launch_pdl(swiglu8_fwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, gu, act, q, scales, M, F, nb, rows);
+  } else {
+    launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+  }
 }
 
 void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M, int F,
@@ -380,9 +598,14 @@ void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const 
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
-  if (F % 8 == 0 && ldd % 8 == 0 && at16(dact) && at16(dgu) && at16(q))
+  if (F % 8 == 0 && ldd % 8 == 0 && at16(dact) && at16(dgu) && at16(q)) {
     launch_pdl(swiglu8_bwd_kernel<true>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
-  else launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
+  } else if (ldd == F && 2 * F <= kOddValues) {
+    const int rows = tile_rows(M, 2 * F);
+    launch_pdl(swiglu8_bwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, dact, q, scales, dgu, M, F, nb, rows);
+  } else {
+    launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
+  }
 }
 
 void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,
@@ -391,12 +614,8 @@ void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const in
   if (R <= 0 || F <= 0) return;
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(R, kWarps)), block(kThreads);
-  const bool vec = F % 8 == 0 && at16(s) && at16(dgu) && at16(act_w) && (gu ? at16(gu) : at16(q));
-#define TB_EXPERT(Q, V) \
-  launch_pdl(expert_swiglu_bwd_kernel<Q, V>, grid, block, 0, stream, s, gu, q, scales, weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb)
-  if (gu) { if (vec) TB_EXPERT(false, true); else TB_EXPERT(false, false); }
-  else { if (vec) TB_EXPERT(true, true); else TB_EXPERT(true, false); }
-#undef TB_EXPERT
+  if (gu) launch_pdl(expert_swiglu_bwd_kernel<false>, grid, block, 0, stream, s, gu, q, scales, weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb);
+  else launch_pdl(expert_swiglu_bwd_kernel<true>, grid, block, 0, stream, s, gu, q, scales, weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb);
 }
 
 }  // namespace tb

@@ -79,7 +79,8 @@ void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const 
                  cudaStream_t stream);
 // The experts' SwiGLU backward, over choices i = t k + j with row r = slots[i] and weight w = weights[i]; s [R, F] = dout W_down.
 // Gate and up come from gu (bf16) or, where gu is nullptr, from (q, scales).  dgu[r] = d(gate) | d(up) for d(act) = w s,
-// act_w[r] = w act, dweights[i] = <act, s>; zeros in rows of no choice, and 0 for a choice without a row.
+// act_w[r] = w act, dweights[i] = <act, s>; zeros in rows of no choice, and 0 for a choice without a row.  F a multiple of 8, matrices on
+// 16 bytes.
 void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,
                        const int* slots, const int* offsets, __nv_bfloat16* dgu, __nv_bfloat16* act_w, float* dweights, int R, int E,
                        int F, cudaStream_t stream);
