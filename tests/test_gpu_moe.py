@@ -414,6 +414,53 @@ def test_expert_mlp_of_a_few_tokens(T, E, k, D, F, capacity, dtype, logit):
         assert not closed or (out[T - 1] == 0).all()
 
 
+@pytest.mark.parametrize("T,E,k,D,F", [(100, 8, 2, 256, 136), (130, 40, 4, 72, 64), (61, 16, 4, 1024, 200), (300, 20, 2, 264, 72)])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_expert_mlp_of_uneven_groups(T, E, k, D, F, bits):
+    """Few rows per expert on average, but one expert has every token (more than one tile of rows), others have none."""
+    x, logits, wgu, wd = mlp_inputs(T, E, D, F)
+    logits[:, E // 2] += 100
+    logits[:, ::3] = NINF
+    leaves = [t.clone().requires_grad_() for t in (x, logits, wgu, wd)]
+    out, aux = moe.expert_mlp(*leaves, k, act_bits=bits)
+    dout = rand(T, D, seed=9)
+    out.backward(dout)
+    ref = [t.detach().cpu().double().requires_grad_() for t in (x, logits, wgu, wd)]
+    want, _ = oracle.expert_mlp(*ref, k, 0, bits)
+    want.backward(dout.cpu().double())
+    assert rel(out.detach().cpu(), want.detach()) < 5 * RMS
+    for got, r in list(zip(leaves, ref))[2:]:
+        assert rel(got.grad.cpu(), r.grad) < (5 * RMS if bits == 16 else 5 * RMS + 2 * 2.5 / 127)
+        assert not got.grad[moe.route(logits, k).counts == 0].any()
+    with torch.no_grad():
+        assert rel(moe.expert_mlp(x, logits, wgu, wd, k)[0].cpu(), want.detach()) < 5 * RMS
+
+
+def test_expert_mlp_reads_matrices_that_were_just_written():
+    """The kernels of a pass overlap, and read matrices early: never before what wrote them has ended, whoever wrote them."""
+    E, D, F = 8, 512, 384
+    x, logits, _, _ = mlp_inputs(64, E, D, F)
+    r = moe.route(torch.randn(4096, 8, device="cuda", generator=gen(5)), 1)
+    sources = [rand(4096, E * F * D * 3 // 4096, seed=s, std=D ** -0.5) for s in range(4)]
+
+    def split(flat):
+        flat = flat.reshape(-1)
+        return flat[:E * 2 * F * D].view(E, 2 * F, D), flat[E * 2 * F * D:].view(E, D, F)
+
+    with torch.no_grad():
+        order = [src[r.rows.long()] for src in sources]
+        want = [moe.expert_mlp(x, logits, *split(o), 2)[0] for o in order]
+        torch.cuda.synchronize()
+        held = torch.empty_like(order[0])
+        for i in range(40):
+            if i % 2:
+                held.copy_(order[i % 4])
+                got = moe.expert_mlp(x, logits, *split(held), 2)[0]
+            else:
+                got = moe.expert_mlp(x, logits, *split(moe.dispatch(sources[i % 4], r)), 2)[0]
+            assert torch.equal(got, want[i % 4])
+
+
 def test_expert_mlp_gradient_of_aux_alone_and_no_tokens():
     x, logits, wgu, wd = mlp_inputs(32, 4, 64, 64)
     logits.requires_grad_()

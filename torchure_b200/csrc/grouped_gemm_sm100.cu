@@ -23,7 +23,9 @@
 // are then all the traffic there is, and what counts is how evenly it is spread and how many copies are on their way.  There the
 // group's rows may be listed (places of token rows in expert order) and are gathered four to a copy (tile::gather4), which spares a
 // launch.  A copy of four rows costs about 72 cycles, so that tiles of many rows do better with the rows put in order first (the pair
-// kernels with listed rows took 270 us instead of 88 + 9.6).
+// kernels with listed rows took 270 us instead of 88 + 9.6).  In a feed-forward pass of few rows, whose launches overlap, the first tile of
+// every group has a CTA that is known beforehand (EARLY): it asks for its first four blocks of the matrix while the kernel before is still at
+// work.
 #include "act8.cuh"
 #include "cta_pair.cuh"
 #include "moe_api.h"
@@ -511,12 +513,14 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 
 // Few rows per group: one CTA has 128 tile rows (64 units of SwiGLU) of one group and up to 64 of its rows; grid (tiles of the matrix,
 // an upper bound of the groups' tiles of rows).  The operand stages hold the epilogue's staging rows once the products are done.
+// EARLY: the matrices are read before the kernel before has ended, which must not write them.  (A template, since the few instructions cost
+// grids of a thousand CTAs 3 % where they are not used.)
 constexpr int FEW_ROWS = 64, FEW_STAGES = 4, FEW_STAGE = A_BYTES + FEW_ROWS * BK * 2;
 constexpr int FEW_SMEM = FEW_STAGES * FEW_STAGE + BAR_BYTES + 1024;
 static_assert(ROW_EPI_BYTES <= FEW_STAGES * FEW_STAGE && kPartBytes<kStore32> <= FEW_STAGES * FEW_STAGE, "staging rows");
 static_assert(2 * (FEW_SMEM + 1024) <= 233472, "two CTAs on an SM");
 
-template <bool W_MN, int EPI, bool LISTED>
+template <bool W_MN, int EPI, bool LISTED, bool EARLY>
 __global__ void __launch_bounds__(FEW_THREADS, 2)
 grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const int* __restrict__ offsets,
                    const __grid_constant__ Rows rows, const __grid_constant__ RowsOut out, int R, int E, int K, int* err) {
@@ -530,18 +534,25 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   int* where = reinterpret_cast<int*>(bars + 2 * FEW_STAGES + 2);      // group, first row, rows, first row of no expert
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 32) {
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
-    for (int s = 0; s < FEW_STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
+  const int n0 = static_cast<int>(blockIdx.x) * UNIT, all_kb = (K + BK - 1) / BK;
+  const int early = EARLY ? E : 0, loaded = static_cast<int>(blockIdx.y) < early ? min(all_kb, FEW_STAGES) : 0;      // k-blocks of the matrix under way
+  if (warp == 1) {      // (warp 0 looks for its rows meanwhile)
+    if (elect_one()) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      for (int s = 0; s < FEW_STAGES; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(tfull, 1);
+      fence_barrier_init();
+      for (int kb = 0; kb < loaded; ++kb) {
+        mbar_expect_more(&full[kb], A_BYTES);
+        load_matrix<W_MN, EPI>(smem + kb * FEW_STAGE, &tmW, out, kb * BK, n0, blockIdx.y, FewLoads{&full[kb]});
+      }
     }
-    mbar_init(tfull, 1);
-    fence_barrier_init();
-  }
-  __syncwarp();
-  if (warp == 1) {
+    __syncwarp();
     tmem_alloc(tmem_slot, FEW_ROWS);
     tmem_relinquish();
     tc_fence_before();
@@ -549,8 +560,9 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   pdl_wait();
   pdl_launch_dependents();
   if (warp == 0) {
-    // the group that tile blockIdx.y of the groups' row tiles belongs to: edges as load_edges has them, 32 groups at a time
-    int run = 0, tiles_before = 0;
+    // the group that tile blockIdx.y of the groups' row tiles belongs to: edges as load_edges has them, 32 groups at a time.  With EARLY
+    // the first tile of each group has a place of its own, and the others follow.
+    int run = 0, tiles_before = early;
     if (lane == 0) where[2] = 0;
     __syncwarp();
     for (int e0 = 0; e0 < E; e0 += 32) {
@@ -564,15 +576,17 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       hi = max(hi, run);
       int lo = __shfl_up_sync(0xffffffffu, hi, 1);
       if (lane == 0) lo = run;
-      const int tiles = (hi - lo + FEW_ROWS - 1) / FEW_ROWS;
+      const int placed = e < early && hi > lo ? 1 : 0, tiles = (hi - lo + FEW_ROWS - 1) / FEW_ROWS - placed;
       int sum = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
       }
-      const int at = static_cast<int>(blockIdx.y) - (tiles_before + sum - tiles);
-      if (at >= 0 && at < tiles) {
+      int at = static_cast<int>(blockIdx.y) - (tiles_before + sum - tiles);
+      const bool mine = placed && e == static_cast<int>(blockIdx.y);
+      if (mine || (at >= 0 && at < tiles)) {
+        at = mine ? 0 : at + placed;
         where[0] = e;
         where[1] = lo + at * FEW_ROWS;
         where[2] = min(FEW_ROWS, hi - lo - at * FEW_ROWS);
@@ -586,9 +600,16 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int e = where[0], r0 = where[1], live = where[2];
-  constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
-  const int n0 = static_cast<int>(blockIdx.x) * UNIT;
-  const int num_kb = live > 0 ? (K + BK - 1) / BK : 0;
+  const int num_kb = live > 0 ? all_kb : 0;
+
+  if (warp == 0 && num_kb == 0) {      // what was asked for arrives before the CTA goes
+    if (elect_one())
+      for (int kb = 0; kb < loaded; ++kb) {
+        mbar_arrive(&full[kb]);
+        if (!mbar_wait(&full[kb], 0, err, kErrMmaFullWait)) break;
+      }
+    __syncwarp();
+  }
 
   if (LISTED && warp == 0) {
     // all lanes: each has four of the rows; the first matrix tiles are on their way before the list is looked at
@@ -597,8 +618,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     const int used = (live + 15) / 16 * 16, ahead = min(num_kb, FEW_STAGES);
     if (lane == 0)
       for (int kb = 0; kb < ahead; ++kb) {
-        mbar_expect_tx(&full[kb], A_BYTES + used * 128);
-        load_matrix<W_MN, EPI>(smem + kb * FEW_STAGE, &tmW, out, kb * BK, n0, e, FewLoads{&full[kb]});
+        mbar_expect_tx(&full[kb], (kb < loaded ? 0 : A_BYTES) + used * 128);
+        if (kb >= loaded) load_matrix<W_MN, EPI>(smem + kb * FEW_STAGE, &tmW, out, kb * BK, n0, e, FewLoads{&full[kb]});
       }
     __syncwarp();
     int from[4];
@@ -621,8 +642,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrProducerEmptyWait)) break;
         uint8_t* sA = smem + stage * FEW_STAGE;
-        mbar_expect_tx(&full[stage], FEW_STAGE);
-        load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, e, FewLoads{&full[stage]});
+        mbar_expect_tx(&full[stage], kb < loaded ? FEW_STAGE - A_BYTES : FEW_STAGE);
+        if (kb >= loaded) load_matrix<W_MN, EPI>(sA, &tmW, out, kb * BK, n0, e, FewLoads{&full[stage]});
         tma_load_2d(sA + A_BYTES, &tmX, &full[stage], kb * BK, r0);
         if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
       }
@@ -960,23 +981,37 @@ int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, 
 
 namespace {
 
-// Up to this many rows per group, on average, the small tiles.
-constexpr int FEW_AVERAGE = 96;
+// Up to this many rows per group, on average, the small tiles.  Small tiles, pairs, us back to back, products of 8 uneven groups (1024 x
+// 1536), of 64 (1024 x 768): 32 rows per group 9.4, 10.0; 24.1, 26.2.  64 rows 9.9, 10.5; 26.7, 30.4.  96 rows 10.2, 11.1; 32.5, 32.2,
+// but the whole feed-forward 46, 43.5; 118, 104.
+constexpr int FEW_AVERAGE = 64;
+// Between these averages a feed-forward's kernels ask for their matrices before they know their rows: with fewer rows many groups would
+// have none, and with more the second tiles of groups, which come last, no longer find their matrices in L2.  The whole feed-forward without
+// and with it, 16 experts of 1024 x 768: 4 rows 30.8, 29.4; 16 rows 31.8, 29.4; 32 rows 35.5, 34.7.  64 experts: 16 rows 80, 77; 32 rows 77.7,
+// 75.6; 64 rows 100, 116.  (The rest of the tile into L2 as well gave nothing with 16 experts and cost 5 % with 64.)
+constexpr int64_t EARLY_FROM = 2, EARLY_TO = 32;
+// Up to this average the rows are gathered by the gate / up product itself.  Put in order before, gathered: 16 experts, 8 rows 30.1, 28.4; 16
+// rows 30.8, 29.4; 24 rows 33.0, 33.0; 64 experts, 8 rows 71.4, 71.0; 16 rows 77.8, 77.8; 24 rows 73, 78.
+constexpr int64_t LISTED_AVERAGE = 16;
 
 template <bool W_MN, int EPI, bool LISTED>
 int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Rows& rows, const int* offsets, const RowsOut& out, int R, int E, int K,
-               int* err, cudaStream_t stream) {
+               bool early, int* err, cudaStream_t stream) {
   constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
-  auto kern = grouped_few_kernel<W_MN, EPI, LISTED>;
-  if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
   // at most: every group with rows ends in a tile that is not full
-  const dim3 grid((out.width + UNIT - 1) / UNIT, R / FEW_ROWS + (E < R ? E : R));
-  return launch_pdl(kern, grid, dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, rows, out, R, E, K, err) == cudaSuccess ? 0 : -21;
+  const auto launch = [&](auto kern, int groups) {
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
+    const dim3 grid((out.width + UNIT - 1) / UNIT, R / FEW_ROWS + groups);
+    return launch_pdl(kern, grid, dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, rows, out, R, E, K, err) == cudaSuccess ? 0 : -21;
+  };
+  if constexpr (EPI != kStore)
+    if (early && R >= EARLY_FROM * E && R <= EARLY_TO * E) return launch(grouped_few_kernel<W_MN, EPI, LISTED, true>, E);
+  return launch(grouped_few_kernel<W_MN, EPI, LISTED, false>, E < R ? E : R);
 }
 
 template <bool W_MN, int EPI>
 int launch_rows(const __nv_bfloat16* x, int64_t ldx, const Rows& rows, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R,
-                int E, int K, int* err, int num_sms, cudaStream_t stream) {
+                int E, int K, bool early, int* err, int num_sms, cudaStream_t stream) {
   const int N = out.width;
   if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || ((reinterpret_cast<uintptr_t>(out.y) | reinterpret_cast<uintptr_t>(out.y32)) & 15) != 0)
     return -1;
@@ -990,11 +1025,11 @@ int launch_rows(const __nv_bfloat16* x, int64_t ldx, const Rows& rows, const __n
   r = rows.list ? make_tmap_2d(&tx, x, 2, rows.count, K, ldx, 1, 64) : make_tmap_2d(&tx, x, 2, R, K, ldx, few ? FEW_ROWS : BNH, 64);
   if (r) return r - 100;
   if constexpr (EPI == kSwiglu)
-    if (rows.list) return launch_few<W_MN, EPI, true>(tw, tx, rows, offsets, out, R, E, K, err, stream);
+    if (rows.list) return launch_few<W_MN, EPI, true>(tw, tx, rows, offsets, out, R, E, K, early, err, stream);
   if constexpr (EPI == kStore32) {
-    return few ? launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream) : -2;
+    return few ? launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, early, err, stream) : -2;
   } else {
-    if (few) return launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, err, stream);
+    if (few) return launch_few<W_MN, EPI, false>(tw, tx, rows, offsets, out, R, E, K, early, err, stream);
     constexpr int UNIT = kGateUp<EPI> ? BM : 2 * BM;
     const int64_t units = (static_cast<int64_t>(R) / BN + (E < R ? E : R)) * ((N + UNIT - 1) / UNIT);
     return launch_pairs(grouped_rows_kernel<W_MN, EPI>, ROW_THREADS, ROW_SMEM, units, num_sms, stream, tw, tx, offsets, out, R, E, K, err);
@@ -1009,30 +1044,30 @@ int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bo
   out.y = y;
   out.width = N;
   const Rows rows{nullptr, FastDiv(1), 0};
-  return w_t ? launch_rows<true, kStore>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream)
-             : launch_rows<false, kStore>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);
+  return w_t ? launch_rows<true, kStore>(x, ldx, rows, w, offsets, out, R, E, K, false, err, num_sms, stream)
+             : launch_rows<false, kStore>(x, ldx, rows, w, offsets, out, R, E, K, false, err, num_sms, stream);
 }
 
 bool grouped_gemm_few(int R, int E) { return R <= static_cast<int64_t>(FEW_AVERAGE) * E; }
 
 int grouped_gemm_f32(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, float* y, int R, int E, int N, int K,
-                     int* err, int num_sms, cudaStream_t stream) {
+                     bool early, int* err, int num_sms, cudaStream_t stream) {
   RowsOut out{};
   out.y32 = y;
   out.width = N;
-  return launch_rows<false, kStore32>(x, ldx, Rows{nullptr, FastDiv(1), 0}, w, offsets, out, R, E, K, err, num_sms, stream);
+  return launch_rows<false, kStore32>(x, ldx, Rows{nullptr, FastDiv(1), 0}, w, offsets, out, R, E, K, early, err, num_sms, stream);
 }
 
-bool grouped_swiglu_listed(int R, int E) { return R <= 32 * static_cast<int64_t>(E); }
+bool grouped_swiglu_listed(int R, int E) { return R <= LISTED_AVERAGE * E; }
 
 int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
-                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms,
-                   cudaStream_t stream) {
+                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, bool early, int* err,
+                   int num_sms, cudaStream_t stream) {
   if (F % 8 != 0 || (gu && q) || ((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) return -1;
   RowsOut out{act, gu, q, scales, F, nullptr};
   const Rows rows{list, FastDiv(list ? k : 1), count};
-  return q ? launch_rows<false, kSwiglu8>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream)
-           : launch_rows<false, kSwiglu>(x, ldx, rows, w, offsets, out, R, E, K, err, num_sms, stream);
+  return q ? launch_rows<false, kSwiglu8>(x, ldx, rows, w, offsets, out, R, E, K, early, err, num_sms, stream)
+           : launch_rows<false, kSwiglu>(x, ldx, rows, w, offsets, out, R, E, K, early, err, num_sms, stream);
 }
 
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,

@@ -43,17 +43,18 @@ void rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_b
 int grouped_gemm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, bool w_t, const int* offsets, __nv_bfloat16* y, int R,
                  int E, int N, int K, int* err, int num_sms, cudaStream_t stream);
 // The same with w_t false and y in fp32, for few rows per expert only (grouped_gemm_few): y is added up over a token's choices afterwards,
-// and costs next to nothing there.
+// and costs next to nothing there.  early (here and below): the kernel before on the stream is one of the same feed-forward pass, so that all
+// that was there before the pass has ended and nothing that still runs writes w; the kernel may then read w before that one has ended.
 bool grouped_gemm_few(int R, int E);
 int grouped_gemm_f32(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, const int* offsets, float* y, int R, int E, int N, int K,
-                     int* err, int num_sms, cudaStream_t stream);
+                     bool early, int* err, int num_sms, cudaStream_t stream);
 // act [R, F] = silu(g) u of g | u = x W[e]^T, W [E, 2F, K] = gate rows over up rows.  Gate and up go to gu [R, 2F] in bf16, or to q
 // [R, 2F] and scales [R, 2 ceil(F / 64)] in 8 bits, or nowhere; rows of no expert: zeros.
 // list (nullptr: the R rows of x are in expert order): row r is row list[r] / k of the `count` rows of x, what `rows` of route_fwd says.
 // Only where grouped_swiglu_listed, and not with q.
 bool grouped_swiglu_listed(int R, int E);
 int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
-                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, int* err, int num_sms,
+                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, bool early, int* err, int num_sms,
                    cudaStream_t stream);
 // dw[e] [N, K] = sum over the rows of e of dy[r]^T x[r], bf16 or fp32; zeros for an expert without rows
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,

@@ -521,7 +521,7 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
     const Tensor xg = listed ? x : do_gather(x, m.r.rows, k, make);
     const int rc = tb::grouped_swiglu(bf(xg), xg.stride(0), listed ? m.r.rows.data_ptr<int>() : nullptr, (int)k, (int)x.size(0), bf(wgu), m.r.offsets.data_ptr<int>(), bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr,
                                       m.q.defined() ? m.q.data_ptr<int8_t>() : nullptr, m.q.defined() ? m.scales.data_ptr<float>() : nullptr,
-                                      (int)R, (int)E, (int)F, (int)D, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+                                      (int)R, (int)E, (int)F, (int)D, true, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
     TORCH_CHECK(rc == 0, "expert_mlp: gate / up product failed with code ", rc);
     g_launches += 1;
   }
@@ -529,7 +529,7 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
   if (R > 0 && tb::grouped_gemm_few((int)R, (int)E)) {
     y = make("expert_mlp.y", {R, D}, wgu.options().dtype(torch::kFloat32));
     const int rc = tb::grouped_gemm_f32(bf(act), F, bf(wd), m.r.offsets.data_ptr<int>(), y.data_ptr<float>(), (int)R, (int)E, (int)D, (int)F,
-                                        attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+                                        true, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
     TORCH_CHECK(rc == 0, "expert_mlp: down product failed with code ", rc);
     g_launches += 1;
   } else {
