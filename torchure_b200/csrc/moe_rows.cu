@@ -3,7 +3,8 @@
 // All three move each byte once and are bound by memory; 8 columns per lane, 16-byte accesses of bf16 rows.  The gather gives a row to a
 // warp, with four loads on their way per lane (8192 x 1024 to 16384 rows 9.5 us, 15 with one).  The sum gives 8 columns of a token to a
 // thread and keeps an SM full of threads, four choices' loads on their way each: one warp per token with as many loads took 19.5 us
-// for the same rows, short-lived warps that each wait for slots, then for rows.  Rows that are no multiple of 8 columns or start
+// for the same rows, short-lived warps that each wait for slots, then for rows; now 12.4.  The gradient of the sum gives a choice to a warp
+// (13.5 for the same).  Rows that are no multiple of 8 columns or start
 // off a 16-byte boundary are read value by value.
 #include "common.cuh"
 #include "moe_api.h"

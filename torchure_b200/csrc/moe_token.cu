@@ -5,7 +5,8 @@
 // -> down -> weighted sum, a launch each on the way for more tokens.  Here every CTA of the first kernel finds the choices itself (a warp
 // per token, about 1 us), and a warp computes gate and up of two units by reading four rows of the matrices; in the second kernel a
 // warp computes one column of one token's output over all its experts.  Matrices are read past L1.  An expert that several tokens chose
-// is read for each of them, from L2, which is why the kernels stop at four tokens.
+// is read for each of them, from L2, which is why the kernels stop at four tokens.  One token, 2 of 8 experts of 1024 x 1536: 7.5 and 8.8 us from
+// cold memory, 13.2 a call with the second kernel's launch under the first (2.9 us at copy bandwidth; the host takes 10.6).
 #include "common.cuh"
 #include "moe_api.h"
 
