@@ -338,6 +338,31 @@ def test_swiglu_8bit(shape):
     assert ((dgu.reshape(-1, 2 * F).double() - k.grad).abs() <= U * k.grad.abs() + slack + 1e-38).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 7), (2000, 33), (300, 2557), (9, 8191), (3, 8193), (100, 64), (1777, 201)])
+@pytest.mark.parametrize("start", [0, 1, 5])
+def test_rows_on_any_boundary(rows, cols, start):
+    """Widths off the vectors, rows that start anywhere and tiles of several rows give the bits of a padded, aligned copy."""
+    def at(n, seed):        # n columns, the first of them `start` values past an aligned address
+        return rand(rows * n + start, seed=seed)[start:].view(rows, n)
+
+    x = at(cols, 1)
+    room = -cols % 64
+    a, b = act8.quantize8(x), act8.quantize8(torch.nn.functional.pad(x, (0, room)))
+    assert torch.equal(a.values, b.values[:, :cols]) and torch.equal(a.scales, b.scales)
+    assert torch.equal(act8.dequantize8(a), act8.dequantize8(b)[:, :cols])
+
+    def halves(t):
+        return torch.nn.functional.pad(t.view(rows, 2, cols), (0, room)).reshape(rows, -1)
+
+    gu, dact = at(2 * cols, 2), at(cols, 3)
+    odd, even = gu.clone().requires_grad_() if start == 0 else gu.requires_grad_(), halves(gu.detach()).requires_grad_()
+    act, want = act8.swiglu_8bit(odd), act8.swiglu_8bit(even)
+    assert torch.equal(act, want[:, :cols])
+    d1, = torch.autograd.grad(act, (odd,), dact)
+    d2, = torch.autograd.grad(want, (even,), torch.nn.functional.pad(dact, (0, room)))
+    assert torch.equal(d1, d2.view(rows, 2, -1)[:, :, :cols].reshape(rows, -1))
+
+
 def test_swiglu_8bit_keeps_half_the_bytes():
     gu = rand(4096, 2048, seed=1).requires_grad_()
     torch.cuda.synchronize()
