@@ -616,8 +616,8 @@ void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const in
   if (R <= 0 || F <= 0) return;
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(R, kWarps)), block(kThreads);
-  if (gu) launch_pdl(expert_swiglu_bwd_kernel<false>, grid, block, 0, stream, s, gu, q, scales, weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb);
-  else launch_pdl(expert_swiglu_bwd_kernel<true>, grid, block, 0, stream, s, gu, q, scales, weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb);
+  launch_pdl(gu ? expert_swiglu_bwd_kernel<false> : expert_swiglu_bwd_kernel<true>, grid, block, 0, stream, s, gu, q, scales, weights, slots,
+             offsets, dgu, act_w, dweights, R, E, F, nb);
 }
 
 }  // namespace tb

@@ -19,8 +19,8 @@
 // fragments.  The activation is taken from the fp32 sums; gate and up are stored beside it in bf16, or in 8 bits with a scale for the
 // CTA's 64 units (act8.cu has the format), or not at all.
 //
-// Bound by the tensor cores at the clock that the power allows (1.58 GHz).  16384 rows in 8 uneven groups, 1024 x 2 x 1536: 74 us forward, 77 for
-// the rows' gradient, 76 for the matrices' (an equally large dense product 71), with SwiGLU 86 (73 if gate and up are not kept, 94 if in 8
+// Bound by the tensor cores at the clock that the power allows (1.58 GHz).  16384 rows in 8 uneven groups, 1024 x 2 x 1536: 74 us forward, 77
+// for the rows' gradient, 76 for the matrices' (an equally large dense product 71), with SwiGLU 86 (73 if gate and up are not kept, 94 if in 8
 // bits); 32768 rows in 32 groups, 1024 x 1536, back to back: 90, 89, 94.  All sums are fp32; results are rounded once, to bf16, which the next
 // product reads (an output that is only added up, of few rows, stays fp32).
 //
@@ -541,7 +541,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int UNIT = kGateUp<EPI> ? BM / 2 : BM;
   const int n0 = static_cast<int>(blockIdx.x) * UNIT, all_kb = (K + BK - 1) / BK;
-  const int early = EARLY ? E : 0, loaded = static_cast<int>(blockIdx.y) < early ? min(all_kb, FEW_STAGES) : 0;      // k-blocks of the matrix under way
+  const int early = EARLY ? E : 0;
+  const int loaded = static_cast<int>(blockIdx.y) < early ? min(all_kb, FEW_STAGES) : 0;      // k-blocks of the matrix under way
   if (warp == 1) {      // (warp 0 looks for its rows meanwhile)
     if (elect_one()) {
       tma_prefetch_desc(&tmW);
@@ -1018,7 +1019,8 @@ template <bool W_MN, int EPI>
 int launch_rows(const __nv_bfloat16* x, int64_t ldx, const Rows& rows, const __nv_bfloat16* w, const int* offsets, const RowsOut& out, int R,
                 int E, int K, bool early, int* err, int num_sms, cudaStream_t stream) {
   const int N = out.width;
-  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 || ((reinterpret_cast<uintptr_t>(out.y) | reinterpret_cast<uintptr_t>(out.y32)) & 15) != 0)
+  if (R < 1 || E < 1 || E > kMaxExperts || N < 1 || K < 1 || N % 8 != 0 ||
+      ((reinterpret_cast<uintptr_t>(out.y) | reinterpret_cast<uintptr_t>(out.y32)) & 15) != 0)
     return -1;
   const bool few = R <= static_cast<int64_t>(FEW_AVERAGE) * E;
   if (rows.list && !(few && EPI == kSwiglu)) return -2;

@@ -54,8 +54,8 @@ int grouped_gemm_f32(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w
 // Only where grouped_swiglu_listed, and not with q.
 bool grouped_swiglu_listed(int R, int E);
 int grouped_swiglu(const __nv_bfloat16* x, int64_t ldx, const int* list, int k, int count, const __nv_bfloat16* w, const int* offsets,
-                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, bool early, int* err, int num_sms,
-                   cudaStream_t stream);
+                   __nv_bfloat16* act, __nv_bfloat16* gu, int8_t* q, float* scales, int R, int E, int F, int K, bool early, int* err,
+                   int num_sms, cudaStream_t stream);
 // dw[e] [N, K] = sum over the rows of e of dy[r]^T x[r], bf16 or fp32; zeros for an expert without rows
 int grouped_wgrad(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* x, int64_t ldx, const int* offsets, void* dw, bool dw_bf16,
                   int R, int E, int N, int K, int* err, int num_sms, cudaStream_t stream);

@@ -47,6 +47,7 @@ std::atomic<int64_t> g_launches{0};      // kernels launched by the calls of thi
 
 const __nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
 __nv_bfloat16* bfm(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+bool at16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
 bool bf16_or_f32(const Tensor& t, const char* what) {
@@ -292,8 +293,7 @@ Tensor do_swiglu8_bwd(const Tensor& dact, const Tensor& q, const Tensor& s, cons
 Tensor rows_of(const Tensor& x) { return x.size(-1) <= 1 || x.stride(-1) == 1 ? x : x.contiguous(); }
 // x [R, K] with columns in eights (zeros behind), the row stride and the base on 16 bytes
 Tensor operand(const Tensor& x) {
-  if (x.size(1) % 8 == 0 && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
-      (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0)
+  if (x.size(1) % 8 == 0 && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) && at16(x))
     return x;
   return x.size(1) % 8 ? at::constant_pad_nd(x, {0, (8 - x.size(1) % 8) % 8}).contiguous() : x.clone(at::MemoryFormat::Contiguous);
 }
@@ -302,7 +302,7 @@ Tensor matrices(const Tensor& w) {
   Tensor b = w.scalar_type() == torch::kBFloat16 ? w : w.to(torch::kBFloat16);
   const int64_t n = (8 - w.size(1) % 8) % 8, k = (8 - w.size(2) % 8) % 8;
   b = n || k ? at::constant_pad_nd(b, {0, k, 0, n}).contiguous() : b.contiguous();
-  return (reinterpret_cast<uintptr_t>(b.data_ptr()) & 15) == 0 ? b : b.clone();
+  return at16(b) ? b : b.clone();
 }
 
 // ---- autograd nodes ----------------------------------------------------------------------------------
@@ -366,7 +366,8 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
 
 Tensor moe_dispatch(const Tensor& x, const Tensor& slots, const Tensor& rows, bool poison) {
   c10::cuda::CUDAGuard guard(x.device());
-  TORCH_CHECK_VALUE(x.dim() == 2 && slots.dim() == 2 && x.size(0) == slots.size(0), "dispatch: ", slots.size(0), " tokens were routed, got ", x.sizes());
+  TORCH_CHECK_VALUE(x.dim() == 2 && slots.dim() == 2 && x.size(0) == slots.size(0), "dispatch: ", slots.size(0), " tokens were routed, got ",
+                    x.sizes());
   check_ints(slots, rows.numel(), x, "dispatch: slots");
   return DispatchNode::apply(rows_of(x), slots, rows, poison);
 }
@@ -390,7 +391,8 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
 Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, const Tensor& offsets, bool f32, bool poison) {
   check_bf16(y, "combine");
   c10::cuda::CUDAGuard guard(y.device());
-  TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ", y.sizes());
+  TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ",
+                    y.sizes());
   check_ints(offsets, offsets.numel(), y, "combine: offsets");
   return CombineNode::apply(y.contiguous(), weights.contiguous(), slots, offsets, f32, poison);
 }
@@ -488,14 +490,16 @@ constexpr int64_t BESIDE_MIN_ROWS = 4096;
 bool runs_by_token(const Tensor& x, int64_t k, const Tensor& wgu, const Tensor& wd) {
   return x.size(0) >= 1 && x.size(0) <= TOKEN_MAX && x.size(0) * k <= tb::kTokenChoices && x.stride(0) % 8 == 0 &&
          x.size(0) * k * wd.size(1) * wd.size(2) * 6 <= TOKEN_BYTES &&
-         ((reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(wgu.data_ptr()) | reinterpret_cast<uintptr_t>(wd.data_ptr())) & 15) == 0;
+         at16(x) && at16(wgu) && at16(wd);
 }
 
 // out, aux
-variable_list mlp_by_token(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, const Outputs& make) {
+variable_list mlp_by_token(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity,
+                           const Outputs& make) {
   const int64_t T = x.size(0), D = x.size(1), E = wd.size(0), F = wd.size(2);
   TORCH_CHECK_VALUE(E <= tb::kMaxExperts, "expert_mlp: 1 to ", tb::kMaxExperts, " experts, got ", E);
-  TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= tb::kMaxChoices, "expert_mlp: top_k of ", k, " among ", E, " experts (at most ", tb::kMaxChoices, ")");
+  TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= tb::kMaxChoices, "expert_mlp: top_k of ", k, " among ", E, " experts (at most ",
+                    tb::kMaxChoices, ")");
   TORCH_CHECK_VALUE(capacity >= 0 && capacity < (1ll << 31), "expert_mlp: capacity ", capacity);
   const Tensor out = make("expert_mlp.out", {T, D}, x.options()), aux = make("expert_mlp.aux", {}, x.options().dtype(torch::kFloat32));
   const Tensor scratch = empty({tb::token_scratch_bytes((int)T, (int)k, (int)F)}, x.options().dtype(torch::kUInt8));
@@ -510,8 +514,8 @@ variable_list mlp_by_token(const Tensor& x, const Tensor& logits, const Tensor& 
 // Whether the gate / up product reads token rows where they lie: few rows per expert, bf16, on 16 bytes.  Others are put in expert order
 // first, rounded where they are fp32.
 bool rows_stay(const Tensor& x, int64_t R, int64_t E, bool in8) {
-  return tb::grouped_swiglu_listed((int)R, (int)E) && !in8 && x.scalar_type() == torch::kBFloat16 && x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
-         (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0;
+  return tb::grouped_swiglu_listed((int)R, (int)E) && !in8 && x.scalar_type() == torch::kBFloat16 && x.stride(1) == 1 &&
+         x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) && at16(x);
 }
 
 // Rounded to bf16 between the kernels are gate and up (kept for the backward pass only), the activation (the down product's operand) and, unless
@@ -532,9 +536,11 @@ Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tens
   if (R > 0) {
     const bool listed = rows_stay(x, R, E, m.q.defined());
     const Tensor xg = listed ? x : do_gather(x, m.r.rows, k, make);
-    const int rc = tb::grouped_swiglu(bf(xg), xg.stride(0), listed ? m.r.rows.data_ptr<int>() : nullptr, (int)k, (int)x.size(0), bf(wgu), m.r.offsets.data_ptr<int>(), bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr,
-                                      m.q.defined() ? m.q.data_ptr<int8_t>() : nullptr, m.q.defined() ? m.scales.data_ptr<float>() : nullptr,
-                                      (int)R, (int)E, (int)F, (int)D, true, attn_err_word().data_ptr<int>(), bind_num_sms(), cur_stream());
+    const int rc = tb::grouped_swiglu(
+        bf(xg), xg.stride(0), listed ? m.r.rows.data_ptr<int>() : nullptr, (int)k, (int)x.size(0), bf(wgu), m.r.offsets.data_ptr<int>(),
+        bfm(act), m.gu.defined() ? bfm(m.gu) : nullptr, m.q.defined() ? m.q.data_ptr<int8_t>() : nullptr,
+        m.q.defined() ? m.scales.data_ptr<float>() : nullptr, (int)R, (int)E, (int)F, (int)D, true, attn_err_word().data_ptr<int>(),
+        bind_num_sms(), cur_stream());
     TORCH_CHECK(rc == 0, "expert_mlp: gate / up product failed with code ", rc);
     g_launches += 1;
   }
@@ -693,7 +699,8 @@ variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& fi
                    wd.scalar_type());
   TORCH_CHECK_VALUE(bits == 8 || bits == 16, "expert_mlp: activations are kept in 8 or 16 bits, not ", bits);
   const bool pair = has(second);
-  TORCH_CHECK_VALUE(!pair || (second->sizes() == first.sizes() && second->scalar_type() == first.scalar_type() && second->device() == first.device()),
+  TORCH_CHECK_VALUE(!pair || (second->sizes() == first.sizes() && second->scalar_type() == first.scalar_type() &&
+                              second->device() == first.device()),
                     "expert_mlp: w_gate and w_up differ");
   TORCH_CHECK_VALUE(wd.dim() == 3 && first.dim() == 3, "expert_mlp: matrices [E, 2F, D] and [E, D, F] expected");
   const int64_t E = wd.size(0), D = wd.size(1), F = wd.size(2);
@@ -705,7 +712,8 @@ variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& fi
                     "expert_mlp: tensors on several GPUs");
   c10::cuda::CUDAGuard guard(x.device());
   const bool keep = at::GradMode::is_enabled() &&
-                    (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() || (pair && second->requires_grad()));
+                    (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() ||
+                     (pair && second->requires_grad()));
   if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, bits, poison);
   const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
   if (runs_by_token(x, k, wgu, wdb)) {

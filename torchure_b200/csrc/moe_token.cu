@@ -5,8 +5,8 @@
 // -> down -> weighted sum, a launch each on the way for more tokens.  Here every CTA of the first kernel finds the choices itself (a warp
 // per token, about 1 us), and a warp computes gate and up of two units by reading four rows of the matrices; in the second kernel a
 // warp computes one column of one token's output over all its experts.  Matrices are read past L1.  An expert that several tokens chose
-// is read for each of them, from L2, which is why the kernels stop at four tokens.  One token, 2 of 8 experts of 1024 x 1536: 7.5 and 8.8 us from
-// cold memory, 13.2 a call with the second kernel's launch under the first (2.9 us at copy bandwidth; the host takes 10.6).
+// is read for each of them, from L2, which is why the kernels stop at four tokens.  One token, 2 of 8 experts of 1024 x 1536: 7.5 and 8.8 us
+// from cold memory, 13 a call with the second kernel's launch under the first (2.9 us at copy bandwidth; the host takes 10.6).
 #include "common.cuh"
 #include "moe_api.h"
 
@@ -241,7 +241,9 @@ int64_t token_scratch_bytes(int T, int k, int F) { return sizeof(Choices) + stat
 int token_mlp(const void* logits, bool logits_bf16, int64_t ldl, const void* x, bool x_bf16, int64_t ldx, const __nv_bfloat16* w_gate_up,
               const __nv_bfloat16* w_down, void* out, float* aux, void* scratch, int T, int E, int k, int capacity, int D, int F,
               cudaStream_t stream) {
-  if (T < 1 || T > kTokenTokens || k < 1 || k > E || T * k > kTokenChoices || E > kMaxExperts || D % 8 != 0 || F % 8 != 0 || ldx % 8 != 0) return -1;
+  if (T < 1 || T > kTokenTokens || k < 1 || k > E || T * k > kTokenChoices || E > kMaxExperts || D % 8 != 0 || F % 8 != 0 ||
+      ldx % 8 != 0)
+    return -1;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w_gate_up) | reinterpret_cast<uintptr_t>(w_down) |
         reinterpret_cast<uintptr_t>(scratch)) & 15) != 0)
     return -11;
