@@ -12,7 +12,7 @@ shuffle is the even-split ``all_to_all``.  Here:
 * ``experts="grouped"`` runs the layer on the operators of ``ops/moe.py``: rows in expert order instead of padded buffers, products
   grouped by expert instead of batched library products, with ``act_bits=8`` gate and up kept in 8 bits for the backward pass.  The
   capacity drops the same choices (``capacity_factor`` 0: none are dropped).  Spread over a mesh axis the exchange keeps its padded
-  buffers and the grouped products run on what arrives.
+  buffers (with ``capacity_factor`` 0 a row for every token of the rank) and the grouped products run on what arrives.
 """
 
 from __future__ import annotations
@@ -80,6 +80,9 @@ class MoELayer(nn.Module):
             self.w_down.copy_(w_down[lo:lo + self.local_E])
 
     def capacity(self, tokens: int) -> int:
+        """Rows of an expert's buffer for ``tokens`` tokens."""
+        if self.experts == "grouped" and self.cf <= 0:
+            return max(1, tokens)          # a token's choices are different experts: nothing can be dropped
         return max(1, int(self.cf * tokens * self.k / self.E + 0.999))
 
     def _grouped_products(self, work: torch.Tensor) -> torch.Tensor:
