@@ -49,3 +49,11 @@ def test_capacity_factor_0_drops_nothing(favourite):
 
 def _without_limit(rank, world, favourite):
     _against_one_piece(rank, world, favourite, capacity_factor=0.0)
+
+
+def test_8_bit_checkpoints_are_taken():
+    run_distributed(_in_8_bits, 2, timeout_s=120)
+
+
+def _in_8_bits(rank, world):
+    _against_one_piece(rank, world, False, capacity_factor=8.0, act_bits=8)

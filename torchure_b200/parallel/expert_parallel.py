@@ -22,7 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from torchure_b200.core.collective import all_to_all
-from torchure_b200.ops import act8, moe
+from torchure_b200.ops import act8, moe, oracle
 
 
 class _AllToAll(torch.autograd.Function):
@@ -93,8 +93,8 @@ class MoELayer(nn.Module):
             rows = rows.to(torch.bfloat16)
         offsets = torch.arange(E + 1, device=work.device, dtype=torch.int32) * R
         gu = moe.grouped_linear(rows, torch.cat([self.w_gate, self.w_up], dim=1), offsets)
-        if self.act_bits == 8 and gu.dtype == torch.bfloat16:
-            act = act8.swiglu_8bit(gu)
+        if self.act_bits == 8:      # (the operator takes bf16, the plain statement what the CPU path has)
+            act = act8.swiglu_8bit(gu) if gu.dtype == torch.bfloat16 else oracle.swiglu_8bit(gu)
         else:
             g, u = gu.chunk(2, dim=-1)
             act = F.silu(g) * u
