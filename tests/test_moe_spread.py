@@ -21,12 +21,12 @@ def _against_one_piece(rank, world, favourite, **kw):
     full, spread = (MoELayer(16, 32, num_experts=4, top_k=2, experts="grouped", **kw) for _ in range(2))
     with torch.no_grad():
         for w in (full.w_gate, full.w_up, full.w_down):
-            w.mul_(10)
+            w.mul_(10 * 64).round_().div_(64)      # gate and up come out exact in any order of the sums, and so do their 8 bits
         if favourite:      # every token prefers one expert
             full.router.weight[:, 0] = torch.tensor([0.0, 9.0, 0.0, 0.0])
     spread.load_state_dict(full.state_dict())
     spread.shard_(Mesh({"ep": world}), "ep")
-    x = torch.randn(64, 16, generator=torch.Generator().manual_seed(rank))
+    x = torch.randn(64, 16, generator=torch.Generator().manual_seed(rank)).mul(16).round().div(16)
     if favourite:
         x[:, 0] = 1.0
     a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
