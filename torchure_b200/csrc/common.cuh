@@ -152,6 +152,21 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code)) != 0;
 }
+// The same for the warps that use named barrier `id` (`threads` threads) behind the wait: one verdict for all of them, so that none goes on
+// to stand in that barrier when another gave up and left.  Every one of these warps comes here, whatever its own poll said.
+__device__ __forceinline__ bool mbar_wait_warps(uint64_t* bar, uint32_t parity, int* err, int code, int id, int threads) {
+  const uint32_t mine = mbar_wait_warp(bar, parity, err, code) ? 1u : 0u;
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(mine), "r"(id), "r"(threads)
+      : "memory");
+  return all != 0;
+}
 __device__ __forceinline__ void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }

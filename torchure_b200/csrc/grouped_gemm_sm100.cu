@@ -489,7 +489,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     for (int n = cluster; ok && at.find(n, r0, live, col); n += num_clusters) {
       const int n0 = col * UNIT + static_cast<int>(rank) * (UNIT / 2);
       const int acc = it & 1;
-      if (!mbar_wait_warp(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait)) { ok = false; break; }
+      if (!mbar_wait_warps(&tfull[acc], (it >> 1) & 1, err, kErrEpilogueTmemFullWait, 1 + part, 128)) { ok = false; break; }
       tc_fence_after();
       const uint32_t lead_tempty = map_to_cta(&tempty[acc], 0);
       rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, q, epi + part * kPartBytes<EPI>, 1 + part, r0,
@@ -678,7 +678,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
   } else {
     const int q = warp & 3;
-    if (num_kb > 0 && mbar_wait_warp(tfull, 0, err, kErrEpilogueTmemFullWait)) {
+    if (num_kb > 0 && mbar_wait_warps(tfull, 0, err, kErrEpilogueTmemFullWait, 1, 128)) {
       tc_fence_after();
       rows_epilogue<EPI>(out, tmem_base + (static_cast<uint32_t>(q * 32) << 16), q, smem, 1, r0, live, 0, EPI_ROWS, n0, [] {});
     }
