@@ -174,6 +174,7 @@ std::tuple<Tensor, Tensor> do_combine_bwd(const Tensor& dout, const Tensor& y, c
   TORCH_CHECK(weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.numel() == T * k, "combine_bwd: weights");
   Tensor dy = make("combine_bwd.dy", {T * k, D}, y.options());
   Tensor dw = make("combine_bwd.dweights", {T, k}, weights.options());
+  if (D == 0) return {dy, dw.zero_()};      // sums of no terms
   const Overlap overlap;
   tb::rows_combine_bwd(dout.data_ptr(), b16, dout.stride(0), bf(y), weights.data_ptr<float>(), slots.data_ptr<int>(),
                        offsets.data_ptr<int>(), bfm(dy), dw.data_ptr<float>(), (int)T, (int)k, (int)E, (int)D, cur_stream());
