@@ -52,3 +52,28 @@ def test_combine_of_rows_without_columns():
     finally:
         debug.enable(False)
     assert out.shape == (5, 0) and dy.shape == (10, 0) and dw.shape == (5, 2) and (dw == 0).all()
+
+
+@pytest.mark.parametrize("name", ["route", "grouped_linear", "expert_mlp of a token", "expert_mlp", "expert_mlp by its matrices", "dispatch",
+                                  "combine", "swiglu_8bit"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(name, grad):
+    """A tangent is never dropped without a word."""
+    x, logits, wgu, wd = mlp_inputs(2 if name.endswith("token") else 40, 4, 64, 64)
+    offsets = edges_of([0, 5, 10, 20, 40])
+    r = moe.route(logits, 2)
+    call, t = {
+        "route": (lambda v: moe.route(v, 2), logits),
+        "grouped_linear": (lambda v: moe.grouped_linear(v, wgu, offsets), x),
+        "expert_mlp of a token": (lambda v: moe.expert_mlp(v, logits, wgu, wd, 2), x),
+        "expert_mlp": (lambda v: moe.expert_mlp(x, v, wgu, wd, 2), logits),
+        "expert_mlp by its matrices": (lambda v: moe.expert_mlp(x, logits, (wgu[:, :64], v), wd, 2), wgu[:, 64:]),
+        "dispatch": (lambda v: moe.dispatch(v, r), x),
+        "combine": (lambda v: moe.combine(v, r), rand(r.rows.numel(), 64)),
+        "swiglu_8bit": (act8.swiglu_8bit, x),
+    }[name]
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = fwd.make_dual(t, torch.ones_like(t))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        call(t)

@@ -313,6 +313,12 @@ using torch::autograd::variable_list;
 void only_once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient itself has no gradient (create_graph is not supported)");
 }
+// A dual tensor asks for no gradient, so that calls without gradients would pass its tangent by
+template <class... Ts>
+void no_tangents(const char* what, const Ts&... tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(... || (tensors.defined() && tensors._fw_grad(0).defined())), what,
+                              ": forward-mode derivatives are not supported");
+}
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 struct RouteNode : torch::autograd::Function<RouteNode> {
@@ -337,6 +343,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
 };
 
 variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
+  no_tangents("route", logits);
   TORCH_CHECK_VALUE(logits.dim() == 2 && logits.is_floating_point(), "route: logits [tokens, experts] expected, got ", logits.scalar_type(),
                     " ", logits.sizes());
   c10::cuda::CUDAGuard guard(logits.device());
@@ -366,6 +373,7 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
 };
 
 Tensor moe_dispatch(const Tensor& x, const Tensor& slots, const Tensor& rows, bool poison) {
+  no_tangents("dispatch", x);
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK_VALUE(x.dim() == 2 && slots.dim() == 2 && x.size(0) == slots.size(0), "dispatch: ", slots.size(0), " tokens were routed, got ",
                     x.sizes());
@@ -390,6 +398,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
 };
 
 Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, const Tensor& offsets, bool f32, bool poison) {
+  no_tangents("combine", y, weights);
   check_bf16(y, "combine");
   c10::cuda::CUDAGuard guard(y.device());
   TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ",
@@ -430,6 +439,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
 };
 
 Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, bool poison) {
+  no_tangents("grouped_linear", x, w);
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3 && x.size(1) == w.size(2), "grouped_linear: rows ", x.sizes(), " and matrices ", w.sizes(),
                     " do not fit");
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() == w.size(0) + 1, "grouped_linear: ", w.size(0) + 1, " offsets expected, got ",
@@ -462,6 +472,7 @@ struct Swiglu8Node : torch::autograd::Function<Swiglu8Node> {
 };
 
 Tensor swiglu_8bit(const Tensor& gu, bool poison) {
+  no_tangents("swiglu_8bit", gu);
   check_bf16(gu, "swiglu_8bit");
   TORCH_CHECK_VALUE(gu.dim() >= 1 && gu.size(-1) % 2 == 0, "swiglu_8bit: gate and up columns expected, got ", gu.sizes());
   c10::cuda::CUDAGuard guard(gu.device());
@@ -692,6 +703,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
 
 variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
                          int64_t capacity, int64_t bits, bool poison) {
+  no_tangents("expert_mlp", x, logits, first, has(second) ? *second : Tensor(), wd);
   check_rows(x, "expert_mlp: x");
   check_rows(logits, "expert_mlp: logits");
   bf16_or_f32(x, "expert_mlp: x");
