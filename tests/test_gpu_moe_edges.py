@@ -77,3 +77,18 @@ def test_forward_mode_is_refused(name, grad):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             call(dual)
         call(t)
+
+
+@pytest.mark.parametrize("N", [64, 33])
+def test_grouped_linear_result_changes_in_place(N):
+    offsets = edges_of([0, 7, 50])
+    x, w, dy = rand(50, 64, seed=1).requires_grad_(), rand(2, N, 64, seed=2).requires_grad_(), rand(50, N, seed=3)
+    y = moe.grouped_linear(x, w, offsets)
+    y.mul_(2)
+    got = torch.autograd.grad(y, (x, w), dy)
+    want = torch.autograd.grad(moe.grouped_linear(x, w, offsets) * 2, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        y = moe.grouped_linear(x, w, offsets)
+    y.mul_(torch.ones(N, device="cuda", requires_grad=True))
+    assert y.requires_grad

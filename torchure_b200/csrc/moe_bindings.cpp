@@ -408,6 +408,7 @@ Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, 
 }
 
 struct GroupedNode : torch::autograd::Function<GroupedNode> {
+  // with columns in eights, as the kernel writes them
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, bool poison) {
     const Tensor xb = operand(x), wb = matrices(w);
     const Tensor y = do_grouped(xb, wb, offsets, false, Outputs{poison});
@@ -416,7 +417,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     ctx->saved_data["k"] = w.size(2);
     ctx->saved_data["type"] = static_cast<int64_t>(w.scalar_type());
     ctx->saved_data["poison"] = poison;
-    return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1));
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once("grouped_linear");
@@ -451,9 +452,11 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, b
   c10::cuda::CUDAGuard guard(x.device());
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad())) {
     const Tensor y = do_grouped(operand(x), matrices(w), offsets.contiguous(), false, Outputs{poison});
-    return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1));
+    return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1)).detach();
   }
-  return GroupedNode::apply(x, w, offsets.contiguous(), poison);
+  // (a view made inside the node, or without gradients and not detached, could not be changed in place)
+  const Tensor y = GroupedNode::apply(x, w, offsets.contiguous(), poison);
+  return y.size(1) == w.size(1) ? y : y.narrow(1, 0, w.size(1));
 }
 
 struct Swiglu8Node : torch::autograd::Function<Swiglu8Node> {
