@@ -92,3 +92,22 @@ def test_grouped_linear_result_changes_in_place(N):
         y = moe.grouped_linear(x, w, offsets)
     y.mul_(torch.ones(N, device="cuda", requires_grad=True))
     assert y.requires_grad
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_experts_of_a_spread_layer_with_the_kernels_off(bits):
+    """What runs on the buffers of a layer spread over ranks, on the plain statements on a GPU: in the layer's own precision."""
+    from torchure_b200.parallel.expert_parallel import MoELayer
+
+    torch.manual_seed(0)
+    layer = MoELayer(64, 72, num_experts=4, top_k=2, experts="grouped", act_bits=bits).cuda()
+    work = torch.randn(4, 9, 64, device="cuda", generator=gen(0))
+    got = layer._grouped_products(work)
+    ops.force_fallback(True)
+    try:
+        plain = layer._grouped_products(work)
+        plain.sum().backward()
+    finally:
+        ops.force_fallback(False)
+    assert plain.dtype == torch.float32 and layer.w_gate.grad is not None
+    assert (got.double() - plain.double()).norm() < 5 * RMS * plain.double().norm()

@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from torchure_b200 import ops
 from torchure_b200.core.collective import all_to_all
 from torchure_b200.ops import act8, moe, oracle
 
@@ -89,7 +90,7 @@ class MoELayer(nn.Module):
         """The experts' feed-forwards on buffers [local_E, rows, hidden] of what the ranks sent."""
         E, R, D = work.shape
         rows = work.reshape(E * R, D)
-        if rows.is_cuda:
+        if rows.is_cuda and ops.available():      # (the plain statements stay in the layer's precision)
             rows = rows.to(torch.bfloat16)
         offsets = torch.arange(E + 1, device=work.device, dtype=torch.int32) * R
         gu = moe.grouped_linear(rows, torch.cat([self.w_gate, self.w_up], dim=1), offsets)
