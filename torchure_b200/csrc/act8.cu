@@ -548,76 +548,84 @@ bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 
-void quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, int64_t M, int N, cudaStream_t stream) {
-  if (M <= 0 || N <= 0) return;
+int quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, int64_t M, int N, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
   const int nb = blocks_of(N);
   const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
+  cudaError_t rc;
   if (N % 8 == 0 && ldx % 8 == 0 && at16(x) && at16(q)) {
-    launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+    rc = launch_pdl(quantize8_kernel<true>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
   } else if (ldx == N && N <= kOddValues) {
     const int rows = tile_rows(M, N);
-    launch_pdl(quantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, x, q, scales, M, N, nb, rows);
+    rc = launch_pdl(quantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, x, q, scales, M, N, nb, rows);
   } else {
-    launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
+    rc = launch_pdl(quantize8_kernel<false>, grid, block, 0, stream, x, ldx, q, scales, units, N, FastDiv(nb));
   }
+  return launch_code(rc);
 }
 
-void dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream) {
-  if (M <= 0 || N <= 0) return;
+int dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
   const int nb = blocks_of(N);
   const dim3 grid(grid_for(M * nb, 4 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
+  cudaError_t rc;
   if (N % 8 == 0 && at16(x) && at16(q)) {
-    launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+    rc = launch_pdl(dequantize8_kernel<true>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
   } else if (N <= kOddValues) {
     const int rows = tile_rows(M, N);
-    launch_pdl(dequantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, q, scales, x, M, N, nb, rows);
+    rc = launch_pdl(dequantize8_rows_kernel, dim3(tile_grid(M, rows)), block, rows * N * 3 + 64, stream, q, scales, x, M, N, nb, rows);
   } else {
-    launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
+    rc = launch_pdl(dequantize8_kernel<false>, grid, block, 0, stream, q, scales, x, units, N, FastDiv(nb));
   }
+  return launch_code(rc);
 }
 
-void swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
+int swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
                  cudaStream_t stream) {
-  if (M <= 0 || F <= 0) return;
+  if (M <= 0 || F <= 0) return 0;
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
+  cudaError_t rc;
   if (F % 8 == 0 && ldgu % 8 == 0 && at16(gu) && at16(act) && at16(q)) {
-    launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+    rc = launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
   } else if (ldgu == 2 * static_cast<int64_t>(F) && 2 * F <= kOddValues) {
     const int rows = tile_rows(M, 2 * F);
-    launch_pdl(swiglu8_fwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, gu, act, q, scales, M, F, nb, rows);
+    rc = launch_pdl(swiglu8_fwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, gu, act, q, scales, M, F, nb, rows);
   } else {
-    launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+    rc = launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
   }
+  return launch_code(rc);
 }
 
-void swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M, int F,
+int swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M, int F,
                  cudaStream_t stream) {
-  if (M <= 0 || F <= 0) return;
+  if (M <= 0 || F <= 0) return 0;
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(M * nb, 2 * kGroups)), block(kThreads);
   const uint32_t units = static_cast<uint32_t>(M * nb);
+  cudaError_t rc;
   if (F % 8 == 0 && ldd % 8 == 0 && at16(dact) && at16(dgu) && at16(q)) {
-    launch_pdl(swiglu8_bwd_kernel<true>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
+    rc = launch_pdl(swiglu8_bwd_kernel<true>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
   } else if (ldd == F && 2 * F <= kOddValues) {
     const int rows = tile_rows(M, 2 * F);
-    launch_pdl(swiglu8_bwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, dact, q, scales, dgu, M, F, nb, rows);
+    rc = launch_pdl(swiglu8_bwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, dact, q, scales, dgu, M, F, nb, rows);
   } else {
-    launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
+    rc = launch_pdl(swiglu8_bwd_kernel<false>, grid, block, 0, stream, dact, ldd, q, scales, dgu, units, F, FastDiv(nb));
   }
+  return launch_code(rc);
 }
 
-void expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,
+int expert_swiglu_bwd(const __nv_bfloat16* s, const __nv_bfloat16* gu, const int8_t* q, const float* scales, const float* weights,
                        const int* slots, const int* offsets, __nv_bfloat16* dgu, __nv_bfloat16* act_w, float* dweights, int R, int E,
                        int F, cudaStream_t stream) {
-  if (R <= 0 || F <= 0) return;
+  if (R <= 0 || F <= 0) return 0;
   const int nb = blocks_of(F);
   const dim3 grid(grid_for(R, kWarps)), block(kThreads);
-  launch_pdl(gu ? expert_swiglu_bwd_kernel<false> : expert_swiglu_bwd_kernel<true>, grid, block, 0, stream, s, gu, q, scales, weights, slots,
-             offsets, dgu, act_w, dweights, R, E, F, nb);
+  return launch_code(launch_pdl(gu ? expert_swiglu_bwd_kernel<false> : expert_swiglu_bwd_kernel<true>, grid, block, 0, stream, s, gu, q, scales,
+                                weights, slots, offsets, dgu, act_w, dweights, R, E, F, nb));
 }
 
 }  // namespace tb

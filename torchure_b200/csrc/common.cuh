@@ -53,6 +53,13 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// What a launcher returns: 0, or -21 for a launch that was refused (which is reported here, and not once more by a later, unrelated check)
+inline int launch_code(cudaError_t rc) {
+  if (rc == cudaSuccess) return 0;
+  cudaGetLastError();
+  return -21;
+}
+
 // The opt-in to more than 48 KB of dynamic shared memory is an attribute of (kernel, device): set it for each pair,
 // with that device current, and again whenever a launch needs more than was granted before.  Returns false if the device cannot be queried or the attribute is refused.
 inline bool ensure_dynamic_smem(const void* kernel, int bytes) {

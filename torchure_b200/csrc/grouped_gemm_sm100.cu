@@ -980,7 +980,7 @@ int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? 0 : -21;
+  return launch_code(cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
 }  // namespace
@@ -1008,7 +1008,7 @@ int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Rows& rows, c
   const auto launch = [&](auto kern, int groups) {
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FEW_SMEM)) return -20;
     const dim3 grid((out.width + UNIT - 1) / UNIT, R / FEW_ROWS + groups);
-    return launch_pdl(kern, grid, dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, rows, out, R, E, K, err) == cudaSuccess ? 0 : -21;
+    return launch_code(launch_pdl(kern, grid, dim3(FEW_THREADS), FEW_SMEM, stream, tw, tx, offsets, rows, out, R, E, K, err));
   };
   if constexpr (EPI != kStore)
     if (early && R >= EARLY_FROM * E && R <= EARLY_TO * E) return launch(grouped_few_kernel<W_MN, EPI, LISTED, true>, E);

@@ -45,6 +45,12 @@ struct Overlap : tb::PdlScope {
 
 std::atomic<int64_t> g_launches{0};      // kernels launched by the calls of this file
 
+// A launcher's code: counted where it launched, an error otherwise
+void done(const char* what, int rc) {
+  TORCH_CHECK(rc == 0, what, " failed with code ", rc);
+  g_launches += 1;
+}
+
 const __nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
 __nv_bfloat16* bfm(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
 bool at16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
@@ -138,8 +144,8 @@ Tensor do_gather(const Tensor& x, const Tensor& rows, int64_t k, const Outputs& 
   check_ints(rows, R, x, "dispatch: rows");
   if (!out.defined()) out = make("dispatch", {R, D}, x.options().dtype(torch::kBFloat16));
   const Overlap overlap;
-  tb::rows_gather(x.data_ptr(), b16, x.stride(0), rows.data_ptr<int>(), bfm(out), (int)T, (int)k, (int)R, (int)D, cur_stream());
-  g_launches += 1;
+  done("dispatch",
+       tb::rows_gather(x.data_ptr(), b16, x.stride(0), rows.data_ptr<int>(), bfm(out), (int)T, (int)k, (int)R, (int)D, cur_stream()));
   return out;
 }
 
@@ -155,9 +161,8 @@ Tensor do_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots
   TORCH_CHECK_VALUE(T * ((D + 7) / 8) < (1ll << 31), "combine: 2^34 values and more are not supported");
   if (!out.defined()) out = make("combine", {T, D}, y.options().dtype(type));
   const Overlap overlap;
-  tb::rows_combine(y.data_ptr(), y16, has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(), out.data_ptr(),
-                   type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream());
-  g_launches += 1;
+  done("combine", tb::rows_combine(y.data_ptr(), y16, has(weights) ? weights->data_ptr<float>() : nullptr, slots.data_ptr<int>(),
+                                   out.data_ptr(), type == torch::kBFloat16, (int)T, (int)k, (int)R, (int)D, cur_stream()));
   return out;
 }
 
@@ -176,9 +181,9 @@ std::tuple<Tensor, Tensor> do_combine_bwd(const Tensor& dout, const Tensor& y, c
   Tensor dw = make("combine_bwd.dweights", {T, k}, weights.options());
   if (D == 0) return {dy, dw.zero_()};      // sums of no terms
   const Overlap overlap;
-  tb::rows_combine_bwd(dout.data_ptr(), b16, dout.stride(0), bf(y), weights.data_ptr<float>(), slots.data_ptr<int>(),
-                       offsets.data_ptr<int>(), bfm(dy), dw.data_ptr<float>(), (int)T, (int)k, (int)E, (int)D, cur_stream());
-  g_launches += 1;
+  done("combine backward",
+       tb::rows_combine_bwd(dout.data_ptr(), b16, dout.stride(0), bf(y), weights.data_ptr<float>(), slots.data_ptr<int>(),
+                            offsets.data_ptr<int>(), bfm(dy), dw.data_ptr<float>(), (int)T, (int)k, (int)E, (int)D, cur_stream()));
   return {dy, dw};
 }
 
@@ -238,8 +243,7 @@ std::tuple<Tensor, Tensor> do_quantize(const Tensor& x) {
   Tensor q = empty({M, N}, x.options().dtype(torch::kInt8));
   Tensor s = empty({M, blocks_of(N)}, x.options().dtype(torch::kFloat32));
   const Overlap overlap;
-  tb::quantize8(bf(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)N, cur_stream());
-  g_launches += 1;
+  done("quantize8", tb::quantize8(bf(x), x.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)N, cur_stream()));
   return {q, s};
 }
 
@@ -255,8 +259,7 @@ Tensor do_dequantize(const Tensor& q, const Tensor& s, const Outputs& make) {
   check_blocks(q.size(0), q.size(1), "dequantize8");
   Tensor x = make("dequantize8", q.sizes(), q.options().dtype(torch::kBFloat16));
   const Overlap overlap;
-  tb::dequantize8(q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(x), q.size(0), (int)q.size(1), cur_stream());
-  g_launches += 1;
+  done("dequantize8", tb::dequantize8(q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(x), q.size(0), (int)q.size(1), cur_stream()));
   return x;
 }
 
@@ -271,8 +274,7 @@ std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, const Outputs& m
   Tensor q = empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
   Tensor s = empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
   const Overlap overlap;
-  tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)F, cur_stream());
-  g_launches += 1;
+  done("swiglu_8bit", tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)F, cur_stream()));
   return {act, q, s};
 }
 
@@ -284,8 +286,8 @@ Tensor do_swiglu8_bwd(const Tensor& dact, const Tensor& q, const Tensor& s, cons
   TORCH_CHECK(q.size(0) == M && q.size(1) == 2 * F && q.device() == dact.device(), "swiglu_8bit backward: shapes");
   Tensor dgu = make("swiglu_8bit.bwd", {M, 2 * F}, dact.options());
   const Overlap overlap;
-  tb::swiglu8_bwd(bf(dact), dact.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(dgu), M, (int)F, cur_stream());
-  g_launches += 1;
+  done("swiglu_8bit backward",
+       tb::swiglu8_bwd(bf(dact), dact.stride(0), q.data_ptr<int8_t>(), s.data_ptr<float>(), bfm(dgu), M, (int)F, cur_stream()));
   return dgu;
 }
 
@@ -637,10 +639,10 @@ variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x
   if (wanted.gate_up) beside.run([&] { do_gather(x, r.rows, k, make, xg); });
   s = do_grouped(dg, wd, r.offsets, true, make);
   const bool kept16 = gu.defined();
-  tb::expert_swiglu_bwd(bf(s), kept16 ? bf(gu) : nullptr, kept16 ? nullptr : q.data_ptr<int8_t>(), kept16 ? nullptr : scales.data_ptr<float>(),
-                        r.weights.data_ptr<float>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), bfm(dgu), bfm(act_w),
-                        dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream());
-  g_launches += 1;
+  done("expert_mlp backward",
+       tb::expert_swiglu_bwd(bf(s), kept16 ? bf(gu) : nullptr, kept16 ? nullptr : q.data_ptr<int8_t>(),
+                             kept16 ? nullptr : scales.data_ptr<float>(), r.weights.data_ptr<float>(), r.slots.data_ptr<int>(),
+                             r.offsets.data_ptr<int>(), bfm(dgu), bfm(act_w), dweights.data_ptr<float>(), (int)R, (int)E, (int)F, cur_stream()));
   if (wanted.x) dxg = do_grouped(dgu, wgu, r.offsets, true, make);
   if (wanted.x || wanted.logits)
     beside.run([&] {

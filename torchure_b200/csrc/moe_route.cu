@@ -433,13 +433,10 @@ int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t str
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(route_fwd_kernel<T, L, V>), smem) ||                                \
         !ensure_dynamic_smem(reinterpret_cast<const void*>(route_plan_kernel), 4 * plan))                                      \
       return -20;                                                                                                             \
-    if (launch_pdl(route_fwd_kernel<T, L, V>, dim3(chunks), dim3(kThreads), smem, stream, logits, a, chunks == 1 ? 1 : 0) !=   \
-        cudaSuccess)                                                                                                          \
-      return -21;                                                                                                             \
-    if (chunks > 1 && launch_pdl(route_plan_kernel, dim3(chunks), dim3(kThreads), 4 * static_cast<size_t>(plan), stream, a) != \
-                          cudaSuccess)                                                                                        \
-      return -21;                                                                                                             \
-    return 0;                                                                                                                 \
+    int rc = launch_code(launch_pdl(route_fwd_kernel<T, L, V>, dim3(chunks), dim3(kThreads), smem, stream, logits, a, chunks == 1 ? 1 : 0)); \
+    if (rc == 0 && chunks > 1)                                                                                                \
+      rc = launch_code(launch_pdl(route_plan_kernel, dim3(chunks), dim3(kThreads), 4 * static_cast<size_t>(plan), stream, a)); \
+    return rc;                                                                                                                \
   }
   TB_ROUTE_SIZES(CASE)
 #undef CASE
@@ -484,7 +481,7 @@ int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, c
              : launch_pdl(route_bwd_kernel<float, L, V>, dim3(grid), dim3(kBwdThreads), 0, stream,                                  \
                           static_cast<const float*>(logits), ld, weights, experts, counts, dweights, daux,                       \
                           static_cast<float*>(dlogits), T, E, k);                                                                \
-    return rc == cudaSuccess ? 0 : -21;                                                                                          \
+    return launch_code(rc);                                                                                                      \
   }
   TB_ROUTE_SIZES(CASE)
 #undef CASE

@@ -221,46 +221,52 @@ bool whole(const void* p, int64_t ld, int D) { return (reinterpret_cast<uintptr_
 
 }  // namespace
 
-void rows_gather(const void* x, bool x_bf16, int64_t ldx, const int* rows, __nv_bfloat16* out, int T, int k, int R, int D,
+int rows_gather(const void* x, bool x_bf16, int64_t ldx, const int* rows, __nv_bfloat16* out, int T, int k, int R, int D,
                  cudaStream_t stream) {
-  if (R <= 0 || D <= 0) return;
+  if (R <= 0 || D <= 0) return 0;
   const dim3 grid(grid_for(R)), block(kThreads);
   const bool vec = whole(x, ldx, D) && whole(out, D, D);
-#define TB_GATHER(X, V) launch_pdl(rows_gather_kernel<X, V>, grid, block, 0, stream, static_cast<const X*>(x), ldx, rows, out, T, k, R, D)
+  cudaError_t rc;
+#define TB_GATHER(X, V) rc = launch_pdl(rows_gather_kernel<X, V>, grid, block, 0, stream, static_cast<const X*>(x), ldx, rows, out, T, k, R, D)
   if (x_bf16) { if (vec) TB_GATHER(__nv_bfloat16, true); else TB_GATHER(__nv_bfloat16, false); }
   else { if (vec) TB_GATHER(float, true); else TB_GATHER(float, false); }
 #undef TB_GATHER
+  return launch_code(rc);
 }
 
-void rows_combine(const void* y, bool y_bf16, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
+int rows_combine(const void* y, bool y_bf16, const float* weights, const int* slots, void* out, bool out_bf16, int T, int k, int R, int D,
                   cudaStream_t stream) {
-  if (T <= 0 || D <= 0) return;
+  if (T <= 0 || D <= 0) return 0;
   const int chunks = (D + 7) / 8;
   const int64_t total = static_cast<int64_t>(T) * chunks, need = (total + kThreads - 1) / kThreads;
   const dim3 grid(static_cast<int>(need < 148 * 16 ? need : 148 * 16)), block(kThreads);
   const bool vec = whole(y, D, D) && whole(out, D, D);
-#define TB_COMBINE(Y, O, V)                                                                                                                  \
-  launch_pdl(rows_combine_kernel<Y, O, V>, grid, block, 0, stream, static_cast<const Y*>(y), weights, slots, static_cast<O*>(out), total, k, \
-             R, D, FastDiv(chunks))
+  cudaError_t rc;
+#define TB_COMBINE(Y, O, V)                                                                                                             \
+  rc = launch_pdl(rows_combine_kernel<Y, O, V>, grid, block, 0, stream, static_cast<const Y*>(y), weights, slots, static_cast<O*>(out), \
+                  total, k, R, D, FastDiv(chunks))
 #define TB_COMBINE_OF(Y)                                                                                                 \
   if (out_bf16) { if (vec) TB_COMBINE(Y, __nv_bfloat16, true); else TB_COMBINE(Y, __nv_bfloat16, false); }               \
   else { if (vec) TB_COMBINE(Y, float, true); else TB_COMBINE(Y, float, false); }
   if (y_bf16) { TB_COMBINE_OF(__nv_bfloat16) } else { TB_COMBINE_OF(float) }
 #undef TB_COMBINE_OF
 #undef TB_COMBINE
+  return launch_code(rc);
 }
 
-void rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_bfloat16* y, const float* weights, const int* slots,
+int rows_combine_bwd(const void* dout, bool dout_bf16, int64_t ld, const __nv_bfloat16* y, const float* weights, const int* slots,
                       const int* offsets, __nv_bfloat16* dy, float* dweights, int T, int k, int E, int D, cudaStream_t stream) {
-  if (T <= 0 || D <= 0) return;
+  if (T <= 0 || D <= 0) return 0;
   const dim3 grid(grid_for(T * k)), block(kThreads);
   const bool vec = whole(dout, ld, D) && whole(y, D, D) && whole(dy, D, D);
-#define TB_COMBINE_BWD(O, V) \
-  launch_pdl(rows_combine_bwd_kernel<O, V>, grid, block, 0, stream, static_cast<const O*>(dout), ld, y, weights, slots, offsets, dy, \
-             dweights, T, k, E, D)
+  cudaError_t rc;
+#define TB_COMBINE_BWD(O, V)                                                                                                              \
+  rc = launch_pdl(rows_combine_bwd_kernel<O, V>, grid, block, 0, stream, static_cast<const O*>(dout), ld, y, weights, slots, offsets, dy, \
+                  dweights, T, k, E, D)
   if (dout_bf16) { if (vec) TB_COMBINE_BWD(__nv_bfloat16, true); else TB_COMBINE_BWD(__nv_bfloat16, false); }
   else { if (vec) TB_COMBINE_BWD(float, true); else TB_COMBINE_BWD(float, false); }
 #undef TB_COMBINE_BWD
+  return launch_code(rc);
 }
 
 }  // namespace tb

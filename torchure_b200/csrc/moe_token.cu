@@ -261,10 +261,10 @@ int token_mlp(const void* logits, bool logits_bf16, int64_t ldl, const void* x, 
   else rc = x_bf16 ? TB_UP(float, __nv_bfloat16) : TB_UP(float, float);
 #undef TB_UP
 #undef TB_UP_OF
-  if (rc != cudaSuccess) return -21;
+  if (rc != cudaSuccess) return launch_code(rc);
   rc = x_bf16 ? launch_pdl(token_down_kernel<__nv_bfloat16>, down, block, 0, stream, c, h, w_down, static_cast<__nv_bfloat16*>(out), T, k, D, F)
               : launch_pdl(token_down_kernel<float>, down, block, 0, stream, c, h, w_down, static_cast<float*>(out), T, k, D, F);
-  return rc == cudaSuccess ? 0 : -21;
+  return launch_code(rc);
 }
 
 }  // namespace tb
