@@ -111,3 +111,13 @@ def test_experts_of_a_spread_layer_with_the_kernels_off(bits):
         ops.force_fallback(False)
     assert plain.dtype == torch.float32 and layer.w_gate.grad is not None
     assert (got.double() - plain.double()).norm() < 5 * RMS * plain.double().norm()
+
+
+def test_kernels_are_counted():
+    """Few tokens are routed by one kernel, many by two."""
+    for T, want in ((16, 1), (4096, 2)):
+        logits = torch.randn(T, 8, device="cuda", generator=gen(0))
+        moe.route(logits, 2)
+        before = ops.launches()
+        moe.route(logits, 2)
+        assert ops.launches() - before == want

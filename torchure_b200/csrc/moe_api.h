@@ -22,6 +22,7 @@ constexpr int kActBlock = 64;      // values of a row that share a scale in an 8
 // rows [T k] (t k + j of each row, -1 behind offsets[E]), counts [E] (choices made, before the capacity), aux [1].
 // scratch: route_scratch_ints(T, E, k) 32-bit words.  capacity 0: no limit.
 int64_t route_scratch_ints(int T, int E, int k);
+int route_kernels(int T, int E, int k);      // that route_fwd launches
 [[nodiscard]] int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts,
                             int* slots, int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream);
 // dlogits [T, E] (the logits' type) from dweights [T, k] (nullptr: none) and daux [1] (nullptr: none)

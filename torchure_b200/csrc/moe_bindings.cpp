@@ -109,8 +109,8 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, r.weights.data_ptr<float>(),
                                r.experts.data_ptr<int>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), r.rows.data_ptr<int>(),
                                r.counts.data_ptr<int>(), r.aux.data_ptr<float>(), scratch.data_ptr<int>(), cur_stream());
-  g_launches += 1;
   TORCH_CHECK(rc == 0, "route failed with code ", rc);
+  g_launches += tb::route_kernels((int)T, (int)E, (int)k);
   return r;
 }
 

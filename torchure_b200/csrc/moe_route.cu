@@ -451,6 +451,12 @@ int64_t route_scratch_ints(int T, int E, int k) {
   return 2 * static_cast<int64_t>(chunks) * E;
 }
 
+int route_kernels(int T, int E, int k) {
+  int chunks, chunk;
+  chunks_for(T, E, k, chunks, chunk);
+  return chunks > 1 ? 2 : 1;
+}
+
 int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts, int* slots,
               int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream) {
   if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices || static_cast<int64_t>(T) * k > (1ll << 30)) return -1;
