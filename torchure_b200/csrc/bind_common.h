@@ -5,7 +5,7 @@
 
 #include "api.h"
 
-torch::Tensor attn_err_word();   // device int32[4], set by bounded waits that expired
+torch::Tensor attn_err_word();   // device int32[4], set by bounded waits that expired; refused on another GPU than the process's first
 int bind_num_sms();              // SMs a persistent kernel may use
 void bind_gemm(const torch::Tensor& a, const torch::Tensor& b, torch::Tensor& out, bool a_mn, bool b_mn, int64_t out_mode,
                int64_t splits = 0, int64_t tile_n = 0, bool b_is_old = false);

@@ -27,10 +27,20 @@ int num_sms() {
 // of `n` SMs with a communication CTA those that compute kernels may use as well
 int unreserved_sms(int64_t n) { return n > g_sm_reserve ? (int)n - g_sm_reserve : 0; }
 
-// one error word per process (one process drives one GPU)
-torch::Tensor& err_word() {
+// One error word per process, on the GPU of the first call: one process drives one GPU.
+torch::Tensor& error_word() {
   static torch::Tensor t;
   if (!t.defined()) t = torch::zeros({4}, torch::dtype(torch::kInt32).device(torch::kCUDA));
+  return t;
+}
+void check_one_gpu(int64_t home, int64_t now) {
+  TORCH_CHECK_VALUE(home == now, "one process drives one GPU: its kernels' error word is on cuda:", home, ", the operands of this call are on cuda:",
+                    now);
+}
+// What a kernel on the current device may poll.  A kernel on another GPU would read memory that is not its own.
+torch::Tensor& err_word() {
+  torch::Tensor& t = error_word();
+  check_one_gpu(t.get_device(), at::cuda::current_device());
   return t;
 }
 
@@ -308,8 +318,6 @@ void bucket_pack_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, co
                         opt_mptr<float>(sq), cur_stream());
 }
 
-torch::Tensor error_word() { return err_word(); }
-
 // Tensors that a captured graph reads at every replay (the host bytes of copy nodes) are owned by the graph: CUDA calls back
 // when neither the graph nor an executable made from it is left.  The callback may not call CUDA, as releasing pinned memory
 // does, so it only hands the tensors over; they go when a table is next asked for.
@@ -404,7 +412,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("stream_place", &stream_place, "(current stream of a device, id of the capture it is in or 0)");
   m.def("keep_with_graph", &keep_with_graph, "the graph being captured on the current stream owns these tensors");
   m.def("graph_keeps", [] { release_gone(); return g_graph_keeps.load(); }, "how many keep_with_graph sets are alive");
-  m.def("error_word", &error_word, "device int32[4]; [0] is set when a bounded wait of a kernel expired");
+  m.def("error_word", [] { return error_word(); }, "device int32[4]; [0] is set when a bounded wait of a kernel expired");
+  m.def("check_one_gpu", &check_one_gpu, "raises unless the device of the error word and of a call are the same");
   m.def("add_rmsnorm_fwd", &add_rmsnorm_fwd);
   m.def("rmsnorm_bwd", &rmsnorm_bwd, pybind11::arg("dh"), pybind11::arg("x"), pybind11::arg("w"), pybind11::arg("rstd"),
         pybind11::arg("dx_in"), pybind11::arg("dx"), pybind11::arg("dx_bf16"), pybind11::arg("dw"),
