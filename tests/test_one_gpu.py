@@ -29,3 +29,21 @@ def test_kernels_get_the_error_word_through_the_check():
     for path in CSRC.glob("*_bindings.cpp"):
         if path.name != "comm_bindings.cpp":          # (the collectives have a word of their own)
             assert not re.search(r"torch::zeros\(\{4\}", path.read_text()), path.name
+
+
+def test_available_asks_the_current_gpu(monkeypatch):
+    """A machine with a GPU that runs the kernels and one that does not: the answer is the current one's, whichever was asked first."""
+    now = [0]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda device=None: ((10, 0), (9, 0))[now[0]])
+    monkeypatch.setattr(ops, "ext", lambda: object())
+    monkeypatch.setattr(ops, "_FOUND", type(ops._FOUND)())
+    for device in (1, 0, 1, 0):
+        now[0] = device
+        assert ops.available() == (device == 0)
+    ops.force_fallback(True)
+    try:
+        assert not ops.available()
+    finally:
+        ops.force_fallback(False)

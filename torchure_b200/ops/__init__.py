@@ -36,7 +36,7 @@ def ext():
 
 
 _FORCED_OFF = False
-_FOUND = False      # the extension and a GPU that runs it were there once; they stay
+_FOUND: set[int] = set()      # GPUs that run the extension, which was there with them; both stay
 
 
 def force_fallback(flag: bool = True) -> None:
@@ -46,12 +46,15 @@ def force_fallback(flag: bool = True) -> None:
 
 
 def available() -> bool:
-    global _FOUND
+    """Whether the kernels run on the current GPU."""
     if _FORCED_OFF:
         return False
-    if not _FOUND:
-        _FOUND = torch.cuda.is_available() and ext() is not None and torch.cuda.get_device_capability()[0] == 10
-    return _FOUND
+    if _FOUND and torch.cuda.current_device() in _FOUND:
+        return True
+    if not torch.cuda.is_available() or ext() is None or torch.cuda.get_device_capability()[0] != 10:
+        return False
+    _FOUND.add(torch.cuda.current_device())
+    return True
 
 
 # launch counter: every Python wrapper that launches one of OUR kernels adds to it; the mixture-of-experts operators count in C++
