@@ -1,0 +1,21 @@
+"""The plain path of the mixture-of-experts operators takes the arguments that the kernels take."""
+
+import pytest
+import torch
+
+from torchure_b200.ops import moe
+
+
+@pytest.mark.parametrize("have", [torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("want", [None, torch.bfloat16, torch.float32])
+def test_combine_gives_the_type_that_was_asked_for(have, want):
+    g = torch.Generator().manual_seed(0)
+    r = moe.route(torch.randn(9, 4, generator=g), 2)
+    y = torch.randn(18, 6, generator=g).to(have)
+    out = moe.combine(y, r) if want is None else moe.combine(y, r, want)
+    assert out.dtype == (want or have)
+    exact = (r.weights.double()[:, :, None] * y.double()[r.slots.long()]).sum(1)
+    # terms and sum of two of them, each rounded to the narrower type: 2^-8 (bf16) or 2^-23 of the terms' magnitudes
+    size = (r.weights.double()[:, :, None] * y.double()[r.slots.long()].abs()).sum(1)
+    unit = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -23
+    assert ((out.double() - exact).abs() <= 4 * unit * size).all()

@@ -79,13 +79,15 @@ def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     return _C().moe_dispatch(x, routing.slots, routing.rows, debug.enabled())
 
 
-def combine(y: torch.Tensor, routing: Routing, out_dtype: torch.dtype = BF16) -> torch.Tensor:
-    """Weighted sums of the rows y [T k, D] (bf16, expert order) for every token, [T, D] in bf16 or fp32."""
+def combine(y: torch.Tensor, routing: Routing, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Weighted sums of the rows y [T k, D] (bf16, expert order) for every token, [T, D] in bf16 or fp32 (None: y's type)."""
     if y.dim() != 2 or y.shape[0] != routing.slots.numel():
         raise ValueError(f"combine: {routing.slots.numel()} rows expected, got {tuple(y.shape)}")
     if _plain(y, routing.slots):
-        return oracle.combine(y, routing.weights.to(y.dtype), routing.slots)
-    if out_dtype not in (BF16, torch.float32):
+        wide = y.dtype if out_dtype is None else torch.promote_types(y.dtype, out_dtype)
+        out = oracle.combine(y.to(wide), routing.weights.to(wide), routing.slots)
+        return out if out_dtype is None else out.to(out_dtype)
+    if out_dtype not in (None, BF16, torch.float32):
         raise TypeError(f"combine: sums in bf16 or fp32, not {out_dtype}")
     return _C().moe_combine(y, routing.weights, routing.slots, routing.offsets, out_dtype == torch.float32, debug.enabled())
 
