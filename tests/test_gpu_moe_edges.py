@@ -121,3 +121,22 @@ def test_kernels_are_counted():
         before = ops.launches()
         moe.route(logits, 2)
         assert ops.launches() - before == want
+
+
+@pytest.mark.parametrize("rows,F,start", [(64, 256, 0), (1, 1, 0), (77, 519, 0), (9, 1000, 1), (33, 72, 3), (3, 4100, 1), (2, 5000, 0), (0, 64, 0)])
+def test_swiglu_8bit_without_gradients(rows, F, start):
+    """The bits of the activation are the same; a checkpoint that nobody will read is not made."""
+    gu = rand(rows * 2 * F + start, seed=1)[start:].view(rows, 2 * F)
+    want = act8.swiglu_8bit(gu.detach().requires_grad_()).detach()
+    with torch.no_grad():
+        assert torch.equal(act8.swiglu_8bit(gu), want)
+    assert torch.equal(act8.swiglu_8bit(gu), want)
+
+
+def test_swiglu_8bit_without_gradients_makes_no_checkpoint():
+    gu = rand(2048, 2048, seed=1)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    act = act8.swiglu_8bit(gu)
+    assert torch.cuda.max_memory_allocated() - before <= act.numel() * 2 + 4096

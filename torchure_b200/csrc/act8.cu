@@ -14,7 +14,8 @@
 //
 // Bound by memory.  Eight lanes have a block, eight values each (16 bytes of bf16, 8 bytes of int8), four blocks at a time (SwiGLU:
 // two of gate and two of up) so that as many loads are on their way; with one block at a time 16384 x 2560 took 43 us to quantise and
-// 32 to read back, and SwiGLU of 16384 x 1536 54 and 42; now 22, 18, 34 and 33 (128 and 204 MB).
+// 32 to read back, and SwiGLU of 16384 x 1536 54 and 42; now 22, 18, 34 and 33 (128 and 204 MB).  Without gradients SwiGLU writes no
+// checkpoint: 24 (151 MB).
 //
 // Widths that are no multiple of 8: a CTA takes whole rows, which lie one behind the other, brings them into shared memory as they lie (16
 // bytes at a time, the ends value by value), works on them there and sends its results out the same way: 16384 x 2557 in 55 us to quantise
@@ -203,7 +204,8 @@ dequantize8_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale
   }
 }
 
-template <bool VEC>
+// KEEP: gate and up are written in 8 bits beside the activation (without gradients nobody reads them)
+template <bool VEC, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 4)
 swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
                    float* __restrict__ scales, uint32_t units, int F, FastDiv nb) {
@@ -233,6 +235,7 @@ swiglu8_fwd_kernel(const __nv_bfloat16* __restrict__ gu, int64_t ldgu, __nv_bflo
       for (int j = 0; j < 8; ++j) out[j] = g[j] * sigmoid(g[j]) * v[j];
       const int64_t at = row[i] * F + c[i];
       store8<VEC>(act + at, left, out);
+      if constexpr (!KEEP) continue;
       const bool first = u < units && (threadIdx.x & 7) == 0;
       float* scale = scales + (u + row[i] * static_cast<int>(nb.d));
       int8_t* to = q + (at + row[i] * F);
@@ -397,6 +400,7 @@ dequantize8_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ 
   }
 }
 
+template <bool KEEP>
 __global__ void __launch_bounds__(kThreads)
 swiglu8_fwd_rows_kernel(const __nv_bfloat16* __restrict__ gu, __nv_bfloat16* __restrict__ act, int8_t* __restrict__ q,
                         float* __restrict__ scales, int64_t M, int F, int nb, int rows) {
@@ -422,13 +426,14 @@ swiglu8_fwd_rows_kernel(const __nv_bfloat16* __restrict__ gu, __nv_bfloat16* __r
         up[i] = in ? odd_load(sg + row * F * 4 + F * 2, c, F) : 0.f;
         if (in) odd_store(sa + row * F * 2, c, F, gate[i] * sigmoid(gate[i]) * up[i]);
       }
+      if constexpr (!KEEP) continue;
       float* scale = scales + (r0 + row) * 2 * nb + b;
       odd_keep(gate, sq + row * 2 * F, c0, F, scale, in);
       odd_keep(up, sq + row * 2 * F + F, c0, F, scale + nb, in);
     }
     __syncthreads();
     stage_out(act + r0 * F, sa, n * F * 2);
-    stage_out(q + r0 * 2 * F, sq, n * F * 2);
+    if constexpr (KEEP) stage_out(q + r0 * 2 * F, sq, n * F * 2);
   }
 }
 
@@ -590,12 +595,15 @@ int swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_
   const uint32_t units = static_cast<uint32_t>(M * nb);
   cudaError_t rc;
   if (F % 8 == 0 && ldgu % 8 == 0 && at16(gu) && at16(act) && at16(q)) {
-    rc = launch_pdl(swiglu8_fwd_kernel<true>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+    rc = launch_pdl(q ? swiglu8_fwd_kernel<true, true> : swiglu8_fwd_kernel<true, false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units,
+                    F, FastDiv(nb));
   } else if (ldgu == 2 * static_cast<int64_t>(F) && 2 * F <= kOddValues) {
     const int rows = tile_rows(M, 2 * F);
-    rc = launch_pdl(swiglu8_fwd_rows_kernel, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream, gu, act, q, scales, M, F, nb, rows);
+    rc = launch_pdl(q ? swiglu8_fwd_rows_kernel<true> : swiglu8_fwd_rows_kernel<false>, dim3(tile_grid(M, rows)), block, rows * F * 8 + 96, stream,
+                    gu, act, q, scales, M, F, nb, rows);
   } else {
-    rc = launch_pdl(swiglu8_fwd_kernel<false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units, F, FastDiv(nb));
+    rc = launch_pdl(q ? swiglu8_fwd_kernel<false, true> : swiglu8_fwd_kernel<false, false>, grid, block, 0, stream, gu, ldgu, act, q, scales, units,
+                    F, FastDiv(nb));
   }
   return launch_code(rc);
 }

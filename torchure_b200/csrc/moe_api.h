@@ -76,7 +76,8 @@ int64_t token_scratch_bytes(int T, int k, int F);
 // zeros, NaN for one that holds a value that is not finite).  q [M, N], scales [M, ceil(N / 64)].
 [[nodiscard]] int quantize8(const __nv_bfloat16* x, int64_t ldx, int8_t* q, float* scales, int64_t M, int N, cudaStream_t stream);
 [[nodiscard]] int dequantize8(const int8_t* q, const float* scales, __nv_bfloat16* x, int64_t M, int N, cudaStream_t stream);
-// act [M, F] = silu(g) u of gu [M, 2F] = g | u; q [M, 2F] and scales [M, 2 ceil(F / 64)]: both halves as quantize8 keeps them
+// act [M, F] = silu(g) u of gu [M, 2F] = g | u; q [M, 2F] and scales [M, 2 ceil(F / 64)]: both halves as quantize8 keeps them (nullptr: not
+// kept)
 [[nodiscard]] int swiglu8_fwd(const __nv_bfloat16* gu, int64_t ldgu, __nv_bfloat16* act, int8_t* q, float* scales, int64_t M, int F,
                               cudaStream_t stream);
 [[nodiscard]] int swiglu8_bwd(const __nv_bfloat16* dact, int64_t ldd, const int8_t* q, const float* scales, __nv_bfloat16* dgu, int64_t M,

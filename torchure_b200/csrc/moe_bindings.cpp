@@ -263,18 +263,22 @@ Tensor do_dequantize(const Tensor& q, const Tensor& s, const Outputs& make) {
   return x;
 }
 
-// act, q, scales
-std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, const Outputs& make) {
+// act, and with `keep` q and scales
+std::tuple<Tensor, Tensor, Tensor> do_swiglu8(const Tensor& gu, bool keep, const Outputs& make) {
   check_rows(gu, "swiglu_8bit");
   check_bf16(gu, "swiglu_8bit");
   TORCH_CHECK(gu.size(1) % 2 == 0, "swiglu_8bit: gate and up columns expected, got an odd number: ", gu.size(1));
   const int64_t M = gu.size(0), F = gu.size(1) / 2;
   check_blocks(M, F, "swiglu_8bit");
   Tensor act = make("swiglu_8bit", {M, F}, gu.options());
-  Tensor q = empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
-  Tensor s = empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
+  Tensor q, s;
+  if (keep) {
+    q = empty({M, 2 * F}, gu.options().dtype(torch::kInt8));
+    s = empty({M, 2 * blocks_of(F)}, gu.options().dtype(torch::kFloat32));
+  }
   const Overlap overlap;
-  done("swiglu_8bit", tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), q.data_ptr<int8_t>(), s.data_ptr<float>(), M, (int)F, cur_stream()));
+  done("swiglu_8bit", tb::swiglu8_fwd(bf(gu), gu.stride(0), bfm(act), keep ? q.data_ptr<int8_t>() : nullptr,
+                                      keep ? s.data_ptr<float>() : nullptr, M, (int)F, cur_stream()));
   return {act, q, s};
 }
 
@@ -463,7 +467,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, b
 
 struct Swiglu8Node : torch::autograd::Function<Swiglu8Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& gu, bool poison) {
-    auto r = do_swiglu8(gu, Outputs{poison});
+    auto r = do_swiglu8(gu, true, Outputs{poison});
     ctx->save_for_backward({std::get<1>(r), std::get<2>(r)});
     ctx->saved_data["poison"] = poison;
     return std::get<0>(r);
@@ -481,11 +485,12 @@ Tensor swiglu_8bit(const Tensor& gu, bool poison) {
   check_bf16(gu, "swiglu_8bit");
   TORCH_CHECK_VALUE(gu.dim() >= 1 && gu.size(-1) % 2 == 0, "swiglu_8bit: gate and up columns expected, got ", gu.sizes());
   c10::cuda::CUDAGuard guard(gu.device());
-  if (gu.dim() == 2) return Swiglu8Node::apply(rows_of(gu), poison);
   auto shape = gu.sizes().vec();
-  const Tensor act = Swiglu8Node::apply(rows_of(gu.reshape({-1, shape.back()})), poison);
+  const Tensor rows = rows_of(gu.dim() == 2 ? gu : gu.reshape({-1, shape.back()}));
+  const bool keep = at::GradMode::is_enabled() && gu.requires_grad();
+  const Tensor act = keep ? Swiglu8Node::apply(rows, poison) : std::get<0>(do_swiglu8(rows, false, Outputs{poison}));
   shape.back() /= 2;
-  return act.view(shape);
+  return gu.dim() == 2 ? act : act.view(shape);
 }
 
 // ---- the whole feed-forward -------------------------------------------------------------------------

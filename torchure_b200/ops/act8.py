@@ -58,7 +58,7 @@ def dequantize8(kept: Act8) -> torch.Tensor:
 
 def swiglu_8bit(gu: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of ``gu`` [..., 2F] = gate | up (bf16), [..., F].  Until the backward pass ``gu`` is kept in 8 bits, gate and
-    up in blocks of their own; the gradient is the formula's at the values read back."""
+    up in blocks of their own; the gradient is the formula's at the values read back.  Without gradients nothing is kept."""
     if ops.available() and gu.is_cuda:
         return _C().swiglu_8bit(gu, debug.enabled())
     if gu.dim() < 1 or gu.shape[-1] % 2:
