@@ -45,3 +45,10 @@ def test_every_launcher_returns_a_code_that_callers_look_at():
     for m in re.finditer(rf"\btb::({'|'.join(launchers)})\(", calls):
         head = calls[:m.start()].rstrip()
         assert head.endswith("rc =") or re.search(r"\bdone\(\"[\w /]+\",$", head), m.group()
+
+
+def test_launchers_keep_nothing_in_plain_globals():
+    """Forward and backward passes launch from different threads: what a launcher finds out once stands behind a lock, by kernel and device."""
+    for name in ("grouped_gemm_sm100.cu", "moe_route.cu", "moe_rows.cu", "moe_token.cu", "act8.cu"):
+        text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+        assert not re.search(r"^(?:static )?(?:int|bool|int64_t) g?_?\w+ = [^;]*;", text, re.M), name

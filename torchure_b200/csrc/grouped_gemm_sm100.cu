@@ -951,8 +951,21 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmDy, const __grid_cons
   }
 }
 
-// CTA pairs that the device holds at once (the two CTAs sit on the two SMs of one TPC)
-int g_pairs = 0;
+// CTA pairs of a kernel that the current device holds at once (the two CTAs sit on the two SMs of one TPC), 0 if it cannot be told.  Asked once
+// for each kernel and device; forward and backward passes launch from different threads.
+int pairs_at_once(const void* kernel, cudaLaunchConfig_t cfg) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, int> found;
+  int dev = 0, sms = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  int& kept = found[{kernel, dev}];
+  if (kept > 0) return kept;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  cfg.gridDim = dim3(2 * (sms / 2));
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) return 0;
+  return kept = n < sms / 2 ? n : sms / 2;
+}
 
 template <class... Params, class... Args>
 int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, int num_sms, cudaStream_t stream, Args... args) {
@@ -966,15 +979,10 @@ int launch_pairs(void (*kern)(Params...), int threads, int smem, int64_t units, 
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  if (g_pairs == 0) {
-    int dev = 0, all_sms = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&all_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -23;
-    cfg.gridDim = dim3(2 * (all_sms / 2));
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) return -23;
-    g_pairs = n < all_sms / 2 ? n : all_sms / 2;
-  }
-  const int pairs = g_pairs < num_sms / 2 ? g_pairs : num_sms / 2;
+  cfg.numAttrs = 1;
+  const int at_once = pairs_at_once(reinterpret_cast<const void*>(kern), cfg);
+  if (at_once == 0) return -23;
+  const int pairs = at_once < num_sms / 2 ? at_once : num_sms / 2;
   cfg.gridDim = dim3(2 * static_cast<int>(units < pairs ? units : pairs));
   cfg.stream = stream;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
