@@ -19,3 +19,12 @@ def test_combine_gives_the_type_that_was_asked_for(have, want):
     size = (r.weights.double()[:, :, None] * y.double()[r.slots.long()].abs()).sum(1)
     unit = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -23
     assert ((out.double() - exact).abs() <= 4 * unit * size).all()
+
+
+@pytest.mark.parametrize("edges,meant", [([0, 60, 20, 100], [0, 60, 60, 100]), ([0, -5, 50, 4000], [0, 0, 50, 100]), ([9, 30, 40, 90], [0, 30, 40, 90])])
+def test_wrong_offsets_count_as_on_the_gpu(edges, meant):
+    """Offsets that fall, are negative or pass the end: the largest so far, within the rows, from 0 on."""
+    g = torch.Generator().manual_seed(2)
+    x, w = torch.randn(100, 6, generator=g), torch.randn(3, 5, 6, generator=g)
+    got, want = (moe.grouped_linear(x, w, torch.tensor(e, dtype=torch.int32)) for e in (edges, meant))
+    assert got.shape == (100, 5) and torch.equal(got, want)
