@@ -9,7 +9,7 @@ Rows of expert e are offsets[e] .. offsets[e + 1] - 1, in the order of (token, c
 for it.  Group sizes are free: an expert may have no rows, all of them, or any number between.  bf16 operands, fp32 sums; gradients
 of bf16 matrices are bf16, of fp32 ones (rounded to bf16 for the products) fp32.
 
-On tensors that are not on a GPU the plain statements of ``ops/oracle.py`` run, in the operands' precision.
+On tensors that are not on a GPU the plain statements of ``ops/oracle.py`` run, in the precision of the rows and at any width.
 """
 
 from __future__ import annotations

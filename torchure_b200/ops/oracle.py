@@ -84,12 +84,12 @@ def route(logits, k, capacity=0):
 
 
 def grouped_linear(x, w, offsets):
-    """Row r of x [R, K] times w[e]^T, w [E, N, K], for offsets[e] <= r < offsets[e + 1]; zeros behind offsets[E].
+    """Row r of x [R, K] times w[e]^T, w [E, N, K] in the type of x, for offsets[e] <= r < offsets[e + 1]; zeros behind offsets[E].
     Offsets count from 0, do not fall and stay within the rows; others are brought there."""
     edge = [0]
     for v in offsets[1:].tolist():
         edge.append(max(edge[-1], min(v, x.shape[0])))
-    parts = [x[a:b] @ w[e].t() for e, (a, b) in enumerate(zip(edge[:-1], edge[1:]))]
+    parts = [x[a:b] @ w[e].t().to(x.dtype) for e, (a, b) in enumerate(zip(edge[:-1], edge[1:]))]
     return torch.cat(parts + [x.new_zeros(x.shape[0] - edge[-1], w.shape[1])])
 
 
