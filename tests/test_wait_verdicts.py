@@ -57,3 +57,15 @@ def test_the_helper_votes_over_the_barrier():
     body = text[text.index("bool mbar_wait_warps("):]
     body = body[:body.index("\n}")]
     assert "mbar_wait_warp(" in body and "bar.red.and.pred" in body
+
+
+def test_dependents_are_let_in_behind_the_wait():
+    """Kernels that read matrices before the kernel before has ended rely on it: whoever lets them in has waited, so that all that came before
+    it on the stream, what wrote the matrices included, has ended."""
+    seen = 0
+    for path in CSRC.glob("*.cu"):
+        text = _code(path.name)
+        for m in re.finditer(r"\bpdl_launch_dependents\(\);", text):
+            assert text[:m.start()].rstrip().endswith("pdl_wait();"), path.name
+            seen += 1
+    assert seen >= 20

@@ -539,7 +539,7 @@ int grid_for(int64_t units, int per_cta) {
   const int64_t need = (units + per_cta - 1) / per_cta;
   return static_cast<int>(need < 148 * 16 ? need : 148 * 16);
 }
-// Rows of a tile that go through shared memory, and its bytes; a value of the widest tensor costs `bytes` of all areas.
+// Rows of a tile that go through shared memory; `width`: of the widest tensor
 int tile_rows(int64_t M, int width) {
   const int fit = kOddValues / width;
   const int64_t spread = (M + 148 * 6 - 1) / (148 * 6);      // small matrices: over all SMs

@@ -27,6 +27,8 @@ namespace tb {
 // and gained nothing (51.86 against 51.36 ms), so it is off unless TORCHURE_B200_PDL=1 or a launch sequence turns it on for
 // itself (pdl.h; the block's forward with few tokens).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Always behind pdl_wait(): kernels that read matrices ahead of their own wait (grouped_few_kernel with EARLY, gemm_small_kernel with early_b)
+// rely on it that the kernel which lets them in has itself waited, so that everything older on the stream has ended.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 inline bool pdl_enabled() {
@@ -389,7 +391,7 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int m, int n, bool a_mn_m
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// n / d for n < 2^31 (multiplication by a rounded reciprocal of 33 bits)
+// n / d for n < 2^31: division by an invariant integer (Granlund and Montgomery), a multiplication by a rounded reciprocal of 33 bits
 struct FastDiv {
   uint32_t d, mul, shift;
   explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {

@@ -5,8 +5,8 @@
 // instruction's M, fixed), the group's rows its columns (the instruction's N, any multiple of 32 up to 256).  Groups end anywhere, and
 // what a group's last tile costs in arithmetic goes with its rows: 2049 rows take 8.1 tiles, not 9.  Nothing is padded in memory: a
 // tile reads rows of the next group along, whose columns of the tile are not stored.  The epilogue turns the accumulator round on its
-// way out: fragments of 16 lanes x 8 columns (tcgen05.ld.16x256b) are rounded to pairs and stored transposed (stmatrix), so that rows
-// of the output leave in pieces of 64 bytes.
+// way out: fragments of 16 lanes x 8 columns (tcgen05.ld.16x256b) are rounded to pairs and stored transposed (stmatrix) into staging rows
+// of four warps, from which the output leaves in whole lines of 128 bytes.
 //
 // The gradient of the matrices, dW[e] = sum of dy[r]^T x[r]: the group's rows are the reduction.  Blocks of 64 rows; of a last block
 // that is not full only the steps of 16 rows that hold some are multiplied, and in a step that is not full the rows of the next group
