@@ -33,15 +33,22 @@ def test_kernels_get_the_error_word_through_the_check():
 
 def test_available_asks_the_current_gpu(monkeypatch):
     """A machine with a GPU that runs the kernels and one that does not: the answer is the current one's, whichever was asked first."""
-    now = [0]
+    now, kinds = [0], [(10, 0), (9, 0)]
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 2)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
-    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda device=None: ((10, 0), (9, 0))[now[0]])
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda device=None: kinds[now[0] if device is None else device])
     monkeypatch.setattr(ops, "ext", lambda: object())
-    monkeypatch.setattr(ops, "_FOUND", type(ops._FOUND)())
+    monkeypatch.setattr(ops, "_EVERY_GPU", False)
     for device in (1, 0, 1, 0):
         now[0] = device
         assert ops.available() == (device == 0)
+    kinds[1] = (10, 0)          # two of a kind: asked once
+    for device in (1, 0):
+        now[0] = device
+        assert ops.available()
+    monkeypatch.setattr(torch.cuda, "get_device_capability", None)
+    assert ops.available()
     ops.force_fallback(True)
     try:
         assert not ops.available()

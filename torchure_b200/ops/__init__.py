@@ -36,7 +36,7 @@ def ext():
 
 
 _FORCED_OFF = False
-_FOUND: set[int] = set()      # GPUs that run the extension, which was there with them; both stay
+_EVERY_GPU = False      # the extension was there once and every GPU runs it: both stay (asking for the current one takes 1.1 us)
 
 
 def force_fallback(flag: bool = True) -> None:
@@ -49,11 +49,12 @@ def available() -> bool:
     """Whether the kernels run on the current GPU."""
     if _FORCED_OFF:
         return False
-    if _FOUND and torch.cuda.current_device() in _FOUND:
+    global _EVERY_GPU
+    if _EVERY_GPU:
         return True
     if not torch.cuda.is_available() or ext() is None or torch.cuda.get_device_capability()[0] != 10:
         return False
-    _FOUND.add(torch.cuda.current_device())
+    _EVERY_GPU = all(torch.cuda.get_device_capability(i)[0] == 10 for i in range(torch.cuda.device_count()))
     return True
 
 
