@@ -193,3 +193,45 @@ def test_router_gradients_against_differences_along_themselves(T, E, k):
         slope, want = (value(up) - value(down)) / (2 * h), g.double().abs().sum()
         bound = size * (h * h * 16 / 6 + 2.0 ** -20 / h)
         assert want > 10 * bound and (slope - want).abs() <= bound + 2.0 ** -18 * want
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("T", [2, 100])
+def test_expert_mlp_takes_logits_as_route_does(T, dtype):
+    """A router under fp16 autocast, or one in fp64: as ``route``, in fp32, and the gradient in the logits' own type."""
+    x, logits, wgu, wd = mlp_inputs(T, 6, 64, 64)
+    leaf, same = logits.to(dtype).requires_grad_(), logits.to(dtype).float().requires_grad_()
+    out, aux = moe.expert_mlp(x, leaf, wgu, wd, 2)
+    want, waux = moe.expert_mlp(x, same, wgu, wd, 2)
+    assert torch.equal(out, want) and torch.equal(aux, waux)
+    dout = rand(T, 64, seed=9)
+    got, = torch.autograd.grad((out, aux), (leaf,), (dout, torch.ones_like(aux)))
+    ref, = torch.autograd.grad((want, waux), (same,), (dout, torch.ones_like(waux)))
+    assert got.dtype == dtype and torch.equal(got, ref.to(dtype))
+    with torch.no_grad():
+        assert torch.equal(moe.expert_mlp(x, leaf, wgu, wd, 2)[0], moe.expert_mlp(x, same, wgu, wd, 2)[0])
+
+
+@pytest.mark.parametrize("T", [300, 2500])
+def test_expert_mlp_training_in_a_graph(T):
+    """A pass with gradients is captured and replayed, with the second stream of many rows inside."""
+    x, logits, wgu, wd = (t.requires_grad_() for t in mlp_inputs(T, 8, 128, 128))
+    dout = rand(T, 128, seed=9)
+
+    def once():
+        out, aux = moe.expert_mlp(x, logits, wgu, wd, 2)
+        return (out, *torch.autograd.grad((out, aux), (x, logits, wgu, wd), (dout, torch.ones_like(aux))))
+
+    want = [t.detach().clone() for t in once()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))

@@ -348,13 +348,17 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
   }
 };
 
+// Logits as the kernels read them: fp32 or bf16, others in fp32
+Tensor router_logits(const Tensor& t) {
+  return !t.is_floating_point() || t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16 ? t : t.to(torch::kFloat32);
+}
+
 variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
   no_tangents("route", logits);
   TORCH_CHECK_VALUE(logits.dim() == 2 && logits.is_floating_point(), "route: logits [tokens, experts] expected, got ", logits.scalar_type(),
                     " ", logits.sizes());
   c10::cuda::CUDAGuard guard(logits.device());
-  const bool as_is = logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16;
-  const Tensor rows = rows_of(as_is ? logits : logits.to(torch::kFloat32));
+  const Tensor rows = rows_of(router_logits(logits));
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     Routed r = do_route(rows, k, capacity, Outputs{poison});
     return {r.weights, r.aux, r.experts, r.slots, r.offsets, r.rows, r.counts};
@@ -711,11 +715,12 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
   }
 };
 
-variable_list expert_mlp(const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
+variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
                          int64_t capacity, int64_t bits, bool poison) {
-  no_tangents("expert_mlp", x, logits, first, has(second) ? *second : Tensor(), wd);
+  no_tangents("expert_mlp", x, given_logits, first, has(second) ? *second : Tensor(), wd);
   check_rows(x, "expert_mlp: x");
-  check_rows(logits, "expert_mlp: logits");
+  check_rows(given_logits, "expert_mlp: logits");
+  const Tensor logits = router_logits(given_logits);
   bf16_or_f32(x, "expert_mlp: x");
   bf16_or_f32(first, "expert_mlp: w_gate_up");
   TORCH_CHECK_TYPE(first.scalar_type() == wd.scalar_type(), "expert_mlp: matrices of one type expected, got ", first.scalar_type(), " and ",

@@ -52,7 +52,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def route(logits: torch.Tensor, top_k: int, capacity: int = 0) -> Routing:
-    """The ``top_k`` experts of every token by its logits [T, E] (fp32 or bf16; at most 384 experts, 16 choices).
+    """The ``top_k`` experts of every token by its logits [T, E] (fp32 or bf16, others in fp32; at most 384 experts, 16 choices).
 
     Ties go to the lowest index.  A weight is the softmax over the token's choices (the probabilities renormalised over them).  An
     expert whose logit is -inf is closed to the token: such a choice is not made (weight 0, no row), so a padding token can be kept
@@ -112,7 +112,14 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.T
 
     x [T, D] bf16 or fp32 (the output's type), logits [T, E] as ``route`` takes them, ``w_gate_up`` [E, 2F, D] or the pair
     (w_gate, w_up) of [E, F, D], ``w_down`` [E, D, F]; matrices bf16 or fp32 (then rounded for the products, with fp32 gradients);
-    D and F multiples of 8.  ``act_bits`` 8: gate and up are kept in 8 bits (``act8``) for the backward pass instead of bf16."""
+    D and F multiples of 8.  ``act_bits`` 8: gate and up are kept in 8 bits (``act8``) for the backward pass instead of bf16, which
+    takes from them the gradients of gate and up and the activation, and with it the gradients of ``w_down`` and of the weights.
+
+    On a GPU sums, weights and the weighted sum are fp32; what a product reads and writes between is bf16: the rows of x, the
+    activation and, with more than 64 rows per expert on average, the down product's rows; in the backward pass the rows of the
+    output's gradient and of dx, dout W_down, d(gate) | d(up) and the weighted activation.  Up to four tokens without gradients are
+    rounded only at the end.  A pair, and fp32 matrices, are packed into one bf16 stack by every call, all experts of it, and the
+    stack is held for the backward pass; bf16 matrices as [E, 2F, D] are read where they lie."""
     first, second = w_gate_up if isinstance(w_gate_up, (tuple, list)) else (w_gate_up, None)
     if not _plain(x, logits, first, w_down):
         if x.dim() != 2 or logits.dim() != 2:
