@@ -997,7 +997,8 @@ namespace {
 
 // Up to this many rows per group, on average, the small tiles.  Small tiles, pairs, us back to back, products of 8 uneven groups (1024 x
 // 1536), of 64 (1024 x 768): 32 rows per group 9.4, 10.0; 24.1, 26.2.  64 rows 9.9, 10.5; 26.7, 30.4.  96 rows 10.2, 11.1; 32.5, 32.2,
-// but the whole feed-forward 46, 43.5; 118, 104.
+// but the whole feed-forward 46, 43.5; 118, 104.  The average counts experts without rows too (group sizes are on the device).  All rows
+// with one expert, small tiles, pairs: 8 experts, 512 rows 6.8, 10.9; 64 experts, 2048 rows 9.0, 11.1, 4096 rows 14.2, 11.9.
 constexpr int FEW_AVERAGE = 64;
 // Between these averages a feed-forward's kernels ask for their matrices before they know their rows: with fewer rows many groups would
 // have none, and with more the second tiles of groups, which come last, no longer find their matrices in L2.  The whole feed-forward without
