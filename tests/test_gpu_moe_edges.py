@@ -235,3 +235,13 @@ def test_expert_mlp_training_in_a_graph(T):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))
+
+
+def test_combine_needs_offsets():
+    """The gradient reads the end of the last expert: a plan without experts is refused before a kernel looks for it."""
+    r = moe.route(torch.randn(5, 4, device="cuda", generator=gen(0)), 2)
+    y = rand(10, 16, seed=1).requires_grad_()
+    with pytest.raises(ValueError, match="offsets"):
+        moe.combine(y, r._replace(offsets=edges_of([])))
+    with pytest.raises(ValueError, match="offsets"):
+        moe.combine(y, r._replace(offsets=edges_of([10])))

@@ -413,6 +413,7 @@ Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, 
   c10::cuda::CUDAGuard guard(y.device());
   TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ",
                     y.sizes());
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2, "combine: offsets of at least one expert expected, got ", offsets.sizes());
   check_ints(offsets, offsets.numel(), y, "combine: offsets");
   return CombineNode::apply(y.contiguous(), weights.contiguous(), slots, offsets, f32, poison);
 }
