@@ -245,3 +245,39 @@ def test_combine_needs_offsets():
         moe.combine(y, r._replace(offsets=edges_of([])))
     with pytest.raises(ValueError, match="offsets"):
         moe.combine(y, r._replace(offsets=edges_of([10])))
+
+
+def test_sizes_next_to_31_bits_are_refused():
+    """Indexes of 32 bits run past the end by a tile, a block or a grid's stride.  Views without memory of their own: nothing is copied first."""
+    long = 2 ** 31 - 100
+    row = rand(1, 8, seed=1)
+    tall = row.expand(long, 8)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    r = moe.route(torch.randn(4, 3, device="cuda", generator=gen(0)), 2)
+    rows = torch.zeros(1, device="cuda", dtype=torch.int32)
+    calls = {
+        "quantize8": lambda: act8.quantize8(tall),
+        "swiglu_8bit": lambda: act8.swiglu_8bit(tall),
+        "route": lambda: moe.route(tall[:, :4], 1),
+        "grouped_linear, rows": lambda: moe.grouped_linear(tall, row.view(1, 1, 8), edges_of([0, long])),
+        "grouped_linear, matrices": lambda: moe.grouped_linear(row, row.view(1, 1, 8).expand(1, long, 8), edges_of([0, 1])),
+        "expert_mlp, matrices": lambda: moe.expert_mlp(row, torch.zeros(1, 1, device="cuda"), row.view(1, 1, 8).expand(1, 2 ** 31, 8),
+                                                       row[:, :1].expand(8, 2 ** 30).unsqueeze(0), 1),
+        "dispatch": lambda: moe.dispatch(tall[:2 ** 30, :4], r._replace(slots=rows.expand(2 ** 30, 2), rows=rows.expand(2 ** 31))),
+        "combine": lambda: moe.combine(tall[:, :4], r._replace(slots=rows.expand(1, long), weights=rows.float().expand(1, long))),
+    }
+    for name, call in calls.items():
+        with pytest.raises((RuntimeError, ValueError), match="not supported|too many"):
+            call()
+        assert torch.cuda.max_memory_allocated() - before < 2 ** 20, name
+
+
+def test_combine_of_no_choices():
+    r = moe.route(torch.randn(5, 4, device="cuda", generator=gen(0)), 2)
+    none = r._replace(weights=torch.empty(5, 0, device="cuda", requires_grad=True), slots=torch.empty(5, 0, device="cuda", dtype=torch.int32))
+    y = torch.empty(0, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    out = moe.combine(y, none)
+    dy, dw = torch.autograd.grad(out, (y, none.weights), torch.ones_like(out))
+    assert (out == 0).all() and dy.shape == (0, 16) and dw.shape == (5, 0)

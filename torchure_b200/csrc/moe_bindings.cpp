@@ -61,11 +61,17 @@ bool bf16_or_f32(const Tensor& t, const char* what) {
   TORCH_CHECK_TYPE(b || t.scalar_type() == torch::kFloat32, what, ": bf16 or fp32 expected, got ", t.scalar_type());
   return b;
 }
+// Indexes of 32 bits in the kernels run past a size by a tile, a block of columns or a grid's stride
+constexpr int64_t MAX_SIZE = (1ll << 31) - (1 << 16), MAX_CHOICES = 1 << 30;
+void check_size(int64_t n, const char* what) {
+  TORCH_CHECK(n <= MAX_SIZE, what, ": sizes of more than 2^31 - 2^16 are not supported, got ", n);
+}
 // A matrix on the GPU whose rows are contiguous
 void check_rows(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what,
                     ": a matrix on the GPU with contiguous rows expected, got ", t.sizes());
-  TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31), what, ": sizes of 2^31 and more are not supported");
+  check_size(t.size(0), what);
+  check_size(t.size(1), what);
 }
 void check_bf16(const Tensor& t, const char* what) {
   TORCH_CHECK_TYPE(t.scalar_type() == torch::kBFloat16, what, ": bf16 expected, got ", t.scalar_type());
@@ -88,7 +94,7 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   TORCH_CHECK_VALUE(E >= 1 && E <= tb::kMaxExperts, "route: 1 to ", tb::kMaxExperts, " experts, got ", E);
   TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= tb::kMaxChoices, "route: top_k of ", k, " among ", E, " experts (at most ", tb::kMaxChoices, ")");
   TORCH_CHECK_VALUE(capacity >= 0 && capacity < (1ll << 31), "route: capacity ", capacity);
-  TORCH_CHECK_VALUE(T * k <= (1ll << 30), "route: too many choices");
+  TORCH_CHECK_VALUE(T * k <= MAX_CHOICES, "route: too many choices");
   const auto f32 = logits.options().dtype(torch::kFloat32), i32 = logits.options().dtype(torch::kInt32);
   Routed r;
   r.weights = make("route.weights", {T, k}, f32);
@@ -179,7 +185,7 @@ std::tuple<Tensor, Tensor> do_combine_bwd(const Tensor& dout, const Tensor& y, c
   TORCH_CHECK(weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.numel() == T * k, "combine_bwd: weights");
   Tensor dy = make("combine_bwd.dy", {T * k, D}, y.options());
   Tensor dw = make("combine_bwd.dweights", {T, k}, weights.options());
-  if (D == 0) return {dy, dw.zero_()};      // sums of no terms
+  if (D == 0 || k == 0) return {dy, dw.zero_()};      // sums of no terms
   const Overlap overlap;
   done("combine backward",
        tb::rows_combine_bwd(dout.data_ptr(), b16, dout.stride(0), bf(y), weights.data_ptr<float>(), slots.data_ptr<int>(),
@@ -251,7 +257,7 @@ void check_kept(const Tensor& q, const Tensor& s, int64_t blocks, const char* wh
   TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.is_contiguous() && q.scalar_type() == torch::kInt8 && s.is_cuda() && s.is_contiguous() &&
                   s.scalar_type() == torch::kFloat32 && s.dim() == 2 && s.size(0) == q.size(0) && s.size(1) == blocks &&
                   s.device() == q.device(), what, ": values (int8) and scales (fp32, one for ", tb::kActBlock, " values) do not match");
-  TORCH_CHECK(q.size(1) < (1ll << 31), what, ": sizes of 2^31 and more are not supported");
+  check_size(q.size(1), what);
 }
 
 Tensor do_dequantize(const Tensor& q, const Tensor& s, const Outputs& make) {
@@ -387,6 +393,7 @@ Tensor moe_dispatch(const Tensor& x, const Tensor& slots, const Tensor& rows, bo
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK_VALUE(x.dim() == 2 && slots.dim() == 2 && x.size(0) == slots.size(0), "dispatch: ", slots.size(0), " tokens were routed, got ",
                     x.sizes());
+  TORCH_CHECK_VALUE(rows.numel() <= MAX_CHOICES, "dispatch: too many choices");
   check_ints(slots, rows.numel(), x, "dispatch: slots");
   return DispatchNode::apply(rows_of(x), slots, rows, poison);
 }
@@ -413,6 +420,7 @@ Tensor moe_combine(const Tensor& y, const Tensor& weights, const Tensor& slots, 
   c10::cuda::CUDAGuard guard(y.device());
   TORCH_CHECK_VALUE(y.dim() == 2 && slots.dim() == 2 && y.size(0) == slots.numel(), "combine: ", slots.numel(), " rows expected, got ",
                     y.sizes());
+  TORCH_CHECK_VALUE(slots.numel() <= MAX_CHOICES, "combine: too many choices");
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2, "combine: offsets of at least one expert expected, got ", offsets.sizes());
   check_ints(offsets, offsets.numel(), y, "combine: offsets");
   return CombineNode::apply(y.contiguous(), weights.contiguous(), slots, offsets, f32, poison);
@@ -460,6 +468,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, b
                    "grouped_linear: bf16 rows and bf16 or fp32 matrices expected, got ", x.scalar_type(), " and ", w.scalar_type());
   TORCH_CHECK_VALUE(offsets.scalar_type() == torch::kInt32 && offsets.device() == x.device() && w.device() == x.device(),
                     "grouped_linear: int32 offsets and matrices on the GPU of the rows expected");
+  for (const int64_t n : {x.size(0), x.size(1), w.size(1)}) check_size(n, "grouped_linear");
   c10::cuda::CUDAGuard guard(x.device());
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad())) {
     const Tensor y = do_grouped(operand(x), matrices(w), offsets.contiguous(), false, Outputs{poison});
@@ -737,6 +746,8 @@ variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tens
                         logits.size(0) == x.size(0) && logits.size(1) == E, "expert_mlp: x ", x.sizes(), ", logits ", logits.sizes(),
                     ", w_gate_up ", first.sizes(), ", w_down ", wd.sizes(), " do not fit");
   TORCH_CHECK_VALUE(D % 8 == 0 && F % 8 == 0 && D > 0 && F > 0, "expert_mlp: widths in multiples of 8 expected, got D ", D, " and F ", F);
+  check_size(D, "expert_mlp");
+  check_size(2 * F, "expert_mlp");
   TORCH_CHECK_VALUE(x.device() == logits.device() && x.device() == first.device() && x.device() == wd.device(),
                     "expert_mlp: tensors on several GPUs");
   c10::cuda::CUDAGuard guard(x.device());
