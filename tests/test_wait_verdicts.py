@@ -56,7 +56,7 @@ def test_the_helper_votes_over_the_barrier():
     text = _code("common.cuh")
     body = text[text.index("bool mbar_wait_warps("):]
     body = body[:body.index("\n}")]
-    assert "mbar_wait_warp(" in body and "bar.red.and.pred" in body
+    assert "mbar_wait_warp(" in body and "__syncwarp();" in body[:body.index("bar.red.and.pred")]
 
 
 def test_dependents_are_let_in_behind_the_wait():

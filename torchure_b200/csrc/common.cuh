@@ -166,6 +166,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
 __device__ __forceinline__ bool mbar_wait_warps(uint64_t* bar, uint32_t parity, int* err, int code, int id, int threads) {
   const uint32_t mine = mbar_wait_warp(bar, parity, err, code) ? 1u : 0u;
   uint32_t all;
+  __syncwarp();      // (an aligned instruction: whole warps arrive)
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
