@@ -20,14 +20,27 @@ constexpr int kActBlock = 64;      // values of a row that share a scale in an 8
 // Choices of one row of logits: the k largest, ties to the lowest index; a choice whose logit is -inf is not made.
 // weights [T, k], experts [T, k], slots [T, k] (row of the choice, -1: not made or beyond the capacity), offsets [E + 1],
 // rows [T k] (t k + j of each row, -1 behind offsets[E]), counts [E] (choices made, before the capacity), aux [1].
-// scratch: route_scratch_ints(T, E, k) 32-bit words.  capacity 0: no limit.
-int64_t route_scratch_ints(int T, int E, int k);
-int route_kernels(int T, int E, int k);      // that route_fwd launches
-[[nodiscard]] int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts,
-                            int* slots, int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream);
+// scratch: route_scratch_ints(T, E, how) 32-bit words.  capacity 0: no limit.
+// how (nullptr: the logits choose, weights are the softmax over the chosen): choice by scores, see moe_route.cu.
+constexpr int kMaxExpertGroups = 32;
+struct RouteScore {
+  bool sigmoid;            // else softmax
+  const float* bias;       // [E], nullptr: none
+  int groups, top_groups;  // experts in `groups` equal parts, `top_groups` of which stay open to a token
+  bool normalize;          // weights over their sum
+  float scale;             // times this, not 0
+};
+int64_t route_scratch_ints(int T, int E, const RouteScore* how);
+int route_kernels(int T, int E, const RouteScore* how);      // that route_fwd launches
+[[nodiscard]] int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, const RouteScore* how,
+                            float* weights, int* experts, int* slots, int* offsets, int* rows, int* counts, float* aux, int* scratch,
+                            cudaStream_t stream);
 // dlogits [T, E] (the logits' type) from dweights [T, k] (nullptr: none) and daux [1] (nullptr: none)
 [[nodiscard]] int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* experts, const int* counts,
-                            const float* dweights, const float* daux, void* dlogits, int T, int E, int k, cudaStream_t stream);
+                            const float* dweights, const float* daux, void* dlogits, int T, int E, int k, const RouteScore* how,
+                            cudaStream_t stream);      // (of `how` the bias and the groups are not looked at)
+// bias[e] += rate sign(mean of counts - counts[e])
+[[nodiscard]] int balance_bias(float* bias, const int* counts, int E, float rate, cudaStream_t stream);
 
 // ---- rows to expert order and back (moe_rows.cu) -----------------------------------------------------
 // out[r] = bf16(x[rows[r] / k]), zeros where rows[r] < 0

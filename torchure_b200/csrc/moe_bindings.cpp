@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "bind_common.h"
 #include "moe_api.h"
@@ -87,7 +88,41 @@ struct Routed {
   Tensor weights, experts, slots, offsets, rows, counts, aux;
 };
 
-Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs& make) {
+// Choice by scores (moe_api.h); without one the logits choose
+struct Scoring {
+  bool sigmoid = false;
+  Tensor bias;      // not defined: none
+  int64_t groups = 1, top_groups = 1;
+  bool normalize = true;
+  double scale = 1.0;
+};
+using OptScoring = c10::optional<Scoring>;
+using PyScoring = c10::optional<std::tuple<bool, OptTensor, int64_t, int64_t, bool, double>>;
+
+tb::RouteScore raw(const Scoring& s) {
+  return {s.sigmoid, s.bias.defined() ? s.bias.data_ptr<float>() : nullptr, (int)s.groups, (int)s.top_groups, s.normalize, (float)s.scale};
+}
+
+OptScoring check_scoring(const PyScoring& given, const Tensor& logits, int64_t k, const char* what) {
+  if (!given) return c10::nullopt;
+  const auto& [sigmoid, bias, groups, top_groups, normalize, scale] = *given;
+  const int64_t E = logits.size(1);
+  TORCH_CHECK_VALUE(groups >= 1 && groups <= tb::kMaxExpertGroups && E % groups == 0, what, ": ", E, " experts in ", groups,
+                    " equal groups (at most ", tb::kMaxExpertGroups, ")");
+  TORCH_CHECK_VALUE(top_groups >= 1 && top_groups <= groups, what, ": ", top_groups, " of ", groups, " groups");
+  TORCH_CHECK_VALUE(k <= top_groups * (E / groups), what, ": top_k of ", k, " among ", top_groups, " groups of ", E / groups, " experts");
+  TORCH_CHECK_VALUE(std::isnormal((float)scale) && scale > 0, what, ": scale ", scale);
+  Scoring s{sigmoid, {}, groups, top_groups, normalize, scale};
+  if (has(bias)) {
+    TORCH_CHECK_TYPE(bias->scalar_type() == torch::kFloat32, what, ": a bias in fp32 expected, got ", bias->scalar_type());
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits.device(), what, ": a bias of ", E,
+                      " elements on the GPU of the logits expected, got ", bias->sizes());
+    s.bias = bias->detach().contiguous();
+  }
+  return s;
+}
+
+Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const OptScoring& how, const Outputs& make) {
   check_rows(logits, "route");
   const bool b16 = bf16_or_f32(logits, "route: logits");
   const int64_t T = logits.size(0), E = logits.size(1);
@@ -110,18 +145,20 @@ Routed do_route(const Tensor& logits, int64_t k, int64_t capacity, const Outputs
   }
   r.offsets = empty({E + 1}, i32);
   r.counts = empty({E}, i32);
-  const Tensor scratch = empty({tb::route_scratch_ints((int)T, (int)E, (int)k)}, i32);
+  const tb::RouteScore score = how ? raw(*how) : tb::RouteScore{};
+  const tb::RouteScore* scored = how ? &score : nullptr;
+  const Tensor scratch = empty({tb::route_scratch_ints((int)T, (int)E, scored)}, i32);
   const Overlap overlap;
-  const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, r.weights.data_ptr<float>(),
-                               r.experts.data_ptr<int>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), r.rows.data_ptr<int>(),
+  const int rc = tb::route_fwd(logits.data_ptr(), b16, logits.stride(0), (int)T, (int)E, (int)k, (int)capacity, scored,
+                               r.weights.data_ptr<float>(), r.experts.data_ptr<int>(), r.slots.data_ptr<int>(), r.offsets.data_ptr<int>(), r.rows.data_ptr<int>(),
                                r.counts.data_ptr<int>(), r.aux.data_ptr<float>(), scratch.data_ptr<int>(), cur_stream());
   TORCH_CHECK(rc == 0, "route failed with code ", rc);
-  g_launches += tb::route_kernels((int)T, (int)E, (int)k);
+  g_launches += tb::route_kernels((int)T, (int)E, scored);
   return r;
 }
 
 Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& experts, const Tensor& counts, const OptTensor& dweights,
-                    const OptTensor& daux, const Outputs& make, Tensor dl = {}) {
+                    const OptTensor& daux, const OptScoring& how, const Outputs& make, Tensor dl = {}) {
   check_rows(logits, "route_bwd");
   const bool b16 = bf16_or_f32(logits, "route_bwd: logits");
   const int64_t T = logits.size(0), E = logits.size(1), k = weights.size(1);
@@ -133,10 +170,12 @@ Tensor do_route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& e
   TORCH_CHECK(!has(daux) || (daux->is_cuda() && daux->scalar_type() == torch::kFloat32 && daux->numel() == 1), "route_bwd: daux");
   if (!dl.defined()) dl = make("route_bwd", {T, E}, logits.options());
   if (T == 0) return dl;
+  const tb::RouteScore score = how ? raw(*how) : tb::RouteScore{};
   const Overlap overlap;
   const int rc = tb::route_bwd(logits.data_ptr(), b16, logits.stride(0), weights.data_ptr<float>(), experts.data_ptr<int>(),
                                counts.data_ptr<int>(), has(dweights) ? dweights->data_ptr<float>() : nullptr,
-                               has(daux) ? daux->data_ptr<float>() : nullptr, dl.data_ptr(), (int)T, (int)E, (int)k, cur_stream());
+                               has(daux) ? daux->data_ptr<float>() : nullptr, dl.data_ptr(), (int)T, (int)E, (int)k, how ? &score : nullptr,
+                               cur_stream());
   g_launches += 1;
   TORCH_CHECK(rc == 0, "route_bwd failed with code ", rc);
   return dl;
@@ -333,10 +372,24 @@ void no_tangents(const char* what, const Ts&... tensors) {
 }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
+// What a gradient needs to know of the scores, from one pass to the other
+void keep_scoring(AutogradContext* ctx, const OptScoring& how) {
+  ctx->saved_data["scored"] = how.has_value();
+  if (!how) return;
+  ctx->saved_data["sigmoid"] = how->sigmoid;
+  ctx->saved_data["normalize"] = how->normalize;
+  ctx->saved_data["scale"] = how->scale;
+}
+OptScoring kept_scoring(AutogradContext* ctx) {
+  if (!ctx->saved_data["scored"].toBool()) return c10::nullopt;
+  return Scoring{ctx->saved_data["sigmoid"].toBool(), {}, 1, 1, ctx->saved_data["normalize"].toBool(), ctx->saved_data["scale"].toDouble()};
+}
+
 struct RouteNode : torch::autograd::Function<RouteNode> {
   // weights, aux, experts, slots, offsets, rows, counts
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
-    Routed r = do_route(logits, k, capacity, Outputs{poison});
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, int64_t capacity, const OptScoring& how, bool poison) {
+    Routed r = do_route(logits, k, capacity, how, Outputs{poison});
+    keep_scoring(ctx, how);
     ctx->save_for_backward({logits, r.weights, r.experts, r.counts});
     ctx->saved_data["poison"] = poison;
     ctx->set_materialize_grads(false);
@@ -346,11 +399,12 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once("route");
     const auto s = ctx->get_saved_variables();
-    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
     c10::cuda::CUDAGuard guard(s[0].device());
     const Tensor dw = grads[0].defined() ? grads[0].to(torch::kFloat32).contiguous() : grads[0];
     const Tensor da = grads[1].defined() ? grads[1].to(torch::kFloat32) : grads[1];
-    return {do_route_bwd(s[0], s[1], s[2], s[3], opt(dw), opt(da), Outputs{ctx->saved_data["poison"].toBool()}), Tensor(), Tensor(), Tensor()};
+    return {do_route_bwd(s[0], s[1], s[2], s[3], opt(dw), opt(da), kept_scoring(ctx), Outputs{ctx->saved_data["poison"].toBool()}), Tensor(),
+            Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -359,17 +413,33 @@ Tensor router_logits(const Tensor& t) {
   return !t.is_floating_point() || t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16 ? t : t.to(torch::kFloat32);
 }
 
-variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, bool poison) {
+variable_list moe_route(const Tensor& logits, int64_t k, int64_t capacity, const PyScoring& scoring, bool poison) {
   no_tangents("route", logits);
   TORCH_CHECK_VALUE(logits.dim() == 2 && logits.is_floating_point(), "route: logits [tokens, experts] expected, got ", logits.scalar_type(),
                     " ", logits.sizes());
   c10::cuda::CUDAGuard guard(logits.device());
   const Tensor rows = rows_of(router_logits(logits));
+  const OptScoring how = check_scoring(scoring, rows, k, "route");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
-    Routed r = do_route(rows, k, capacity, Outputs{poison});
+    Routed r = do_route(rows, k, capacity, how, Outputs{poison});
     return {r.weights, r.aux, r.experts, r.slots, r.offsets, r.rows, r.counts};
   }
-  return RouteNode::apply(rows, k, capacity, poison);
+  return RouteNode::apply(rows, k, capacity, how, poison);
+}
+
+Tensor moe_balance_bias(Tensor bias, const Tensor& counts, double rate) {
+  TORCH_CHECK_TYPE(bias.scalar_type() == torch::kFloat32, "balance_bias_: a bias in fp32 expected, got ", bias.scalar_type());
+  TORCH_CHECK_VALUE(bias.dim() == 1 && bias.is_contiguous() && !(bias.requires_grad() && at::GradMode::is_enabled()),
+                    "balance_bias_: a contiguous vector without gradient expected");
+  check_ints(counts, bias.numel(), bias, "balance_bias_: counts");
+  TORCH_CHECK_VALUE(std::isfinite((float)rate), "balance_bias_: rate ", rate);
+  if (bias.numel() == 0) return bias;
+  check_size(bias.numel(), "balance_bias_");
+  c10::cuda::CUDAGuard guard(bias.device());
+  const Overlap overlap;
+  done("balance_bias_", tb::balance_bias(bias.data_ptr<float>(), counts.data_ptr<int>(), (int)bias.numel(), (float)rate, cur_stream()));
+  bias.unsafeGetTensorImpl()->bump_version();
+  return bias;
 }
 
 struct DispatchNode : torch::autograd::Function<DispatchNode> {
@@ -557,11 +627,11 @@ bool rows_stay(const Tensor& x, int64_t R, int64_t E, bool in8) {
 // Rounded to bf16 between the kernels are gate and up (kept for the backward pass only), the activation (the down product's operand) and, unless
 // rows are few, the down product's rows, which the weighted sum reads back: in fp32 they would be 67 MB more of traffic (16384 rows of 1024).
 // Weights, sums and the weighted sum are fp32.
-Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool keep,
-            const Outputs& make) {
+Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, const OptScoring& how,
+            int64_t bits, bool keep, const Outputs& make) {
   Mlp m;
   const Overlap overlap;
-  m.r = do_route(logits, k, capacity, make);
+  m.r = do_route(logits, k, capacity, how, make);
   const int64_t R = x.size(0) * k, F = wd.size(2), E = wd.size(0), D = x.size(1);
   const Tensor act = make("expert_mlp.act", {R, F}, wgu.options());
   if (keep && bits == 16) m.gu = make("expert_mlp.gu", {R, 2 * F}, wgu.options());
@@ -640,7 +710,7 @@ struct Wanted {
 // dx, dlogits, dw_gate_up, dw_down, undefined where not wanted
 variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd,
                       const Routed& r, const Tensor& gu, const Tensor& q, const Tensor& scales, at::ScalarType wtype, const Wanted& wanted,
-                      const Outputs& make) {
+                      const OptScoring& how, const Outputs& make) {
   const int64_t T = x.size(0), k = r.slots.size(1), R = T * k, E = logits.size(1), F = wd.size(2);
   if (R == 0)
     return {at::zeros_like(x), at::zeros_like(logits), at::zeros(wgu.sizes(), wgu.options().dtype(wtype)),
@@ -666,7 +736,7 @@ variable_list mlp_bwd(const Tensor& dout, const OptTensor& daux, const Tensor& x
   if (wanted.x || wanted.logits)
     beside.run([&] {
       if (wanted.x) do_combine(dxg, c10::nullopt, r.slots, x.scalar_type(), make, dx);
-      if (wanted.logits) do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, make, dl);
+      if (wanted.logits) do_route_bwd(logits, r.weights, r.experts, r.counts, dweights, daux, how, make, dl);
     });
   if (wanted.down) dwd = do_wgrad(dg, act_w, r.offsets, wtype, make);
   beside.join();
@@ -686,9 +756,10 @@ Tensor stack_of(const Tensor& first, const OptTensor& second) {
 
 struct MlpNode : torch::autograd::Function<MlpNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second,
-                               const Tensor& wd, int64_t k, int64_t capacity, int64_t bits, bool poison) {
+                               const Tensor& wd, int64_t k, int64_t capacity, const OptScoring& how, int64_t bits, bool poison) {
     const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
-    Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, bits, true, Outputs{poison});
+    Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, bits, true, Outputs{poison});
+    keep_scoring(ctx, how);
     ctx->save_for_backward({x, logits, wgu, wdb, m.r.weights, m.r.experts, m.r.slots, m.r.offsets, m.r.rows, m.r.counts, m.gu, m.q, m.scales});
     ctx->saved_data["type"] = static_cast<int64_t>(wd.scalar_type());
     ctx->saved_data["pair"] = has(second);
@@ -700,12 +771,12 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     only_once("expert_mlp");
     const auto s = ctx->get_saved_variables();
     const Outputs make{ctx->saved_data["poison"].toBool()};
-    variable_list out(9);
+    variable_list out(10);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     c10::cuda::CUDAGuard guard(s[0].device());
     const Tensor daux = grads[1].defined() ? grads[1].to(torch::kFloat32) : grads[1];
     if (!grads[0].defined()) {
-      out[1] = do_route_bwd(s[1], s[4], s[5], s[9], c10::nullopt, opt(daux), make);
+      out[1] = do_route_bwd(s[1], s[4], s[5], s[9], c10::nullopt, opt(daux), kept_scoring(ctx), make);
       return out;
     }
     Routed r{s[4], s[5], s[6], s[7], s[8], s[9], Tensor()};
@@ -714,7 +785,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     const Wanted wanted{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2) || (pair && ctx->needs_input_grad(3)),
                         ctx->needs_input_grad(pair ? 4 : 3)};
     auto g = mlp_bwd(rows_of(grads[0]), opt(daux), s[0], s[1], s[2], s[3], r, s[10], s[11], s[12],
-                     static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), wanted, make);
+                     static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), wanted, kept_scoring(ctx), make);
     const int64_t F = s[3].size(2);
     out[0] = g[0];
     out[1] = g[1];
@@ -726,7 +797,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
 };
 
 variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
-                         int64_t capacity, int64_t bits, bool poison) {
+                         int64_t capacity, const PyScoring& scoring, int64_t bits, bool poison) {
   no_tangents("expert_mlp", x, given_logits, first, has(second) ? *second : Tensor(), wd);
   check_rows(x, "expert_mlp: x");
   check_rows(given_logits, "expert_mlp: logits");
@@ -751,16 +822,17 @@ variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tens
   TORCH_CHECK_VALUE(x.device() == logits.device() && x.device() == first.device() && x.device() == wd.device(),
                     "expert_mlp: tensors on several GPUs");
   c10::cuda::CUDAGuard guard(x.device());
+  const OptScoring how = check_scoring(scoring, logits, k, "expert_mlp");
   const bool keep = at::GradMode::is_enabled() &&
                     (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() ||
                      (pair && second->requires_grad()));
-  if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, bits, poison);
+  if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, how, bits, poison);
   const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
-  if (runs_by_token(x, k, wgu, wdb)) {
+  if (!how && runs_by_token(x, k, wgu, wdb)) {      // (the token kernels choose by logits)
     const Overlap overlap;
     return mlp_by_token(x, logits, wgu, wdb, k, capacity, Outputs{poison});
   }
-  Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, bits, false, Outputs{poison});
+  Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, bits, false, Outputs{poison});
   return {m.out, m.r.aux};
 }
 
@@ -768,6 +840,7 @@ variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tens
 
 void register_moe(pybind11::module_& m) {
   m.def("moe_route", &moe_route, "(weights, aux, experts, slots, offsets, rows, counts)");
+  m.def("moe_balance_bias", &moe_balance_bias);
   m.def("moe_dispatch", &moe_dispatch);
   m.def("moe_combine", &moe_combine);
   m.def("grouped_linear", &grouped_linear);

@@ -1,5 +1,5 @@
 // The router of a mixture of experts: top-k choice, weights, the order of rows by expert, the load-balancing term, and the
-// gradient of weights and term.
+// gradient of weights and term; the same by scores, with a bias and groups of experts, and the bias' update.
 //
 // Per token, logits l over E experts, k of them chosen in falling order (ties to the lowest index):
 //   w_j = exp(l_j) / sum over the chosen of exp(l_i),  p = softmax(l),  aux = E sum_e share_e mean_t p[t, e]
@@ -169,6 +169,93 @@ __device__ void plan_rows(const RouteArgs& a, const int* codes, const int* all_h
 
 constexpr int plan_smem_ints(int E) { return 3 * E + 1 + kWarps * (E | 1) + kWarps; }
 
+// The k largest keys of a token, in falling order, the lowest index among equals: choice j in thread j of the token's (its key and index).  A
+// thread's indices rise.  PACKED: a key carries its index in the low 16 bits, falling.
+template <int VALS, bool PACKED>
+__device__ __forceinline__ void choose(uint32_t (&key)[VALS], int (&index)[VALS], int k, int gl, uint32_t mask, uint32_t& my_key, int& my_e) {
+  if constexpr (VALS <= 4) {           // falling keys; equal ones stay in the order of their indices
+#pragma unroll
+    for (int i = 1; i < VALS; ++i)
+#pragma unroll
+      for (int v = VALS - 1; v >= i; --v) {
+        const bool swap = key[v] > key[v - 1];
+        const uint32_t lo = swap ? key[v - 1] : key[v], hi = swap ? key[v] : key[v - 1];
+        const int ilo = swap ? index[v - 1] : index[v], ihi = swap ? index[v] : index[v - 1];
+        key[v] = lo;
+        key[v - 1] = hi;
+        index[v] = ilo;
+        index[v - 1] = ihi;
+      }
+  }
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = key[0];
+    if constexpr (VALS > 4) {
+#pragma unroll
+      for (int v = 1; v < VALS; ++v) best = max(best, key[v]);
+    }
+    best = __reduce_max_sync(mask, best);
+    int at = 0x7fffffff;
+    if constexpr (!PACKED) {
+      if constexpr (VALS <= 4) {
+        if (key[0] == best) at = index[0];
+      } else {
+#pragma unroll
+        for (int v = VALS - 1; v >= 0; --v)
+          if (key[v] == best) at = index[v];
+      }
+      at = __reduce_min_sync(mask, at);
+    } else {
+      at = 0xffff - static_cast<int>(best & 0xffffu);
+    }
+    if constexpr (VALS <= 4) {
+      if (index[0] == at) {
+#pragma unroll
+        for (int v = 0; v + 1 < VALS; ++v) {
+          key[v] = key[v + 1];
+          index[v] = index[v + 1];
+        }
+        key[VALS - 1] = 0;
+        index[VALS - 1] = -1;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VALS; ++v)
+        if (index[v] == at) key[v] = 0;
+    }
+    if (gl == j) { my_key = best; my_e = at; }
+  }
+}
+
+// What a CTA leaves of its tokens: the counts of its choices and the sums of its probabilities (acc, of the experts `index`), or with one CTA
+// the whole plan.
+template <int LANES, int VALS>
+__device__ __forceinline__ void close_chunk(const RouteArgs& a, float (&acc)[VALS], const int (&index)[VALS], const int* codes, int* hist,
+                                            float* psum, int* rest, int single) {
+  const int E = a.E, tid = threadIdx.x, lane = tid & 31;
+  float* part = reinterpret_cast<float*>(rest);           // [kWarps][E | 1]
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) {
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
+    if (lane < LANES && index[v] < E) part[(tid >> 5) * (E | 1) + index[v]] = acc[v];
+  }
+  __syncthreads();
+  for (int e = tid >> 5; e < E; e += kWarps) {      // a warp adds up the warps' sums of one expert
+    const float s = group_sum<32>(part[lane * (E | 1) + e], 0xffffffffu);
+    if (lane != 0) continue;
+    if (single) {
+      psum[e] = s;
+    } else {
+      a.psum[static_cast<int64_t>(blockIdx.x) * E + e] = s;
+      a.hist[static_cast<int64_t>(blockIdx.x) * E + e] = hist[e];
+    }
+  }
+  if (single) {
+    __syncthreads();
+    plan_rows(a, codes, hist, psum, 0, 1, rest);
+  }
+}
+
 template <class T, int LANES, int VALS>
 __global__ void __launch_bounds__(kThreads)
 route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
@@ -182,10 +269,10 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
   float* psum = reinterpret_cast<float*>(sm + E);         // [E]
   int* codes = sm + 2 * E;                                // [T k] with one CTA
   int* rest = codes + (single ? a.T * a.k : 0);
-  float* part = reinterpret_cast<float*>(rest);           // [kWarps][E | 1]
   for (int e = tid; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
   float acc[VALS];
+  int index[VALS];
 #pragma unroll
   for (int v = 0; v < VALS; ++v) acc[v] = 0.f;
   const int t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
@@ -210,60 +297,9 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
 #pragma unroll
       for (int v = 0; v < VALS; ++v) key[v] = key[v] ? (key[v] & 0xffff0000u) | (0xffffu - (v * LANES + gl)) : 0u;
     }
-    int index[VALS];
 #pragma unroll
     for (int v = 0; v < VALS; ++v) index[v] = v * LANES + gl;
-    if constexpr (VALS <= 4) {           // falling keys; equal ones stay in the order of their indices
-#pragma unroll
-      for (int i = 1; i < VALS; ++i)
-#pragma unroll
-        for (int v = VALS - 1; v >= i; --v) {
-          const bool swap = key[v] > key[v - 1];
-          const uint32_t lo = swap ? key[v - 1] : key[v], hi = swap ? key[v] : key[v - 1];
-          const int ilo = swap ? index[v - 1] : index[v], ihi = swap ? index[v] : index[v - 1];
-          key[v] = lo;
-          key[v - 1] = hi;
-          index[v] = ilo;
-          index[v - 1] = ihi;
-        }
-    }
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = key[0];
-      if constexpr (VALS > 4) {
-#pragma unroll
-        for (int v = 1; v < VALS; ++v) best = max(best, key[v]);
-      }
-      best = __reduce_max_sync(mask, best);
-      int at = 0x7fffffff;
-      if constexpr (sizeof(T) == 4) {
-        if constexpr (VALS <= 4) {
-          if (key[0] == best) at = index[0];
-        } else {
-#pragma unroll
-          for (int v = VALS - 1; v >= 0; --v)
-            if (key[v] == best) at = index[v];
-        }
-        at = __reduce_min_sync(mask, at);
-      } else {
-        at = 0xffff - static_cast<int>(best & 0xffffu);
-      }
-      if constexpr (VALS <= 4) {
-        if (index[0] == at) {
-#pragma unroll
-          for (int v = 0; v + 1 < VALS; ++v) {
-            key[v] = key[v + 1];
-            index[v] = index[v + 1];
-          }
-          key[VALS - 1] = 0;
-          index[VALS - 1] = -1;
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < VALS; ++v)
-          if (index[v] == at) key[v] = 0;
-      }
-      if (gl == j) { my_key = best; my_e = at; }
-    }
+    choose<VALS, sizeof(T) == 2>(key, index, a.k, gl, mask, my_key, my_e);
     // the key of a bf16 value: its low bits as to_key leaves them
     if constexpr (sizeof(T) == 2) my_key = (my_key >> 31) ? my_key & 0xffff0000u : my_key | 0xffffu;
     const float top = from_key(__shfl_sync(mask, my_key, 0, LANES));
@@ -293,27 +329,8 @@ route_fwd_kernel(const T* __restrict__ logits, RouteArgs a, int single) {
     }
   }
 #pragma unroll
-  for (int v = 0; v < VALS; ++v) {
-    const int e = v * LANES + gl;
-#pragma unroll
-    for (int o = LANES; o < 32; o <<= 1) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
-    if (lane < LANES && e < E) part[(tid >> 5) * (E | 1) + e] = acc[v];
-  }
-  __syncthreads();
-  for (int e = tid >> 5; e < E; e += kWarps) {      // a warp adds up the warps' sums of one expert
-    const float s = group_sum<32>(part[lane * (E | 1) + e], 0xffffffffu);
-    if (lane != 0) continue;
-    if (single) {
-      psum[e] = s;
-    } else {
-      a.psum[static_cast<int64_t>(blockIdx.x) * E + e] = s;
-      a.hist[static_cast<int64_t>(blockIdx.x) * E + e] = hist[e];
-    }
-  }
-  if (single) {
-    __syncthreads();
-    plan_rows(a, codes, hist, psum, 0, 1, rest);
-  }
+  for (int v = 0; v < VALS; ++v) index[v] = v * LANES + gl;
+  close_chunk<LANES, VALS>(a, acc, index, codes, hist, psum, rest, single);
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -394,6 +411,280 @@ route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restri
   }
 }
 
+// ---- choice by scores, with a bias and groups of experts -----------------------------------------------
+// s = sigmoid(l) or softmax(l), rounded to fp32 from 64 bits; with a bias or groups the choice goes by c = s + bias, else by l.  A group's score is
+// the sum of its two largest c; the experts of the top_groups largest groups stay open (ties to the lowest index).  Weights of the choices made:
+//   w_j = scale s_j / (normalize: sum over the chosen of s_i, else 1);  aux = E sum_e share_e mean_t P[t, e], P = s / sum over all of s
+// and with what = w / scale, d = 1 - s (sigmoid) or 1 (softmax):
+//   dl_j += d_j what_j (scale dw_j - (normalize ? inner : 0)), inner = sum_i what_i scale dw_i;  softmax, not normalized: dl_e -= s_e inner
+//   dl_e += daux E / T d_e P_e (share_e - sum_i share_i P_i)
+// Scores 1e-7 apart decide which expert a token goes to and with it the order of all rows behind; computed in 32 bits they would depend on the
+// machine's exp, rounded once from 64 they do not.
+struct ScoreArgs {
+  const float* bias;       // nullptr: none
+  int groups, top_groups, each;      // each: experts of a group
+  int groups_log2;         // of the power of two that holds `groups`
+  int sigmoid, normalize;
+  float scale;
+};
+
+// s over exp(shift) for scores that may all be tiny: sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|))
+__device__ __forceinline__ float sigmoid_over(float l, float shift) { return expf(fminf(l, 0.f) - shift) / (1.f + expf(-fabsf(l))); }
+
+template <int LANES>
+__device__ __forceinline__ float group_max(float v, uint32_t mask) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o, LANES));
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ double group_sum64(double v, uint32_t mask) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o, LANES);
+  return v;
+}
+
+// The experts of a group lie with neighbouring threads: of the token's threads, LANES / 2^groups_log2 for each group.
+template <class T, int LANES, int VALS>
+__global__ void __launch_bounds__(kThreads)
+route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, int single) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ int sm[];
+  constexpr int GROUPS = kThreads / LANES;
+  const int E = a.E, tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1), group = tid / LANES;
+  const uint32_t mask = group_mask<LANES>(lane);
+  const int per = LANES >> how.groups_log2, mine = gl / per, sub = gl - mine * per;      // threads of a group of experts, the group, the place in it
+  int* hist = sm;                                         // [E]
+  float* psum = reinterpret_cast<float*>(sm + E);         // [E]
+  int* codes = sm + 2 * E;                                // [T k] with one CTA
+  int* rest = codes + (single ? a.T * a.k : 0);
+  for (int e = tid; e < E; e += kThreads) hist[e] = 0;
+  __syncthreads();
+  const bool by_score = how.bias != nullptr || how.groups > 1;
+  float acc[VALS], bias[VALS];
+  int expert[VALS];
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) {
+    const int in = v * per + sub;
+    expert[v] = mine < how.groups && in < how.each ? mine * how.each + in : 0x7fffffff;
+    acc[v] = 0.f;
+    bias[v] = how.bias != nullptr && expert[v] < E ? how.bias[expert[v]] : 0.f;
+  }
+  const int t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
+  float next[VALS];      // the logits of the token after the one that is worked on
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) next[v] = t < t1 && expert[v] < E ? load_logit(logits + t * a.ld + expert[v]) : -INFINITY;
+  };
+  fetch(t0 + group);
+  for (int t = t0 + group; t < t1; t += GROUPS) {
+    float x[VALS], top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      x[v] = next[v];
+      top = fmaxf(top, x[v]);
+    }
+    fetch(t + GROUPS);
+    top = group_max<LANES>(top, mask);
+    float s[VALS];
+    if (how.sigmoid) {
+#pragma unroll
+      for (int v = 0; v < VALS; ++v)
+        s[v] = by_score ? static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(x[v])))) : sigmoid_over(x[v], 0.f);
+    } else {
+      double e[VALS], sum = 0.0;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) {
+        e[v] = top == -INFINITY ? 0.0 : exp(static_cast<double>(x[v]) - static_cast<double>(top));
+        sum += e[v];
+      }
+      sum = group_sum64<LANES>(sum, mask);
+      const double r = sum > 0.0 || sum != sum ? 1.0 / sum : 0.0;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) s[v] = static_cast<float>(e[v] * r);
+    }
+    uint32_t key[VALS];
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const float c = !by_score ? x[v] : x[v] == -INFINITY ? -INFINITY : s[v] + bias[v];
+      key[v] = expert[v] < E ? to_key(c) : 0u;
+    }
+    if (how.groups > 1) {
+      uint32_t first = 0, second = 0;      // the largest two of the group
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) {
+        second = max(second, min(first, key[v]));
+        first = max(first, key[v]);
+      }
+      for (int o = per / 2; o > 0; o >>= 1) {
+        const uint32_t f = __shfl_xor_sync(mask, first, o, LANES), g = __shfl_xor_sync(mask, second, o, LANES);
+        second = max(max(second, g), min(first, f));
+        first = max(first, f);
+      }
+      const uint32_t total = second <= kKeyMinusInf ? first : to_key(from_key(first) + from_key(second));
+      int ahead = 0;
+      for (int g = 0; g < how.groups; ++g) {
+        const uint32_t other = __shfl_sync(mask, total, g * per, LANES);
+        ahead += other > total || (other == total && g < mine);
+      }
+      if (ahead >= how.top_groups) {
+#pragma unroll
+        for (int v = 0; v < VALS; ++v) key[v] = min(key[v], kKeyMinusInf);
+      }
+    }
+    uint32_t my_key = 0;
+    int my_e = 0, index[VALS];
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) index[v] = expert[v];
+    choose<VALS, false>(key, index, a.k, gl, mask, my_key, my_e);
+    const bool made = gl < a.k && my_key != kKeyMinusInf;
+    const float l = made ? load_logit(logits + t * a.ld + my_e) : -INFINITY;
+    float shift = 0.f;
+    if (how.normalize) shift = group_max<LANES>(how.sigmoid ? (made ? fminf(l, 0.f) : -INFINITY) : l, mask);
+    float w = 0.f;
+    if (made) w = how.sigmoid ? sigmoid_over(l, shift) : expf(l - (how.normalize ? shift : top));
+    float whole = 1.f;
+    if (how.normalize) {
+      whole = group_sum<LANES>(w, mask);
+    } else if (!how.sigmoid) {
+      whole = 0.f;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) whole += top == -INFINITY ? 0.f : expf(x[v] - top);
+      whole = group_sum<LANES>(whole, mask);
+    }
+    if (gl < a.k) {
+      const int64_t i = static_cast<int64_t>(t) * a.k + gl;
+      a.weights[i] = made ? how.scale * (w / whole) : 0.f;
+      a.experts[i] = my_e;
+      const int code = made ? my_e : -1;
+      if (single) codes[i] = code;
+      else a.slots[i] = code;
+      if (made) atomicAdd(&hist[my_e], 1);
+    }
+    if (how.sigmoid) {
+      // scores below 2^-115 have lost bits in fp32: where there are no others, all over the largest one's
+      if (top < -80.f && top != -INFINITY) {
+#pragma unroll
+        for (int v = 0; v < VALS; ++v) s[v] = sigmoid_over(x[v], top);
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) sum += s[v];
+      sum = group_sum<LANES>(sum, mask);
+      const float r = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) acc[v] += s[v] * r;
+    } else {
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) acc[v] += s[v];
+    }
+  }
+  close_chunk<LANES, VALS>(a, acc, expert, codes, hist, psum, rest, single);
+}
+
+template <class T, int LANES, int VALS>
+__global__ void __launch_bounds__(kBwdThreads)
+route_scored_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ weights, const int* __restrict__ experts,
+                        const int* __restrict__ counts, const float* __restrict__ dweights, const float* __restrict__ daux,
+                        T* __restrict__ dlogits, int n_tokens, int E, int k, int sigmoid, int normalize, float scale) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int GROUPS = kBwdThreads / LANES;
+  const int tid = threadIdx.x, lane = tid & 31, gl = tid & (LANES - 1);
+  const uint32_t mask = group_mask<LANES>(lane);
+  const float pull = daux ? *daux * static_cast<float>(E) / static_cast<float>(n_tokens) : 0.f;
+  const float per = 1.f / (static_cast<float>(n_tokens) * static_cast<float>(k));
+  float share[VALS];
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) share[v] = v * LANES + gl < E ? static_cast<float>(counts[v * LANES + gl]) * per : 0.f;
+  for (int t = blockIdx.x * GROUPS + tid / LANES; t < n_tokens; t += gridDim.x * GROUPS) {
+    float x[VALS], top = -INFINITY;
+    bool odd = false;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const int e = v * LANES + gl;
+      x[v] = e < E ? load_logit(logits + t * ld + e) : -INFINITY;
+      odd |= x[v] != x[v];
+      top = fmaxf(top, x[v]);
+    }
+    top = group_max<LANES>(top, mask);
+    odd = __any_sync(mask, odd);      // a NaN among the logits makes the whole row's gradient NaN
+    const bool none = top == -INFINITY;
+    const float shift = sigmoid ? fminf(top, 0.f) : top;
+    float p[VALS], s = 0.f, mean = 0.f;
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      p[v] = none ? 0.f : sigmoid ? sigmoid_over(x[v], shift) : expf(x[v] - top);
+      s += p[v];
+      mean += p[v] * share[v];
+    }
+    s = group_sum<LANES>(s, mask);
+    mean = group_sum<LANES>(mean, mask);
+    const float r = none ? 0.f : 1.f / s;
+    mean *= r;
+    float w = 0.f, dw = 0.f, inner = 0.f, g = 0.f;
+    int e_j = -1;
+    if (dweights) {
+      if (gl < k) {
+        const int64_t i = static_cast<int64_t>(t) * k + gl;
+        w = weights[i] / scale;
+        e_j = experts[i];
+        dw = w != 0.f ? scale * dweights[i] : 0.f;
+      }
+      inner = group_sum<LANES>(w * dw, mask);
+      g = w * (dw - (normalize ? inner : 0.f));
+      // (an expert of a choice that was not made may have any logit)
+      if (sigmoid && g != 0.f && e_j >= 0 && e_j < E) g *= sigmoid_over(-load_logit(logits + t * ld + e_j), 0.f);
+      if (normalize || sigmoid) inner = 0.f;      // from here on what every expert pays for a softmax's sum
+    }
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const float q = p[v] * r;
+      float d = pull == 0.f ? 0.f : pull * q * (share[v] - mean);
+      if (sigmoid) d = d == 0.f ? 0.f : d * sigmoid_over(-x[v], 0.f);
+      else d -= q * inner;
+      x[v] = odd ? __uint_as_float(0x7fffffffu) : d;
+    }
+    if (dweights) {
+      for (int j = 0; j < k; ++j) {
+        const float gj = __shfl_sync(mask, g, j, LANES);
+        const int ej = __shfl_sync(mask, e_j, j, LANES);
+#pragma unroll
+        for (int v = 0; v < VALS; ++v)
+          if (ej == v * LANES + gl) x[v] += gj;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VALS; ++v) {
+      const int e = v * LANES + gl;
+      if (e < E) dlogits[static_cast<int64_t>(t) * E + e] = static_cast<T>(x[v]);
+    }
+  }
+}
+
+// bias[e] += rate sign(mean of the counts - counts[e]), the comparison in whole numbers
+__global__ void __launch_bounds__(kThreads)
+balance_bias_kernel(float* __restrict__ bias, const int* __restrict__ counts, int E, float rate) {
+  pdl_wait();
+  pdl_launch_dependents();
+  __shared__ long long parts[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31;
+  long long sum = 0;
+  for (int e = tid; e < E; e += kThreads) sum += counts[e];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) parts[tid >> 5] = sum;
+  __syncthreads();
+  sum = parts[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int e = tid; e < E; e += kThreads) {
+    const long long over = static_cast<long long>(counts[e]) * E - sum;
+    bias[e] += over < 0 ? rate : over > 0 ? -rate : 0.f;
+  }
+}
+
 int lanes_for(int E) {
   int l = 4;
   while (l < E && l < 32) l <<= 1;
@@ -401,8 +692,8 @@ int lanes_for(int E) {
 }
 
 // (chunks, tokens of a chunk)
-void chunks_for(int T, int E, int k, int& chunks, int& chunk) {
-  const int groups = kThreads / lanes_for(E);
+void chunks_for(int T, int lanes, int& chunks, int& chunk) {
+  const int groups = kThreads / lanes;
   // One CTA for as many tokens as it has groups.  One CTA, two kernels, us: 128 tokens x 8 experts 6.3, 7.5 and 256 tokens (two rounds) 8.2,
   // 7.5; 32 x 256 12.2, 13.8 and 64 (two rounds) 17.1, 13.8.
   if (T <= groups) {
@@ -421,6 +712,29 @@ int vals_for(int E) {
   int v = 1;
   while (v * 32 < E) v <<= 1;
   return v;
+}
+
+bool score_fits(int E, int k, const RouteScore& how) {
+  return how.groups >= 1 && how.groups <= kMaxExpertGroups && E % how.groups == 0 && how.top_groups >= 1 && how.top_groups <= how.groups &&
+         k <= how.top_groups * (E / how.groups);
+}
+
+// Threads of a token, logits of a thread and log2 of the groups' places: each group has the same power of two of threads.
+void scored_shape(int E, const RouteScore& how, int& lanes, int& vals, int& groups_log2) {
+  groups_log2 = 0;
+  while ((1 << groups_log2) < how.groups) ++groups_log2;
+  const int each = E / how.groups;
+  lanes = 4;
+  while (lanes < 32 && (lanes >> groups_log2) < each) lanes <<= 1;
+  vals = 1;
+  while (vals * (lanes >> groups_log2) < each) vals <<= 1;
+}
+
+int lanes_of(int E, const RouteScore* how) {
+  if (how == nullptr) return lanes_for(E);
+  int lanes, vals, log2;
+  scored_shape(E, *how, lanes, vals, log2);
+  return lanes;
 }
 
 template <class T>
@@ -443,41 +757,95 @@ int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t str
   return -2;
 }
 
+// (groups that are no power of two leave threads without experts: up to 22 logits for the others)
+#define TB_SCORED_SIZES(CASE) TB_ROUTE_SIZES(CASE) CASE(32, 32)
+
+template <class T>
+int launch_scored(const T* logits, const RouteArgs& a, const RouteScore& how, int chunks, cudaStream_t stream) {
+  int lanes, vals;
+  ScoreArgs s{};
+  scored_shape(a.E, how, lanes, vals, s.groups_log2);
+  s.bias = how.bias; s.groups = how.groups; s.top_groups = how.top_groups; s.each = a.E / how.groups;
+  s.sigmoid = how.sigmoid; s.normalize = how.normalize; s.scale = how.scale;
+  const int plan = plan_smem_ints(a.E), sums = kWarps * (a.E | 1);
+  const int smem = 4 * (chunks == 1 ? 2 * a.E + a.T * a.k + (sums > plan ? sums : plan) : 2 * a.E + sums);
+#define CASE(L, V)                                                                                                                 \
+  if (lanes == L && vals == V) {                                                                                                   \
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(route_scored_kernel<T, L, V>), smem) ||                                  \
+        !ensure_dynamic_smem(reinterpret_cast<const void*>(route_plan_kernel), 4 * plan))                                           \
+      return -20;                                                                                                                  \
+    int rc = launch_code(                                                                                                          \
+        launch_pdl(route_scored_kernel<T, L, V>, dim3(chunks), dim3(kThreads), smem, stream, logits, a, s, chunks == 1 ? 1 : 0));     \
+    if (rc == 0 && chunks > 1)                                                                                                     \
+      rc = launch_code(launch_pdl(route_plan_kernel, dim3(chunks), dim3(kThreads), 4 * static_cast<size_t>(plan), stream, a));      \
+    return rc;                                                                                                                     \
+  }
+  TB_SCORED_SIZES(CASE)
+#undef CASE
+  return -2;
+}
+
 }  // namespace
 
-int64_t route_scratch_ints(int T, int E, int k) {
+int balance_bias(float* bias, const int* counts, int E, float rate, cudaStream_t stream) {
+  if (E < 1) return -1;
+  return launch_code(launch_pdl(balance_bias_kernel, dim3(1), dim3(kThreads), 0, stream, bias, counts, E, rate));
+}
+
+int64_t route_scratch_ints(int T, int E, const RouteScore* how) {
   int chunks, chunk;
-  chunks_for(T, E, k, chunks, chunk);
+  chunks_for(T, lanes_of(E, how), chunks, chunk);
   return 2 * static_cast<int64_t>(chunks) * E;
 }
 
-int route_kernels(int T, int E, int k) {
+int route_kernels(int T, int E, const RouteScore* how) {
   int chunks, chunk;
-  chunks_for(T, E, k, chunks, chunk);
+  chunks_for(T, lanes_of(E, how), chunks, chunk);
   return chunks > 1 ? 2 : 1;
 }
 
-int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, float* weights, int* experts, int* slots,
-              int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream) {
+int route_fwd(const void* logits, bool bf16, int64_t ld, int T, int E, int k, int capacity, const RouteScore* how, float* weights,
+              int* experts, int* slots, int* offsets, int* rows, int* counts, float* aux, int* scratch, cudaStream_t stream) {
   if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices || static_cast<int64_t>(T) * k > (1ll << 30)) return -1;
+  if (how != nullptr && !score_fits(E, k, *how)) return -1;
   RouteArgs a{};
   a.ld = ld; a.T = T; a.E = E; a.k = k; a.capacity = capacity;
   a.weights = weights; a.experts = experts; a.slots = slots; a.offsets = offsets; a.rows = rows; a.counts = counts; a.aux = aux;
   int chunks;
-  chunks_for(T, E, k, chunks, a.chunk);
+  chunks_for(T, lanes_of(E, how), chunks, a.chunk);
   a.hist = scratch;
   a.psum = reinterpret_cast<float*>(scratch + static_cast<int64_t>(chunks) * E);
+  if (how != nullptr)
+    return bf16 ? launch_scored(static_cast<const __nv_bfloat16*>(logits), a, *how, chunks, stream)
+                : launch_scored(static_cast<const float*>(logits), a, *how, chunks, stream);
   return bf16 ? launch_fwd(static_cast<const __nv_bfloat16*>(logits), a, chunks, stream)
               : launch_fwd(static_cast<const float*>(logits), a, chunks, stream);
 }
 
 int route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* experts, const int* counts,
-              const float* dweights, const float* daux, void* dlogits, int T, int E, int k, cudaStream_t stream) {
+              const float* dweights, const float* daux, void* dlogits, int T, int E, int k, const RouteScore* how, cudaStream_t stream) {
   if (T < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxChoices) return -1;
+  if (how != nullptr && !score_fits(E, k, *how)) return -1;
   const int lanes = lanes_for(E), vals = vals_for(E);
   const int groups = kBwdThreads / lanes;
   const int need = (T + groups - 1) / groups;
   const int grid = need < 148 * 8 ? need : 148 * 8;
+  if (how != nullptr) {
+#define CASE(L, V)                                                                                                              \
+  if (lanes == L && vals == V) {                                                                                                \
+    const cudaError_t rc =                                                                                                      \
+        bf16 ? launch_pdl(route_scored_bwd_kernel<__nv_bfloat16, L, V>, dim3(grid), dim3(kBwdThreads), 0, stream,                  \
+                          static_cast<const __nv_bfloat16*>(logits), ld, weights, experts, counts, dweights, daux,               \
+                          static_cast<__nv_bfloat16*>(dlogits), T, E, k, how->sigmoid ? 1 : 0, how->normalize ? 1 : 0, how->scale) \
+             : launch_pdl(route_scored_bwd_kernel<float, L, V>, dim3(grid), dim3(kBwdThreads), 0, stream,                          \
+                          static_cast<const float*>(logits), ld, weights, experts, counts, dweights, daux,                       \
+                          static_cast<float*>(dlogits), T, E, k, how->sigmoid ? 1 : 0, how->normalize ? 1 : 0, how->scale);        \
+    return launch_code(rc);                                                                                                      \
+  }
+  TB_ROUTE_SIZES(CASE)
+#undef CASE
+    return -2;
+  }
 #define CASE(L, V)                                                                                                              \
   if (lanes == L && vals == V) {                                                                                                \
     const cudaError_t rc =                                                                                                      \

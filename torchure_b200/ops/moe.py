@@ -1,6 +1,7 @@
 """Operators of a mixture-of-experts feed-forward: router, rows by expert and back, products grouped by expert.
 
-``route``           top-k choice, weights, the order of rows by expert, the load-balancing term
+``route``           top-k choice (by logits, or by scores with a bias and groups of experts), weights, the order of rows by expert, the
+                    load-balancing term;   ``balance_bias_``  the bias of the next step
 ``dispatch``        token rows in expert order;   ``combine``  their weighted sums back in token order
 ``grouped_linear``  rows grouped by expert times each expert's matrix
 ``expert_mlp``      all of it: router, gate / up product, SwiGLU, down product, weighted sum, in one native call per direction
@@ -28,9 +29,9 @@ BF16 = torch.bfloat16
 class Routing(NamedTuple):
     """What ``route`` found, T tokens and k choices each."""
 
-    weights: torch.Tensor     # fp32 [T, k], sum 1 over the choices made; differentiable
+    weights: torch.Tensor     # fp32 [T, k], sum 1 over the choices made (`normalize`; times `scale`); differentiable
     aux_loss: torch.Tensor    # fp32, 0-dim; differentiable
-    experts: torch.Tensor     # int32 [T, k], falling logits
+    experts: torch.Tensor     # int32 [T, k], falling logits (or biased scores)
     slots: torch.Tensor       # int32 [T, k]: row of the choice in expert order; -1: not made, or beyond the capacity
     offsets: torch.Tensor     # int32 [E + 1]: first row of each expert
     rows: torch.Tensor        # int32 [T k]: t k + j of each row; -1 behind offsets[E]
@@ -51,23 +52,82 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
-def route(logits: torch.Tensor, top_k: int, capacity: int = 0) -> Routing:
+class Scoring(NamedTuple):
+    """How ``route`` scores experts, where the softmax over the chosen logits is not what is wanted."""
+
+    score: str = "softmax"            # or "sigmoid"
+    bias: torch.Tensor | None = None  # fp32 [E], added to the scores for the choice only; no gradient
+    groups: int = 1                   # experts in so many equal, consecutive groups
+    top_groups: int = 1               # groups that stay open to a token
+    normalize: bool = True            # weights over their sum
+    scale: float = 1.0                # ... times this
+
+
+def _scoring(experts: int, top_k: int, score: str, bias, groups: int, top_groups: int, normalize: bool, scale: float):
+    """The ``Scoring`` of these arguments, or None where they ask for the plain choice by logits."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f'route: scores are "softmax" or "sigmoid", not {score!r}')
+    if groups < 1 or experts % groups:
+        raise ValueError(f"route: {experts} experts in {groups} equal groups")
+    if groups == 1 and top_groups in (0, 1):
+        top_groups = 1
+    elif not 1 <= top_groups <= groups:
+        raise ValueError(f"route: {top_groups} of {groups} groups")
+    if top_k > top_groups * (experts // groups):
+        raise ValueError(f"route: top_k of {top_k} among {top_groups} groups of {experts // groups} experts")
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"route: scale {scale}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (experts,)):
+        raise ValueError(f"route: a bias of {experts} fp32 elements expected, got {bias.dtype} {tuple(bias.shape)}")
+    if score == "softmax" and bias is None and groups == 1 and normalize and scale == 1.0:
+        return None
+    return Scoring(score, bias, groups, top_groups, bool(normalize), float(scale))
+
+
+def _native(how: Scoring | None):
+    return None if how is None else (how.score == "sigmoid", how.bias, how.groups, how.top_groups, how.normalize, how.scale)
+
+
+def route(logits: torch.Tensor, top_k: int, capacity: int = 0, *, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+          top_groups: int = 0, normalize: bool = True, scale: float = 1.0) -> Routing:
     """The ``top_k`` experts of every token by its logits [T, E] (fp32 or bf16, others in fp32; at most 384 experts, 16 choices).
 
     Ties go to the lowest index.  A weight is the softmax over the token's choices (the probabilities renormalised over them).  An
     expert whose logit is -inf is closed to the token: such a choice is not made (weight 0, no row), so a padding token can be kept
     out of every expert.  ``capacity``: rows an expert takes at most, the first in token order; 0: no limit.  ``aux_loss`` is
-    E * sum_e (share of the choices, before the capacity, that went to e) * (mean probability of e)."""
+    E * sum_e (share of the choices, before the capacity, that went to e) * (mean probability of e).
+
+    ``score`` "sigmoid": an expert's score s is the sigmoid of its logit, not its softmax.  ``bias`` (fp32 [E]) is added to the scores for
+    the choice alone, see ``balance_bias_``.  ``groups``: the experts lie in so many equal groups, of which the ``top_groups`` whose two
+    largest (biased) scores have the largest sum are open to a token.  With a bias or groups the choice goes by biased scores (each score
+    rounded to fp32 once, so that it is the same on every machine), else by the logits.  ``normalize`` False: weights are the scores
+    themselves, not divided by their sum over the choices; ``scale`` multiplies them.  The load-balancing term's probabilities are the
+    scores over their sum.  A bias of -inf closes its expert to the choice."""
+    how = None
+    if not (score == "softmax" and bias is None and groups == 1 and top_groups == 0 and normalize and scale == 1.0) and logits.dim() == 2:
+        how = _scoring(logits.shape[1], top_k, score, bias, groups, top_groups, normalize, scale)
     if not _plain(logits):
-        return Routing(*_C().moe_route(logits, top_k, capacity, debug.enabled()))
+        return Routing(*_C().moe_route(logits, top_k, capacity, _native(how), debug.enabled()))
     if logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError(f"route: logits [tokens, experts] expected, got {logits.dtype} {tuple(logits.shape)}")
     if not 1 <= top_k <= logits.shape[1]:
         raise ValueError(f"route: top_k of {top_k} among {logits.shape[1]} experts")
     if capacity < 0:
         raise ValueError(f"route: capacity {capacity}")
-    weights, experts, slots, offsets, rows, counts, aux = oracle.route(logits, top_k, capacity)
+    found = oracle.route(logits, top_k, capacity) if how is None else oracle.route_scored(logits, top_k, capacity, *how)
+    weights, experts, slots, offsets, rows, counts, aux = found
     return Routing(weights, aux, experts, slots, offsets, rows, counts)
+
+
+def balance_bias_(bias: torch.Tensor, counts: torch.Tensor, rate: float) -> torch.Tensor:
+    """``bias`` (fp32 [E], in place) for the next step: ``rate`` more for an expert with fewer choices than the mean of ``counts`` (int32 [E],
+    ``Routing.counts``, of several ranks or micro-batches their sum), ``rate`` less for one with more."""
+    if not _plain(bias, counts):
+        return _C().moe_balance_bias(bias, counts, rate)
+    if bias.dim() != 1 or bias.shape != counts.shape or counts.dtype != torch.int32 or bias.dtype != torch.float32:
+        raise ValueError(f"balance_bias_: fp32 [E] and int32 [E] expected, got {bias.dtype} {tuple(bias.shape)} and {counts.dtype} "
+                         f"{tuple(counts.shape)}")
+    return bias.copy_(oracle.balance_bias(bias, counts, rate))
 
 
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
@@ -107,13 +167,14 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> t
 
 
 def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.Tensor, top_k: int, capacity: int = 0,
-               act_bits: int = 16) -> tuple[torch.Tensor, torch.Tensor]:
+               act_bits: int = 16, scoring: Scoring | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(out [T, D], aux_loss): every token through its ``top_k`` experts' SwiGLU feed-forwards, weighted by the router.
 
     x [T, D] bf16 or fp32 (the output's type), logits [T, E] as ``route`` takes them, ``w_gate_up`` [E, 2F, D] or the pair
     (w_gate, w_up) of [E, F, D], ``w_down`` [E, D, F]; matrices bf16 or fp32 (then rounded for the products, with fp32 gradients);
     D and F multiples of 8.  ``act_bits`` 8: gate and up are kept in 8 bits (``act8``) for the backward pass instead of bf16, which
     takes from them the gradients of gate and up and the activation, and with it the gradients of ``w_down`` and of the weights.
+    ``scoring``: the further arguments of ``route``.
 
     On a GPU sums, weights and the weighted sum are fp32; what a product reads and writes between is bf16: the rows of x, the
     activation and, with more than 64 rows per expert on average, the down product's rows; in the backward pass the rows of the
@@ -121,10 +182,13 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.T
     rounded only at the end.  A pair, and fp32 matrices, are packed into one bf16 stack by every call, all experts of it, and the
     stack is held for the backward pass; bf16 matrices as [E, 2F, D] are read where they lie."""
     first, second = w_gate_up if isinstance(w_gate_up, (tuple, list)) else (w_gate_up, None)
+    if scoring is not None and logits.dim() == 2:
+        scoring = _scoring(logits.shape[1], top_k, *scoring)
     if not _plain(x, logits, first, w_down):
         if x.dim() != 2 or logits.dim() != 2:
             raise ValueError(f"expert_mlp: x [T, D] and logits [T, E] expected, got {tuple(x.shape)} and {tuple(logits.shape)}")
-        out, aux = _C().expert_mlp(_rows(x), _rows(logits), first, second, w_down, top_k, capacity, act_bits, debug.enabled())
+        out, aux = _C().expert_mlp(_rows(x), _rows(logits), first, second, w_down, top_k, capacity, _native(scoring),
+                                   act_bits, debug.enabled())
         return out, aux
     if x.dim() != 2 or logits.dim() != 2 or first.dim() != 3 or w_down.dim() != 3:
         raise ValueError("expert_mlp: x [T, D], logits [T, E], w_gate_up [E, 2F, D] and w_down [E, D, F] expected")
@@ -139,4 +203,4 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.T
         raise ValueError(f"expert_mlp: x {tuple(x.shape)}, logits {tuple(logits.shape)}, w_gate_up {tuple(first.shape)}, w_down "
                          f"{tuple(w_down.shape)} do not fit")
     wgu = first if second is None else torch.cat([first, second], dim=1)
-    return oracle.expert_mlp(x, logits, wgu, w_down, top_k, capacity, act_bits)
+    return oracle.expert_mlp(x, logits, wgu, w_down, top_k, capacity, act_bits, scoring)

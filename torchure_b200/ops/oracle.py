@@ -69,18 +69,68 @@ def route(logits, k, capacity=0):
     closed = ~made.any(1, keepdim=True)              # no expert at all: zeros instead of 0 / 0
     weights = torch.softmax(torch.where(closed, torch.zeros_like(top), top), -1) * made
     p = torch.softmax(torch.where(closed, torch.zeros_like(x), x), -1) * ~closed
+    slots, offsets, rows, counts = _plan_rows(experts, made, E, capacity)
+    aux = E * (counts.to(p.dtype) / max(1, T * k) * p.sum(0) / max(1, T)).sum()
+    return weights, experts.int(), slots, offsets, rows, counts.int(), aux
+
+
+def _plan_rows(experts, made, E, capacity):
+    """(slots, offsets, rows, counts) of choices [T, k]: rows in the order of (expert, token, choice)."""
+    T, k = experts.shape
     of = torch.where(made, experts, E).reshape(-1)
     counts = torch.bincount(of, minlength=E + 1)[:E]
     kept = counts.clamp_max(capacity) if capacity else counts
     offsets = torch.cat([kept.new_zeros(1), kept.cumsum(0)])
-    slots = torch.full((T * k,), -1, dtype=torch.int64, device=x.device)
-    rows = torch.full((T * k,), -1, dtype=torch.int64, device=x.device)
+    slots = torch.full((T * k,), -1, dtype=torch.int64, device=of.device)
+    rows = torch.full((T * k,), -1, dtype=torch.int64, device=of.device)
     for e in range(E):
         mine = (of == e).nonzero()[:, 0][:int(kept[e])]
-        slots[mine] = offsets[e] + torch.arange(mine.numel(), device=x.device)
+        slots[mine] = offsets[e] + torch.arange(mine.numel(), device=of.device)
         rows[offsets[e]:offsets[e + 1]] = mine
+    return slots.view(T, k).int(), offsets.int(), rows.int(), counts
+
+
+def route_scored(logits, k, capacity=0, score="softmax", bias=None, groups=1, top_groups=1, normalize=True, scale=1.0):
+    """``route`` by scores: s = sigmoid or softmax of the logits, rounded to fp32 from 64 bits for the choice; with a bias or groups the choice goes
+    by s + bias inside the ``top_groups`` groups whose two largest have the largest sums, else by the logits."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    T, E = x.shape
+    lowest = torch.full((), float("-inf"), device=x.device)
+    low = x.detach()
+    is_open = low != lowest
+    closed = ~is_open.any(1, keepdim=True)             # no expert at all: zeros instead of 0 / 0
+    safe = torch.where(closed, torch.zeros_like(x), x)
+    if bias is None and groups == 1:
+        key = low
+    else:
+        wide = safe.detach().double()
+        s = (torch.sigmoid(wide) if score == "sigmoid" else torch.softmax(wide, -1)).float()
+        key = torch.where(is_open, s if bias is None else s + bias.detach(), lowest)
+    if groups > 1:
+        two = key.view(T, groups, E // groups).sort(-1, descending=True).values[..., :2]
+        total = torch.where((two == lowest)[..., 1:].any(-1) | (two.shape[-1] == 1), two[..., 0], two.sum(-1))
+        best = torch.sort(total, dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        stays = torch.zeros(T, groups, dtype=torch.bool, device=x.device).scatter_(1, best, True)
+        key = torch.where(stays.repeat_interleave(E // groups, 1), key, lowest)
+    experts = torch.sort(key, dim=-1, descending=True, stable=True).indices[:, :k]
+    made = key.gather(1, experts) != lowest
+    # logarithms of the scores: they may all be tiny
+    log_s = F.logsigmoid(safe) if score == "sigmoid" else torch.log_softmax(safe, -1)
+    top = log_s.gather(1, experts)
+    none = ~made.any(1, keepdim=True)
+    if normalize:
+        weights = torch.softmax(torch.where(none, torch.zeros_like(top), torch.where(made, top, lowest)), -1) * made
+    else:
+        weights = torch.where(made, torch.exp(top), torch.zeros_like(top))
+    p = torch.softmax(log_s, -1) * ~closed
+    slots, offsets, rows, counts = _plan_rows(experts, made, E, capacity)
     aux = E * (counts.to(p.dtype) / max(1, T * k) * p.sum(0) / max(1, T)).sum()
-    return weights, experts.int(), slots.view(T, k).int(), offsets.int(), rows.int(), counts.int(), aux
+    return scale * weights, experts.int(), slots, offsets, rows, counts.int(), aux
+
+
+def balance_bias(bias, counts, rate):
+    n = counts.long()
+    return bias + rate * torch.sign(n.sum() - n * n.numel()).to(bias.dtype)
 
 
 def grouped_linear(x, w, offsets):
@@ -103,9 +153,9 @@ def combine(y, weights, slots):
     return (weights[..., None] * got).sum(1)
 
 
-def expert_mlp(x, logits, w_gate_up, w_down, k, capacity=0, act_bits=16):
-    """(out, aux) in the operands' precision."""
-    weights, _, slots, offsets, rows, _, aux = route(logits, k, capacity)
+def expert_mlp(x, logits, w_gate_up, w_down, k, capacity=0, act_bits=16, scoring=None):
+    """(out, aux) in the operands' precision.  scoring: the further arguments of ``route_scored``."""
+    weights, _, slots, offsets, rows, _, aux = route(logits, k, capacity) if scoring is None else route_scored(logits, k, capacity, *scoring)
     gu = grouped_linear(dispatch(x, rows, k), w_gate_up, offsets)
     act = swiglu_8bit(gu) if act_bits == 8 else swiglu_plain(gu)
     return combine(grouped_linear(act, w_down, offsets), weights.to(x.dtype), slots), aux
