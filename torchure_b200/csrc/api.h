@@ -139,6 +139,27 @@ struct TensorList {           // device-resident table (built once per parameter
   int n_blocks;
 };
 constexpr int kChunkElems = 16384;
+// The same with as many pointer columns as the operation has, one after the other (adamw8.cu).  p, grad (flag bit 0: bf16), codes and scales of
+// the moments (m, v codes, then m, v scales) and the optional bf16 shadow; scales have one fp32 value for kStateBlock codes.
+constexpr int kStateBlock = 128;
+struct State8List {
+  const int64_t* ptrs;
+  const int64_t* numel;
+  const int32_t* flags;
+  const int32_t* block_tensor;
+  const int32_t* block_chunk;
+  int n_tensors, n_blocks;
+};
+struct Adam8Scalars {
+  float beta1, rest1, beta2, rest2, eps;      // rest: 1 - beta
+  float step_size, root, decay;               // lr / (1 - beta1^t), (1 - beta2^t)^-1/2, 1 - lr weight decay
+  uint32_t key;                               // of the step's random bits
+  int maximize;
+};
+// hyper (optional, device): {step_size, root, decay, key's bits} instead of those of `s`
+[[nodiscard]] int adamw8_multi(const State8List& t, const Adam8Scalars& s, const float* grad_scale, const float* hyper, cudaStream_t stream);
+// columns: codes, scales, the values' place in `out` in elements
+[[nodiscard]] int state8_values_multi(const State8List& t, bool is_signed, void* out, bool bf16, cudaStream_t stream);
 // fp32 master p, fp32/bf16 grad g (flag bit0 = grad is bf16), m, v fp32, optional bf16 shadow (ptr 0 = none).
 // `hyper` (optional, device): {lr, bias1, bias2} overriding the scalar arguments at run time.
 void adamw_multi(const TensorList& t, float lr, float beta1, float beta2, float eps, float weight_decay,

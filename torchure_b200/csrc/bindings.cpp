@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -299,6 +300,106 @@ void adamw_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const to
                   (float)bias1, (float)bias2, opt_ptr<float>(grad_scale), maximize ? 1 : 0, opt_ptr<float>(hyper),
                   cur_stream());
 }
+// ---- moments in 8 bits --------------------------------------------------------------------------------
+using Tensors = std::vector<torch::Tensor>;
+using OptTensors = std::vector<c10::optional<torch::Tensor>>;
+
+tb::State8List as_state8(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt,
+                         const torch::Tensor& bc) {
+  return {ptrs.data_ptr<int64_t>(), numel.data_ptr<int64_t>(), flags.data_ptr<int32_t>(), bt.data_ptr<int32_t>(), bc.data_ptr<int32_t>(),
+          (int)numel.numel(), (int)bt.numel()};
+}
+
+// Checks what the kernel is going to read through addresses, and appends them
+void add_column(std::vector<int64_t>& out, const torch::Tensor& t, int64_t n, const torch::Device& dev, std::initializer_list<at::ScalarType> types,
+                const char* what) {
+  TORCH_CHECK_VALUE(t.device() == dev && t.is_contiguous() && t.numel() == n, what, ": a contiguous tensor of ", n, " elements on ", dev,
+                    " expected, got ", t.sizes(), " on ", t.device());
+  TORCH_CHECK_TYPE(std::find(types.begin(), types.end(), t.scalar_type()) != types.end(), what, ": unexpected type ", t.scalar_type());
+  out.push_back(reinterpret_cast<int64_t>(t.data_ptr()));
+}
+
+// (addresses, elements, flags) of an 8-bit AdamW step's tensors
+std::tuple<std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>> adamw8_columns(
+    const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, const Tensors& ms, const Tensors& vs, const OptTensors& shadows) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(n > 0 && grads.size() == n && m.size() == n && v.size() == n && ms.size() == n && vs.size() == n && shadows.size() == n,
+                    "adamw8_step: lists of one length expected");
+  const auto dev = params[0].device();
+  TORCH_CHECK_VALUE(dev.is_cuda(), "adamw8_step: tensors on a GPU expected");
+  std::vector<int64_t> ptrs, numel, flags;
+  ptrs.reserve(7 * n);
+  const auto f32 = torch::kFloat32, b16 = torch::kBFloat16, u8 = torch::kUInt8;
+  for (size_t i = 0; i < n; ++i) {
+    numel.push_back(params[i].numel());
+    flags.push_back(grads[i].scalar_type() == b16);
+    add_column(ptrs, params[i], numel[i], dev, {f32}, "adamw8_step: parameter");
+  }
+  for (size_t i = 0; i < n; ++i) add_column(ptrs, grads[i], numel[i], dev, {f32, b16}, "adamw8_step: gradient");
+  for (size_t i = 0; i < n; ++i) add_column(ptrs, m[i], numel[i], dev, {u8}, "adamw8_step: first moment");
+  for (size_t i = 0; i < n; ++i) add_column(ptrs, v[i], numel[i], dev, {u8}, "adamw8_step: second moment");
+  const auto blocks = [&](size_t i) { return (numel[i] + tb::kStateBlock - 1) / tb::kStateBlock; };
+  for (size_t i = 0; i < n; ++i) add_column(ptrs, ms[i], blocks(i), dev, {f32}, "adamw8_step: first moment's scales");
+  for (size_t i = 0; i < n; ++i) add_column(ptrs, vs[i], blocks(i), dev, {f32}, "adamw8_step: second moment's scales");
+  for (size_t i = 0; i < n; ++i) {
+    if (shadows[i].has_value()) add_column(ptrs, *shadows[i], numel[i], dev, {b16}, "adamw8_step: shadow");
+    else ptrs.push_back(0);
+  }
+  return {ptrs, numel, flags};
+}
+
+// (columns, elements) of moments in 8 bits; the third column is the place of a tensor's values in one buffer, in elements, each on 16 bytes
+std::tuple<std::vector<int64_t>, std::vector<int64_t>> state8_columns(const Tensors& codes, const Tensors& scales) {
+  const size_t n = codes.size();
+  TORCH_CHECK_VALUE(n > 0 && scales.size() == n, "state8_values: lists of one length expected");
+  const auto dev = codes[0].device();
+  TORCH_CHECK_VALUE(dev.is_cuda(), "state8_values: tensors on a GPU expected");
+  std::vector<int64_t> ptrs, numel;
+  for (size_t i = 0; i < n; ++i) {
+    numel.push_back(codes[i].numel());
+    add_column(ptrs, codes[i], numel[i], dev, {torch::kUInt8}, "state8_values: codes");
+  }
+  for (size_t i = 0; i < n; ++i)
+    add_column(ptrs, scales[i], (numel[i] + tb::kStateBlock - 1) / tb::kStateBlock, dev, {torch::kFloat32}, "state8_values: scales");
+  int64_t at = 0;
+  for (size_t i = 0; i < n; ++i) {
+    ptrs.push_back(at);
+    at += (numel[i] + 7) / 8 * 8;
+  }
+  return {ptrs, numel};
+}
+
+void adamw8_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt, const torch::Tensor& bc,
+                  double beta1, double beta2, double eps, double step_size, double root, double decay, int64_t key,
+                  c10::optional<torch::Tensor> grad_scale, bool maximize, c10::optional<torch::Tensor> hyper) {
+  TORCH_CHECK(!hyper || (hyper->is_cuda() && hyper->scalar_type() == torch::kFloat32 && hyper->numel() >= 4), "adamw8_step: hyper");
+  TORCH_CHECK_VALUE(!grad_scale || (grad_scale->device() == ptrs.device() && grad_scale->scalar_type() == torch::kFloat32 && grad_scale->numel() == 1),
+                    "adamw8_step: grad_scale must be one fp32 element on the GPU of the parameters");
+  const tb::Adam8Scalars s{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)step_size, (float)root,
+                           (float)decay, (uint32_t)key, maximize ? 1 : 0};
+  c10::cuda::CUDAGuard guard(ptrs.device());
+  const int rc = tb::adamw8_multi(as_state8(ptrs, numel, flags, bt, bc), s, opt_ptr<float>(grad_scale), opt_ptr<float>(hyper), cur_stream());
+  TORCH_CHECK(rc == 0, "adamw8_step failed with code ", rc);
+}
+
+// The values of all tensors, a view of one buffer for each
+Tensors state8_values_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt,
+                            const torch::Tensor& bc, const Tensors& codes, bool is_signed, bool bf16) {
+  c10::cuda::CUDAGuard guard(ptrs.device());
+  int64_t total = 0;
+  for (const auto& c : codes) total += (c.numel() + 7) / 8 * 8;
+  const auto all = torch::empty({total}, codes[0].options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
+  const int rc = tb::state8_values_multi(as_state8(ptrs, numel, flags, bt, bc), is_signed, all.data_ptr(), bf16, cur_stream());
+  TORCH_CHECK(rc == 0, "state8_values failed with code ", rc);
+  Tensors out;
+  int64_t at = 0;
+  for (const auto& c : codes) {
+    out.push_back(all.narrow(0, at, c.numel()).view(c.sizes()));
+    at += (c.numel() + 7) / 8 * 8;
+  }
+  return out;
+}
+
 void sqnorm_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags,
                   const torch::Tensor& bt, const torch::Tensor& bc, torch::Tensor& out) {
   tb::sqnorm_multi(as_list(ptrs, numel, flags, bt, bc), out.data_ptr<float>(), cur_stream());
@@ -389,6 +490,7 @@ void register_comm(pybind11::module_& m);
 void register_attn(pybind11::module_& m);
 void register_block(pybind11::module_& m);
 void register_moe(pybind11::module_& m);
+void register_embedding(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", [](const torch::Tensor& a, const torch::Tensor& b, torch::Tensor& out, bool a_mn, bool b_mn, int64_t out_mode,
@@ -473,6 +575,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cast_to_bf16", &cast_to_bf16);
   m.def("scale_inplace", &scale_inplace);
   m.def("adamw_multi", &adamw_multi);
+  m.def("adamw8_columns", &adamw8_columns);
+  m.def("state8_columns", &state8_columns);
+  m.def("adamw8_multi", &adamw8_multi);
+  m.def("state8_values_multi", &state8_values_multi);
   m.def("sqnorm_multi", &sqnorm_multi);
   m.def("finalize_norm", [](const torch::Tensor& partials, double max_norm, double eps, torch::Tensor& out) {
     TORCH_CHECK(partials.scalar_type() == torch::kFloat32 && partials.is_contiguous() && out.numel() >= 2 &&
@@ -487,4 +593,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_attn(m);
   register_block(m);
   register_moe(m);
+  register_embedding(m);
 }

@@ -3,8 +3,6 @@
 // here; in the poison mode (ops/debug.py) each is filled and remembered before its kernel runs.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -13,7 +11,6 @@
 
 #include "bind_common.h"
 #include "moe_api.h"
-#include "pdl.h"
 
 namespace {
 
@@ -22,29 +19,7 @@ using OptTensor = c10::optional<Tensor>;
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-// torch::empty for GPU tensors without the dispatcher (0.6 us instead of 1.8)
-Tensor empty(c10::IntArrayRef size, const at::TensorOptions& options) { return at::detail::empty_cuda(size, options); }
-
-// Backward passes run in threads of autograd's, which do not hold the interpreter's lock.
-struct Outputs {
-  bool poisoned;
-  Tensor operator()(const char* name, c10::IntArrayRef size, const at::TensorOptions& options) const {
-    Tensor t = empty(size, options);
-    if (poisoned) {
-      pybind11::gil_scoped_acquire lock;
-      pybind11::module_::import("torchure_b200.ops.debug").attr("track")(name, t);
-    }
-    return t;
-  }
-};
-
-// Launches overlap (pdl.h): a kernel comes up while the one before ends, and waits before it reads.  The feed-forward forward, us, without and
-// with: 8 experts of 1024 x 1536, 512 rows 48, 39; 4096 rows 83, 70; 32768 rows 284, 278.  (A graph keeps plain edges.)
-struct Overlap : tb::PdlScope {
-  Overlap() : tb::PdlScope(at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) {}
-};
-
-std::atomic<int64_t> g_launches{0};      // kernels launched by the calls of this file
+std::atomic<int64_t> g_launches{0};      // kernels launched by the operators with autograd nodes in C++
 
 // A launcher's code: counted where it launched, an error otherwise
 void done(const char* what, int rc) {
@@ -361,15 +336,6 @@ Tensor matrices(const Tensor& w) {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void only_once(const char* what) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient itself has no gradient (create_graph is not supported)");
-}
-// A dual tensor asks for no gradient, so that calls without gradients would pass its tangent by
-template <class... Ts>
-void no_tangents(const char* what, const Ts&... tensors) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!(... || (tensors.defined() && tensors._fw_grad(0).defined())), what,
-                              ": forward-mode derivatives are not supported");
-}
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 // What a gradient needs to know of the scores, from one pass to the other
@@ -838,6 +804,8 @@ variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tens
 
 }  // namespace
 
+void bind_count_launches(int64_t n) { g_launches += n; }
+
 void register_moe(pybind11::module_& m) {
   m.def("moe_route", &moe_route, "(weights, aux, experts, slots, offsets, rows, counts)");
   m.def("moe_balance_bias", &moe_balance_bias);
@@ -857,5 +825,5 @@ void register_moe(pybind11::module_& m) {
   });
   m.def("swiglu_8bit", &swiglu_8bit);
   m.def("moe_launches", [](bool reset) { return reset ? g_launches.exchange(0) : g_launches.load(); },
-        "kernels launched by the operators of this file since the last reset");
+        "kernels launched by the operators with autograd nodes in C++ since the last reset");
 }

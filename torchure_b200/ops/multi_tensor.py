@@ -1,4 +1,4 @@
-"""Multi-tensor kernels (AdamW, grad norm, scaling, DDP bucket fill) driven by device-resident tables.
+"""Multi-tensor kernels (AdamW, also with moments in 8 bits, grad norm, scaling, DDP bucket fill) driven by device-resident tables.
 
 A ``TensorTable`` records, for a fixed list of tensors, up to five pointer columns, the element counts,
 per-tensor flags and the (tensor, chunk) assignment of every thread block.  It is uploaded once; while the
@@ -19,12 +19,16 @@ from __future__ import annotations
 import torch
 
 from torchure_b200 import ops
+from torchure_b200.ops import oracle
 
 CHUNK = 16384
 
 
 def available() -> bool:
     return ops.available()
+
+
+STATE_BLOCK = oracle.STATE8_BLOCK      # values of a moment in 8 bits that share a scale
 
 
 def _addresses(columns) -> tuple:
@@ -83,12 +87,14 @@ def _place(device: torch.device) -> tuple[int, int]:
     return ops.ext().stream_place(device.index) if device.type == "cuda" else (0, 0)
 
 
-def _table(tag: str, columns, flags=None) -> TensorTable:
+def _table(tag: str, columns, flags=None, ptrs: tuple | None = None, numel: tuple | None = None) -> TensorTable:
+    """`ptrs`, `numel`: the columns' entries and the elements of each tensor where the caller has them already."""
     first = columns[0]
     stream, capture = _place(first[0].device)
-    slot = (tag, len(columns), tuple(t.numel() for t in first), tuple(flags) if flags is not None else (),
-            first[0].device.index, stream)
-    ptrs = _addresses(columns)
+    slot = (tag, len(columns), numel if numel is not None else tuple(t.numel() for t in first),
+            tuple(flags) if flags is not None else (), first[0].device.index, stream)
+    if ptrs is None:
+        ptrs = _addresses(columns)
     cache = _CACHE
     if capture:
         if capture not in _CAPTURES and len(_CAPTURES) >= 4:
@@ -150,6 +156,49 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, shadows, lr, beta1, beta2, 
     gs = grad_scale.to(torch.float32) if grad_scale is not None else None
     ops.ext().adamw_multi(*tab.args(), lr, beta1, beta2, eps, weight_decay, bias1, bias2, gs, maximize, hyper)
     ops.count_launch()
+
+
+def adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed=0) -> tuple[float, float, float, int]:
+    """What an 8-bit AdamW step takes of its step: lr / (1 - beta1^t), (1 - beta2^t)^-1/2, 1 - lr weight_decay, the key of its random bits."""
+    return lr / (1.0 - beta1 ** step), (1.0 - beta2 ** step) ** -0.5, 1.0 - lr * weight_decay, oracle.state8_key(seed, step)
+
+
+def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, shadows, lr, beta1, beta2, eps, weight_decay,
+                step, grad_scale=None, maximize=False, hyper=None, seed=0) -> None:
+    """One AdamW step over all tensors with both moments in 8 bits (uint8 codes of the parameter's shape, an fp32 scale for every 128
+    values), in place.  params fp32, grads fp32 or bf16, shadows bf16 or None; all contiguous.
+
+    The step is ``adamw_step``'s on the moments read back; what they are then is rounded to 8 bits with random bits of (seed, step, tensor's
+    place in the list, element), so that the mean over steps is right (``oracle.state8_encode`` has the format).  `grad_scale`: device
+    scalar that multiplies the gradients.  `hyper`: optional device tensor of what ``adamw8_scalars`` gives (the key as the pattern of a
+    float), in its place at run time (graph replay)."""
+    if not params:
+        return
+    if not (ops.available() and params[0].is_cuda):
+        oracle.adamw8(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, shadows, lr, beta1, beta2, eps, weight_decay,
+                      step, grad_scale, maximize, seed)
+        return
+    ptrs, numel, flags = ops.ext().adamw8_columns(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, shadows)
+    tab = _table("adamw8", [params], flags, tuple(ptrs), tuple(numel))
+    size, root, decay, key = adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed)
+    gs = grad_scale.to(torch.float32) if grad_scale is not None else None
+    ops.ext().adamw8_multi(*tab.args(), beta1, beta2, eps, size, root, decay, key, gs, maximize, hyper)
+    ops.count_launch()
+
+
+def state8_values(codes, scales, signed: bool, dtype=torch.float32) -> list[torch.Tensor]:
+    """What moments in 8 bits stand for (signed: the first, else the second), fp32 or bf16, views of one buffer."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"state8_values: values in fp32 or bf16, not {dtype}")
+    if not codes:
+        return []
+    if not (ops.available() and codes[0].is_cuda):
+        return [oracle.state8_decode(c, s, signed).to(dtype) for c, s in zip(codes, scales, strict=True)]
+    ptrs, numel = ops.ext().state8_columns(codes, scales)
+    tab = _table("state8", [codes], None, tuple(ptrs), tuple(numel))
+    out = ops.ext().state8_values_multi(*tab.args(), codes, signed, dtype == torch.bfloat16)
+    ops.count_launch()
+    return out
 
 
 def bucket_pack(grads, dst_views, accumulate: bool, post_scale: float, sq_out: torch.Tensor | None) -> None:

@@ -57,6 +57,116 @@ def adamw(p, g, m, v, lr, b1, b2, eps, wd, step):
     return p, m, v
 
 
+class _Embedding(torch.autograd.Function):
+    """Rows in fp32 (or the table's wider type), scaled and rounded once; a row's gradient likewise."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding, dtype):
+        if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < table.shape[0]):
+            raise IndexError(f"embedding: ids from {int(ids.min())} to {int(ids.max())} in a table of {table.shape[0]} rows")
+        ctx.save_for_backward(ids)
+        ctx.how = table.shape, table.dtype, scale, padding
+        wide = torch.promote_types(table.dtype, torch.float32)
+        return (table[ids.long()].to(wide) * scale).to(dtype)
+
+    @staticmethod
+    def backward(ctx, dout):
+        ids, = ctx.saved_tensors
+        shape, dtype, scale, padding = ctx.how
+        wide = torch.promote_types(dtype, torch.float32)
+        d = torch.zeros(shape, dtype=wide, device=dout.device)
+        d.index_add_(0, ids.reshape(-1).long(), dout.reshape(ids.numel(), shape[1]).to(wide))
+        d = d * scale
+        if padding is not None:
+            d[padding] = 0
+        return None, d.to(dtype), None, None, None
+
+
+def embedding(ids, table, scale=1.0, padding=None, dtype=None):
+    return _Embedding.apply(ids, table, scale, padding, table.dtype if dtype is None else dtype)
+
+
+# ---- moments in 8 bits --------------------------------------------------------------------------------
+# A block of 128 values shares the scale a / TOP, a its largest magnitude.  y = |x| TOP / a + FIRST is held as its fp32 pattern cut to 3 bits
+# of mantissa, counted from FIRST's.  First moment: 7 bits and a sign; second moment: 8 bits.  A value goes to one of its two neighbours
+# by 16 random bits, so that the mean is its own; a second moment above zero keeps at least the first step.  fp32, one rounding for each
+# operation: the kernel's results have the same bits.
+STATE8_BLOCK = 128
+_S8 = {True: (2.0 ** -15, 896, 127, 1.875 - 2.0 ** -15), False: (2.0 ** -31, 768, 255, 1.875)}      # FIRST, its pattern >> 20, last code, TOP
+_LOW32 = 0xFFFFFFFF
+
+
+def _mix32(x):
+    x = (x ^ (x >> 16)) * 0x7FEB352D & _LOW32
+    x = (x ^ (x >> 15)) * 0x846CA68B & _LOW32
+    return x ^ (x >> 16)
+
+
+def state8_key(seed: int, step: int) -> int:
+    return _mix32((seed + 0x9E3779B9 * step) & _LOW32)
+
+
+def state8_bits(n: int, key: int, index: int, device) -> torch.Tensor:
+    """32 random bits (int64) for each of the n values of the `index`-th tensor: the lower 16 for the first moment."""
+    i = torch.arange(n, device=device)
+    if n <= 1 << 32:
+        return _mix32((i & _LOW32) ^ _mix32((key + 0x85EBCA6B * index) & _LOW32))
+    return _mix32((i & _LOW32) ^ _mix32((key + 0x85EBCA6B * index + 0xC2B2AE35 * (i >> 32)) & _LOW32))
+
+
+def _blocks128(x):
+    x = x.reshape(-1)
+    return F.pad(x, (0, -x.numel() % STATE8_BLOCK)).view(-1, STATE8_BLOCK)
+
+
+def state8_encode(x, bits, signed):
+    """(uint8 codes of x's shape, fp32 scales) of x in fp32; `bits`: 0 to 65535 for each value (32768: nearly to the nearest)."""
+    first, base, last, most = _S8[signed]
+    b = _blocks128(x)
+    top = b.abs().amax(-1, keepdim=True) if x.numel() else b.new_zeros(b.shape[0], 1)
+    y = b.abs() * (top.reciprocal() * most) + first
+    code = ((y.view(torch.int32) + (_blocks128(bits) << 4).int()) >> 20) - base
+    code = code.clamp_max(last)
+    code = torch.where(b < 0, code + 128, code) if signed else torch.where(b > 0, code.clamp_min(1), code)
+    tiny = top < 2.0 ** -100
+    fine = (top < float("inf")) & ~tiny
+    code = torch.where(fine, code, torch.zeros_like(code))
+    scale = torch.where(fine, top * torch.tensor(1.0 / most, dtype=torch.float32, device=x.device),
+                        torch.where(tiny, torch.zeros_like(top), torch.full_like(top, float("nan"))))
+    return code.view(-1)[:x.numel()].view(x.shape).to(torch.uint8), scale.view(-1)
+
+
+def state8_decode(codes, scales, signed):
+    first, base, _, _ = _S8[signed]
+    c = _blocks128(codes).int()
+    y = ((((c & 127) if signed else c) + base << 20).view(torch.float32) - first) * scales[:, None]
+    if signed:
+        y = torch.where(c >= 128, -y, y)
+    return y.view(-1)[:codes.numel()].view(codes.shape)
+
+
+def adamw8(params, grads, ms, m_scales, vs, v_scales, shadows, lr, b1, b2, eps, wd, step, grad_scale=None, maximize=False, seed=0):
+    """AdamW in place with moments in 8 bits."""
+    size, root, key = lr / (1.0 - b1 ** step), (1.0 - b2 ** step) ** -0.5, state8_key(seed, step)
+    for i, (p, g, mc, msc, vc, vsc, sh) in enumerate(zip(params, grads, ms, m_scales, vs, v_scales, shadows, strict=True)):
+        g = g.float()
+        if grad_scale is not None:
+            g = g * grad_scale.float()
+        if maximize:
+            g = -g
+        m = state8_decode(mc, msc, True) * b1 + g * (1.0 - b1)
+        v = state8_decode(vc, vsc, False) * b2 + (g * (1.0 - b2)) * g
+        r = torch.sqrt(v.double()).float()          # correctly rounded (a CPU's fp32 root need not be)
+        p.copy_(p * (1.0 - lr * wd) - (m / (r * root + eps)) * size)
+        if sh is not None:
+            sh.copy_(p)
+        bits = state8_bits(p.numel(), key, i, p.device).view(p.shape)
+        for x, r, codes, scales, signed in ((m, bits & 0xFFFF, mc, msc, True), (v, bits >> 16, vc, vsc, False)):
+            c, s = state8_encode(x, r, signed)
+            codes.copy_(c)
+            scales.copy_(s)
+
+
 # ---- mixture of experts -----------------------------------------------------------------------------
 def route(logits, k, capacity=0):
     """(weights, experts, slots, offsets, rows, counts, aux), weights and aux differentiable; ties go to the lowest index, a choice
