@@ -195,7 +195,7 @@ def state8_values(codes, scales, signed: bool, dtype=torch.float32) -> list[torc
     if not (ops.available() and codes[0].is_cuda):
         return [oracle.state8_decode(c, s, signed).to(dtype) for c, s in zip(codes, scales, strict=True)]
     ptrs, numel = ops.ext().state8_columns(codes, scales)
-    tab = _table("state8", [codes], None, tuple(ptrs), tuple(numel))
+    tab = _table("state8+" if signed else "state8", [codes], None, tuple(ptrs), tuple(numel))
     out = ops.ext().state8_values_multi(*tab.args(), codes, signed, dtype == torch.bfloat16)
     ops.count_launch()
     return out
