@@ -26,6 +26,7 @@ namespace tb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSmallChunk = kChunkElems / 4;      // where there are too few chunks of kChunkElems for the SMs
 constexpr float kFirstM = 3.0517578125e-05f, kFirstV = 4.656612873077393e-10f;      // 2^-15, 2^-31
 constexpr uint32_t kKeyM = 896, kKeyV = 768;                                            // their patterns >> 20
 constexpr float kTopM = 1.875f - 3.0517578125e-05f, kTopV = 1.875f;
@@ -219,13 +220,13 @@ struct Chunk {               // where a chunk's tensors begin
   __nv_bfloat16* sh;
 };
 
-// A chunk of kChunkElems on 16-byte boundaries, a warp per block of 128, four values a thread.  The values of the next three rounds are on their
+// A chunk of whole rounds on 16-byte boundaries, a warp per block of 128, four values a thread.  The values of the next three rounds are on their
 // way to shared memory meanwhile: held in registers they would leave room for too few warps, and without them the loads of a round wait
 // behind the stores of the one before, which for all the compiler knows could be to the same place.
 template <bool G16, bool SHADOW>
-__device__ __forceinline__ void whole_chunk(const Chunk& c, const Adam8Scalars& s, float gs, uint32_t key, uint32_t i0, Stage* stages) {
+__device__ __forceinline__ void whole_chunk(const Chunk& c, int count, const Adam8Scalars& s, float gs, uint32_t key, uint32_t i0, Stage* stages) {
   constexpr int kStep = kThreads / 32 * kStateBlock, kAhead = kStages - 1;
-  static_assert(kChunkElems % (kStages * kStep) == 0, "whole rounds");
+  static_assert(kSmallChunk % (kStages * kStep) == 0 && kChunkElems % kSmallChunk == 0, "whole rounds");
   const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * kStateBlock, at = first + lane * 4;
   // each thread's places, moved on by kStages rounds at a time
   float* p = c.p + at;
@@ -248,7 +249,7 @@ __device__ __forceinline__ void whole_chunk(const Chunk& c, const Adam8Scalars& 
   }
   uint32_t i = i0 + at;
 #pragma unroll 1
-  for (int left = kChunkElems / kStep; left > 0; left -= kStages) {
+  for (int left = count / kStep; left > 0; left -= kStages) {
 #pragma unroll
     for (int r = 0; r < kStages; ++r) {
       // (the stage that is filled here was read by all lanes in the round before)
@@ -296,8 +297,8 @@ adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale
     key = __float_as_uint(hyper[3]);
   }
   const int ti = t.block_tensor[blockIdx.x], n_tensors = t.n_tensors;
-  const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * kChunkElems;
-  const int count = static_cast<int>(lo + kChunkElems < n ? kChunkElems : n - lo);
+  const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * t.chunk;
+  const int count = static_cast<int>(lo + t.chunk < n ? t.chunk : n - lo);
   const int64_t* ptr = t.ptrs + ti;
   float* p = reinterpret_cast<float*>(ptr[0]) + lo;
   const char* g = reinterpret_cast<const char*>(ptr[n_tensors]);
@@ -315,14 +316,14 @@ adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale
   key = mix32(key + 0x85ebca6bu * static_cast<uint32_t>(ti) + 0xc2b2ae35u * static_cast<uint32_t>(lo >> 32));
   const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * kStateBlock;
   constexpr int kStep = kThreads / 32 * kStateBlock;
-  if (count == kChunkElems && vp && vg && vm && vv && vs) {
+  if (count == t.chunk && vp && vg && vm && vv && vs) {
     extern __shared__ __align__(16) uint8_t dynamic[];      // [warps][kStages]
     Stage* stages = reinterpret_cast<Stage*>(dynamic);
     const Chunk c{p, g, m, v, m_scale, v_scale, sh};
     Stage* mine = stages + (threadIdx.x >> 5) * kStages;
     const uint32_t i0 = static_cast<uint32_t>(lo);
-    if (g16) sh ? whole_chunk<true, true>(c, s, gs, key, i0, mine) : whole_chunk<true, false>(c, s, gs, key, i0, mine);
-    else sh ? whole_chunk<false, true>(c, s, gs, key, i0, mine) : whole_chunk<false, false>(c, s, gs, key, i0, mine);
+    if (g16) sh ? whole_chunk<true, true>(c, count, s, gs, key, i0, mine) : whole_chunk<true, false>(c, count, s, gs, key, i0, mine);
+    else sh ? whole_chunk<false, true>(c, count, s, gs, key, i0, mine) : whole_chunk<false, false>(c, count, s, gs, key, i0, mine);
     return;
   }
   // a tensor's last chunk, or one that does not lie on 16 bytes: what is not there is read as zero, which is no block's largest
@@ -353,19 +354,22 @@ state8_values_kernel(State8List t, T* __restrict__ all) {
   pdl_wait();
   pdl_launch_dependents();
   const int ti = t.block_tensor[blockIdx.x];
-  const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * kChunkElems;
-  const int64_t hi = lo + kChunkElems < n ? lo + kChunkElems : n;
+  const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * t.chunk;
+  const int64_t hi = lo + t.chunk < n ? lo + t.chunk : n;
   const uint8_t* codes = reinterpret_cast<const uint8_t*>(t.ptrs[ti]);
   const float* scales = reinterpret_cast<const float*>(t.ptrs[t.n_tensors + ti]);
   T* out = all + t.ptrs[2 * t.n_tensors + ti];
   const bool vc = on(codes, 4), vo = on(out, 4 * sizeof(T));
-  if (hi - lo == kChunkElems && on(codes, 8) && on(out, 16)) {      // eight values a thread: whole lines in and out
-    constexpr int kRounds = kChunkElems / (kThreads * 8), kFlight = 4;
+  if (hi - lo == t.chunk && on(codes, 8) && on(out, 16)) {      // eight values a thread: whole lines in and out
+    const int rounds = t.chunk / (kThreads * 8);
     const uint2* from = reinterpret_cast<const uint2*>(codes + lo) + threadIdx.x;
     const float* scale = scales + lo / kStateBlock + threadIdx.x / (kStateBlock / 8);
     T* to = out + lo + threadIdx.x * 8;
+    const auto go = [&](auto flight) {      // so many rounds' loads on their way at once
+      constexpr int kFlight = decltype(flight)::value;
+      static_assert(kSmallChunk % (2 * kThreads * 8) == 0 && kChunkElems % (4 * kThreads * 8) == 0, "whole rounds");
 #pragma unroll 1
-    for (int r0 = 0; r0 < kRounds; r0 += kFlight) {
+    for (int r0 = 0; r0 < rounds; r0 += kFlight) {
       uint2 c[kFlight];
       float s[kFlight];
 #pragma unroll
@@ -391,6 +395,9 @@ state8_values_kernel(State8List t, T* __restrict__ all) {
         }
       }
     }
+    };
+    if (rounds % 4 == 0) go(Num<4>{});
+    else go(Num<2>{});
     return;
   }
   for (int64_t i = lo + threadIdx.x * 4; i < hi; i += kThreads * 4) {
@@ -410,6 +417,7 @@ state8_values_kernel(State8List t, T* __restrict__ all) {
 
 int adamw8_multi(const State8List& t, const Adam8Scalars& s, const float* grad_scale, const float* hyper, cudaStream_t stream) {
   if (t.n_blocks <= 0) return 0;
+  if (t.chunk != kChunkElems && t.chunk != kSmallChunk) return -1;
   constexpr int kBytes = kThreads / 32 * kStages * static_cast<int>(sizeof(Stage));
   if (!ensure_dynamic_smem(reinterpret_cast<const void*>(adamw8_kernel), kBytes)) return -20;
   return launch_code(launch_pdl(adamw8_kernel, dim3(t.n_blocks), dim3(kThreads), kBytes, stream, t, s, grad_scale, hyper));
@@ -417,6 +425,7 @@ int adamw8_multi(const State8List& t, const Adam8Scalars& s, const float* grad_s
 
 int state8_values_multi(const State8List& t, bool is_signed, void* out, bool bf16, cudaStream_t stream) {
   if (t.n_blocks <= 0) return 0;
+  if (t.chunk != kChunkElems && t.chunk != kSmallChunk) return -1;
   const dim3 grid(t.n_blocks), block(kThreads);
   const auto run = [&](auto* kernel, auto* to) { return launch_code(launch_pdl(kernel, grid, block, 0, stream, t, to)); };
   if (bf16)

@@ -149,6 +149,7 @@ struct State8List {
   const int32_t* block_tensor;
   const int32_t* block_chunk;
   int n_tensors, n_blocks;
+  int chunk;                  // elements of a block's chunk: kChunkElems or a quarter of it
 };
 struct Adam8Scalars {
   float beta1, rest1, beta2, rest2, eps;      // rest: 1 - beta

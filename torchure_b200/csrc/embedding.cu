@@ -23,6 +23,7 @@ constexpr int kMaxChunks = 148;
 constexpr int kSegThreads = 256;
 constexpr int kSegChunks = 148 * 8;      // chunks of the sorted list, at most (about)
 constexpr int kSegMin = 16;              // tokens of a chunk, at least
+constexpr int kJoinCols = 128;           // columns of a CTA that joins parts
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -42,32 +43,92 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
 }
 
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 template <class I>
 __device__ __forceinline__ int64_t id_at(const I* ids, int64_t t) { return static_cast<int64_t>(ids[t]); }
 
 // ---- lookup -------------------------------------------------------------------------------------------
-// A row's columns go to gridDim.y CTAs of 4 columns a thread (VEC) or 1; blockIdx.x strides over the rows.
-template <class I, class S, class O, bool VEC>
+// A warp has kRowCols columns of a row (blockIdx.y says which), at addresses that are constants behind one base: four next to each other for a thread
+// and round (kRowsFours), or one (kRowsOnes).  bf16 rows of an odd width or stride are read and written as 32-bit words all the same
+// (kRowsPairs): pairs of columns as the output's words have them, put together from two neighbouring words where the table's lie one column off.
+// The ids of the rows to come are on their way meanwhile.  65521 rows of 1003 columns, us: ones 50, pairs PAIRS_US.
+constexpr int kRowCols = 512;
+enum RowsBy { kRowsFours, kRowsOnes, kRowsPairs };
+
+template <class I, class S, class O, RowsBy BY>
 __global__ void __launch_bounds__(256)
 embedding_rows_kernel(const I* __restrict__ ids, const S* __restrict__ table, int64_t ld, O* __restrict__ out, float scale, int64_t T, int64_t V,
                       int D) {
   pdl_wait();
   pdl_launch_dependents();
-  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * (VEC ? 4 : 1);
-  if (col >= D) return;
-#pragma unroll 4
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < T; t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    const int64_t id = id_at(ids, t);
+  constexpr int W = BY == kRowsFours ? 4 : BY == kRowsPairs ? 2 : 1, N = kRowCols / 32 / W;
+  const int lane = threadIdx.x & 31, begin = blockIdx.y * kRowCols, end = min(D, begin + kRowCols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32);
+  int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
+  int64_t next = t < T ? id_at(ids, t) : 0;
+  for (; t < T; t += step) {
+    const int64_t id = next;
+    if (t + step < T) next = id_at(ids, t + step);
     const bool there = id >= 0 && id < V;
-    const S* row = table + (there ? id : 0) * ld + col;
-    if constexpr (VEC) {
-      float x[4];
-      load4(row, x);
+    const float by = there ? scale : __uint_as_float(0x7fffffffu);      // (an id outside the table: NaN times its first row)
+    const S* from = table + (there ? id : 0) * ld;
+    O* to = out + t * D;
+    const auto ones = [&](int first, int last) {
+      for (int c0 = first; c0 < last; c0 += 512) {
+        S x[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = there ? x[j] * scale : __uint_as_float(0x7fffffffu);
-      store4(out + t * D + col, x);
+        for (int n = 0; n < 16; ++n)
+          if (c0 + lane + n * 32 < last) x[n] = from[c0 + lane + n * 32];
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          if (c0 + lane + n * 32 < last) put(to + c0 + lane + n * 32, to_f(x[n]) * by);
+      }
+    };
+    if constexpr (BY == kRowsFours) {
+      const int col = begin + lane * 4;
+      const auto part = [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        float x[N][4];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (kWhole || col + n * 128 < end) load4(from + col + n * 128, x[n]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[n][j] *= by;
+          if (kWhole || col + n * 128 < end) store4(to + col + n * 128, x[n]);
+        }
+      };
+      if (end - begin == kRowCols) part(Yes{});
+      else part(No{});
+    } else if constexpr (BY == kRowsOnes) {
+      ones(begin, end);
     } else {
-      put(out + t * D + col, there ? to_f(*row) * scale : __uint_as_float(0x7fffffffu));
+      // (a last row's words could reach behind the table)
+      if (!there || id + 1 == V) {
+        ones(begin, end);
+        continue;
+      }
+      const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(to + begin) >> 1) & 1;      // columns before the output's first word
+      const int first = begin + lead, pairs = (end - first) / 2;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(from + first);
+      const bool off = (at & 2) != 0;
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+      const int n_words = pairs + (off ? 1 : 0);
+      uint32_t* put_words = reinterpret_cast<uint32_t*>(to + first);
+      uint32_t x[N + 1];
+#pragma unroll
+      for (int n = 0; n <= N; ++n) x[n] = lane + n * 32 < n_words ? words[lane + n * 32] : 0u;
+      if (lane == 0 && lead) put(to + begin, to_f(from[begin]) * by);
+      if (lane == 1 && first + 2 * pairs < end) put(to + end - 1, to_f(from[end - 1]) * by);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        uint32_t w = x[n];
+        if (off) w = __funnelshift_r(w, __shfl_sync(0xffffffffu, lane == 0 ? x[n + 1] : w, (lane + 1) & 31), 16);
+        if (lane + n * 32 < pairs)
+          put_words[lane + n * 32] = pack_bf16x2(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xffff0000u) * by);
+      }
     }
   }
 }
@@ -77,14 +138,22 @@ struct Zero {                // a part of the table's gradient that CTAs from `f
   char* base;
   int64_t lo, hi;            // bytes
   int from;
+  int* spans;                // set to 0 too
 };
 
 __device__ void fill_zero(const Zero& z) {
-  const int64_t n = static_cast<int64_t>(gridDim.x - z.from) * blockDim.x, i0 = static_cast<int64_t>(blockIdx.x - z.from) * blockDim.x + threadIdx.x;
-  const int64_t quads = (z.hi - z.lo) >> 4;
-  uint4* p = reinterpret_cast<uint4*>(z.base + z.lo);
-  for (int64_t i = i0; i < quads; i += n) p[i] = make_uint4(0, 0, 0, 0);
-  for (int64_t i = z.lo + (quads << 4) + i0; i < z.hi; i += n) z.base[i] = 0;
+  constexpr int kPiece = 4 * kThreads;      // 64 KB
+  const int64_t ctas = gridDim.x - z.from, me = blockIdx.x - z.from, quads = (z.hi - z.lo) >> 4;
+  uint4* p = reinterpret_cast<uint4*>(z.base + z.lo) + threadIdx.x;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int64_t q = me * kPiece; q < quads; q += ctas * kPiece) {
+    const int64_t left = quads - q - threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j * kThreads < left) p[q + j * kThreads] = zero;
+  }
+  if (me == 0 && threadIdx.x == 0) *z.spans = 0;
+  if (me == 0 && threadIdx.x < ((z.hi - z.lo) & 15)) z.base[z.lo + (quads << 4) + threadIdx.x] = 0;
 }
 
 struct SortArgs {
@@ -119,36 +188,34 @@ sort_count_kernel(From from, SortArgs a, int* __restrict__ hist, Zero z) {
   for (int b = threadIdx.x; b < a.bins; b += kThreads) hist[static_cast<int64_t>(blockIdx.x) * a.bins + b] = count[b];
 }
 
-// [kWarps][bins | 1] counts of the warps, and the first place of each bin for this CTA
-constexpr int rank_smem(int bins) { return 4 * (kWarps * (bins | 1) + bins + kWarps); }
+// One stable counting sort of a CTA's tokens by a digit.  `entry(i)`: token i of `count`, in parts of consecutive ones for each warp;
+// `others(bin)`: (tokens of this bin in all CTAs, in those before), or nothing but the own; `put(place, entry)` takes what was sorted.
+// cnt [kWarps][bins | 1], place [bins], sums [kWarps]
+constexpr int rank_ints(int bins) { return kWarps * (bins | 1) + bins + kWarps; }
 
-template <class From>
-__global__ void __launch_bounds__(kThreads)
-sort_rank_kernel(From from, SortArgs a, const int* __restrict__ hist, int chunks, uint2* __restrict__ out, Zero z) {
-  pdl_wait();
-  pdl_launch_dependents();
-  if (static_cast<int>(blockIdx.x) >= z.from) return fill_zero(z);
-  extern __shared__ int sm[];
-  const int S = a.bins | 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = blockIdx.x;
-  int* cnt = sm;                       // [kWarps][S]
-  int* place = sm + kWarps * S;        // [bins]
-  int* sums = place + a.bins;          // [kWarps]
+template <class Entry, class Others, class Put>
+__device__ __forceinline__ void sort_pass(int count, int shift, int bins, int* sm, Entry entry, Others others, Put put) {
+  const int S = bins | 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;      // (odd: the counts of a bin lie in different banks)
+  int* cnt = sm;
+  int* place = sm + kWarps * S;
+  int* sums = place + bins;
   for (int i = tid; i < kWarps * S; i += kThreads) cnt[i] = 0;
   __syncthreads();
-  // this CTA's tokens, a consecutive part for each warp
-  const int lo = c * a.chunk, count = min(a.T - lo, a.chunk);
   const int part = ((count + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int wlo = min(count, warp * part), whi = min(count, wlo + part);
-  for (int i = wlo + lane; i < whi; i += 32) atomicAdd(&cnt[warp * S + ((from(lo + i, a).x >> a.shift) & (a.bins - 1))], 1);
-  // (bins are at most half the threads) counts of all CTAs, and of those before
+  const int lo = min(count, warp * part), hi = min(count, lo + part);
+  for (int i = lo + lane; i < hi; i += 32) atomicAdd(&cnt[warp * S + ((entry(i).x >> shift) & (bins - 1))], 1);
   int all = 0, before = 0;
-  if (tid < a.bins) {
+  const bool given = others(tid, all, before);      // (bins are at most half the threads)
+  __syncthreads();
+  if (tid < bins) {                                 // the warps' counts become how many tokens of the bin earlier warps have
+    int run = 0;
 #pragma unroll 8
-    for (int i = 0; i < chunks; ++i) {
-      const int v = hist[static_cast<int64_t>(i) * a.bins + tid];
-      all += v;
-      before += i < c ? v : 0;
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = cnt[w * S + tid];
+      cnt[w * S + tid] = run;
+      run += n;
     }
+    if (!given) all = run;
   }
   int up = all;
 #pragma unroll
@@ -158,34 +225,69 @@ sort_rank_kernel(From from, SortArgs a, const int* __restrict__ hist, int chunks
   }
   if (lane == 31) sums[warp] = up;
   __syncthreads();
-  if (tid < a.bins) {
+  if (tid < bins) {
     int base = 0;
     for (int w = 0; w < warp; ++w) base += sums[w];
     place[tid] = base + up - all + before;
   }
   __syncthreads();
-  for (int b = warp; b < a.bins; b += kWarps) {      // a lane per warp's count
-    const int n = cnt[lane * S + b];
-    int s = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += v;
-    }
-    cnt[lane * S + b] = place[b] + s - n;
-  }
-  __syncthreads();
-  for (int i0 = wlo; i0 < whi; i0 += 32) {
+  for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
-    const uint2 e = i < whi ? from(lo + i, a) : make_uint2(0, 0);
-    const int b = i < whi ? static_cast<int>((e.x >> a.shift) & (a.bins - 1)) : -1;
+    const uint2 e = i < hi ? entry(i) : make_uint2(0, 0);
+    const int b = i < hi ? static_cast<int>((e.x >> shift) & (bins - 1)) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, b);
     const int rank = __popc(same & ((1u << lane) - 1u));
-    const int at = b >= 0 ? cnt[warp * S + b] + rank : 0;
+    const int at = b >= 0 ? place[b] + cnt[warp * S + b] + rank : 0;
     __syncwarp();
     if (b >= 0 && rank == 0) cnt[warp * S + b] += __popc(same);
     __syncwarp();
-    if (b >= 0) out[at] = e;
+    if (b >= 0) put(at, e);
+  }
+}
+
+template <class From>
+__global__ void __launch_bounds__(kThreads)
+sort_rank_kernel(From from, SortArgs a, const int* __restrict__ hist, int chunks, uint2* __restrict__ out, Zero z) {
+  pdl_wait();
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= z.from) return fill_zero(z);
+  extern __shared__ int sm[];
+  const int lo = blockIdx.x * a.chunk;
+  sort_pass(min(a.T - lo, a.chunk), a.shift, a.bins, sm, [&](int i) { return from(lo + i, a); },
+            [&](int bin, int& all, int& before) {
+              if (bin < a.bins) {
+#pragma unroll 16
+                for (int c = 0; c < chunks; ++c) {
+                  const int v = hist[static_cast<int64_t>(c) * a.bins + bin];
+                  all += v;
+                  before += c < static_cast<int>(blockIdx.x) ? v : 0;
+                }
+              }
+              return true;
+            },
+            [&](int at, uint2 e) { out[at] = e; });
+}
+
+// The whole sort in one CTA, between two lists in shared memory, while the other CTAs fill the gradient with zeros
+constexpr int kSmallSort = 8192;
+template <class From>
+__global__ void __launch_bounds__(kThreads)
+sort_small_kernel(From from, SortArgs a, int passes, uint2* __restrict__ out, Zero z) {
+  pdl_wait();
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= z.from) return fill_zero(z);
+  extern __shared__ int sm[];
+  uint2* list[2] = {reinterpret_cast<uint2*>(sm), reinterpret_cast<uint2*>(sm) + a.T};
+  int* counts = sm + 4 * a.T;
+  const auto own = [](int, int&, int&) { return false; };
+  for (int t = threadIdx.x; t < a.T; t += kThreads) list[0][t] = from(t, a);
+  __syncthreads();
+  int bits = 31 - __clz(a.bins);
+  for (int p = 0; p < passes; ++p) {
+    const uint2* in = list[p & 1];
+    uint2* to = p + 1 == passes ? out : list[(p + 1) & 1];
+    sort_pass(a.T, p * bits, a.bins, counts, [&](int i) { return in[i]; }, own, [&](int at, uint2 e) { to[at] = e; });
+    __syncthreads();
   }
 }
 
@@ -195,119 +297,219 @@ struct SumArgs {
   int T, chunk, V, D;
   int64_t ld;
   float scale;
+  int* spans;                // how many runs go on behind the chunk that they begin in, and those chunks, in no order
   float* parts;              // [2 chunks][D]: what a chunk adds to the run that came in, and what it begins of the one that goes on
 };
 
-// A thread's four columns: next to each other (VEC) or a CTA's width apart
-template <bool VEC, class T>
-__device__ __forceinline__ void load_cols(const T* row, int col, int step, int D, float (&x)[4]) {
-  if constexpr (VEC) {
-    load4(row + col, x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = col + j * step < D ? to_f(row[col + j * step]) : 0.f;
-  }
+// A thread's four columns: next to each other (kFours), a CTA's width apart (kOnes), or two pairs that far apart (kPairs), which bf16 rows of an odd
+// width or stride are read in, as 32-bit words, put together from two neighbouring ones where a row lies one column off them.
+enum ColsBy { kFours, kOnes, kPairs };
+template <ColsBy BY>
+__device__ __forceinline__ int first_col(int step) {
+  return blockIdx.y * step * 4 + threadIdx.x * (BY == kFours ? 4 : BY == kPairs ? 2 : 1);
 }
-template <bool VEC, class T>
+template <ColsBy BY>
+__device__ __forceinline__ int col_of(int col, int step, int j) {
+  return BY == kFours ? col + j : BY == kOnes ? col + j * step : col + (j >> 1) * 2 * step + (j & 1);
+}
+
+// What a thread reads of a row, as it lies in memory (a conversion next to the load would wait for it).  at: its columns, those that are not there
+// brought to 0 (they are not stored).  last: the row is the matrix' last one, behind which nothing is read.
+template <ColsBy BY, class T>
+struct Cols;
+template <>
+struct Cols<kFours, float> {
+  float4 x;
+  __device__ __forceinline__ void load(const float* row, const int (&at)[4], bool) { x = *reinterpret_cast<const float4*>(row + at[0]); }
+  __device__ __forceinline__ void add(float (&acc)[4]) const { acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w; }
+};
+template <>
+struct Cols<kFours, __nv_bfloat16> {
+  uint2 x;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, const int (&at)[4], bool) { x = *reinterpret_cast<const uint2*>(row + at[0]); }
+  __device__ __forceinline__ void add(float (&acc)[4]) const {
+    acc[0] += __uint_as_float(x.x << 16);
+    acc[1] += __uint_as_float(x.x & 0xffff0000u);
+    acc[2] += __uint_as_float(x.y << 16);
+    acc[3] += __uint_as_float(x.y & 0xffff0000u);
+  }
+};
+template <class T>
+struct Cols<kOnes, T> {
+  T x[4];
+  __device__ __forceinline__ void load(const T* row, const int (&at)[4], bool) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = row[at[j]];
+  }
+  __device__ __forceinline__ void add(float (&acc)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += to_f(x[j]);
+  }
+};
+template <>
+struct Cols<kPairs, __nv_bfloat16> {
+  uint32_t x[2][2];
+  bool off;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, const int (&at)[4], bool last) {
+    off = (reinterpret_cast<uintptr_t>(row) & 2) != 0;      // (columns of pairs are even)
+    const char* words = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(3));
+    if (!last) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        x[h][0] = *reinterpret_cast<const uint32_t*>(words + at[2 * h] * 2);
+        x[h][1] = off ? *reinterpret_cast<const uint32_t*>(words + at[2 * h] * 2 + 4) : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {      // (at[2 h + 1] is the pair's second column, or 0)
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(row + at[2 * h]) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + at[2 * h + 1])) << 16;
+        x[h][0] = off ? w << 16 : w;
+        x[h][1] = w >> 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void add(float (&acc)[4]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = off ? __funnelshift_r(x[h][0], x[h][1], 16) : x[h][0];
+      acc[2 * h] += __uint_as_float(w << 16);
+      acc[2 * h + 1] += __uint_as_float(w & 0xffff0000u);
+    }
+  }
+};
+
+template <ColsBy BY, class T>
 __device__ __forceinline__ void store_cols(T* row, int col, int step, int D, const float (&x)[4]) {
-  if constexpr (VEC) {
+  if constexpr (BY == kFours) {
     store4(row + col, x);
   } else {
+    T* first = row + col;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j * step < D) put(row + col + j * step, x[j]);
+    for (int j = 0; j < 4; ++j) {
+      const int c = col_of<BY>(0, step, j);
+      if (col + c < D) put(first + c, x[j]);
+    }
   }
 }
 
-template <class S, class O, bool VEC>
-__global__ void __launch_bounds__(kSegThreads)
+template <class S, class O, ColsBy BY, int STEP>
+__global__ void __launch_bounds__(STEP)
 segment_sum_kernel(SumArgs a, const S* __restrict__ dout, O* __restrict__ dtable) {
   pdl_wait();
   pdl_launch_dependents();
-  const int step = blockDim.x, col = blockIdx.y * step * 4 + threadIdx.x * (VEC ? 4 : 1);
+  constexpr int step = STEP;
+  const int col = first_col<BY>(step);
   const int lo = blockIdx.x * a.chunk, hi = min(a.T, lo + a.chunk);
-  if (VEC && col >= a.D) return;
+  if (col >= a.D) return;
+  int at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) at[j] = col_of<BY>(col, step, j) < a.D ? col_of<BY>(col, step, j) : 0;
   const uint32_t none = static_cast<uint32_t>(a.V);
   const uint32_t came = lo > 0 ? a.sorted[lo - 1].x : none, goes = hi < a.T ? a.sorted[hi].x : none;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   uint32_t run = a.sorted[lo].x;
   bool open = run == came;           // the run began before this chunk
+  // a run that begins here and goes on is one for the next kernel
+  if (threadIdx.x == 0 && blockIdx.y == 0 && goes != none && a.sorted[hi - 1].x == goes && came != goes) a.spans[1 + atomicAdd(a.spans, 1)] = blockIdx.x;
   if (run == none) return;
   constexpr int U = 8;
+  static_assert(kSegMin % U == 0, "chunks of whole steps");
+  uint2 next[U];                     // entries behind the end: no row, and the first token's to read
+  const auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = i0 + u < hi ? a.sorted[i0 + u] : make_uint2(none, 0);
+  };
+  fetch(lo);
   for (int i0 = lo; i0 < hi; i0 += U) {
-    uint2 e[U];
-    float x[U][4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) e[u] = i0 + u < hi ? a.sorted[i0 + u] : make_uint2(none, 0);
+    uint32_t id[U];
+    Cols<BY, S> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (e[u].x != none) load_cols<VEC>(dout + static_cast<int64_t>(e[u].y) * a.ld, col, step, a.D, x[u]);
+      id[u] = next[u].x;
+      x[u].load(dout + static_cast<int64_t>(next[u].y) * a.ld, at, static_cast<int>(next[u].y) + 1 == a.T);
     }
+    fetch(i0 + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (e[u].x != run) {
+      if (id[u] != run) {
         if (open) {
-          store_cols<VEC>(a.parts + static_cast<int64_t>(2 * blockIdx.x) * a.D, col, step, a.D, acc);
-        } else if (run != none && !(i0 + u >= hi && run == goes)) {
+          store_cols<BY>(a.parts + static_cast<int64_t>(2 * blockIdx.x) * a.D, col, step, a.D, acc);
+        } else if (!(i0 + u >= hi && run == goes)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j] *= a.scale;
-          store_cols<VEC>(dtable + static_cast<int64_t>(run) * a.D, col, step, a.D, acc);
-        } else if (run != none) {
-          store_cols<VEC>(a.parts + static_cast<int64_t>(2 * blockIdx.x + 1) * a.D, col, step, a.D, acc);
+          store_cols<BY>(dtable + static_cast<int64_t>(run) * a.D, col, step, a.D, acc);
+        } else {
+          store_cols<BY>(a.parts + static_cast<int64_t>(2 * blockIdx.x + 1) * a.D, col, step, a.D, acc);
         }
-        if (e[u].x == none) return;
-        run = e[u].x;
+        if (id[u] == none) return;
+        run = id[u];
         open = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += x[u][j];
+      x[u].add(acc);
     }
   }
-  // a chunk of a multiple of U tokens: its last run
+  // a chunk of whole steps: its last run
   if (open) {
-    store_cols<VEC>(a.parts + static_cast<int64_t>(2 * blockIdx.x) * a.D, col, step, a.D, acc);
+    store_cols<BY>(a.parts + static_cast<int64_t>(2 * blockIdx.x) * a.D, col, step, a.D, acc);
   } else if (run == goes) {
-    store_cols<VEC>(a.parts + static_cast<int64_t>(2 * blockIdx.x + 1) * a.D, col, step, a.D, acc);
+    store_cols<BY>(a.parts + static_cast<int64_t>(2 * blockIdx.x + 1) * a.D, col, step, a.D, acc);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] *= a.scale;
-    store_cols<VEC>(dtable + static_cast<int64_t>(run) * a.D, col, step, a.D, acc);
+    store_cols<BY>(dtable + static_cast<int64_t>(run) * a.D, col, step, a.D, acc);
   }
 }
 
-// Runs over several chunks, each by the CTAs of the chunk that it begins in: its part there, and those of the chunks up to its end
+// Runs over several chunks: what a run left in the chunk that it begins in, and in those up to its end
 template <class O>
 __global__ void __launch_bounds__(kSegThreads)
 segment_join_kernel(SumArgs a, O* __restrict__ dtable) {
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x, lo = c * a.chunk, hi = min(a.T, lo + a.chunk);
-  if (hi >= a.T) return;
-  const uint32_t run = a.sorted[hi - 1].x;
-  if (run == static_cast<uint32_t>(a.V) || a.sorted[hi].x != run || (lo > 0 && a.sorted[lo - 1].x == run)) return;
-  int first = hi, last = a.T;              // the run ends before `last`
-  while (first < last) {
-    const int mid = first + (last - first) / 2;
-    if (a.sorted[mid].x == run) first = mid + 1;
-    else last = mid;
-  }
-  const int end = (first - 1) / a.chunk;   // its last chunk
-  __shared__ float part[kSegThreads / 32][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * 32 + lane;
-  float s = 0.f;
-  if (col < a.D) {
+  const int tiles = (a.D + kJoinCols - 1) / kJoinCols, items = a.spans[0] * tiles;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int c = a.spans[1 + item / tiles], tile = item % tiles;
+    const uint32_t run = a.sorted[(c + 1) * a.chunk].x;
+    // its last chunk: the first one behind this whose last token is another's (all chunks that could be are asked at once)
+    __shared__ int ends;
+    __syncthreads();
+    if (threadIdx.x == 0) ends = 0x7fffffff;
+    __syncthreads();
+    for (int i0 = c + 1; ends == 0x7fffffff; i0 += kSegThreads) {
+      const int i = i0 + threadIdx.x;
+      const int64_t behind = (static_cast<int64_t>(i) + 1) * a.chunk;
+      const bool over = behind >= a.T || a.sorted[behind - 1].x != run || a.sorted[behind].x != run;
+      __syncthreads();
+      if (over) atomicMin(&ends, i);
+      __syncthreads();
+    }
+    const int end = ends;
+    // a warp adds up every eighth part, four columns a thread
+    constexpr int kTeams = kSegThreads / 32;
+    __shared__ float sums[kTeams][kJoinCols];
+    const int team = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int i = c + warp; i <= end; i += kSegThreads / 32) s += a.parts[static_cast<int64_t>(2 * i + (i == c ? 1 : 0)) * a.D + col];
-  }
-  part[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0 && col < a.D) {
-    s = 0.f;
+    for (int i = c + team; i <= end; i += kTeams) {
+      const float* part = a.parts + static_cast<int64_t>(2 * i + (i == c ? 1 : 0)) * a.D;
 #pragma unroll
-    for (int w = 0; w < kSegThreads / 32; ++w) s += part[w][lane];
-    put(dtable + static_cast<int64_t>(run) * a.D + col, s * a.scale);
+      for (int j = 0; j < 4; ++j) {
+        const int col = tile * kJoinCols + lane + j * 32;
+        acc[j] += part[col < a.D ? col : 0];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[team][lane + j * 32] = acc[j];
+    __syncthreads();
+    const int n = threadIdx.x, col = tile * kJoinCols + n;
+    if (n < kJoinCols && col < a.D) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTeams; ++w) s += sums[w][n];
+      put(dtable + static_cast<int64_t>(run) * a.D + col, s * a.scale);
+    }
   }
 }
 
@@ -317,6 +519,7 @@ int bits_of(int64_t n) {             // of the largest value below n
   return b;
 }
 struct Plan {
+  bool small;                        // sorted by one CTA
   int passes, bits, chunks, chunk, seg_chunk, seg_chunks;
 };
 Plan plan_for(int64_t T, int64_t V) {
@@ -324,8 +527,9 @@ Plan plan_for(int64_t T, int64_t V) {
   const int bits = bits_of(V + 1);
   p.passes = (bits + kDigit - 1) / kDigit;
   p.bits = (bits + p.passes - 1) / p.passes;
+  p.small = T <= kSmallSort;
   p.chunk = static_cast<int>((T + kMaxChunks - 1) / kMaxChunks);
-  p.chunk = (p.chunk + kThreads - 1) / kThreads * kThreads;
+  p.chunk = p.small ? static_cast<int>(T) : p.chunk < 2 * kThreads ? 2 * kThreads : (p.chunk + kThreads - 1) / kThreads * kThreads;
   p.chunks = static_cast<int>((T + p.chunk - 1) / p.chunk);
   p.seg_chunk = static_cast<int>((T + kSegChunks - 1) / kSegChunks);
   p.seg_chunk = p.seg_chunk < kSegMin ? kSegMin : (p.seg_chunk + 7) / 8 * 8;
@@ -338,26 +542,35 @@ bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 template <class I, class S, class O>
 int launch_rows(const I* ids, const S* table, int64_t ld, O* out, float scale, int64_t T, int64_t V, int D, cudaStream_t stream) {
   const bool vec = D % 4 == 0 && ld % 4 == 0 && aligned(table, 4 * sizeof(S)) && aligned(out, 4 * sizeof(O));
-  const int units = vec ? D / 4 : D;
-  int width = 32;
-  while (width < 256 && width < units) width *= 2;
-  const dim3 block(width, 256 / width);
-  const int64_t rows = (T + block.y - 1) / block.y;
-  const dim3 grid(static_cast<unsigned>(rows < 148 * 32 ? rows : 148 * 32), (units + width - 1) / width);
-  return launch_code(vec ? launch_pdl(embedding_rows_kernel<I, S, O, true>, grid, block, 0, stream, ids, table, ld, out, scale, T, V, D)
-                         : launch_pdl(embedding_rows_kernel<I, S, O, false>, grid, block, 0, stream, ids, table, ld, out, scale, T, V, D));
+  const int warps = T < 8 ? static_cast<int>(T) : 8, slices = (D + kRowCols - 1) / kRowCols;
+  int64_t rows = (T + warps - 1) / warps;
+  const int64_t most = (148 * 8 + slices - 1) / slices;
+  const dim3 block(32 * warps), grid(static_cast<unsigned>(rows < most ? rows : most), slices);
+  const auto run = [&](auto* kernel) { return launch_code(launch_pdl(kernel, grid, block, 0, stream, ids, table, ld, out, scale, T, V, D)); };
+  if (vec) return run(embedding_rows_kernel<I, S, O, kRowsFours>);
+  if constexpr (sizeof(S) == 2 && sizeof(O) == 2) {
+    if (aligned(table, 4) && aligned(out, 4)) return run(embedding_rows_kernel<I, S, O, kRowsPairs>);
+  }
+  return run(embedding_rows_kernel<I, S, O, kRowsOnes>);
 }
 
 template <class S, class O>
 int launch_sums(const SumArgs& a, int chunks, const S* dout, O* dtable, cudaStream_t stream) {
   const bool vec = a.D % 4 == 0 && a.ld % 4 == 0 && aligned(dout, 4 * sizeof(S)) && aligned(dtable, 4 * sizeof(O));
-  int width = 32;
-  while (width < kSegThreads && width * 4 < a.D) width *= 2;
-  const dim3 grid(chunks, (a.D + width * 4 - 1) / (width * 4));
-  int rc = launch_code(vec ? launch_pdl(segment_sum_kernel<S, O, true>, grid, dim3(width), 0, stream, a, dout, dtable)
-                           : launch_pdl(segment_sum_kernel<S, O, false>, grid, dim3(width), 0, stream, a, dout, dtable));
-  if (rc == 0 && chunks > 1)
-    rc = launch_code(launch_pdl(segment_join_kernel<O>, dim3(chunks, (a.D + 31) / 32), dim3(kSegThreads), 0, stream, a, dtable));
+  const auto run = [&](auto* kernel, int width) {
+    return launch_code(launch_pdl(kernel, dim3(chunks, (a.D + width * 4 - 1) / (width * 4)), dim3(width), 0, stream, a, dout, dtable));
+  };
+  constexpr ColsBy kWords = sizeof(S) == 2 ? kPairs : kOnes;
+  const bool words = sizeof(S) == 2 && aligned(dout, 4), wide = a.D > 256;      // narrow rows take CTAs of two warps
+  int rc;
+  if (vec) rc = wide ? run(segment_sum_kernel<S, O, kFours, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kFours, 64>, 64);
+  else if (words) rc = wide ? run(segment_sum_kernel<S, O, kWords, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kWords, 64>, 64);
+  else rc = wide ? run(segment_sum_kernel<S, O, kOnes, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kOnes, 64>, 64);
+  if (rc == 0 && chunks > 1) {
+    const int64_t items = static_cast<int64_t>(chunks - 1) * ((a.D + kJoinCols - 1) / kJoinCols);
+    rc = launch_code(launch_pdl(segment_join_kernel<O>, dim3(static_cast<unsigned>(items < 148 * 8 ? items : 148 * 8)), dim3(kSegThreads), 0, stream,
+                                a, dtable));
+  }
   return rc;
 }
 
@@ -369,12 +582,12 @@ bool fits(int64_t T, int64_t V, int D) {
 
 int64_t embedding_scratch_bytes(int64_t T, int64_t V, int D) {
   const Plan p = plan_for(T, V);
-  return 2 * on16(8 * T) + on16(4ll * p.chunks << p.bits) + 8ll * p.seg_chunks * D;
+  return 2 * on16(8 * T) + on16(4ll * p.chunks << p.bits) + on16(4ll * (p.seg_chunks + 1)) + 8ll * p.seg_chunks * D;
 }
 
 int embedding_grad_kernels(int64_t T, int64_t V) {
   const Plan p = plan_for(T, V);
-  return 2 * p.passes + (p.seg_chunks > 1 ? 2 : 1);
+  return (p.small ? 1 : 2 * p.passes) + (p.seg_chunks > 1 ? 2 : 1);
 }
 
 int embedding_rows(const void* ids, bool ids64, const void* table, bool table16, int64_t ld, void* out, bool out16, float scale, int64_t T,
@@ -399,21 +612,31 @@ int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, i
   at += 2 * on16(8 * T);
   int* hist = reinterpret_cast<int*>(at);
   at += on16(4ll * p.chunks << p.bits);
+  int* spans = reinterpret_cast<int*>(at);
+  at += on16(4ll * (p.seg_chunks + 1));
   SortArgs a{};
   a.T = static_cast<int>(T); a.chunk = p.chunk; a.bins = 1 << p.bits; a.V = static_cast<int>(V); a.padding = static_cast<int>(padding);
   const int64_t bytes = V * D * (dtable16 ? 2 : 4);
   // each of the sorting kernels fills its share of the gradient
-  const int kernels = 2 * p.passes;
+  const int kernels = p.small ? 1 : 2 * p.passes;
   int64_t done = 0;
-  Zero z{static_cast<char*>(dtable), 0, 0, p.chunks};
+  Zero z{static_cast<char*>(dtable), 0, 0, p.chunks, spans};
   const auto share = [&](int i) {
     z.lo = done;
     z.hi = done = i + 1 == kernels ? bytes : bytes * (i + 1) / kernels / 16 * 16;
     int64_t ctas = (z.hi - z.lo + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
     if (ctas > 148 * 2) ctas = 148 * 2;
+    if (p.small && ctas > 147) ctas = 147;      // (the sort's shared memory leaves an SM one CTA)
     return static_cast<int>(ctas < 1 ? 1 : ctas);
   };
-  const int smem = rank_smem(a.bins);
+  const int smem = 4 * rank_ints(a.bins) + (p.small ? 16 * a.T : 0);
+  const auto whole = [&](auto from) {
+    using From = decltype(from);
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(sort_small_kernel<From>), smem)) return -20;
+    const int more = share(0);
+    return launch_code(launch_pdl(sort_small_kernel<From>, dim3(1 + more), dim3(kThreads), static_cast<size_t>(smem), stream, from, a, p.passes,
+                                  lists[0], z));
+  };
   const auto pass = [&](auto from, int i) {
     using From = decltype(from);
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(sort_rank_kernel<From>), smem)) return -20;
@@ -425,15 +648,20 @@ int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, i
     return launch_code(launch_pdl(sort_rank_kernel<From>, dim3(p.chunks + more), dim3(kThreads), static_cast<size_t>(smem), stream, from, a,
                                   hist, p.chunks, lists[i & 1], z));
   };
-  for (int i = 0; i < p.passes; ++i) {
+  if (p.small) {
+    const int rc = ids64 ? whole(FromIds64{static_cast<const int64_t*>(ids)}) : whole(FromIds32{static_cast<const int*>(ids)});
+    if (rc) return rc;
+  }
+  for (int i = 0; i < p.passes && !p.small; ++i) {
     const int rc = i > 0 ? pass(FromPass{lists[(i - 1) & 1]}, i)
                    : ids64 ? pass(FromIds64{static_cast<const int64_t*>(ids)}, i)
                            : pass(FromIds32{static_cast<const int*>(ids)}, i);
     if (rc) return rc;
   }
   SumArgs s{};
-  s.sorted = lists[(p.passes - 1) & 1];
+  s.sorted = lists[p.small ? 0 : (p.passes - 1) & 1];
   s.T = a.T; s.chunk = p.seg_chunk; s.V = a.V; s.D = D; s.ld = ld; s.scale = scale;
+  s.spans = spans;
   s.parts = reinterpret_cast<float*>(at);
   const auto sums = [&](auto* d) {
     return dtable16 ? launch_sums(s, p.seg_chunks, d, static_cast<__nv_bfloat16*>(dtable), stream)

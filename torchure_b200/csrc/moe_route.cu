@@ -428,8 +428,39 @@ struct ScoreArgs {
   float scale;
 };
 
+// exp(-a) for a >= 0 in 64 bits, within about 2^-46: exp(-a) = 2^n exp(r), |r| <= ln 2 / 2, and Taylor's series to r^11 / 11!.  Above 700: what it is
+// there, 2^-1010, next to which the result is zero in fp32.
+__device__ __forceinline__ double exp_minus(float a) {
+  const double x = static_cast<double>(fminf(a, 700.f));
+  constexpr double kRound = 6755399441055744.0;      // 1.5 2^52: the sum's last bits are the rounded number
+  const double t = fma(x, -1.4426950408889634, kRound);
+  const double r = fma(t - kRound, -0.6931471805599453, -x);
+  double p = 1.0 / 39916800.0;
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+// sigmoid(l), rounded once to fp32: e = exp(-|l|), 1 / (1 + e) by two of Newton's steps
+__device__ __forceinline__ float sigmoid64(float l) {
+  const double e = exp_minus(fabsf(l)), d = 1.0 + e;
+  double q = static_cast<double>(__fdividef(1.f, static_cast<float>(d)));
+  q = fma(q, fma(-d, q, 1.0), q);
+  q = fma(q, fma(-d, q, 1.0), q);
+  const float s = static_cast<float>(l < 0.f ? e * q : q);
+  return l != l ? l : s;
+}
 // s over exp(shift) for scores that may all be tiny: sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|))
 __device__ __forceinline__ float sigmoid_over(float l, float shift) { return expf(fminf(l, 0.f) - shift) / (1.f + expf(-fabsf(l))); }
+constexpr float kTinyScores = -80.f;      // a score below 2^-115: others may be too small for fp32
 
 template <int LANES>
 __device__ __forceinline__ float group_max(float v, uint32_t mask) {
@@ -479,28 +510,30 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
   };
   fetch(t0 + group);
   for (int t = t0 + group; t < t1; t += GROUPS) {
-    float x[VALS], top = -INFINITY;
+    float x[VALS], s[VALS], top = -INFINITY;
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {
       x[v] = next[v];
       top = fmaxf(top, x[v]);
     }
     fetch(t + GROUPS);
-    top = group_max<LANES>(top, mask);
-    float s[VALS];
+    // (of sigmoids the largest logit is asked for only where all scores are tiny)
+    const bool tiny = how.sigmoid && !__any_sync(mask, top >= kTinyScores);
+    if (!how.sigmoid || tiny) top = group_max<LANES>(top, mask);
     if (how.sigmoid) {
 #pragma unroll
-      for (int v = 0; v < VALS; ++v)
-        s[v] = by_score ? static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(x[v])))) : sigmoid_over(x[v], 0.f);
+      for (int v = 0; v < VALS; ++v) s[v] = sigmoid64(x[v]);
     } else {
       double e[VALS], sum = 0.0;
+      const bool none = top == -INFINITY;
 #pragma unroll
       for (int v = 0; v < VALS; ++v) {
-        e[v] = top == -INFINITY ? 0.0 : exp(static_cast<double>(x[v]) - static_cast<double>(top));
+        const float below = top - x[v];
+        e[v] = none ? 0.0 : below != below ? static_cast<double>(below) : exp_minus(below);
         sum += e[v];
       }
       sum = group_sum64<LANES>(sum, mask);
-      const double r = sum > 0.0 || sum != sum ? 1.0 / sum : 0.0;
+      const double r = none ? 0.0 : 1.0 / sum;
 #pragma unroll
       for (int v = 0; v < VALS; ++v) s[v] = static_cast<float>(e[v] * r);
     }
@@ -540,14 +573,21 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
     choose<VALS, false>(key, index, a.k, gl, mask, my_key, my_e);
     const bool made = gl < a.k && my_key != kKeyMinusInf;
     const float l = made ? load_logit(logits + t * a.ld + my_e) : -INFINITY;
-    float shift = 0.f;
-    if (how.normalize) shift = group_max<LANES>(how.sigmoid ? (made ? fminf(l, 0.f) : -INFINITY) : l, mask);
-    float w = 0.f;
-    if (made) w = how.sigmoid ? sigmoid_over(l, shift) : expf(l - (how.normalize ? shift : top));
-    float whole = 1.f;
-    if (how.normalize) {
+    float w = 0.f, whole = 1.f;
+    if (how.sigmoid) {
+      if (how.normalize && !__any_sync(mask, made && l >= kTinyScores)) {
+        const float shift = group_max<LANES>(made ? l : -INFINITY, mask);
+        if (made) w = sigmoid_over(l, fminf(shift, 0.f));
+      } else if (made) {
+        w = sigmoid64(l);
+      }
+      if (how.normalize) whole = group_sum<LANES>(w, mask);
+    } else if (how.normalize) {
+      const float shift = group_max<LANES>(l, mask);
+      if (made) w = expf(l - shift);
       whole = group_sum<LANES>(w, mask);
-    } else if (!how.sigmoid) {
+    } else {
+      if (made) w = expf(l - top);
       whole = 0.f;
 #pragma unroll
       for (int v = 0; v < VALS; ++v) whole += top == -INFINITY ? 0.f : expf(x[v] - top);
@@ -563,8 +603,7 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
       if (made) atomicAdd(&hist[my_e], 1);
     }
     if (how.sigmoid) {
-      // scores below 2^-115 have lost bits in fp32: where there are no others, all over the largest one's
-      if (top < -80.f && top != -INFINITY) {
+      if (tiny && top != -INFINITY) {      // over the largest one's
 #pragma unroll
         for (int v = 0; v < VALS; ++v) s[v] = sigmoid_over(x[v], top);
       }
@@ -572,7 +611,7 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
 #pragma unroll
       for (int v = 0; v < VALS; ++v) sum += s[v];
       sum = group_sum<LANES>(sum, mask);
-      const float r = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
+      const float r = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int v = 0; v < VALS; ++v) acc[v] += s[v] * r;
     } else {
@@ -611,11 +650,17 @@ route_scored_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* _
     top = group_max<LANES>(top, mask);
     odd = __any_sync(mask, odd);      // a NaN among the logits makes the whole row's gradient NaN
     const bool none = top == -INFINITY;
-    const float shift = sigmoid ? fminf(top, 0.f) : top;
-    float p[VALS], s = 0.f, mean = 0.f;
+    float p[VALS], steep[VALS], s = 0.f, mean = 0.f;
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {
-      p[v] = none ? 0.f : sigmoid ? sigmoid_over(x[v], shift) : expf(x[v] - top);
+      if (sigmoid) {
+        const float e = expf(-fabsf(x[v])), q = __fdividef(1.f, 1.f + e);
+        p[v] = x[v] < 0.f ? e * q : q;
+        steep[v] = x[v] < 0.f ? q : e * q;
+        if (top < kTinyScores) p[v] = none ? 0.f : sigmoid_over(x[v], top);
+      } else {
+        p[v] = none ? 0.f : expf(x[v] - top);
+      }
       s += p[v];
       mean += p[v] * share[v];
     }
@@ -642,7 +687,7 @@ route_scored_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* _
     for (int v = 0; v < VALS; ++v) {
       const float q = p[v] * r;
       float d = pull == 0.f ? 0.f : pull * q * (share[v] - mean);
-      if (sigmoid) d = d == 0.f ? 0.f : d * sigmoid_over(-x[v], 0.f);
+      if (sigmoid) d *= steep[v];
       else d -= q * inner;
       x[v] = odd ? __uint_as_float(0x7fffffffu) : d;
     }
