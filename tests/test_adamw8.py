@@ -298,7 +298,7 @@ def test_optimizer_follows_the_32_bit_one(device):
     (a, _), (b, _) = train(device, 10, 8), train(device, 10, 32)
     start, _ = train(device, 0, 32)
     for p, q, s in zip(a, b, start):
-        assert float((p - q).norm()) < 0.25 * float((q - s).norm())
+        assert float((p - q).detach().norm()) < 0.25 * float((q - s).detach().norm())
 
 
 @pytest.mark.parametrize("device", ["cpu", GPU])

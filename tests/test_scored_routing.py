@@ -215,7 +215,7 @@ def test_refusals(device):
 def test_no_tokens(device):
     x = torch.randn(0, 8, device=device, requires_grad=True)
     r = moe.route(x, 2, score="sigmoid", bias=torch.zeros(8, device=device), groups=4, top_groups=2)
-    assert r.weights.shape == (0, 2) and r.offsets.tolist() == [0] * 9 and float(r.aux_loss) == 0
+    assert r.weights.shape == (0, 2) and r.offsets.tolist() == [0] * 9 and float(r.aux_loss.detach()) == 0
     grad, = torch.autograd.grad((r.weights.sum() + r.aux_loss,), (x,))
     assert grad.shape == (0, 8)
 

@@ -594,10 +594,11 @@ bool rows_stay(const Tensor& x, int64_t R, int64_t E, bool in8) {
 // rows are few, the down product's rows, which the weighted sum reads back: in fp32 they would be 67 MB more of traffic (16384 rows of 1024).
 // Weights, sums and the weighted sum are fp32.
 Mlp mlp_fwd(const Tensor& x, const Tensor& logits, const Tensor& wgu, const Tensor& wd, int64_t k, int64_t capacity, const OptScoring& how,
-            int64_t bits, bool keep, const Outputs& make) {
+            const OptTensor& counts, int64_t bits, bool keep, const Outputs& make) {
   Mlp m;
   const Overlap overlap;
   m.r = do_route(logits, k, capacity, how, make);
+  if (has(counts)) at::Tensor(*counts).add_(m.r.counts);
   const int64_t R = x.size(0) * k, F = wd.size(2), E = wd.size(0), D = x.size(1);
   const Tensor act = make("expert_mlp.act", {R, F}, wgu.options());
   if (keep && bits == 16) m.gu = make("expert_mlp.gu", {R, 2 * F}, wgu.options());
@@ -722,9 +723,9 @@ Tensor stack_of(const Tensor& first, const OptTensor& second) {
 
 struct MlpNode : torch::autograd::Function<MlpNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& logits, const Tensor& first, const OptTensor& second,
-                               const Tensor& wd, int64_t k, int64_t capacity, const OptScoring& how, int64_t bits, bool poison) {
+                               const Tensor& wd, int64_t k, int64_t capacity, const OptScoring& how, const OptTensor& counts, int64_t bits, bool poison) {
     const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
-    Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, bits, true, Outputs{poison});
+    Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, counts, bits, true, Outputs{poison});
     keep_scoring(ctx, how);
     ctx->save_for_backward({x, logits, wgu, wdb, m.r.weights, m.r.experts, m.r.slots, m.r.offsets, m.r.rows, m.r.counts, m.gu, m.q, m.scales});
     ctx->saved_data["type"] = static_cast<int64_t>(wd.scalar_type());
@@ -737,7 +738,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     only_once("expert_mlp");
     const auto s = ctx->get_saved_variables();
     const Outputs make{ctx->saved_data["poison"].toBool()};
-    variable_list out(10);
+    variable_list out(11);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     c10::cuda::CUDAGuard guard(s[0].device());
     const Tensor daux = grads[1].defined() ? grads[1].to(torch::kFloat32) : grads[1];
@@ -763,7 +764,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
 };
 
 variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tensor& first, const OptTensor& second, const Tensor& wd, int64_t k,
-                         int64_t capacity, const PyScoring& scoring, int64_t bits, bool poison) {
+                         int64_t capacity, const PyScoring& scoring, const OptTensor& counts, int64_t bits, bool poison) {
   no_tangents("expert_mlp", x, given_logits, first, has(second) ? *second : Tensor(), wd);
   check_rows(x, "expert_mlp: x");
   check_rows(given_logits, "expert_mlp: logits");
@@ -789,16 +790,17 @@ variable_list expert_mlp(const Tensor& x, const Tensor& given_logits, const Tens
                     "expert_mlp: tensors on several GPUs");
   c10::cuda::CUDAGuard guard(x.device());
   const OptScoring how = check_scoring(scoring, logits, k, "expert_mlp");
+  if (has(counts)) check_ints(*counts, E, x, "expert_mlp: counts");
   const bool keep = at::GradMode::is_enabled() &&
                     (x.requires_grad() || logits.requires_grad() || first.requires_grad() || wd.requires_grad() ||
                      (pair && second->requires_grad()));
-  if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, how, bits, poison);
+  if (keep) return MlpNode::apply(x, logits, first, second, wd, k, capacity, how, counts, bits, poison);
   const Tensor wgu = stack_of(first, second), wdb = matrices(wd);
-  if (!how && runs_by_token(x, k, wgu, wdb)) {      // (the token kernels choose by logits)
+  if (!how && !has(counts) && runs_by_token(x, k, wgu, wdb)) {      // (the token kernels choose by logits and count nothing)
     const Overlap overlap;
     return mlp_by_token(x, logits, wgu, wdb, k, capacity, Outputs{poison});
   }
-  Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, bits, false, Outputs{poison});
+  Mlp m = mlp_fwd(x, logits, wgu, wdb, k, capacity, how, counts, bits, false, Outputs{poison});
   return {m.out, m.r.aux};
 }
 

@@ -5,7 +5,9 @@ so that the expert-parallel layer (``parallel/expert_parallel.py``) has a model 
 keeps the dense model's attention and norms and swaps the MLP for ``MoELayer``.  The blocks run the PyTorch path
 (``impl`` is fixed to "torch"); ``experts: "grouped"`` runs the feed-forwards on the sm_100a operators of ``ops/moe.py``
 instead of batched library products over padded buffers, and ``act_bits: 8`` keeps their gate and up in 8 bits between the
-passes.
+passes.  ``router`` ({"score", "groups", "top_groups", "normalize", "scale", "bias_rate"}) chooses experts by scores, with a bias that
+the Trainer moves after every step; ``embedding: "sorted"`` looks tokens up with ``ops/embedding.py``, whose gradient sums a
+token's rows in a fixed order, and ``embed_scale`` multiplies the rows.
 
 With ``mesh: {"dp": D, "ep": E}`` the Trainer calls ``shard_experts``: rank r of an ``ep`` group keeps experts
 [r E_total / E, (r + 1) E_total / E) of every layer, tokens travel to their experts' owners and back through the
@@ -17,7 +19,9 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from torchure_b200.core.collective import all_reduce
 from torchure_b200.models.qwen3 import Qwen3, RMSNorm
+from torchure_b200.ops.embedding import embedding
 from torchure_b200.parallel.expert_parallel import MoELayer
 
 
@@ -27,16 +31,21 @@ class Qwen3MoE(Qwen3):
                  capacity_factor: float = 2.0, aux_loss_coef: float = 0.01, ffn_dim: int | None = None,
                  norm_eps: float = 1e-6,
                  rope_theta: float = 1_000_000.0, qk_norm: bool = True, tie_embeddings: bool = True,
-                 impl: str = "torch", experts: str = "capacity", act_bits: int = 16):
+                 impl: str = "torch", experts: str = "capacity", act_bits: int = 16, router: dict | None = None,
+                 embedding: str = "torch", embed_scale: float = 1.0):
         super().__init__(num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, emb_dim=emb_dim,
                          head_dim=head_dim, vocab_size=vocab_size, ffn_dim=ffn_dim, norm_eps=norm_eps,
                          rope_theta=rope_theta, qk_norm=qk_norm, tie_embeddings=tie_embeddings, impl="torch")
+        if embedding not in ("torch", "sorted"):
+            raise ValueError(f'Qwen3MoE: the embedding is "torch" or "sorted", not {embedding!r}')
         width = moe_ffn_dim if moe_ffn_dim is not None else self.cfg["ffn_dim"]
         self.cfg.update(num_experts=num_experts, top_k=top_k, moe_ffn_dim=width, capacity_factor=capacity_factor,
-                        aux_loss_coef=aux_loss_coef, experts=experts, act_bits=act_bits)
+                        aux_loss_coef=aux_loss_coef, experts=experts, act_bits=act_bits, router=router,
+                        embedding=embedding, embed_scale=embed_scale)
         self.aux_loss_coef = aux_loss_coef
         for block in self.blocks:
-            block.ffn = MoELayer(emb_dim, width, num_experts, top_k, capacity_factor, experts=experts, act_bits=act_bits)
+            block.ffn = MoELayer(emb_dim, width, num_experts, top_k, capacity_factor, experts=experts, act_bits=act_bits,
+                                 router=router)
 
     @torch.no_grad()
     def init_weights(self, std: float = 0.02) -> None:
@@ -54,6 +63,27 @@ class Qwen3MoE(Qwen3):
         for b in self.blocks:
             b.gqa.o_proj.weight.mul_(scale)
             b.ffn.w_down.mul_(scale)
+
+    def embed(self, ids: torch.Tensor) -> torch.Tensor:
+        scale = self.cfg["embed_scale"]
+        if self.cfg["embedding"] == "sorted":
+            return embedding(ids, self.token_emb.weight, scale)
+        h = super().embed(ids)
+        return h if scale == 1.0 else h * scale
+
+    @torch.no_grad()
+    def balance_routers(self, mesh=None, dim: str | None = None) -> None:
+        """After a training step: every router's bias against the choices counted since the last call, over all ranks of `dim`."""
+        layers = [b.ffn for b in self.blocks if b.ffn.bias_rate]
+        if not layers:
+            return
+        counts = torch.stack([layer.router_counts for layer in layers])
+        if mesh is not None and mesh.size(dim) > 1:
+            wide = counts.long()
+            all_reduce(wide, mesh, dim, "sum")
+            counts = wide.clamp_max(2 ** 31 - 1).int()
+        for layer, mine in zip(layers, counts):
+            layer.balance(mine)
 
     def aux_loss(self) -> torch.Tensor:
         """Mean over the layers of the routers' load-balancing terms of the LAST forward pass; the objective adds

@@ -63,8 +63,9 @@ class Scoring(NamedTuple):
     scale: float = 1.0                # ... times this
 
 
-def _scoring(experts: int, top_k: int, score: str, bias, groups: int, top_groups: int, normalize: bool, scale: float):
-    """The ``Scoring`` of these arguments, or None where they ask for the plain choice by logits."""
+def scoring(experts: int, top_k: int, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1, top_groups: int = 0,
+            normalize: bool = True, scale: float = 1.0) -> Scoring | None:
+    """The ``Scoring`` of these arguments for a router of so many experts, or None where they ask for the plain choice by logits."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f'route: scores are "softmax" or "sigmoid", not {score!r}')
     if groups < 1 or experts % groups:
@@ -82,6 +83,9 @@ def _scoring(experts: int, top_k: int, score: str, bias, groups: int, top_groups
     if score == "softmax" and bias is None and groups == 1 and normalize and scale == 1.0:
         return None
     return Scoring(score, bias, groups, top_groups, bool(normalize), float(scale))
+
+
+_checked = scoring      # (where an argument has its name)
 
 
 def _native(how: Scoring | None):
@@ -105,7 +109,7 @@ def route(logits: torch.Tensor, top_k: int, capacity: int = 0, *, score: str = "
     scores over their sum.  A bias of -inf closes its expert to the choice."""
     how = None
     if not (score == "softmax" and bias is None and groups == 1 and top_groups == 0 and normalize and scale == 1.0) and logits.dim() == 2:
-        how = _scoring(logits.shape[1], top_k, score, bias, groups, top_groups, normalize, scale)
+        how = scoring(logits.shape[1], top_k, score, bias, groups, top_groups, normalize, scale)
     if not _plain(logits):
         return Routing(*_C().moe_route(logits, top_k, capacity, _native(how), debug.enabled()))
     if logits.dim() != 2 or not logits.is_floating_point():
@@ -167,14 +171,14 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> t
 
 
 def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.Tensor, top_k: int, capacity: int = 0,
-               act_bits: int = 16, scoring: Scoring | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+               act_bits: int = 16, scoring: Scoring | None = None, counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(out [T, D], aux_loss): every token through its ``top_k`` experts' SwiGLU feed-forwards, weighted by the router.
 
     x [T, D] bf16 or fp32 (the output's type), logits [T, E] as ``route`` takes them, ``w_gate_up`` [E, 2F, D] or the pair
     (w_gate, w_up) of [E, F, D], ``w_down`` [E, D, F]; matrices bf16 or fp32 (then rounded for the products, with fp32 gradients);
     D and F multiples of 8.  ``act_bits`` 8: gate and up are kept in 8 bits (``act8``) for the backward pass instead of bf16, which
     takes from them the gradients of gate and up and the activation, and with it the gradients of ``w_down`` and of the weights.
-    ``scoring``: the further arguments of ``route``.
+    ``scoring``: the further arguments of ``route``.  ``counts`` (int32 [E]): the choices made for each expert are added to it.
 
     On a GPU sums, weights and the weighted sum are fp32; what a product reads and writes between is bf16: the rows of x, the
     activation and, with more than 64 rows per expert on average, the down product's rows; in the backward pass the rows of the
@@ -183,12 +187,12 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.T
     stack is held for the backward pass; bf16 matrices as [E, 2F, D] are read where they lie."""
     first, second = w_gate_up if isinstance(w_gate_up, (tuple, list)) else (w_gate_up, None)
     if scoring is not None and logits.dim() == 2:
-        scoring = _scoring(logits.shape[1], top_k, *scoring)
+        scoring = _checked(logits.shape[1], top_k, *scoring)
     if not _plain(x, logits, first, w_down):
         if x.dim() != 2 or logits.dim() != 2:
             raise ValueError(f"expert_mlp: x [T, D] and logits [T, E] expected, got {tuple(x.shape)} and {tuple(logits.shape)}")
         out, aux = _C().expert_mlp(_rows(x), _rows(logits), first, second, w_down, top_k, capacity, _native(scoring),
-                                   act_bits, debug.enabled())
+                                   counts, act_bits, debug.enabled())
         return out, aux
     if x.dim() != 2 or logits.dim() != 2 or first.dim() != 3 or w_down.dim() != 3:
         raise ValueError("expert_mlp: x [T, D], logits [T, E], w_gate_up [E, 2F, D] and w_down [E, D, F] expected")
@@ -202,5 +206,7 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_gate_up, w_down: torch.T
     if first.shape != (E, 2 * f if second is None else f, D) or x.shape[1] != D or logits.shape != (x.shape[0], E):
         raise ValueError(f"expert_mlp: x {tuple(x.shape)}, logits {tuple(logits.shape)}, w_gate_up {tuple(first.shape)}, w_down "
                          f"{tuple(w_down.shape)} do not fit")
+    if counts is not None and (counts.shape != (E,) or counts.dtype != torch.int32):
+        raise ValueError(f"expert_mlp: counts int32 [{E}] expected, got {counts.dtype} {tuple(counts.shape)}")
     wgu = first if second is None else torch.cat([first, second], dim=1)
-    return oracle.expert_mlp(x, logits, wgu, w_down, top_k, capacity, act_bits, scoring)
+    return oracle.expert_mlp(x, logits, wgu, w_down, top_k, capacity, act_bits, scoring, counts)

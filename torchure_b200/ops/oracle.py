@@ -263,9 +263,11 @@ def combine(y, weights, slots):
     return (weights[..., None] * got).sum(1)
 
 
-def expert_mlp(x, logits, w_gate_up, w_down, k, capacity=0, act_bits=16, scoring=None):
+def expert_mlp(x, logits, w_gate_up, w_down, k, capacity=0, act_bits=16, scoring=None, counts=None):
     """(out, aux) in the operands' precision.  scoring: the further arguments of ``route_scored``."""
-    weights, _, slots, offsets, rows, _, aux = route(logits, k, capacity) if scoring is None else route_scored(logits, k, capacity, *scoring)
+    weights, _, slots, offsets, rows, made, aux = route(logits, k, capacity) if scoring is None else route_scored(logits, k, capacity, *scoring)
+    if counts is not None:
+        counts += made
     gu = grouped_linear(dispatch(x, rows, k), w_gate_up, offsets)
     act = swiglu_8bit(gu) if act_bits == 8 else swiglu_plain(gu)
     return combine(grouped_linear(act, w_down, offsets), weights.to(x.dtype), slots), aux

@@ -13,6 +13,9 @@ shuffle is the even-split ``all_to_all``.  Here:
   grouped by expert instead of batched library products, with ``act_bits=8`` gate and up kept in 8 bits for the backward pass.  The
   capacity drops the same choices (``capacity_factor`` 0: none are dropped).  Spread over a mesh axis the exchange keeps its padded
   buffers (with ``capacity_factor`` 0 a row for every token of the rank) and the grouped products run on what arrives.
+* ``router`` ({"score", "groups", "top_groups", "normalize", "scale", "bias_rate"}) chooses experts by scores (``ops/moe.py::route``).
+  With a ``bias_rate`` every expert has a bias for the choice, a buffer: ``balance`` moves it by that much against the choices
+  that training passes have counted since the last call.
 """
 
 from __future__ import annotations
@@ -39,7 +42,7 @@ class _AllToAll(torch.autograd.Function):
 
 class MoELayer(nn.Module):
     def __init__(self, hidden: int, ffn: int, num_experts: int, top_k: int = 2, capacity_factor: float = 2.0,
-                 mesh=None, dim: str = "ep", experts: str = "capacity", act_bits: int = 16):
+                 mesh=None, dim: str = "ep", experts: str = "capacity", act_bits: int = 16, router: dict | None = None):
         super().__init__()
         if experts not in ("capacity", "grouped"):
             raise ValueError(f'MoELayer: experts are "capacity" or "grouped", not {experts!r}')
@@ -52,6 +55,17 @@ class MoELayer(nn.Module):
         self.r = mesh.coordinate(dim) if mesh is not None else 0
         assert num_experts % self.n == 0, "experts must divide evenly over the ep axis"
         self.local_E = num_experts // self.n
+        how = dict(router or {})
+        self.bias_rate = float(how.pop("bias_rate", 0.0))
+        if not 0.0 <= self.bias_rate < float("inf"):
+            raise ValueError(f"MoELayer: bias_rate {self.bias_rate}")
+        if unknown := set(how) - {"score", "groups", "top_groups", "normalize", "scale"}:
+            raise ValueError(f"MoELayer: unknown router keys {sorted(unknown)}")
+        self.scoring = moe.scoring(num_experts, top_k, bias=torch.zeros(num_experts) if self.bias_rate else None, **how)
+        if self.bias_rate:
+            self.scoring = self.scoring._replace(bias=None)
+            self.register_buffer("router_bias", torch.zeros(num_experts))
+            self.register_buffer("router_counts", torch.zeros(num_experts, dtype=torch.int32), persistent=False)
         self.router = nn.Linear(hidden, num_experts, bias=False)
         self.aux_loss = None
         self.w_gate = nn.Parameter(torch.empty(self.local_E, ffn, hidden))
@@ -80,6 +94,23 @@ class MoELayer(nn.Module):
             self.w_up.copy_(w_up[lo:lo + self.local_E])
             self.w_down.copy_(w_down[lo:lo + self.local_E])
 
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kw) -> None:
+        if self.bias_rate:      # weights of a layer without a bias: it starts at zero
+            state_dict.setdefault(prefix + "router_bias", torch.zeros_like(self.router_bias))
+        super()._load_from_state_dict(state_dict, prefix, *args, **kw)
+
+    @torch.no_grad()
+    def balance(self, counts: torch.Tensor | None = None) -> None:
+        """Move the bias against what was counted (``counts``: the same summed over ranks) and start counting anew."""
+        moe.balance_bias_(self.router_bias, self.router_counts if counts is None else counts, self.bias_rate)
+        self.router_counts.zero_()
+
+    def _how(self):
+        """(scoring with the bias as it is, where to count choices), each None where there is none."""
+        if not self.bias_rate:
+            return self.scoring, None
+        return self.scoring._replace(bias=self.router_bias.float()), self.router_counts if self.training and torch.is_grad_enabled() else None
+
     def capacity(self, tokens: int) -> int:
         """Rows of an expert's buffer for ``tokens`` tokens."""
         if self.experts == "grouped" and self.cf <= 0:
@@ -105,19 +136,26 @@ class MoELayer(nn.Module):
         shape = x.shape
         x = x.reshape(-1, self.hidden)
         T = x.shape[0]
+        scoring, counts = self._how()
         if self.experts == "grouped" and self.n == 1:
             out, self.aux_loss = moe.expert_mlp(x, self.router(x), (self.w_gate, self.w_up), self.w_down, self.k,
-                                                self.capacity(T) if self.cf > 0 else 0, self.act_bits)
+                                                self.capacity(T) if self.cf > 0 else 0, self.act_bits, scoring, counts)
             return out.view(shape)
         C = self.capacity(T)
-        probs = F.softmax(self.router(x).float(), dim=-1)
-        gate, expert = probs.topk(self.k, dim=-1)                 # (T, k)
-        gate = gate / gate.sum(-1, keepdim=True)
-        # load-balancing term (Switch Transformer): E * sum_e (share of the assignments that went to e) * (mean router
-        # probability of e); 1 when routing is uniform, larger when experts are over-subscribed.  Over this rank's
-        # tokens; the owner of the loss reads `aux_loss` after the forward pass
-        share = F.one_hot(expert, self.E).sum(dim=(0, 1)).float() / (T * self.k)
-        self.aux_loss = self.E * (share * probs.mean(0)).sum()
+        if scoring is not None:
+            r = moe.route(self.router(x), self.k, **scoring._asdict())
+            gate, expert, self.aux_loss = r.weights, r.experts.long(), r.aux_loss
+            if counts is not None:
+                counts += r.counts
+        else:
+            probs = F.softmax(self.router(x).float(), dim=-1)
+            gate, expert = probs.topk(self.k, dim=-1)                 # (T, k)
+            gate = gate / gate.sum(-1, keepdim=True)
+            # load-balancing term (Switch Transformer): E * sum_e (share of the assignments that went to e) * (mean router
+            # probability of e); 1 when routing is uniform, larger when experts are over-subscribed.  Over this rank's
+            # tokens; the owner of the loss reads `aux_loss` after the forward pass
+            share = F.one_hot(expert, self.E).sum(dim=(0, 1)).float() / (T * self.k)
+            self.aux_loss = self.E * (share * probs.mean(0)).sum()
         # slot of every (token, choice) inside its expert's buffer; choices beyond the capacity are dropped
         flat_e = expert.reshape(-1)
         onehot = F.one_hot(flat_e, self.E)

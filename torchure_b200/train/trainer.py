@@ -520,6 +520,8 @@ class Trainer:
         if hasattr(self.ddp, "mark_updated"):
             self.ddp.mark_updated()
         self.optimizer.zero_grad()
+        if hasattr(self.model, "balance_routers"):
+            self.model.balance_routers(self.mesh, self.grad_axis)
         if slot is not None:
             self.ddp.reducer.comm.all_reduce_symmetric_(slot, "avg", blocks=1)
             loss = slot[0].clone()
@@ -599,6 +601,7 @@ class Trainer:
             torch._foreach_mul_(expert_grads + shared_grads, torch.clamp(self.max_norm / (grad_norm + 1e-6), max=1.0))
         self.optimizer.step()
         self.optimizer.zero_grad()
+        self.model.balance_routers(self.mesh, self.grad_axis)
         self._loss_averaged = False
         return loss, grad_norm
 
