@@ -624,9 +624,9 @@ int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, i
   const auto share = [&](int i) {
     z.lo = done;
     z.hi = done = i + 1 == kernels ? bytes : bytes * (i + 1) / kernels / 16 * 16;
-    int64_t ctas = (z.hi - z.lo + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
-    if (ctas > 148 * 2) ctas = 148 * 2;
-    if (p.small && ctas > 147) ctas = 147;      // (the sort's shared memory leaves an SM one CTA)
+    // 256 KB for each, so that SMs which are done take more (147 CTAs that share it out: 105 us for 622 MB, so 89), 64 KB where that leaves SMs idle
+    const int64_t n = z.hi - z.lo, idle = (n + (1 << 16) - 1) >> 16, many = (n + (1 << 18) - 1) >> 18;
+    const int64_t ctas = idle < 147 ? idle : many < 147 ? 147 : many;
     return static_cast<int>(ctas < 1 ? 1 : ctas);
   };
   const int smem = 4 * rank_ints(a.bins) + (p.small ? 16 * a.T : 0);
