@@ -118,6 +118,28 @@ def test_ids_outside_the_table_on_the_cpu():
             embedding(torch.tensor(ids), torch.randn(5, 8))
 
 
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("D", [1, 7, 8, 33])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_broadcast_rows_and_gradients(device, D, dtype):
+    """One row expanded to a table, and gradients that are one row, or one number, for all tokens."""
+    ids, table = problem(70, 12, D, dtype, seed=3)
+    row = table[:1].to(device, copy=True).requires_grad_()
+    wide = row.expand(12, D)
+    one = torch.randn(D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    for dout in (one.expand(70, D), one[:1].expand(70, D)):
+        out = embedding(ids.to(device), wide, 2.0)
+        w = table.to(device, copy=True).requires_grad_()
+        full = embedding(ids.to(device), w, 2.0)
+        dtable, = torch.autograd.grad(full, w, dout.to(device))
+        check(ids, table, dout, full, dtable, 2.0)
+        check(ids, table[:1].expand(12, D), dout, out, dtable, 2.0)
+        drow, = torch.autograd.grad(out, row, dout.to(device))
+        assert drow.shape == (1, D)
+    # (strides that a reshape keeps)
+    assert torch.equal(embedding(ids.to(device)[:0], wide), wide[:0])
+
+
 @pytest.mark.gpu
 def test_operands_on_one_gpu():
     with pytest.raises(ValueError):

@@ -83,8 +83,8 @@ Tensor embedding(const Tensor& ids, const Tensor& table, double scale, c10::opti
   TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1, "embedding: a table [rows, width] expected, got ", table.sizes());
   TORCH_CHECK_VALUE(table.is_cuda() && ids.device() == table.device(), "embedding: ids on ", ids.device(), " and a table on ", table.device());
   const int64_t V = table.size(0);
-  TORCH_CHECK_VALUE(ids.numel() <= 1ll << 30 && V <= 1ll << 30 && table.size(1) <= 1 << 20, "embedding: ", ids.numel(), " tokens, a table of ",
-                    table.sizes(), ": more than 2^30 tokens or rows, or 2^20 columns, are not supported");
+  TORCH_CHECK_VALUE(ids.numel() <= 1ll << 30 && V <= 1ll << 30 && table.size(1) <= 1 << 16, "embedding: ", ids.numel(), " tokens, a table of ",
+                    table.sizes(), ": more than 2^30 tokens or rows, or 2^16 columns, are not supported");
   TORCH_CHECK_VALUE(!padding || (*padding >= -V && *padding < V), "embedding: padding_idx ", padding.value_or(0), " in a table of ", V, " rows");
   TORCH_CHECK_VALUE(std::isfinite((float)scale), "embedding: scale ", scale);
   c10::cuda::CUDAGuard guard(table.device());

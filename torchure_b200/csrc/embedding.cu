@@ -549,7 +549,7 @@ int launch_rows(const I* ids, const S* table, int64_t ld, O* out, float scale, i
   const auto run = [&](auto* kernel) { return launch_code(launch_pdl(kernel, grid, block, 0, stream, ids, table, ld, out, scale, T, V, D)); };
   if (vec) return run(embedding_rows_kernel<I, S, O, kRowsFours>);
   if constexpr (sizeof(S) == 2 && sizeof(O) == 2) {
-    if (aligned(table, 4) && aligned(out, 4)) return run(embedding_rows_kernel<I, S, O, kRowsPairs>);
+    if (aligned(table, 4) && aligned(out, 4) && ld >= D) return run(embedding_rows_kernel<I, S, O, kRowsPairs>);
   }
   return run(embedding_rows_kernel<I, S, O, kRowsOnes>);
 }
@@ -561,7 +561,7 @@ int launch_sums(const SumArgs& a, int chunks, const S* dout, O* dtable, cudaStre
     return launch_code(launch_pdl(kernel, dim3(chunks, (a.D + width * 4 - 1) / (width * 4)), dim3(width), 0, stream, a, dout, dtable));
   };
   constexpr ColsBy kWords = sizeof(S) == 2 ? kPairs : kOnes;
-  const bool words = sizeof(S) == 2 && aligned(dout, 4), wide = a.D > 256;      // narrow rows take CTAs of two warps
+  const bool words = sizeof(S) == 2 && aligned(dout, 4) && a.ld >= a.D, wide = a.D > 256;      // narrow rows take CTAs of two warps
   int rc;
   if (vec) rc = wide ? run(segment_sum_kernel<S, O, kFours, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kFours, 64>, 64);
   else if (words) rc = wide ? run(segment_sum_kernel<S, O, kWords, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kWords, 64>, 64);
@@ -575,7 +575,7 @@ int launch_sums(const SumArgs& a, int chunks, const S* dout, O* dtable, cudaStre
 }
 
 bool fits(int64_t T, int64_t V, int D) {
-  return T >= 1 && T <= (1ll << 30) && V >= 1 && V <= (1ll << 30) && D >= 1 && D <= (1 << 20);
+  return T >= 1 && T <= (1ll << 30) && V >= 1 && V <= (1ll << 30) && D >= 1 && D <= (1 << 16);
 }
 
 }  // namespace
