@@ -393,6 +393,32 @@ def test_replayed_steps_equal_eager_ones():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 64, 65, 300])
+def test_few_and_many_tensors(count):
+    """Up to 64 tensors' addresses travel with the launch, those of more lie in a table; either way other tensors of the same sizes are other tensors."""
+    sets = []
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        shapes = [(int(torch.randint(1, 700, (1,), generator=g)),) for _ in range(1)] + [(129 + i % 40,) for i in range(count - 1)]
+        shapes[0] = (500,)
+        s = dict(params=[torch.randn(n, generator=g) for n in shapes], grads=[torch.randn(n, generator=g) for n in shapes])
+        s["ms"], s["vs"] = ([torch.zeros(n, dtype=torch.uint8) for n in shapes] for _ in range(2))
+        s["mscales"], s["vscales"] = ([torch.zeros(-(-n[0] // 128)) for n in shapes] for _ in range(2))
+        s["shadows"] = [None] * count
+        sets.append((s, {n: [None if t is None else t.cuda() for t in ts] for n, ts in s.items()}))
+    for t in (1, 2):
+        for a, b in sets:
+            step(a, plain, step=t, seed=t)
+            step(b, multi_tensor.adamw8_step, step=t, seed=t)
+    for a, b in sets:
+        for name in ("ms", "mscales", "vs", "vscales"):
+            assert all(torch.equal(x, y.cpu()) for x, y in zip(a[name], b[name])), name
+        for signed, codes, scales in ((True, "ms", "mscales"), (False, "vs", "vscales")):
+            got = multi_tensor.state8_values(b[codes], b[scales], signed)
+            assert all(torch.equal(x.cpu(), oracle.state8_decode(c, sc, signed)) for x, c, sc in zip(got, a[codes], a[scales]))
+
+
+@pytest.mark.gpu
 def test_on_another_stream():
     a, b = problem(6, "cuda"), problem(6, "cuda")
     side = torch.cuda.Stream()

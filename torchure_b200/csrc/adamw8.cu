@@ -153,6 +153,20 @@ __device__ __forceinline__ float update(float p, float m, float v, const Adam8Sc
   return fmaf(-s.step_size, m * over, p * s.decay);
 }
 
+// The addresses of up to kState8ByValue tensors as an argument of the kernel: new gradients, at new addresses every step, then cost no copy to the
+// device (30 us of the host's time for a pinned one).  COLUMNS 0: they lie on the device.
+template <int COLUMNS>
+struct Addresses {
+  int64_t p[COLUMNS * kState8ByValue];
+};
+template <>
+struct Addresses<0> {};
+template <int COLUMNS>
+__device__ __forceinline__ int64_t address(const State8List& t, const Addresses<COLUMNS>& a, int column, int ti) {
+  if constexpr (COLUMNS == 0) return t.ptrs[column * t.n_tensors + ti];
+  else return a.p[column * t.n_tensors + ti];
+}
+
 struct Four {
   float p[4], g[4];
   uint32_t m, v;           // codes
@@ -286,8 +300,10 @@ __device__ __forceinline__ void whole_chunk(const Chunk& c, int count, const Ada
   }
 }
 
+template <int COLUMNS>
 __global__ void __launch_bounds__(kThreads, 4)
-adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale, const float* __restrict__ hyper) {
+adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale, const float* __restrict__ hyper,
+              const __grid_constant__ Addresses<COLUMNS> addresses) {
   pdl_wait();
   pdl_launch_dependents();
   uint32_t key = s.key;
@@ -297,17 +313,17 @@ adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale
     s.decay = hyper[2];
     key = __float_as_uint(hyper[3]);
   }
-  const int ti = t.block_tensor[blockIdx.x], n_tensors = t.n_tensors;
+  const int ti = t.block_tensor[blockIdx.x];
   const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * t.chunk;
   const int count = static_cast<int>(lo + t.chunk < n ? t.chunk : n - lo);
-  const int64_t* ptr = t.ptrs + ti;
-  float* p = reinterpret_cast<float*>(ptr[0]) + lo;
-  const char* g = reinterpret_cast<const char*>(ptr[n_tensors]);
-  uint8_t* m = reinterpret_cast<uint8_t*>(ptr[2 * n_tensors]) + lo;
-  uint8_t* v = reinterpret_cast<uint8_t*>(ptr[3 * n_tensors]) + lo;
-  float* m_scale = reinterpret_cast<float*>(ptr[4 * n_tensors]) + lo / kStateBlock;
-  float* v_scale = reinterpret_cast<float*>(ptr[5 * n_tensors]) + lo / kStateBlock;
-  __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(ptr[6 * n_tensors]);
+  const auto ptr = [&](int column) { return address<COLUMNS>(t, addresses, column, ti); };
+  float* p = reinterpret_cast<float*>(ptr(0)) + lo;
+  const char* g = reinterpret_cast<const char*>(ptr(1));
+  uint8_t* m = reinterpret_cast<uint8_t*>(ptr(2)) + lo;
+  uint8_t* v = reinterpret_cast<uint8_t*>(ptr(3)) + lo;
+  float* m_scale = reinterpret_cast<float*>(ptr(4)) + lo / kStateBlock;
+  float* v_scale = reinterpret_cast<float*>(ptr(5)) + lo / kStateBlock;
+  __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(ptr(6));
   const bool g16 = (t.flags[ti] & 1) != 0;
   g += lo * (g16 ? 2 : 4);
   if (sh) sh += lo;
@@ -349,17 +365,18 @@ adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale
 }
 
 // ptrs: codes, scales, and the values' place in `all`, in elements
-template <class T, bool SIGNED>
+template <class T, bool SIGNED, int COLUMNS>
 __global__ void __launch_bounds__(kThreads)
-state8_values_kernel(State8List t, T* __restrict__ all) {
+state8_values_kernel(State8List t, T* __restrict__ all, const __grid_constant__ Addresses<COLUMNS> addresses) {
   pdl_wait();
   pdl_launch_dependents();
   const int ti = t.block_tensor[blockIdx.x];
   const int64_t n = t.numel[ti], lo = static_cast<int64_t>(t.block_chunk[blockIdx.x]) * t.chunk;
   const int64_t hi = lo + t.chunk < n ? lo + t.chunk : n;
-  const uint8_t* codes = reinterpret_cast<const uint8_t*>(t.ptrs[ti]);
-  const float* scales = reinterpret_cast<const float*>(t.ptrs[t.n_tensors + ti]);
-  T* out = all + t.ptrs[2 * t.n_tensors + ti];
+  const auto ptr = [&](int column) { return address<COLUMNS>(t, addresses, column, ti); };
+  const uint8_t* codes = reinterpret_cast<const uint8_t*>(ptr(0));
+  const float* scales = reinterpret_cast<const float*>(ptr(1));
+  T* out = all + ptr(2);
   const bool vc = on(codes, 4), vo = on(out, 4 * sizeof(T));
   if (hi - lo == t.chunk && on(codes, 8) && on(out, 16)) {      // eight values a thread: whole lines in and out
     const int rounds = t.chunk / (kThreads * 8);
@@ -414,26 +431,47 @@ state8_values_kernel(State8List t, T* __restrict__ all) {
   }
 }
 
+template <int COLUMNS>
+Addresses<COLUMNS> addresses_of(const State8List& t) {
+  Addresses<COLUMNS> a{};
+  if constexpr (COLUMNS > 0)
+    for (int i = 0; i < COLUMNS * t.n_tensors; ++i) a.p[i] = t.host_ptrs[i];
+  return a;
+}
+
+bool fits(const State8List& t) {
+  return (t.chunk == kChunkElems || t.chunk == kSmallChunk) && (t.host_ptrs == nullptr || t.n_tensors <= kState8ByValue);
+}
+
+template <int COLUMNS>
+int launch_step(const State8List& t, const Adam8Scalars& s, const float* grad_scale, const float* hyper, cudaStream_t stream) {
+  constexpr int kBytes = kThreads / 32 * kStages * static_cast<int>(sizeof(Stage));
+  if (!ensure_dynamic_smem(reinterpret_cast<const void*>(adamw8_kernel<COLUMNS>), kBytes)) return -20;
+  return launch_code(launch_pdl(adamw8_kernel<COLUMNS>, dim3(t.n_blocks), dim3(kThreads), kBytes, stream, t, s, grad_scale, hyper,
+                                addresses_of<COLUMNS>(t)));
+}
+
+template <int COLUMNS, class T>
+int launch_values(const State8List& t, bool is_signed, T* out, cudaStream_t stream) {
+  const auto run = [&](auto* kernel) {
+    return launch_code(launch_pdl(kernel, dim3(t.n_blocks), dim3(kThreads), 0, stream, t, out, addresses_of<COLUMNS>(t)));
+  };
+  return is_signed ? run(state8_values_kernel<T, true, COLUMNS>) : run(state8_values_kernel<T, false, COLUMNS>);
+}
+
 }  // namespace
 
 int adamw8_multi(const State8List& t, const Adam8Scalars& s, const float* grad_scale, const float* hyper, cudaStream_t stream) {
   if (t.n_blocks <= 0) return 0;
-  if (t.chunk != kChunkElems && t.chunk != kSmallChunk) return -1;
-  constexpr int kBytes = kThreads / 32 * kStages * static_cast<int>(sizeof(Stage));
-  if (!ensure_dynamic_smem(reinterpret_cast<const void*>(adamw8_kernel), kBytes)) return -20;
-  return launch_code(launch_pdl(adamw8_kernel, dim3(t.n_blocks), dim3(kThreads), kBytes, stream, t, s, grad_scale, hyper));
+  if (!fits(t)) return -1;
+  return t.host_ptrs ? launch_step<7>(t, s, grad_scale, hyper, stream) : launch_step<0>(t, s, grad_scale, hyper, stream);
 }
 
 int state8_values_multi(const State8List& t, bool is_signed, void* out, bool bf16, cudaStream_t stream) {
   if (t.n_blocks <= 0) return 0;
-  if (t.chunk != kChunkElems && t.chunk != kSmallChunk) return -1;
-  const dim3 grid(t.n_blocks), block(kThreads);
-  const auto run = [&](auto* kernel, auto* to) { return launch_code(launch_pdl(kernel, grid, block, 0, stream, t, to)); };
-  if (bf16)
-    return is_signed ? run(state8_values_kernel<__nv_bfloat16, true>, static_cast<__nv_bfloat16*>(out))
-                     : run(state8_values_kernel<__nv_bfloat16, false>, static_cast<__nv_bfloat16*>(out));
-  return is_signed ? run(state8_values_kernel<float, true>, static_cast<float*>(out))
-                   : run(state8_values_kernel<float, false>, static_cast<float*>(out));
+  if (!fits(t)) return -1;
+  const auto run = [&](auto* to) { return t.host_ptrs ? launch_values<3>(t, is_signed, to, stream) : launch_values<0>(t, is_signed, to, stream); };
+  return bf16 ? run(static_cast<__nv_bfloat16*>(out)) : run(static_cast<float*>(out));
 }
 
 }  // namespace tb

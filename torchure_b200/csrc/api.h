@@ -142,8 +142,10 @@ constexpr int kChunkElems = 16384;
 // The same with as many pointer columns as the operation has, one after the other (adamw8.cu).  p, grad (flag bit 0: bf16), codes and scales of
 // the moments (m, v codes, then m, v scales) and the optional bf16 shadow; scales have one fp32 value for kStateBlock codes.
 constexpr int kStateBlock = 128;
+constexpr int kState8ByValue = 64;
 struct State8List {
-  const int64_t* ptrs;
+  const int64_t* ptrs;        // on the device
+  const int64_t* host_ptrs;   // or, where this is given, on the host: n_tensors <= kState8ByValue, they travel with the launch
   const int64_t* numel;
   const int32_t* flags;
   const int32_t* block_tensor;

@@ -305,8 +305,8 @@ using Tensors = std::vector<torch::Tensor>;
 using OptTensors = std::vector<c10::optional<torch::Tensor>>;
 
 tb::State8List as_state8(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt,
-                         const torch::Tensor& bc, int64_t chunk) {
-  return {ptrs.data_ptr<int64_t>(), numel.data_ptr<int64_t>(), flags.data_ptr<int32_t>(), bt.data_ptr<int32_t>(), bc.data_ptr<int32_t>(),
+                         const torch::Tensor& bc, int64_t chunk, const std::vector<int64_t>& host_ptrs) {
+  return {ptrs.data_ptr<int64_t>(), numel.numel() <= tb::kState8ByValue && !host_ptrs.empty() ? host_ptrs.data() : nullptr, numel.data_ptr<int64_t>(), flags.data_ptr<int32_t>(), bt.data_ptr<int32_t>(), bc.data_ptr<int32_t>(),
           (int)numel.numel(), (int)bt.numel(), (int)chunk};
 }
 
@@ -370,7 +370,7 @@ std::tuple<std::vector<int64_t>, std::vector<int64_t>> state8_columns(const Tens
 }
 
 void adamw8_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt, const torch::Tensor& bc,
-                  int64_t chunk, double beta1, double beta2, double eps, double step_size, double root, double decay, int64_t key,
+                  int64_t chunk, const std::vector<int64_t>& host_ptrs, double beta1, double beta2, double eps, double step_size, double root, double decay, int64_t key,
                   c10::optional<torch::Tensor> grad_scale, bool maximize, c10::optional<torch::Tensor> hyper) {
   TORCH_CHECK(!hyper || (hyper->is_cuda() && hyper->scalar_type() == torch::kFloat32 && hyper->numel() >= 4), "adamw8_step: hyper");
   TORCH_CHECK_VALUE(!grad_scale || (grad_scale->device() == ptrs.device() && grad_scale->scalar_type() == torch::kFloat32 && grad_scale->numel() == 1),
@@ -378,18 +378,19 @@ void adamw8_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const t
   const tb::Adam8Scalars s{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)step_size, (float)root,
                            (float)decay, (uint32_t)key, maximize ? 1 : 0};
   c10::cuda::CUDAGuard guard(ptrs.device());
-  const int rc = tb::adamw8_multi(as_state8(ptrs, numel, flags, bt, bc, chunk), s, opt_ptr<float>(grad_scale), opt_ptr<float>(hyper), cur_stream());
+  const int rc = tb::adamw8_multi(as_state8(ptrs, numel, flags, bt, bc, chunk, host_ptrs), s, opt_ptr<float>(grad_scale), opt_ptr<float>(hyper), cur_stream());
   TORCH_CHECK(rc == 0, "adamw8_step failed with code ", rc);
 }
 
 // The values of all tensors, a view of one buffer for each
 Tensors state8_values_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt,
-                            const torch::Tensor& bc, int64_t chunk, const Tensors& codes, bool is_signed, bool bf16) {
+                            const torch::Tensor& bc, int64_t chunk, const std::vector<int64_t>& host_ptrs, const Tensors& codes, bool is_signed,
+                            bool bf16) {
   c10::cuda::CUDAGuard guard(ptrs.device());
   int64_t total = 0;
   for (const auto& c : codes) total += (c.numel() + 7) / 8 * 8;
   const auto all = torch::empty({total}, codes[0].options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
-  const int rc = tb::state8_values_multi(as_state8(ptrs, numel, flags, bt, bc, chunk), is_signed, all.data_ptr(), bf16, cur_stream());
+  const int rc = tb::state8_values_multi(as_state8(ptrs, numel, flags, bt, bc, chunk, host_ptrs), is_signed, all.data_ptr(), bf16, cur_stream());
   TORCH_CHECK(rc == 0, "state8_values failed with code ", rc);
   Tensors out;
   out.reserve(codes.size());

@@ -634,6 +634,11 @@ route_scored_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* _
   const uint32_t mask = group_mask<LANES>(lane);
   const float pull = daux ? *daux * static_cast<float>(E) / static_cast<float>(n_tokens) : 0.f;
   const float per = 1.f / (static_cast<float>(n_tokens) * static_cast<float>(k));
+  __shared__ float rows[GROUPS][LANES * VALS];
+  float* row = rows[tid / LANES];
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) row[v * LANES + gl] = 0.f;
+  __syncwarp(mask);
   float share[VALS];
 #pragma unroll
   for (int v = 0; v < VALS; ++v) share[v] = v * LANES + gl < E ? static_cast<float>(counts[v * LANES + gl]) * per : 0.f;
@@ -691,14 +696,15 @@ route_scored_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* _
       else d -= q * inner;
       x[v] = odd ? __uint_as_float(0x7fffffffu) : d;
     }
-    if (dweights) {
-      for (int j = 0; j < k; ++j) {
-        const float gj = __shfl_sync(mask, g, j, LANES);
-        const int ej = __shfl_sync(mask, e_j, j, LANES);
+    if (dweights) {      // each choice's share to its expert's thread, through the token's row in shared memory
+      const bool gives = e_j >= 0 && e_j < E;
+      if (gives) row[e_j] = g;
+      __syncwarp(mask);
 #pragma unroll
-        for (int v = 0; v < VALS; ++v)
-          if (ej == v * LANES + gl) x[v] += gj;
-      }
+      for (int v = 0; v < VALS; ++v) x[v] += row[v * LANES + gl];
+      __syncwarp(mask);
+      if (gives) row[e_j] = 0.f;
+      __syncwarp(mask);
     }
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {

@@ -28,7 +28,8 @@ def available() -> bool:
     return ops.available()
 
 
-STATE_BLOCK = oracle.STATE8_BLOCK      # values of a moment in 8 bits that share a scale
+BY_VALUE = 64
+_NO_ADDRESSES = (0,)
 
 
 def _addresses(columns) -> tuple:
@@ -42,7 +43,7 @@ class TensorTable:
                  ptrs: tuple | None = None, like: "TensorTable | None" = None, chunk: int = CHUNK):
         """columns: up to 5 equally long tensor lists (None entries become null pointers).  `ptrs`: their addresses when
         the caller has them already.  `like`: a table of the same sizes and flags made on this stream, whose device
-        copies of everything but the addresses are shared: fresh gradients then cost one upload instead of five.  `chunk`:
+        copies of everything but the addresses are shared: fresh gradients then cost one upload instead of two.  `chunk`:
         elements of a thread block."""
         n = len(columns[0])
         assert n > 0 and all(len(c) == n for c in columns)
@@ -62,18 +63,24 @@ class TensorTable:
             chunks = [(ne + chunk - 1) // chunk for ne in numel]
             bt = np.repeat(np.arange(n, dtype=np.int32), chunks)
             bc = np.concatenate([np.arange(c, dtype=np.int32) for c in chunks]) if chunks else np.zeros(0, np.int32)
-            sizes = [torch.tensor(numel, dtype=torch.int64),
-                     torch.tensor(flags if flags is not None else [0] * n, dtype=torch.int32),
-                     torch.from_numpy(bt), torch.from_numpy(bc)]
-            self.sizes = [upload(h) for h in sizes]
+            # one upload (in a graph one node): the element counts in 64 bits, then flags, tensors and chunks in 32
+            ints = np.concatenate([np.asarray(flags if flags is not None else [0] * n, dtype=np.int32), bt, bc,
+                                   np.zeros((n + 2 * len(bt)) % 2, np.int32)])
+            self.sizes = [upload(torch.from_numpy(np.concatenate([np.asarray(numel, dtype=np.int64), ints.view(np.int64)])))]
+            both = self.sizes[0][1]
+            self.numel, ints = both[:n], both[n:].view(torch.int32)
+            self.flags, self.bt, self.bc = ints[:n], ints[n:n + len(bt)], ints[n + len(bt):n + 2 * len(bt)]
         else:
             self.sizes = like.sizes
-        self.numel, self.flags, self.bt, self.bc = (d for _, d in self.sizes)
-        self.host_ptrs, self.ptrs = upload(torch.tensor(self.key, dtype=torch.int64))
+            self.numel, self.flags, self.bt, self.bc = like.numel, like.flags, like.bt, like.bc
+        if self.key == _NO_ADDRESSES:
+            self.host_ptrs, self.ptrs = None, self.numel
+        else:
+            self.host_ptrs, self.ptrs = upload(torch.tensor(self.key, dtype=torch.int64))
 
     def host(self) -> list[torch.Tensor]:
         """The staging buffers the uploads read."""
-        return [h for h, _ in self.sizes] + [self.host_ptrs]
+        return [h for h, _ in self.sizes] + ([] if self.host_ptrs is None else [self.host_ptrs])
 
     def args(self):
         return self.ptrs, self.numel, self.flags, self.bt, self.bc
@@ -165,6 +172,14 @@ def _chunk8(numel) -> int:
     return CHUNK // 4 if sum(numel) < 1 << 24 else CHUNK
 
 
+def _table8(tag: str, first, flags, ptrs, numel, chunk):
+    """(table, addresses that travel with the launch): up to BY_VALUE tensors' addresses are an argument of the kernel and the table holds sizes
+    only, so that it is made once; more lie on the device, in the table."""
+    if len(numel) <= BY_VALUE:
+        return _table(tag + " sizes", [first], flags, _NO_ADDRESSES, tuple(numel), chunk), ptrs
+    return _table(tag, [first], flags, tuple(ptrs), tuple(numel), chunk), []
+
+
 def adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed=0) -> tuple[float, float, float, int]:
     """What an 8-bit AdamW step takes of its step: lr / (1 - beta1^t), (1 - beta2^t)^-1/2, 1 - lr weight_decay, the key of its random bits."""
     return lr / (1.0 - beta1 ** step), (1.0 - beta2 ** step) ** -0.5, 1.0 - lr * weight_decay, oracle.state8_key(seed, step)
@@ -187,10 +202,10 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
         return
     ptrs, numel, flags = ops.ext().adamw8_columns(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, shadows)
     chunk = _chunk8(numel)
-    tab = _table("adamw8", [params], flags, tuple(ptrs), tuple(numel), chunk)
+    tab, ptrs = _table8("adamw8", params, flags, ptrs, numel, chunk)
     size, root, decay, key = adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed)
     gs = grad_scale.to(torch.float32) if grad_scale is not None else None
-    ops.ext().adamw8_multi(*tab.args(), chunk, beta1, beta2, eps, size, root, decay, key, gs, maximize, hyper)
+    ops.ext().adamw8_multi(*tab.args(), chunk, ptrs, beta1, beta2, eps, size, root, decay, key, gs, maximize, hyper)
     ops.count_launch()
 
 
@@ -204,8 +219,8 @@ def state8_values(codes, scales, signed: bool, dtype=torch.float32) -> list[torc
         return [oracle.state8_decode(c, s, signed).to(dtype) for c, s in zip(codes, scales, strict=True)]
     ptrs, numel = ops.ext().state8_columns(codes, scales)
     chunk = _chunk8(numel)
-    tab = _table("state8+" if signed else "state8", [codes], None, tuple(ptrs), tuple(numel), chunk)
-    out = ops.ext().state8_values_multi(*tab.args(), chunk, codes, signed, dtype == torch.bfloat16)
+    tab, ptrs = _table8("state8+" if signed else "state8", codes, None, ptrs, numel, chunk)
+    out = ops.ext().state8_values_multi(*tab.args(), chunk, ptrs, codes, signed, dtype == torch.bfloat16)
     ops.count_launch()
     return out
 
