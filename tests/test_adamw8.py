@@ -204,6 +204,41 @@ def test_not_finite_gradients_stay_in_their_block():
 
 
 @pytest.mark.gpu
+def test_a_second_moment_that_overflows():
+    """The step itself divides by infinity; the block's second moment is NaN from then on, and the next step's parameters say so."""
+    a, b = problem(8, "cpu"), problem(8, "cuda")
+    for s in (a, b):
+        s["grads"][8][0, 5] = 1e25
+    for t in (1, 2):
+        step(a, plain, step=t)
+        step(b, multi_tensor.adamw8_step, step=t)
+        bad = torch.isnan(a["params"][8])
+        assert torch.equal(bad, torch.isnan(b["params"][8]).cpu()) and int(bad.sum()) == (0 if t == 1 else 128)
+        assert torch.isfinite(b["params"][8][~bad.cuda()]).all()
+        for name in ("ms", "vs"):
+            assert torch.equal(a[name][8], b[name][8].cpu())
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+def test_zero_and_tiny_gradients(device, eps):
+    """Nothing where nothing came; with eps 0 too, where 0 / 0 would be."""
+    p = torch.linspace(-1, 1, 1000)
+    for value in (0.0, 1e-30, 1e-20):
+        s = dict(params=[p.to(device, copy=True)], grads=[torch.zeros(1000, device=device)], ms=[torch.zeros(1000, dtype=torch.uint8, device=device)],
+                 vs=[torch.zeros(1000, dtype=torch.uint8, device=device)], mscales=[torch.zeros(8, device=device)],
+                 vscales=[torch.zeros(8, device=device)], shadows=[None])
+        s["grads"][0][:500] = value
+        for t in (1, 2):
+            step(s, multi_tensor.adamw8_step, step=t, eps=eps)
+        got = s["params"][0].cpu()
+        assert torch.isfinite(got).all()
+        assert torch.allclose(got[500:], p[500:] * (1 - 1e-3) ** 2, rtol=1e-6, atol=0)
+        # at most the two updates of lr, whatever came
+        assert ((got[:500] - p[:500] * (1 - 1e-3) ** 2).abs() <= 2.1e-2).all()
+
+
+@pytest.mark.gpu
 def test_a_tensor_beyond_32_bits():
     """Indexes and random bits of the last elements, as the plain statement has them."""
     n = (1 << 32) + 300

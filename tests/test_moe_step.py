@@ -227,3 +227,41 @@ def test_trainer_runs_the_shipped_configuration(tmp_path, monkeypatch):
         assert all(h["loss"] == h["loss"] for h in history)
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_dense_trainer_with_8_bit_moments_in_a_graph(tmp_path, monkeypatch):
+    """The dense model on the kernel engine, its step captured: the shadow weights follow the masters, the replayed step counts its steps, and a run
+    without the graph ends nearly where this one does (the engine's gradients differ in the order of their sums, and an update is at most
+    some lr a step)."""
+    monkeypatch.setenv("TORCHURE_B200_HOME", str(tmp_path))
+    monkeypatch.setenv("MASTER_ADDR", "127.0.0.1")
+    import torch.distributed as dist
+
+    from tests.dist_utils import free_port
+    from tests.tiny import parity_config
+    from torchure_b200.train.trainer import Trainer
+
+    monkeypatch.setenv("MASTER_PORT", str(free_port()))
+    if not dist.is_initialized():
+        dist.init_process_group("nccl", rank=0, world_size=1)
+    try:
+        ends = []
+        for graph in (False, True):
+            cfg = parity_config(world=1, steps=8, accumulation=1)
+            cfg["model"]["config"].update(num_layers=2, num_heads=4, num_kv_heads=2, emb_dim=256, head_dim=128, vocab_size=1024, ffn_dim=512)
+            cfg["optimizer"]["config"].update(fused=True, state_bits=8)
+            cfg.update(cuda_graph=graph, cuda_graph_warmup=2)
+            tr = Trainer(cfg, 0, 0, 1, benchmark=True)
+            history = tr.train_n_step_test(6)
+            tr.check_device_errors()
+            assert all(h["loss"] == h["loss"] for h in history) and (tr._graph is not None) == graph
+            states = tr.optimizer.state
+            assert all(st["exp_avg"].dtype == torch.uint8 and float(st["step"]) == 6 for st in states.values())
+            for p, shadow in tr.model.engine().shadow_pairs():
+                assert torch.equal(shadow.reshape(p.shape), p.detach().bfloat16())
+            ends.append([p.detach().clone() for p in tr.model.parameters()])
+        for a, b in zip(*ends):
+            assert float((a - b).abs().max()) <= 6 * 2 * 3e-4
+    finally:
+        dist.destroy_process_group()

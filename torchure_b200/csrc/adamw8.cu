@@ -148,7 +148,8 @@ __device__ __forceinline__ bool on(const void* p, int bytes) { return (reinterpr
 // kernel 1.6 times slower.  They touch the parameters only, by 2^-21 of an update; the moments keep the bits of the plain statement.
 __device__ __forceinline__ float update(float p, float m, float v, const Adam8Scalars& s) {
   float root, over;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(fmaxf(v, 1.17549435e-38f)));      // (not zero: also with eps 0 no 0 / 0)
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(root) : "f"(v), "f"(1.17549435e-38f));      // (not zero: also with eps 0 no 0 / 0; a NaN stays one)
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(root));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(fmaf(root, s.root, s.eps)));
   return fmaf(-s.step_size, m * over, p * s.decay);
 }

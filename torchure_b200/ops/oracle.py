@@ -156,7 +156,8 @@ def adamw8(params, grads, ms, m_scales, vs, v_scales, shadows, lr, b1, b2, eps, 
             g = -g
         m = state8_decode(mc, msc, True) * b1 + g * (1.0 - b1)
         v = state8_decode(vc, vsc, False) * b2 + (g * (1.0 - b2)) * g
-        r = torch.sqrt(v.double()).float()          # correctly rounded (a CPU's fp32 root need not be)
+        # correctly rounded (a CPU's fp32 root need not be), and not of zero: no 0 / 0 with eps 0
+        r = torch.sqrt(v.clamp_min(2.0 ** -126).double()).float()
         p.copy_(p * (1.0 - lr * wd) - (m / (r * root + eps)) * size)
         if sh is not None:
             sh.copy_(p)
