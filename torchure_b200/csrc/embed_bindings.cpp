@@ -45,13 +45,13 @@ Tensor do_grad(const Tensor& ids, const Tensor& given, int64_t V, at::ScalarType
   if (D == 0) return dtable;
   if (T == 0) return dtable.zero_();
   const Tensor dout = rows_of(given.reshape({T, D}));
-  const Tensor scratch = empty({tb::embedding_scratch_bytes(T, V, (int)D)}, given.options().dtype(torch::kUInt8));
+  const Tensor scratch = empty({tb::embedding_scratch_bytes(T, V, (int)D, type == torch::kBFloat16)}, given.options().dtype(torch::kUInt8));
   const Overlap overlap;
   const int rc = tb::embedding_grad(ids.data_ptr(), ids.scalar_type() == torch::kInt64, dout.data_ptr(), is16(dout), dout.stride(0),
                                     dtable.data_ptr(), type == torch::kBFloat16, (float)how.scale, how.padding, T, V, (int)D, scratch.data_ptr(),
                                     cur_stream());
   TORCH_CHECK(rc == 0, "embedding backward failed with code ", rc);
-  bind_count_launches(tb::embedding_grad_kernels(T, V));
+  bind_count_launches(tb::embedding_grad_kernels(T, V, (int)D, type == torch::kBFloat16));
   return dtable;
 }
 

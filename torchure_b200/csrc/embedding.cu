@@ -8,7 +8,9 @@
 // in scratch memory, and a last kernel adds up the parts of such runs: however often one token occurs, its rows are read by many CTAs.
 // The table's gradient is mostly rows of no token: they are zeroed by CTAs of the sorting kernels, whose own work fills few SMs.
 //
-// Bound by memory: V D values of the gradient to write, T D to read.
+// Bound by memory: V D values of the gradient to write, T D to read.  8192 tokens, a table of 151936 x 1024 in fp32: lookup 10.3 us (6.5 TB/s), sort
+// and zeros 86 (7.2 TB/s of zeros), sums 12.7, runs over chunks 6.3; the whole pass 120, of which the bytes take 110 at copy bandwidth.  65521 tokens of
+// 1003 columns in bf16, 30 % padding: 45, 30, 39, 12.  Few tokens: a chain of kernels of 3 - 5 us.
 #include "common.cuh"
 #include "embed_api.h"
 
@@ -52,7 +54,8 @@ __device__ __forceinline__ int64_t id_at(const I* ids, int64_t t) { return stati
 // A warp has kRowCols columns of a row (blockIdx.y says which), at addresses that are constants behind one base: four next to each other for a thread
 // and round (kRowsFours), or one (kRowsOnes).  bf16 rows of an odd width or stride are read and written as 32-bit words all the same
 // (kRowsPairs): pairs of columns as the output's words have them, put together from two neighbouring words where the table's lie one column off.
-// The ids of the rows to come are on their way meanwhile.  65521 rows of 1003 columns, us: ones 50, pairs PAIRS_US.
+// The ids of the rows to come are on their way meanwhile.  65521 rows of 1003 columns 50 us by ones and 45 by
+// pairs.
 constexpr int kRowCols = 512;
 enum RowsBy { kRowsFours, kRowsOnes, kRowsPairs };
 
@@ -175,10 +178,9 @@ struct FromPass { const uint2* p; __device__ uint2 operator()(int t, const SortA
 
 template <class From>
 __global__ void __launch_bounds__(kThreads)
-sort_count_kernel(From from, SortArgs a, int* __restrict__ hist, Zero z) {
+sort_count_kernel(From from, SortArgs a, int* __restrict__ hist) {
   pdl_wait();
   pdl_launch_dependents();
-  if (static_cast<int>(blockIdx.x) >= z.from) return fill_zero(z);
   __shared__ int count[1 << kDigit];
   for (int b = threadIdx.x; b < a.bins; b += kThreads) count[b] = 0;
   __syncthreads();
@@ -203,7 +205,15 @@ __device__ __forceinline__ void sort_pass(int count, int shift, int bins, int* s
   __syncthreads();
   const int part = ((count + kWarps - 1) / kWarps + 31) / 32 * 32;
   const int lo = min(count, warp * part), hi = min(count, lo + part);
-  for (int i = lo + lane; i < hi; i += 32) atomicAdd(&cnt[warp * S + ((entry(i).x >> shift) & (bins - 1))], 1);
+  constexpr int U = 8;                              // entries of a thread that are on their way at once
+  for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
+    uint32_t key[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) key[u] = i0 + u * 32 < hi ? entry(i0 + u * 32).x : 0u;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * 32 < hi) atomicAdd(&cnt[warp * S + ((key[u] >> shift) & (bins - 1))], 1);
+  }
   int all = 0, before = 0;
   const bool given = others(tid, all, before);      // (bins are at most half the threads)
   __syncthreads();
@@ -231,17 +241,22 @@ __device__ __forceinline__ void sort_pass(int count, int shift, int bins, int* s
     place[tid] = base + up - all + before;
   }
   __syncthreads();
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    const uint2 e = i < hi ? entry(i) : make_uint2(0, 0);
-    const int b = i < hi ? static_cast<int>((e.x >> shift) & (bins - 1)) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, b);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    const int at = b >= 0 ? place[b] + cnt[warp * S + b] + rank : 0;
-    __syncwarp();
-    if (b >= 0 && rank == 0) cnt[warp * S + b] += __popc(same);
-    __syncwarp();
-    if (b >= 0) put(at, e);
+  for (int i0 = lo; i0 < hi; i0 += 32 * U) {
+    uint2 e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = i0 + u * 32 + lane < hi ? entry(i0 + u * 32 + lane) : make_uint2(0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * 32 >= hi) break;
+      const int b = i0 + u * 32 + lane < hi ? static_cast<int>((e[u].x >> shift) & (bins - 1)) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, b);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int at = b >= 0 ? place[b] + cnt[warp * S + b] + rank : 0;
+      __syncwarp();
+      if (b >= 0 && rank == 0) cnt[warp * S + b] += __popc(same);
+      __syncwarp();
+      if (b >= 0) put(at, e[u]);
+    }
   }
 }
 
@@ -268,25 +283,28 @@ sort_rank_kernel(From from, SortArgs a, const int* __restrict__ hist, int chunks
             [&](int at, uint2 e) { out[at] = e; });
 }
 
-// The whole sort in one CTA, between two lists in shared memory, while the other CTAs fill the gradient with zeros
-constexpr int kSmallSort = 8192;
+// The whole sort in one CTA while the others fill the gradient with zeros, the lists between its passes in shared memory up to kSharedSort tokens and in
+// scratch memory above.
+constexpr int kSharedSort = 8192;
 template <class From>
 __global__ void __launch_bounds__(kThreads)
-sort_small_kernel(From from, SortArgs a, int passes, uint2* __restrict__ out, Zero z) {
+sort_whole_kernel(From from, SortArgs a, int passes, uint2* __restrict__ out, uint2* __restrict__ other, Zero z) {
   pdl_wait();
   pdl_launch_dependents();
   if (static_cast<int>(blockIdx.x) >= z.from) return fill_zero(z);
   extern __shared__ int sm[];
-  uint2* list[2] = {reinterpret_cast<uint2*>(sm), reinterpret_cast<uint2*>(sm) + a.T};
-  int* counts = sm + 4 * a.T;
+  const int bits = 31 - __clz(a.bins);
+  const bool shared = a.T <= kSharedSort;
+  int* counts = sm + (shared ? 4 * a.T : 0);
+  uint2* lists[2] = {shared ? reinterpret_cast<uint2*>(sm) : (passes & 1) ? out : other,      // (the last pass of an even number writes to `out`)
+                     shared ? reinterpret_cast<uint2*>(sm) + a.T : (passes & 1) ? other : out};
   const auto own = [](int, int&, int&) { return false; };
-  for (int t = threadIdx.x; t < a.T; t += kThreads) list[0][t] = from(t, a);
-  __syncthreads();
-  int bits = 31 - __clz(a.bins);
   for (int p = 0; p < passes; ++p) {
-    const uint2* in = list[p & 1];
-    uint2* to = p + 1 == passes ? out : list[(p + 1) & 1];
-    sort_pass(a.T, p * bits, a.bins, counts, [&](int i) { return in[i]; }, own, [&](int at, uint2 e) { to[at] = e; });
+    const uint2* in = lists[(p + 1) & 1];
+    uint2* to = p + 1 == passes ? out : lists[p & 1];
+    const auto write = [&](int at, uint2 e) { to[at] = e; };
+    if (p == 0) sort_pass(a.T, 0, a.bins, counts, [&](int i) { return from(i, a); }, own, write);
+    else sort_pass(a.T, p * bits, a.bins, counts, [&](int i) { return in[i]; }, own, write);
     __syncthreads();
   }
 }
@@ -518,18 +536,22 @@ int bits_of(int64_t n) {             // of the largest value below n
   while ((1ll << b) < n) ++b;
   return b;
 }
+// One CTA sorts what fits its shared memory, and up to twice that where the zeros take longer than it does: 16384 tokens over 102 MB of bf16
+// rows 80 us so and 66 by many CTAs in four kernels, over 311 MB 90 and 100, over 622 MB of fp32 rows 185 and 194; 32768 over 622 MB 274 and 271.
+bool sorts_whole(int64_t T, int64_t bytes) { return T <= kSharedSort || (T <= 2 * kSharedSort && bytes >= 18000 * T); }
+
 struct Plan {
-  bool small;                        // sorted by one CTA
+  bool whole;                        // sorted by one CTA
   int passes, bits, chunks, chunk, seg_chunk, seg_chunks;
 };
-Plan plan_for(int64_t T, int64_t V) {
+Plan plan_for(int64_t T, int64_t V, int64_t bytes) {
   Plan p{};
   const int bits = bits_of(V + 1);
   p.passes = (bits + kDigit - 1) / kDigit;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.small = T <= kSmallSort;
+  p.whole = sorts_whole(T, bytes);
   p.chunk = static_cast<int>((T + kMaxChunks - 1) / kMaxChunks);
-  p.chunk = p.small ? static_cast<int>(T) : p.chunk < 2 * kThreads ? 2 * kThreads : (p.chunk + kThreads - 1) / kThreads * kThreads;
+  p.chunk = p.whole ? static_cast<int>(T) : p.chunk < 2 * kThreads ? 2 * kThreads : (p.chunk + kThreads - 1) / kThreads * kThreads;
   p.chunks = static_cast<int>((T + p.chunk - 1) / p.chunk);
   p.seg_chunk = static_cast<int>((T + kSegChunks - 1) / kSegChunks);
   p.seg_chunk = p.seg_chunk < kSegMin ? kSegMin : (p.seg_chunk + 7) / 8 * 8;
@@ -580,14 +602,14 @@ bool fits(int64_t T, int64_t V, int D) {
 
 }  // namespace
 
-int64_t embedding_scratch_bytes(int64_t T, int64_t V, int D) {
-  const Plan p = plan_for(T, V);
+int64_t embedding_scratch_bytes(int64_t T, int64_t V, int D, bool dtable16) {
+  const Plan p = plan_for(T, V, V * D * (dtable16 ? 2 : 4));
   return 2 * on16(8 * T) + on16(4ll * p.chunks << p.bits) + on16(4ll * (p.seg_chunks + 1)) + 8ll * p.seg_chunks * D;
 }
 
-int embedding_grad_kernels(int64_t T, int64_t V) {
-  const Plan p = plan_for(T, V);
-  return (p.small ? 1 : 2 * p.passes) + (p.seg_chunks > 1 ? 2 : 1);
+int embedding_grad_kernels(int64_t T, int64_t V, int D, bool dtable16) {
+  const Plan p = plan_for(T, V, V * D * (dtable16 ? 2 : 4));
+  return (p.whole ? 1 : 2 * p.passes) + (p.seg_chunks > 1 ? 2 : 1);
 }
 
 int embedding_rows(const void* ids, bool ids64, const void* table, bool table16, int64_t ld, void* out, bool out16, float scale, int64_t T,
@@ -606,7 +628,8 @@ int embedding_rows(const void* ids, bool ids64, const void* table, bool table16,
 int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, int64_t ld, void* dtable, bool dtable16, float scale,
                    int64_t padding, int64_t T, int64_t V, int D, void* scratch, cudaStream_t stream) {
   if (!fits(T, V, D) || padding < -1 || padding >= V || !aligned(dtable, 16) || !aligned(scratch, 16)) return -1;
-  const Plan p = plan_for(T, V);
+  const int64_t bytes = V * D * (dtable16 ? 2 : 4);
+  const Plan p = plan_for(T, V, bytes);
   char* at = static_cast<char*>(scratch);
   uint2* lists[2] = {reinterpret_cast<uint2*>(at), reinterpret_cast<uint2*>(at + on16(8 * T))};
   at += 2 * on16(8 * T);
@@ -616,9 +639,8 @@ int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, i
   at += on16(4ll * (p.seg_chunks + 1));
   SortArgs a{};
   a.T = static_cast<int>(T); a.chunk = p.chunk; a.bins = 1 << p.bits; a.V = static_cast<int>(V); a.padding = static_cast<int>(padding);
-  const int64_t bytes = V * D * (dtable16 ? 2 : 4);
-  // each of the sorting kernels fills its share of the gradient
-  const int kernels = p.small ? 1 : 2 * p.passes;
+  // the kernels that rank tokens fill the gradient, each its share (those that count are done before a share would be)
+  const int kernels = p.whole ? 1 : p.passes;
   int64_t done = 0;
   Zero z{static_cast<char*>(dtable), 0, 0, p.chunks, spans};
   const auto share = [&](int i) {
@@ -629,37 +651,36 @@ int embedding_grad(const void* ids, bool ids64, const void* dout, bool dout16, i
     const int64_t ctas = idle < 147 ? idle : many < 147 ? 147 : many;
     return static_cast<int>(ctas < 1 ? 1 : ctas);
   };
-  const int smem = 4 * rank_ints(a.bins) + (p.small ? 16 * a.T : 0);
+  const int smem = 4 * rank_ints(a.bins) + (p.whole && T <= kSharedSort ? 16 * a.T : 0);
   const auto whole = [&](auto from) {
     using From = decltype(from);
-    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(sort_small_kernel<From>), smem)) return -20;
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(sort_whole_kernel<From>), smem)) return -20;
     const int more = share(0);
-    return launch_code(launch_pdl(sort_small_kernel<From>, dim3(1 + more), dim3(kThreads), static_cast<size_t>(smem), stream, from, a, p.passes,
-                                  lists[0], z));
+    return launch_code(launch_pdl(sort_whole_kernel<From>, dim3(1 + more), dim3(kThreads), static_cast<size_t>(smem), stream, from, a, p.passes,
+                                  lists[0], lists[1], z));
   };
   const auto pass = [&](auto from, int i) {
     using From = decltype(from);
     if (!ensure_dynamic_smem(reinterpret_cast<const void*>(sort_rank_kernel<From>), smem)) return -20;
     a.shift = i * p.bits;
-    int more = share(2 * i);
-    int rc = launch_code(launch_pdl(sort_count_kernel<From>, dim3(p.chunks + more), dim3(kThreads), 0, stream, from, a, hist, z));
+    const int rc = launch_code(launch_pdl(sort_count_kernel<From>, dim3(p.chunks), dim3(kThreads), 0, stream, from, a, hist));
     if (rc) return rc;
-    more = share(2 * i + 1);
+    const int more = share(i);
     return launch_code(launch_pdl(sort_rank_kernel<From>, dim3(p.chunks + more), dim3(kThreads), static_cast<size_t>(smem), stream, from, a,
                                   hist, p.chunks, lists[i & 1], z));
   };
-  if (p.small) {
+  if (p.whole) {
     const int rc = ids64 ? whole(FromIds64{static_cast<const int64_t*>(ids)}) : whole(FromIds32{static_cast<const int*>(ids)});
     if (rc) return rc;
   }
-  for (int i = 0; i < p.passes && !p.small; ++i) {
+  for (int i = 0; i < p.passes && !p.whole; ++i) {
     const int rc = i > 0 ? pass(FromPass{lists[(i - 1) & 1]}, i)
                    : ids64 ? pass(FromIds64{static_cast<const int64_t*>(ids)}, i)
                            : pass(FromIds32{static_cast<const int*>(ids)}, i);
     if (rc) return rc;
   }
   SumArgs s{};
-  s.sorted = lists[p.small ? 0 : (p.passes - 1) & 1];
+  s.sorted = lists[p.whole ? 0 : (p.passes - 1) & 1];
   s.T = a.T; s.chunk = p.seg_chunk; s.V = a.V; s.D = D; s.ld = ld; s.scale = scale;
   s.spans = spans;
   s.parts = reinterpret_cast<float*>(at);
