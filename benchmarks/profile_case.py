@@ -4,7 +4,7 @@
 
 Cases: gemm_fwd, gemm_dgrad, gemm_wgrad, gemm_small, gemm_swiglu, gemm_swiglu_bwd, gemm_ce, attn_fwd, attn_bwd (single pass), attn_bwd_split, attn_prep, rmsnorm, rmsnorm_bwd, qknorm_rope,
 qknorm_rope_bwd, qknorm_rope_bwd_acc, swiglu, swiglu_bwd, ce, adamw, moe_train, moe_few, moe_token (all kernels of a pass of the
-experts' feed-forward), route, swiglu8, store8.  Each case builds inputs
+experts' feed-forward), route, route_scored, swiglu8, store8, adamw8, state8, embedding, embedding_odd.  Each case builds inputs
 larger than the 126 MB L2 but well under a few GB, launches the kernel `iters` times (default 4) and prints the
 CUDA-event time of the last launch with the achieved FLOP/s or bytes/s, so the same command serves a plain timing run
 and an `ncu -k regex:<kernel> -s 2 -c 1` capture.
@@ -170,6 +170,33 @@ def main(argv=None) -> None:
         dw = torch.randn(16389, 8, device=dev)
         fn = lambda: torch.autograd.grad(moe.route(logits, 8).weights, logits, dw)
         bytes_ = 16389 * (128 * 4 + 8 * 20)
+    elif args.case == "route_scored":
+        from torchure_b200.ops import moe
+
+        logits = torch.randn(32768, 128, device=dev).bfloat16().requires_grad_()
+        bias, dw = torch.randn(128, device=dev) * 0.02, torch.randn(32768, 8, device=dev)
+        fn = lambda: torch.autograd.grad(moe.route(logits, 8, score="sigmoid", bias=bias).weights, logits, dw)
+        bytes_ = 32768 * (128 * 4 + 8 * 20)
+    elif args.case in ("adamw8", "state8"):
+        n = 64 << 20
+        p, g = torch.randn(n, device=dev), torch.randn(n, device=dev) * 1e-3
+        m, v = (torch.randint(0, 256, (n,), device=dev, dtype=torch.uint8) for _ in range(2))
+        ms, vs = torch.rand(n // 128, device=dev) * 1e-3, torch.rand(n // 128, device=dev) * 1e-6
+        sh = torch.empty(n, dtype=torch.bfloat16, device=dev)
+        if args.case == "adamw8":
+            fn = lambda: multi_tensor.adamw8_step([p], [g], [m], [ms], [v], [vs], [sh], 1e-3, 0.9, 0.95, 1e-8, 0.1, 3)
+            bytes_ = n * 18.125
+        else:
+            fn = lambda: multi_tensor.state8_values([m], [ms], True, torch.bfloat16)
+            bytes_ = n * 3
+    elif args.case in ("embedding", "embedding_odd"):
+        from torchure_b200.ops.embedding import embedding
+
+        T, V, W, dt = (M, 151936, D, torch.float32) if args.case == "embedding" else (8 * M, 50257, 1003, torch.bfloat16)
+        ids = (float(V) ** torch.rand(T, device=dev, dtype=torch.float64)).long().sub_(1).clamp_(0, V - 1)
+        table, dout = torch.randn(V, W, device=dev).to(dt).requires_grad_(), torch.randn(T, W, device=dev).to(dt)
+        fn = lambda: torch.autograd.grad(embedding(ids, table), table, dout)
+        bytes_ = table.element_size() * W * (V + 3 * T)
     elif args.case == "swiglu8":
         from torchure_b200.ops import act8
 
