@@ -17,7 +17,8 @@
 // statements in plain tensor operations, bit for bit.
 //
 // Bound by memory: an element reads 4 + 4 + 1 + 1 bytes and writes 4 + 1 + 1 (+ 2 of the bf16 shadow), 18.1 with the scales, against 30 with the
-// moments in fp32.
+// moments in fp32.  64 Mi elements with the shadow 208 us (5.9 TB/s; a plain copy has 6.55), 73 instructions an element and issue slots 69 % taken;
+// 275 M in 17 tensors 817 us, 760 at copy bandwidth.  A moment read back as bf16: 275 M values in 127 us, 126 at copy bandwidth; 64 Mi in 36.
 #include "api.h"
 #include "common.cuh"
 

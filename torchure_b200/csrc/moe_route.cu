@@ -420,6 +420,9 @@ route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restri
 //   dl_e += daux E / T d_e P_e (share_e - sum_i share_i P_i)
 // Scores 1e-7 apart decide which expert a token goes to and with it the order of all rows behind; computed in 32 bits they would depend on the
 // machine's exp, rounded once from 64 they do not.
+//
+// Bound by instructions: a score in 64 bits takes 33 of them, a choice 25, and every token a warp.  8192 tokens x 256 experts in 8 groups, 8 choices:
+// 25 us, 9 for the rows, 9 for the gradient; 32768 x 128, 8 choices (8.4 MB of logits, 1.3 us): 32, 9 and 19; one token 7.6.
 struct ScoreArgs {
   const float* bias;       // nullptr: none
   int groups, top_groups, each;      // each: experts of a group
