@@ -70,6 +70,45 @@ def test_weights_without_a_bias_load():
     assert "router_bias" in biased.state_dict() and (biased.router_bias == 0).all() and "router_counts" not in biased.state_dict()
 
 
+def _sharded(rank, world, out):
+    from torchure_b200.core.mesh import Mesh
+    from torchure_b200.parallel.fsdp import FSDP
+
+    torch.manual_seed(1)
+    model = build_model("qwen3_moe", dict(MODEL, emb_dim=64, head_dim=16, moe_ffn_dim=32, router=None))
+    ids = torch.arange(30).view(2, 15)
+    want = model(ids).detach()
+    FSDP(model, Mesh({"dp_shard": world}), "dp_shard")
+    torch.save((want, model(ids).detach()), f"{out}.{rank}")
+
+
+def test_lookup_of_a_sharded_table(tmp_path):
+    """The table of a sharded model is gathered when its module is called: the lookup by sorting is such a call."""
+    run_distributed(_sharded, 2, str(tmp_path / "out"))
+    for rank in range(2):
+        want, got = torch.load(tmp_path / f"out.{rank}")
+        _same(got, want)
+
+
+def test_a_pipeline_stage_scales_its_rows():
+    class One:
+        def size(self, dim):
+            return 1
+
+        def coordinate(self, dim):
+            return 0
+
+    from torchure_b200.parallel.pipeline import PipelineStage
+
+    for kind in ("torch", "sorted"):
+        torch.manual_seed(2)
+        model = build_model("qwen3_moe", dict(MODEL, embedding=kind))
+        assert model.lm_head.weight is model.token_emb.weight and "token_emb.weight" in model.state_dict()
+        ids = torch.arange(12).view(1, 12)
+        with torch.no_grad():
+            _same(PipelineStage(model, One())(ids), model(ids))
+
+
 def _run(rank, world, cfg, home, out, emulate_world):
     os.environ["TORCHURE_B200_HOME"] = home
     from torchure_b200.train.trainer import Trainer

@@ -274,10 +274,6 @@ class Qwen3(nn.Module):
             self._engine = Sm100Engine(self)
         return self._engine
 
-    def embed(self, ids: torch.Tensor) -> torch.Tensor:
-        """Token rows as the first block takes them (PyTorch path)."""
-        return self.token_emb(ids)
-
     def forward(self, x: torch.Tensor, attention_mask: torch.Tensor | None = None,
                 return_hidden_states: bool = False, return_final_hidden: bool = False):
         if self._use_sm100(x, attention_mask) and not return_hidden_states:
@@ -302,7 +298,7 @@ class Qwen3(nn.Module):
             attention_mask = attention_mask.bool()
             pos = (attention_mask.long().cumsum(dim=1) - 1).masked_fill(~attention_mask, 0)
             cos, sin = self.rope(pos)
-        h = self.embed(x)
+        h = self.token_emb(x)
         sp = getattr(self, "sp", None)      # (mesh, axis) under tensor parallelism with sequence parallelism
         if sp is not None:
             from torchure_b200.parallel.tensor_parallel import shard_sequence, unshard_sequence

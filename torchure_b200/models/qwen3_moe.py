@@ -25,6 +25,22 @@ from torchure_b200.ops.embedding import embedding
 from torchure_b200.parallel.expert_parallel import MoELayer
 
 
+class TokenEmbedding(nn.Embedding):
+    """The token table `like`, the same parameter, with rows times `scale`; `by_sorting`: looked up by ``ops/embedding.py``.  A module, so that
+    wrappers that hook its forward pass (sharded parameters, pipeline stages) find it where a plain table would be."""
+
+    def __init__(self, like: nn.Embedding, scale: float, by_sorting: bool):
+        super().__init__(*like.weight.shape, _weight=like.weight.detach())
+        self.weight = like.weight
+        self.scale, self.by_sorting = float(scale), by_sorting
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        if self.by_sorting:
+            return embedding(ids, self.weight, self.scale)
+        h = super().forward(ids)
+        return h if self.scale == 1.0 else h * self.scale
+
+
 class Qwen3MoE(Qwen3):
     def __init__(self, num_layers: int, num_heads: int, num_kv_heads: int, emb_dim: int, head_dim: int | None,
                  vocab_size: int, num_experts: int, top_k: int = 2, moe_ffn_dim: int | None = None,
@@ -42,6 +58,7 @@ class Qwen3MoE(Qwen3):
         self.cfg.update(num_experts=num_experts, top_k=top_k, moe_ffn_dim=width, capacity_factor=capacity_factor,
                         aux_loss_coef=aux_loss_coef, experts=experts, act_bits=act_bits, router=router,
                         embedding=embedding, embed_scale=embed_scale)
+        self.token_emb = TokenEmbedding(self.token_emb, embed_scale, embedding == "sorted")
         self.aux_loss_coef = aux_loss_coef
         for block in self.blocks:
             block.ffn = MoELayer(emb_dim, width, num_experts, top_k, capacity_factor, experts=experts, act_bits=act_bits,
@@ -63,13 +80,6 @@ class Qwen3MoE(Qwen3):
         for b in self.blocks:
             b.gqa.o_proj.weight.mul_(scale)
             b.ffn.w_down.mul_(scale)
-
-    def embed(self, ids: torch.Tensor) -> torch.Tensor:
-        scale = self.cfg["embed_scale"]
-        if self.cfg["embedding"] == "sorted":
-            return embedding(ids, self.token_emb.weight, scale)
-        h = super().embed(ids)
-        return h if scale == 1.0 else h * scale
 
     @torch.no_grad()
     def balance_routers(self, mesh=None, dim: str | None = None) -> None:
