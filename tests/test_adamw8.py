@@ -369,6 +369,30 @@ def test_state_dicts_resume_bit_for_bit_and_convert(device, tmp_path):
             assert ((x - y).abs() <= 2.0 ** -20 * x.abs()).all()
 
 
+def test_a_state_dict_for_parameters_in_16_bits():
+    """An optimizer without 8-bit moments may have such parameters: the moments come in their type, rounded once, and the next step runs."""
+    _, opt = train("cpu", 4)
+    sd = copy.deepcopy(opt.state_dict())
+    sd["param_groups"] = [dict(sd["param_groups"][0], params=[0, 1, 2])]
+    half = [torch.nn.Parameter(p.detach().bfloat16()) for g in opt.param_groups for p in g["params"]]
+    wide = AdamW(half)
+    wide.load_state_dict(sd)
+    for i, p in enumerate(half):
+        st = sd["state"][i]
+        assert st["exp_avg"].dtype == torch.uint8      # (the caller's stays)
+        for key, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            assert torch.equal(wide.state[p][key], oracle.state8_decode(st[key], st[key + "_scale"], signed).bfloat16())
+        p.grad = torch.ones_like(p)
+    wide.step()
+
+
+def test_a_refused_group_is_not_kept():
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4))], state_bits=8)
+    with pytest.raises(TypeError):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))]})
+    assert len(opt.param_groups) == 1
+
+
 def test_refusals_of_the_optimizer():
     p = torch.nn.Parameter(torch.randn(4, 4))
     for kw in (dict(state_bits=16), dict(state_bits=8, amsgrad=True)):

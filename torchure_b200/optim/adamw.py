@@ -41,6 +41,7 @@ class AdamW(torch.optim.AdamW):
         if self._state_bits == 8:
             for p in self.param_groups[-1]["params"]:
                 if p.dtype != torch.float32 or not p.is_contiguous():
+                    self.param_groups.pop()
                     raise TypeError(f"AdamW: moments in 8 bits need contiguous fp32 parameters, got {p.dtype} with strides {p.stride()}")
 
     # -- hooks for the trainer -------------------------------------------------------------
@@ -160,22 +161,28 @@ class AdamW(torch.optim.AdamW):
 
     def load_state_dict(self, state_dict) -> None:
         """Also of an optimizer with moments in the other form: read back, or rounded to the nearest."""
-        super().load_state_dict(state_dict)      # (casts what it takes for values to the parameter's type; codes up to 255 survive that)
         from torchure_b200.ops import oracle
 
+        keys = (("exp_avg", True), ("exp_avg_sq", False))
+        if self._state_bits == 32:
+            state_dict = {**state_dict, "state": {i: dict(st) for i, st in state_dict["state"].items()}}
+            for st in state_dict["state"].values():
+                for key, signed in keys:
+                    if key + "_scale" in st:
+                        st[key] = oracle.state8_decode(st[key], st.pop(key + "_scale"), signed)
+        super().load_state_dict(state_dict)      # (casts what it takes for values to the parameter's type, fp32; codes up to 255 survive that)
+        if self._state_bits == 32:
+            return
         for st in self.state.values():
-            for key, signed in (("exp_avg", True), ("exp_avg_sq", False)):
-                if key not in st:
+            for key, signed in keys:
+                if key + "_scale" in st:
+                    codes, scales = st[key].to(torch.uint8), st[key + "_scale"]
+                elif key in st:
+                    x = st[key].contiguous()
+                    codes, scales = oracle.state8_encode(x, torch.full((x.numel(),), 32768, device=x.device), signed)
+                else:
                     continue
-                scales = st.pop(key + "_scale", None)
-                codes = None if scales is None else st[key].to(torch.uint8)
-                if self._state_bits == 8:
-                    if codes is None:
-                        x = st[key].contiguous()
-                        codes, scales = oracle.state8_encode(x, torch.full((x.numel(),), 32768, device=x.device), signed)
-                    st[key], st[key + "_scale"] = codes.contiguous(), scales.contiguous()
-                elif codes is not None:
-                    st[key] = oracle.state8_decode(codes, scales, signed)
+                st[key], st[key + "_scale"] = codes.contiguous(), scales.contiguous()
 
     def _advance_group(self, group, ps) -> tuple[int, float]:
         """Host bookkeeping of one step for one group: state init, step count, current lr."""
@@ -193,8 +200,8 @@ class AdamW(torch.optim.AdamW):
 
     # -- CUDA-graph support -----------------------------------------------------------------------------
     def enable_device_hyper(self, ring: int = 8) -> None:
-        """Keep {lr, 1-beta1^t, 1-beta2^t} (or what an 8-bit step takes of its step) of every group in device memory, refreshed from a ring of pinned host
-        slots before each launch.  A captured step then never bakes a step-dependent scalar into a kernel node."""
+        """Keep {lr, 1-beta1^t, 1-beta2^t} (or what an 8-bit step takes of its step) of every group in device memory, refreshed from a ring of
+        pinned host slots before each launch.  A captured step then never bakes a step-dependent scalar into a kernel node."""
         if self._hyper is not None:
             return
         dev = self.param_groups[0]["params"][0].device
