@@ -288,6 +288,9 @@ def test_refusals_of_the_step():
         step(s, multi_tensor.adamw8_step, step=1)
     with pytest.raises(ValueError):
         step(problem(5, "cuda"), multi_tensor.adamw8_step, step=1, grad_scale=torch.tensor(1.0))
+    for hyper in (torch.zeros(8, device="cuda")[::2], torch.zeros(3, device="cuda"), torch.zeros(4)):
+        with pytest.raises(ValueError):
+            step(problem(5, "cuda"), multi_tensor.adamw8_step, step=1, hyper=hyper)
     with pytest.raises(TypeError):
         multi_tensor.state8_values(s["ms"], s["mscales"], True, torch.float16)
     with pytest.raises(ValueError):

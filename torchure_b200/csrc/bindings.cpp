@@ -306,8 +306,9 @@ using OptTensors = std::vector<c10::optional<torch::Tensor>>;
 
 tb::State8List as_state8(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt,
                          const torch::Tensor& bc, int64_t chunk, const std::vector<int64_t>& host_ptrs) {
-  return {ptrs.data_ptr<int64_t>(), numel.numel() <= tb::kState8ByValue && !host_ptrs.empty() ? host_ptrs.data() : nullptr, numel.data_ptr<int64_t>(), flags.data_ptr<int32_t>(), bt.data_ptr<int32_t>(), bc.data_ptr<int32_t>(),
-          (int)numel.numel(), (int)bt.numel(), (int)chunk};
+  const int n = (int)numel.numel();
+  return {ptrs.data_ptr<int64_t>(), n <= tb::kState8ByValue && !host_ptrs.empty() ? host_ptrs.data() : nullptr, numel.data_ptr<int64_t>(),
+          flags.data_ptr<int32_t>(), bt.data_ptr<int32_t>(), bc.data_ptr<int32_t>(), n, (int)bt.numel(), (int)chunk};
 }
 
 // Checks what the kernel is going to read through addresses, and appends them
@@ -370,15 +371,17 @@ std::tuple<std::vector<int64_t>, std::vector<int64_t>> state8_columns(const Tens
 }
 
 void adamw8_multi(const torch::Tensor& ptrs, const torch::Tensor& numel, const torch::Tensor& flags, const torch::Tensor& bt, const torch::Tensor& bc,
-                  int64_t chunk, const std::vector<int64_t>& host_ptrs, double beta1, double beta2, double eps, double step_size, double root, double decay, int64_t key,
-                  c10::optional<torch::Tensor> grad_scale, bool maximize, c10::optional<torch::Tensor> hyper) {
-  TORCH_CHECK(!hyper || (hyper->is_cuda() && hyper->scalar_type() == torch::kFloat32 && hyper->numel() >= 4), "adamw8_step: hyper");
+                  int64_t chunk, const std::vector<int64_t>& host_ptrs, double beta1, double beta2, double eps, double step_size, double root,
+                  double decay, int64_t key, c10::optional<torch::Tensor> grad_scale, bool maximize, c10::optional<torch::Tensor> hyper) {
+  TORCH_CHECK_VALUE(!hyper || (hyper->device() == ptrs.device() && hyper->scalar_type() == torch::kFloat32 && hyper->is_contiguous() &&
+                               hyper->numel() >= 4), "adamw8_step: hyper must be four fp32 elements in a row on the GPU of the parameters");
   TORCH_CHECK_VALUE(!grad_scale || (grad_scale->device() == ptrs.device() && grad_scale->scalar_type() == torch::kFloat32 && grad_scale->numel() == 1),
                     "adamw8_step: grad_scale must be one fp32 element on the GPU of the parameters");
   const tb::Adam8Scalars s{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)step_size, (float)root,
                            (float)decay, (uint32_t)key, maximize ? 1 : 0};
   c10::cuda::CUDAGuard guard(ptrs.device());
-  const int rc = tb::adamw8_multi(as_state8(ptrs, numel, flags, bt, bc, chunk, host_ptrs), s, opt_ptr<float>(grad_scale), opt_ptr<float>(hyper), cur_stream());
+  const int rc = tb::adamw8_multi(as_state8(ptrs, numel, flags, bt, bc, chunk, host_ptrs), s, opt_ptr<float>(grad_scale), opt_ptr<float>(hyper),
+                                  cur_stream());
   TORCH_CHECK(rc == 0, "adamw8_step failed with code ", rc);
 }
 
