@@ -100,6 +100,10 @@ CASES = [      # T, E, k, score, biased, groups, top_groups, normalize, scale, c
     (37, 384, 16, "sigmoid", False, 1, 0, False, 1.0, 0.0),
     (37, 384, 7, "sigmoid", True, 32, 1, True, 1.0, 0.0),
     (64, 378, 4, "sigmoid", True, 9, 2, True, 1.0, 0.5),
+    (900, 384, 8, "sigmoid", True, 8, 4, True, 2.5, 0.1),        # several tokens of a warp, 12, 16, 24 and 10 experts of a thread
+    (700, 384, 6, "softmax", True, 3, 2, True, 1.0, 0.0),
+    (600, 380, 8, "sigmoid", False, 20, 8, False, 1.0, 0.2),
+    (777, 300, 8, "softmax", True, 1, 0, False, 1.0, 0.0),
 ]
 
 

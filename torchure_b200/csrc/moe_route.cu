@@ -226,19 +226,33 @@ __device__ __forceinline__ void choose(uint32_t (&key)[VALS], int (&index)[VALS]
   }
 }
 
-// What a CTA leaves of its tokens: the counts of its choices and the sums of its probabilities (acc, of the experts `index`), or with one CTA
-// the whole plan.
-template <int LANES, int VALS>
-__device__ __forceinline__ void close_chunk(const RouteArgs& a, float (&acc)[VALS], const int (&index)[VALS], const int* codes, int* hist,
-                                            float* psum, int* rest, int single) {
-  const int E = a.E, tid = threadIdx.x, lane = tid & 31;
-  float* part = reinterpret_cast<float*>(rest);           // [kWarps][E | 1]
+// The same for threads of many keys, whose indices are not held: at(v) is that of key v.
+template <int VALS, class At>
+__device__ __forceinline__ void choose_wide(uint32_t (&key)[VALS], At at, int k, int gl, uint32_t mask, uint32_t& my_key, int& my_e) {
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = key[0];
 #pragma unroll
-  for (int v = 0; v < VALS; ++v) {
+    for (int v = 1; v < VALS; ++v) best = max(best, key[v]);
+    best = __reduce_max_sync(mask, best);
+    int place = VALS;                // of this thread's lowest index with that key
 #pragma unroll
-    for (int o = LANES; o < 32; o <<= 1) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
-    if (lane < LANES && index[v] < E) part[(tid >> 5) * (E | 1) + index[v]] = acc[v];
+    for (int v = VALS - 1; v >= 0; --v)
+      if (key[v] == best) place = v;
+    const int mine = place < VALS ? at(place) : 0x7fffffff, e = __reduce_min_sync(mask, mine);
+    if (mine == e) {
+#pragma unroll
+      for (int v = 0; v < VALS; ++v)
+        if (v == place) key[v] = 0;
+    }
+    if (gl == j) { my_key = best; my_e = e; }
   }
+}
+
+// What a CTA leaves of its tokens: the counts of its choices and the sums of its probabilities (those of each warp in `rest`, or a thread's in acc, of
+// the experts `index`), or with one CTA the whole plan.
+__device__ __forceinline__ void close_chunk(const RouteArgs& a, const int* codes, int* hist, float* psum, int* rest, int single) {
+  const int E = a.E, tid = threadIdx.x, lane = tid & 31;
+  const float* part = reinterpret_cast<const float*>(rest);           // [kWarps][E | 1]
   __syncthreads();
   for (int e = tid >> 5; e < E; e += kWarps) {      // a warp adds up the warps' sums of one expert
     const float s = group_sum<32>(part[lane * (E | 1) + e], 0xffffffffu);
@@ -254,6 +268,19 @@ __device__ __forceinline__ void close_chunk(const RouteArgs& a, float (&acc)[VAL
     __syncthreads();
     plan_rows(a, codes, hist, psum, 0, 1, rest);
   }
+}
+template <int LANES, int VALS>
+__device__ __forceinline__ void close_chunk(const RouteArgs& a, float (&acc)[VALS], const int (&index)[VALS], const int* codes, int* hist,
+                                            float* psum, int* rest, int single) {
+  const int E = a.E, tid = threadIdx.x, lane = tid & 31;
+  float* part = reinterpret_cast<float*>(rest);           // [kWarps][E | 1]
+#pragma unroll
+  for (int v = 0; v < VALS; ++v) {
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], o);
+    if (lane < LANES && index[v] < E) part[(tid >> 5) * (E | 1) + index[v]] = acc[v];
+  }
+  close_chunk(a, codes, hist, psum, rest, single);
 }
 
 template <class T, int LANES, int VALS>
@@ -478,7 +505,9 @@ __device__ __forceinline__ double group_sum64(double v, uint32_t mask) {
   return v;
 }
 
-// The experts of a group lie with neighbouring threads: of the token's threads, LANES / 2^groups_log2 for each group.
+// The experts of a group lie with neighbouring threads: of the token's threads, LANES / 2^groups_log2 for each group.  Of more than eight experts a
+// thread holds scores and keys only (1024 threads leave it 64 registers): sums lie in shared memory, the bias is read anew, the next token's logits are
+// not on their way.  32768 tokens x 384 experts 107 us with the rows' numbers, 200 with all of it in registers; x 256, eight a thread, 81 and 70.
 template <class T, int LANES, int VALS>
 __global__ void __launch_bounds__(kThreads)
 route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, int single) {
@@ -496,30 +525,54 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
   for (int e = tid; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
   const bool by_score = how.bias != nullptr || how.groups > 1;
-  float acc[VALS], bias[VALS];
-  int expert[VALS];
+  constexpr bool kWide = VALS > 8;
+  static_assert(!kWide || LANES == 32, "a warp's sums are a token's threads'");
+  constexpr int kHeld = kWide ? 1 : VALS;
+  const int here = mine < how.groups ? how.each : 0, first_expert = mine * how.each;
+  const auto expert_at = [&](int v) { return v * per + sub < here ? first_expert + v * per + sub : 0x7fffffff; };
+  float acc[kHeld], held_bias[kHeld];
+  int held[kHeld];
+  if constexpr (!kWide) {
 #pragma unroll
-  for (int v = 0; v < VALS; ++v) {
-    const int in = v * per + sub;
-    expert[v] = mine < how.groups && in < how.each ? mine * how.each + in : 0x7fffffff;
-    acc[v] = 0.f;
-    bias[v] = how.bias != nullptr && expert[v] < E ? how.bias[expert[v]] : 0.f;
+    for (int v = 0; v < VALS; ++v) {
+      held[v] = expert_at(v);
+      acc[v] = 0.f;
+      held_bias[v] = how.bias != nullptr && held[v] < E ? how.bias[held[v]] : 0.f;
+    }
   }
+  float* sums = reinterpret_cast<float*>(rest) + (tid >> 5) * (E | 1);      // (kWide) of this warp
+  if constexpr (kWide) {
+    for (int e = lane; e < E; e += 32) sums[e] = 0.f;
+    __syncwarp();
+  }
+  const auto expert = [&](int v) {
+    if constexpr (kWide) return expert_at(v);
+    else return held[v];
+  };
+  const auto bias = [&](int v) {
+    if constexpr (!kWide) return held_bias[v];
+    else return how.bias != nullptr && expert_at(v) < E ? how.bias[expert_at(v)] : 0.f;
+  };
+  const auto gather = [&](float of, int v) {
+    if constexpr (!kWide) acc[v] += of;
+    else if (expert_at(v) < E) sums[expert_at(v)] += of;
+  };
   const int t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
   float next[VALS];      // the logits of the token after the one that is worked on
   auto fetch = [&](int t) {
 #pragma unroll
-    for (int v = 0; v < VALS; ++v) next[v] = t < t1 && expert[v] < E ? load_logit(logits + t * a.ld + expert[v]) : -INFINITY;
+    for (int v = 0; v < VALS; ++v) next[v] = t < t1 && expert(v) < E ? load_logit(logits + t * a.ld + expert(v)) : -INFINITY;
   };
-  fetch(t0 + group);
+  if (!kWide) fetch(t0 + group);
   for (int t = t0 + group; t < t1; t += GROUPS) {
     float x[VALS], s[VALS], top = -INFINITY;
+    if (kWide) fetch(t);
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {
       x[v] = next[v];
       top = fmaxf(top, x[v]);
     }
-    fetch(t + GROUPS);
+    if (!kWide) fetch(t + GROUPS);
     // (of sigmoids the largest logit is asked for only where all scores are tiny)
     const bool tiny = how.sigmoid && !__any_sync(mask, top >= kTinyScores);
     if (!how.sigmoid || tiny) top = group_max<LANES>(top, mask);
@@ -543,8 +596,8 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
     uint32_t key[VALS];
 #pragma unroll
     for (int v = 0; v < VALS; ++v) {
-      const float c = !by_score ? x[v] : x[v] == -INFINITY ? -INFINITY : s[v] + bias[v];
-      key[v] = expert[v] < E ? to_key(c) : 0u;
+      const float c = !by_score ? x[v] : x[v] == -INFINITY ? -INFINITY : s[v] + bias(v);
+      key[v] = expert(v) < E ? to_key(c) : 0u;
     }
     if (how.groups > 1) {
       uint32_t first = 0, second = 0;      // the largest two of the group
@@ -570,10 +623,15 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
       }
     }
     uint32_t my_key = 0;
-    int my_e = 0, index[VALS];
+    int my_e = 0;
+    if constexpr (kWide) {
+      choose_wide<VALS>(key, expert_at, a.k, gl, mask, my_key, my_e);
+    } else {
+      int index[VALS];
 #pragma unroll
-    for (int v = 0; v < VALS; ++v) index[v] = expert[v];
-    choose<VALS, false>(key, index, a.k, gl, mask, my_key, my_e);
+      for (int v = 0; v < VALS; ++v) index[v] = held[v];
+      choose<VALS, false>(key, index, a.k, gl, mask, my_key, my_e);
+    }
     const bool made = gl < a.k && my_key != kKeyMinusInf;
     const float l = made ? load_logit(logits + t * a.ld + my_e) : -INFINITY;
     float w = 0.f, whole = 1.f;
@@ -616,13 +674,14 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
       sum = group_sum<LANES>(sum, mask);
       const float r = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int v = 0; v < VALS; ++v) acc[v] += s[v] * r;
+      for (int v = 0; v < VALS; ++v) gather(s[v] * r, v);
     } else {
 #pragma unroll
-      for (int v = 0; v < VALS; ++v) acc[v] += s[v];
+      for (int v = 0; v < VALS; ++v) gather(s[v], v);
     }
   }
-  close_chunk<LANES, VALS>(a, acc, expert, codes, hist, psum, rest, single);
+  if constexpr (kWide) close_chunk(a, codes, hist, psum, rest, single);
+  else close_chunk<LANES, VALS>(a, acc, held, codes, hist, psum, rest, single);
 }
 
 template <class T, int LANES, int VALS>
@@ -781,7 +840,7 @@ void scored_shape(int E, const RouteScore& how, int& lanes, int& vals, int& grou
   lanes = 4;
   while (lanes < 32 && (lanes >> groups_log2) < each) lanes <<= 1;
   vals = 1;
-  while (vals * (lanes >> groups_log2) < each) vals <<= 1;
+  while (vals * (lanes >> groups_log2) < each) vals = vals < 8 ? vals * 2 : vals + (vals < 16 ? 4 : 8);
 }
 
 int lanes_of(int E, const RouteScore* how) {
@@ -812,7 +871,7 @@ int launch_fwd(const T* logits, const RouteArgs& a, int chunks, cudaStream_t str
 }
 
 // (groups that are no power of two leave threads without experts: up to 22 logits for the others)
-#define TB_SCORED_SIZES(CASE) TB_ROUTE_SIZES(CASE) CASE(32, 32)
+#define TB_SCORED_SIZES(CASE) CASE(4, 1) CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(32, 2) CASE(32, 4) CASE(32, 8) CASE(32, 12) CASE(32, 16) CASE(32, 24)
 
 template <class T>
 int launch_scored(const T* logits, const RouteArgs& a, const RouteScore& how, int chunks, cudaStream_t stream) {
