@@ -262,3 +262,27 @@ def test_launches_are_counted():
     assert ops.launches() == before + 1
     torch.autograd.grad(out, w, torch.ones_like(out))
     assert ops.launches() > before + 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 3, 69, 70])
+@pytest.mark.parametrize("D, gap", [(1, 0), (1, 1), (1, 2), (2, 1), (3, 0), (3, 2), (7, 0), (7, 4), (8, 1), (513, 2), (600, 1)])
+def test_rows_of_16_bits_that_end_in_the_middle_of_a_word(T, D, gap):
+    """Tables and gradients of odd widths and odd strides, the last row at the very end of its storage: rows are read as 32-bit words, and of one
+    column an odd number of them leaves no word for the last."""
+    g = torch.Generator().manual_seed(T)
+    V, scale, wide = 9, 0.7, D + gap
+
+    def rows(n):
+        room = torch.full((n * wide - gap,), float("nan"), dtype=torch.bfloat16)
+        x = room.as_strided((n, D), (wide, 1))
+        x.copy_(torch.randn(n, D, generator=g))
+        return x, room.cuda().as_strided((n, D), (wide, 1))
+
+    ids = torch.randint(0, V, (T,), generator=g)
+    ids[0] = V - 1
+    table, there = rows(V)
+    dout, dthere = rows(T)
+    out = embedding(ids.cuda(), there.requires_grad_(), scale)
+    dtable, = torch.autograd.grad(out, there, dthere)
+    check(ids, table, dout, out, dtable, scale)

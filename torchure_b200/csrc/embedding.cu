@@ -336,7 +336,7 @@ __device__ __forceinline__ int col_of(int col, int step, int j) {
 }
 
 // What a thread reads of a row, as it lies in memory (a conversion next to the load would wait for it).  at: its columns, those that are not there
-// brought to 0 (they are not stored).  last: the row is the matrix' last one, behind which nothing is read.
+// brought to 0 (they are not stored).  last: the row is the matrix' last one, behind which nothing is read (kPairs: of rows of two columns or more).
 template <ColsBy BY, class T>
 struct Cols;
 template <>
@@ -587,7 +587,9 @@ int launch_sums(const SumArgs& a, int chunks, const S* dout, O* dtable, cudaStre
     return launch_code(launch_pdl(kernel, dim3(chunks, (a.D + width * 4 - 1) / (width * 4)), dim3(width), 0, stream, a, dout, dtable));
   };
   constexpr ColsBy kWords = sizeof(S) == 2 ? kPairs : kOnes;
-  const bool words = sizeof(S) == 2 && aligned(dout, 4) && a.ld >= a.D, wide = a.D > 256;      // narrow rows take CTAs of two warps
+  // A pair's second word ends at most two columns behind its row's last: in the next row, unless rows are one value each (of an odd number the last
+  // but one would read behind the matrix).
+  const bool words = sizeof(S) == 2 && aligned(dout, 4) && a.ld >= a.D && a.D > 1, wide = a.D > 256;      // narrow rows take CTAs of two warps
   int rc;
   if (vec) rc = wide ? run(segment_sum_kernel<S, O, kFours, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kFours, 64>, 64);
   else if (words) rc = wide ? run(segment_sum_kernel<S, O, kWords, kSegThreads>, kSegThreads) : run(segment_sum_kernel<S, O, kWords, 64>, 64);
