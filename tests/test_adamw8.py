@@ -502,3 +502,69 @@ def test_kernels_off_runs_the_plain_statement():
         assert torch.isfinite(s["params"][0]).all()
     finally:
         ops.force_fallback(False)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_a_tensors_number_is_what_its_random_bits_go_by(device):
+    """Without numbers: the place in the list.  With them a tensor's step is the same wherever it stands and whatever stands beside it."""
+    a, b, c = (problem(11, device) for _ in range(3))
+    step(a, multi_tensor.adamw8_step, step=3, seed=4)
+    numbers = [7 * i % 10 for i in range(len(SHAPES))]
+    step(b, multi_tensor.adamw8_step, step=3, seed=4, numbers=list(range(len(SHAPES))))
+    assert all(torch.equal(x, y) for name in a for x, y in zip(a[name], b[name]) if x is not None)
+    some = [9, 8, 3, 2]
+    c = {name: [ts[i] for i in some] for name, ts in c.items()}
+    step(c, multi_tensor.adamw8_step, step=3, seed=4, numbers=some)
+    for name in a:
+        assert all(x is None or torch.equal(x, y) for x, y in zip((a[name][i] for i in some), c[name])), name
+    d, e = problem(11, device), problem(11, "cpu")
+    step(d, multi_tensor.adamw8_step, step=3, seed=4, numbers=numbers)
+    step(e, plain, step=3, seed=4, numbers=numbers)
+    for name in ("ms", "mscales", "vs", "vscales"):
+        assert all(torch.equal(x.cpu(), y) for x, y in zip(d[name], e[name])), name
+    assert any(not torch.equal(x, y) for x, y in zip(a["ms"], d["ms"]))
+    if device == "cuda":
+        for bad in (numbers[:-1], [-1] + numbers[1:], [1 << 30] + numbers[1:]):
+            with pytest.raises(ValueError):
+                step(d, multi_tensor.adamw8_step, step=3, numbers=bad)
+        step(d, multi_tensor.adamw8_step, step=3, numbers=[(1 << 30) - 1] + numbers[1:])
+
+
+@pytest.mark.gpu
+def test_numbers_of_many_tensors():
+    """More than 64 tensors: addresses from a table; the numbers come with the sizes all the same."""
+    g = torch.Generator().manual_seed(1)
+    grads = [torch.randn(200 + i, generator=g) for i in range(70)]
+    out = []
+    for order in (range(70), range(69, -1, -1)):
+        s = dict(params=[torch.zeros(200 + i, device="cuda") for i in order], grads=[grads[i].cuda() for i in order], shadows=[None] * 70)
+        s["ms"], s["vs"] = ([torch.zeros(200 + i, dtype=torch.uint8, device="cuda") for i in order] for _ in range(2))
+        s["mscales"], s["vscales"] = ([torch.zeros(-(-(200 + i) // 128), device="cuda") for i in order] for _ in range(2))
+        step(s, multi_tensor.adamw8_step, step=1, seed=2, numbers=[1000 + i for i in order])
+        out.append({n: ts if order[0] == 0 else ts[::-1] for n, ts in s.items()})
+    assert all(torch.equal(x, y) for n in ("params", "ms", "vs", "mscales", "vscales") for x, y in zip(out[0][n], out[1][n]))
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_a_step_that_leaves_a_parameter_out(device):
+    """The others are rounded as they would have been beside it, and a parameter with a number as itself in any group's order."""
+    g = torch.Generator().manual_seed(5)
+    start, grads = ([torch.randn(n, generator=g) for n in (300, 400, 500)] for _ in range(2))
+
+    def run(order, without=(), numbers=None):
+        params = [torch.nn.Parameter(start[i].to(device, copy=True)) for i in order]
+        opt = AdamW(params, lr=1e-2, fused=True, state_bits=8)
+        if numbers:
+            opt.number_tensors({p: numbers[i] for p, i in zip(params, order)})
+        for p, i in zip(params, order):
+            p.grad = None if i in without else grads[i].to(device, copy=True)
+        opt.step()
+        return {i: (p.detach(), opt.state[p].get("exp_avg"), opt.state[p].get("exp_avg_sq")) for p, i in zip(params, order)}
+
+    def same(x, y):
+        return all(torch.equal(u, v) for u, v in zip(x, y))
+
+    whole, part = run([0, 1, 2]), run([0, 1, 2], without=(0,))
+    assert same(whole[1], part[1]) and same(whole[2], part[2])
+    numbered, other = run([0, 1, 2], numbers=[4, 9, 17]), run([2, 0], numbers=[4, 9, 17])
+    assert same(numbered[2], other[2]) and same(numbered[0], other[0]) and not torch.equal(numbered[2][1], whole[2][1])

@@ -488,3 +488,26 @@ def test_resume_is_exact(tmp_path):
         assert torch.equal(got["a"][n], got["b"][n]), n
     assert (tmp_path / "checkpoints" / "resumed" / "5" / ".complete").exists()
     assert sorted(os.listdir(tmp_path / "checkpoints" / "resumed")) == ["3", "5"]
+
+
+def _run_pp8(rank, world, cfg, home, out):
+    os.environ["TORCHURE_B200_HOME"] = home
+    from torchure_b200.train.trainer import Trainer
+
+    tr = Trainer(cfg, rank, rank, world, benchmark=True, device="cpu")
+    tr.train_n_step_test(STEPS)
+    states = {n: tr.optimizer.state[p] for n, p in tr.model.named_parameters()}
+    torch.save({"params": _weights(tr), "states": states}, f"{out}.{rank}")
+
+
+def test_pipeline_of_uneven_stages_keeps_a_tied_table_equal_with_8_bit_moments(tmp_path):
+    """Three layers on two stages: the table stands behind a different number of tensors in the two optimizers, and its moments are rounded alike all
+    the same."""
+    cfg = parity_config(world=1, steps=STEPS, accumulation=4, mesh={"dp": 1, "pp": 2})
+    cfg["model"]["config"]["num_layers"] = 3
+    cfg["optimizer"]["config"]["state_bits"] = 8
+    run_distributed(_run_pp8, 2, cfg, str(tmp_path), str(tmp_path / "pp8.pt"), timeout_s=240)
+    a, b = (torch.load(f"{tmp_path}/pp8.pt.{r}") for r in range(2))
+    assert torch.equal(a["params"]["token_emb.weight"], b["params"]["lm_head.weight"])
+    x, y = a["states"]["token_emb.weight"], b["states"]["lm_head.weight"]
+    assert set(x) == set(y) and x["exp_avg"].dtype == torch.uint8 and all(torch.equal(x[n], y[n]) for n in x)

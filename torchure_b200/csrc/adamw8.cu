@@ -10,7 +10,7 @@
 // no update divides by eps alone where the gradients have been small beside the block's.
 // A block that holds something that is not finite reads back as NaN, one whose largest magnitude is under 2^-100 as zeros.
 //
-// Random bits: h(i) = mix(key ^ low 32 bits of i), key from (seed, step, tensor, high bits of i), mix two rounds of xorshift and multiplication
+// Random bits: h(i) = mix(key ^ low 32 bits of i), key from (seed, step, the tensor's number, high bits of i), mix two rounds of xorshift and multiplication
 // (constants by C. Wellons, 2018); 16 bits for each moment.
 //
 // The moments' arithmetic is fp32, every operation rounded by itself in the order written (no contraction): their codes are those of the same
@@ -326,13 +326,14 @@ adamw8_kernel(State8List t, Adam8Scalars s, const float* __restrict__ grad_scale
   float* m_scale = reinterpret_cast<float*>(ptr(4)) + lo / kStateBlock;
   float* v_scale = reinterpret_cast<float*>(ptr(5)) + lo / kStateBlock;
   __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(ptr(6));
-  const bool g16 = (t.flags[ti] & 1) != 0;
+  const int flags = t.flags[ti];
+  const bool g16 = (flags & 1) != 0;
   g += lo * (g16 ? 2 : 4);
   if (sh) sh += lo;
   const bool vp = on(p, 16), vg = on(g, g16 ? 8 : 16), vm = on(m, 16), vv = on(v, 16), vs = on(sh, 8);
   float gs = grad_scale ? *grad_scale : 1.f;
   if (s.maximize) gs = -gs;
-  key = mix32(key + 0x85ebca6bu * static_cast<uint32_t>(ti) + 0xc2b2ae35u * static_cast<uint32_t>(lo >> 32));
+  key = mix32(key + 0x85ebca6bu * static_cast<uint32_t>(flags >> 1) + 0xc2b2ae35u * static_cast<uint32_t>(lo >> 32));
   const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * kStateBlock;
   constexpr int kStep = kThreads / 32 * kStateBlock;
   if (count == t.chunk && vp && vg && vm && vv && vs) {

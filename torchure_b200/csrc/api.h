@@ -139,7 +139,8 @@ struct TensorList {           // device-resident table (built once per parameter
   int n_blocks;
 };
 constexpr int kChunkElems = 16384;
-// The same with as many pointer columns as the operation has, one after the other (adamw8.cu).  p, grad (flag bit 0: bf16), codes and scales of
+// The same with as many pointer columns as the operation has, one after the other (adamw8.cu).  p, grad (flag bit 0: bf16; the bits above it: the
+// tensor's number for its random bits), codes and scales of
 // the moments (m, v codes, then m, v scales) and the optional bf16 shadow; scales have one fp32 value for kStateBlock codes.
 constexpr int kStateBlock = 128;
 constexpr int kState8ByValue = 64;

@@ -322,10 +322,12 @@ void add_column(std::vector<int64_t>& out, const torch::Tensor& t, int64_t n, co
 
 // (addresses, elements, flags) of an 8-bit AdamW step's tensors
 std::tuple<std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>> adamw8_columns(
-    const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, const Tensors& ms, const Tensors& vs, const OptTensors& shadows) {
+    const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, const Tensors& ms, const Tensors& vs, const OptTensors& shadows,
+    const c10::optional<std::vector<int64_t>>& numbers) {
   const size_t n = params.size();
   TORCH_CHECK_VALUE(n > 0 && grads.size() == n && m.size() == n && v.size() == n && ms.size() == n && vs.size() == n && shadows.size() == n,
                     "adamw8_step: lists of one length expected");
+  TORCH_CHECK_VALUE(!numbers || numbers->size() == n, "adamw8_step: a number for each of ", n, " tensors expected");
   const auto dev = params[0].device();
   TORCH_CHECK_VALUE(dev.is_cuda(), "adamw8_step: tensors on a GPU expected");
   std::vector<int64_t> ptrs, numel, flags;
@@ -333,7 +335,9 @@ std::tuple<std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>> ada
   const auto f32 = torch::kFloat32, b16 = torch::kBFloat16, u8 = torch::kUInt8;
   for (size_t i = 0; i < n; ++i) {
     numel.push_back(params[i].numel());
-    flags.push_back(grads[i].scalar_type() == b16);
+    const int64_t number = numbers ? (*numbers)[i] : static_cast<int64_t>(i);
+    TORCH_CHECK_VALUE(number >= 0 && number < 1ll << 30, "adamw8_step: number ", number, " of a tensor (0 to 2^30 - 1 expected)");
+    flags.push_back(number << 1 | (grads[i].scalar_type() == b16));
     add_column(ptrs, params[i], numel[i], dev, {f32}, "adamw8_step: parameter");
   }
   for (size_t i = 0; i < n; ++i) add_column(ptrs, grads[i], numel[i], dev, {f32, b16}, "adamw8_step: gradient");

@@ -186,21 +186,22 @@ def adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed=0) -> tuple[float,
 
 
 def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, shadows, lr, beta1, beta2, eps, weight_decay,
-                step, grad_scale=None, maximize=False, hyper=None, seed=0) -> None:
+                step, grad_scale=None, maximize=False, hyper=None, seed=0, numbers=None) -> None:
     """One AdamW step over all tensors with both moments in 8 bits (uint8 codes of the parameter's shape, an fp32 scale for every 128
     values), in place.  params fp32, grads fp32 or bf16, shadows bf16 or None; all contiguous.
 
     The step is ``adamw_step``'s on the moments read back; what they are then is rounded to 8 bits with random bits of (seed, step, tensor's
-    place in the list, element), so that the mean over steps is right (``oracle.state8_encode`` has the format).  `grad_scale`: device
+    number, element), so that the mean over steps is right (``oracle.state8_encode`` has the format).  `numbers`: of the tensors, each 0 to
+    2^30 - 1 (None: their places in the list); a tensor that is held twice keeps equal copies only under one number.  `grad_scale`: device
     scalar that multiplies the gradients.  `hyper`: optional device tensor of what ``adamw8_scalars`` gives (the key as the pattern of a
     float), in its place at run time (graph replay)."""
     if not params:
         return
     if not (ops.available() and params[0].is_cuda):
         oracle.adamw8(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, shadows, lr, beta1, beta2, eps, weight_decay,
-                      step, grad_scale, maximize, seed)
+                      step, grad_scale, maximize, seed, numbers)
         return
-    ptrs, numel, flags = ops.ext().adamw8_columns(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, shadows)
+    ptrs, numel, flags = ops.ext().adamw8_columns(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, shadows, numbers)
     chunk = _chunk8(numel)
     tab, ptrs = _table8("adamw8", params, flags, ptrs, numel, chunk)
     size, root, decay, key = adamw8_scalars(lr, beta1, beta2, weight_decay, step, seed)

@@ -107,7 +107,7 @@ def state8_key(seed: int, step: int) -> int:
 
 
 def state8_bits(n: int, key: int, index: int, device) -> torch.Tensor:
-    """32 random bits (int64) for each of the n values of the `index`-th tensor: the lower 16 for the first moment."""
+    """32 random bits (int64) for each of the n values of tensor number `index`: the lower 16 for the first moment."""
     i = torch.arange(n, device=device)
     if n <= 1 << 32:
         return _mix32((i & _LOW32) ^ _mix32((key + 0x85EBCA6B * index) & _LOW32))
@@ -145,10 +145,11 @@ def state8_decode(codes, scales, signed):
     return y.view(-1)[:codes.numel()].view(codes.shape)
 
 
-def adamw8(params, grads, ms, m_scales, vs, v_scales, shadows, lr, b1, b2, eps, wd, step, grad_scale=None, maximize=False, seed=0):
+def adamw8(params, grads, ms, m_scales, vs, v_scales, shadows, lr, b1, b2, eps, wd, step, grad_scale=None, maximize=False, seed=0, numbers=None):
     """AdamW in place with moments in 8 bits."""
+    numbers = range(len(params)) if numbers is None else numbers
     size, root, key = lr / (1.0 - b1 ** step), (1.0 - b2 ** step) ** -0.5, state8_key(seed, step)
-    for i, (p, g, mc, msc, vc, vsc, sh) in enumerate(zip(params, grads, ms, m_scales, vs, v_scales, shadows, strict=True)):
+    for i, p, g, mc, msc, vc, vsc, sh in zip(numbers, params, grads, ms, m_scales, vs, v_scales, shadows, strict=True):
         g = g.float()
         if grad_scale is not None:
             g = g * grad_scale.float()

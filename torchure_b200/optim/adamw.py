@@ -12,8 +12,9 @@ of separate clip-scale, optimizer and autocast-cast passes.
 
 ``state_bits=8`` holds both moments in 8 bits: ``state[p] = {step, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}`` with uint8 codes
 of the parameter's shape and an fp32 scale for every 128 values (``ops/multi_tensor.py::adamw8_step``), 2.06 bytes a parameter instead of
-8.  They are rounded with random bits of (``rounding_seed``, step, parameter, element), so that steps smaller than a code's are kept in the
-mean, runs repeat bit for bit and data-parallel replicas stay equal.  State dicts of both forms load into either.
+8.  They are rounded with random bits of (``rounding_seed``, step, the parameter's number, element), so that steps smaller than a code's are kept in
+the mean, runs repeat bit for bit and data-parallel replicas stay equal.  A parameter's number is its place in its group, or what
+``number_tensors`` gave it: pipeline stages that hold one tensor twice give both copies one number.  State dicts of both forms load into either.
 """
 
 from __future__ import annotations
@@ -32,6 +33,7 @@ class AdamW(torch.optim.AdamW):
         super().__init__(params, lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, **kw)
         self._grad_scale: torch.Tensor | None = None
         self._shadow: dict[torch.Tensor, torch.Tensor] = {}
+        self._numbers: dict[torch.Tensor, int] = {}
         self._hyper: list[torch.Tensor] | None = None   # per group {lr, bias1, bias2} on the device
         self._hyper_cur: int | None = None
         self._graph_groups: dict[int, list[torch.Tensor]] = {}
@@ -52,6 +54,10 @@ class AdamW(torch.optim.AdamW):
     def attach_shadow(self, param: torch.Tensor, shadow: torch.Tensor) -> None:
         """Register a bf16 tensor that receives the updated value of `param` at every step."""
         self._shadow[param] = shadow
+
+    def number_tensors(self, numbers: dict[torch.Tensor, int]) -> None:
+        """Numbers for the random bits of parameters' 8-bit moments, in place of their places in the group."""
+        self._numbers.update(numbers)
 
     def _kernel_ok(self, group) -> bool:
         if not self._want_kernel:
@@ -117,20 +123,22 @@ class AdamW(torch.optim.AdamW):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
                 continue
+            # (also of a step that leaves parameters out: the others keep theirs)
+            numbers = [self._numbers.get(p, i) for i, p in enumerate(group["params"]) if p.grad is not None]
             t, lr = self._advance_group(group, ps)
             states = [self.state[p] for p in ps]
             args = [ps, [p.grad.contiguous() for p in ps], [st["exp_avg"] for st in states], [st["exp_avg_scale"] for st in states],
                     [st["exp_avg_sq"] for st in states], [st["exp_avg_sq_scale"] for st in states], [self._shadow.get(p) for p in ps],
                     lr, *group["betas"], group["eps"], group["weight_decay"], t, scale, group.get("maximize", False)]
             if not (self._want_kernel and multi_tensor.available() and ps[0].is_cuda):
-                oracle.adamw8(*args, seed=self._group_seed(gi))
+                oracle.adamw8(*args, seed=self._group_seed(gi), numbers=numbers)
                 continue
             hyper = None
             if self._hyper is not None:
                 if not capturing:
                     self._upload_hyper(gi, self._hyper_values(gi, group, t, lr))
                 hyper = self._hyper[gi]
-            multi_tensor.adamw8_step(*args, hyper=hyper, seed=self._group_seed(gi))
+            multi_tensor.adamw8_step(*args, hyper=hyper, seed=self._group_seed(gi), numbers=numbers)
             self._graph_groups[gi] = ps
 
     def _group_seed(self, gi: int) -> int:

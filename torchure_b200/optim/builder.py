@@ -30,7 +30,10 @@ def build_optimizer(model: nn.Module | None, name: str, cfg: dict, params=None) 
     ]
     if name not in OPTIMIZERS:
         raise KeyError(f"unknown optimizer {name!r}; known: {sorted(OPTIMIZERS)}")
-    return OPTIMIZERS[name](groups, **cfg)
+    optimizer = OPTIMIZERS[name](groups, **cfg)
+    if hasattr(model, "tensor_numbers") and hasattr(optimizer, "number_tensors"):
+        optimizer.number_tensors(model.tensor_numbers)
+    return optimizer
 
 
 def build_scheduler(optimizer: optim.Optimizer, cfg: dict):

@@ -45,6 +45,9 @@ class PipelineStage(nn.Module):
         # a tied embedding / head lives on two stages: their gradients are summed and their values kept equal
         self.tied_across = (self.stages > 1 and getattr(model, "lm_head", None) is not None
                             and model.lm_head.weight is model.token_emb.weight)
+        # places in the whole model: what an optimizer rounds with random bits is then rounded alike by both holders
+        mine = set(self.parameters())
+        self.tensor_numbers = {p: i for i, p in enumerate(model.parameters()) if p in mine}
 
     def forward(self, x: torch.Tensor, return_final_hidden: bool = False) -> torch.Tensor:
         if self.first:
@@ -79,7 +82,7 @@ class PipelineStage(nn.Module):
 
     def sync_tied_grad(self) -> None:
         """Both holders end with the SUM of the embedding's and the head's gradient, as the tied tensor of an
-        unsplit model has; with the same optimizer state they then apply the same update."""
+        unsplit model has; with the same optimizer state (and, of 8-bit moments, the same number) they then apply the same update."""
         w = self._tied()
         if w is None:
             return
