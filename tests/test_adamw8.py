@@ -568,3 +568,23 @@ def test_a_step_that_leaves_a_parameter_out(device):
     assert same(whole[1], part[1]) and same(whole[2], part[2])
     numbered, other = run([0, 1, 2], numbers=[4, 9, 17]), run([2, 0], numbers=[4, 9, 17])
     assert same(numbered[2], other[2]) and same(numbered[0], other[0]) and not torch.equal(numbered[2][1], whole[2][1])
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_negative_zeros(device):
+    """A first moment that was rounded to -0 and a gradient of -0 (that of nothing, with `maximize`): the code keeps its sign on every device."""
+    codes, _ = oracle.state8_encode(torch.tensor([1.0, -0.0, 0.0, -1.0]), torch.zeros(4, dtype=torch.int64), True)
+    assert codes.tolist() == [127, 128, 0, 255]
+    n = 300
+    m = torch.zeros(n)
+    m[0], m[128], m[256] = 1.0, 1.0, 1.0
+    made, scales = oracle.state8_encode(m, torch.zeros(n, dtype=torch.int64), True)
+    made[5:100] = made[200:250] = 128
+    s = dict(params=[torch.zeros(n)], grads=[torch.zeros(n)], ms=[made], mscales=[scales], vs=[torch.zeros(n, dtype=torch.uint8)],
+             vscales=[torch.zeros(3)], shadows=[None])
+    s = {name: [None if t is None else t.to(device) for t in ts] for name, ts in s.items()}
+    step(s, multi_tensor.adamw8_step, step=1, maximize=True)
+    want = torch.zeros(n, dtype=torch.uint8)
+    want[5:100] = want[200:250] = 128
+    want[0] = want[128] = want[256] = 127
+    assert torch.equal(s["ms"][0].cpu(), want)

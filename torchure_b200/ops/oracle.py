@@ -127,7 +127,7 @@ def state8_encode(x, bits, signed):
     y = b.abs() * (top.reciprocal() * most) + first
     code = ((y.view(torch.int32) + (_blocks128(bits) << 4).int()) >> 20) - base
     code = code.clamp_max(last)
-    code = torch.where(b < 0, code + 128, code) if signed else torch.where(b > 0, code.clamp_min(1), code)
+    code = torch.where(torch.signbit(b), code + 128, code) if signed else torch.where(b > 0, code.clamp_min(1), code)
     tiny = top < 2.0 ** -100
     fine = (top < float("inf")) & ~tiny
     code = torch.where(fine, code, torch.zeros_like(code))
