@@ -304,3 +304,18 @@ def test_dense_trainer_with_8_bit_moments_in_a_graph(tmp_path, monkeypatch):
             assert float((a - b).abs().max()) <= 6 * 2 * 3e-4
     finally:
         dist.destroy_process_group()
+
+
+def test_layer_whose_groups_count_by_their_largest_score():
+    torch.manual_seed(3)
+    router = dict(score="softmax", groups=4, top_groups=2, group_scores=1, normalize=False, scale=4.0)
+    layers = [MoELayer(16, 32, num_experts=8, top_k=2, capacity_factor=8.0, router=router),
+              MoELayer(16, 32, num_experts=8, top_k=2, capacity_factor=0.0, experts="grouped", router=router)]
+    layers[1].load_state_dict(layers[0].state_dict())
+    x = torch.randn(60, 16)
+    _same(layers[1](x), layers[0](x))
+    logits = layers[0].router(x).detach()
+    mine = moe.route(logits, 2, **router)
+    assert not torch.equal(mine.counts, moe.route(logits, 2, **dict(router, group_scores=2)).counts)
+    with pytest.raises(ValueError):
+        MoELayer(16, 32, num_experts=8, top_k=2, router=dict(router, group_scores=3))

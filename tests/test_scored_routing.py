@@ -389,3 +389,64 @@ def test_available_off_runs_the_plain_statements():
         assert moe.route(torch.randn(3, 4), 2, score="sigmoid").weights.shape == (3, 2)
     finally:
         ops.force_fallback(False)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("T, E, k, score, biased, groups, top_groups", [
+    (1, 8, 2, "softmax", False, 4, 2), (65, 160, 6, "softmax", False, 8, 3), (300, 63, 5, "sigmoid", False, 7, 3), (64, 9, 3, "sigmoid", True, 9, 5),
+    (40, 256, 8, "sigmoid", True, 8, 4), (900, 384, 8, "softmax", False, 16, 4), (37, 374, 16, "softmax", True, 17, 4)])
+def test_groups_by_their_largest_score(device, T, E, k, score, biased, groups, top_groups):
+    """``group_scores`` 1, from its definition on whole tensors: the groups of the largest score, then the largest scores in them."""
+    logits, bias = inputs(T, E, seed=E)
+    s = (torch.sigmoid(logits.double()) if score == "sigmoid" else torch.softmax(logits.double(), 1)).float()
+    c = s + bias if biased else s
+    tops = c.view(T, groups, E // groups).amax(2)
+    keep = torch.zeros(T, groups).scatter_(1, tops.topk(top_groups, 1).indices, 1).repeat_interleave(E // groups, 1) > 0
+    want = c.masked_fill(~keep, float("-inf")).topk(k, 1).indices
+    how = dict(score=score, bias=bias.to(device) if biased else None, groups=groups, top_groups=top_groups, normalize=False, scale=16.0)
+    x = logits.to(device).requires_grad_()
+    r = moe.route(x, k, group_scores=1, **how)
+    assert torch.equal(r.experts.cpu().long(), want)
+    _, w, _ = exact(logits, k, want, score, False, 16.0)
+    assert norm_off(r.weights, w) < FP32
+    dw = torch.randn(T, k, generator=torch.Generator().manual_seed(1))
+    l, w, _ = exact(logits, k, want, score, False, 16.0)
+    (w * dw).sum().backward()
+    got, = torch.autograd.grad(r.weights, x, dw.to(device))
+    assert norm_off(got, l.grad) < FP32 * float((w.detach() * dw).norm()) / float(l.grad.norm())
+    assert norm_off(moe.route(x, k, group_scores=2, **how).weights, moe.route(x, k, **how).weights) == 0
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_one_large_score_or_two_good_ones(device):
+    """Where the two rules differ, and where a group has one open expert, or none."""
+    inf = float("inf")
+    logits = torch.tensor([[3.0, -3.0, 2.0, 2.0, 0.0, 0.0], [-inf, 1.0, 0.5, 0.5, -inf, -inf], [-inf] * 6], device=device)
+    one = moe.route(logits, 2, score="sigmoid", groups=3, top_groups=1, group_scores=1)
+    two = moe.route(logits, 2, score="sigmoid", groups=3, top_groups=1)
+    assert one.experts[:2].tolist() == [[0, 1], [1, 0]] and two.experts[:2].tolist() == [[2, 3], [2, 3]]
+    assert (one.slots >= 0).tolist() == [[True, True], [True, False], [False, False]]
+    assert one.counts.tolist() == [1, 2, 0, 0, 0, 0] and float(one.weights[1, 0]) == 1.0
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_refusals_of_group_scores(device):
+    x = torch.randn(4, 12, device=device)
+    for bad in (0, 3, -1):
+        with pytest.raises(ValueError):
+            moe.route(x, 2, groups=3, top_groups=2, group_scores=bad)
+        with pytest.raises(ValueError):
+            moe.route(x, 2, group_scores=bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2, 50])
+def test_expert_mlp_with_group_scores(T):
+    E, D, F, k = 16, 64, 40, 3
+    x, wgu, wd, logits = mlp_inputs(T, E, D, F, "cuda", torch.bfloat16, seed=T)
+    how = moe.Scoring("softmax", None, 4, 2, False, 2.5, 1)
+    counts = torch.zeros(E, dtype=torch.int32, device="cuda")
+    out, _ = moe.expert_mlp(x, logits, wgu, wd, k, scoring=how, counts=counts)
+    want, _ = oracle.expert_mlp(*[t.double() for t in (x, logits, wgu, wd)], k, scoring=how)
+    assert norm_off(out, want) < 8 * RMS
+    assert torch.equal(counts, moe.route(logits, k, score="softmax", groups=4, top_groups=2, normalize=False, group_scores=1).counts)

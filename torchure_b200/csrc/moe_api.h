@@ -29,6 +29,7 @@ struct RouteScore {
   int groups, top_groups;  // experts in `groups` equal parts, `top_groups` of which stay open to a token
   bool normalize;          // weights over their sum
   float scale;             // times this, not 0
+  int group_scores;        // a group counts by its so many largest, 1 or 2
 };
 int64_t route_scratch_ints(int T, int E, const RouteScore* how);
 int route_kernels(int T, int E, const RouteScore* how);      // that route_fwd launches

@@ -70,24 +70,27 @@ struct Scoring {
   int64_t groups = 1, top_groups = 1;
   bool normalize = true;
   double scale = 1.0;
+  int64_t group_scores = 2;
 };
 using OptScoring = c10::optional<Scoring>;
-using PyScoring = c10::optional<std::tuple<bool, OptTensor, int64_t, int64_t, bool, double>>;
+using PyScoring = c10::optional<std::tuple<bool, OptTensor, int64_t, int64_t, bool, double, int64_t>>;
 
 tb::RouteScore raw(const Scoring& s) {
-  return {s.sigmoid, s.bias.defined() ? s.bias.data_ptr<float>() : nullptr, (int)s.groups, (int)s.top_groups, s.normalize, (float)s.scale};
+  return {s.sigmoid, s.bias.defined() ? s.bias.data_ptr<float>() : nullptr, (int)s.groups, (int)s.top_groups, s.normalize, (float)s.scale,
+          (int)s.group_scores};
 }
 
 OptScoring check_scoring(const PyScoring& given, const Tensor& logits, int64_t k, const char* what) {
   if (!given) return c10::nullopt;
-  const auto& [sigmoid, bias, groups, top_groups, normalize, scale] = *given;
+  const auto& [sigmoid, bias, groups, top_groups, normalize, scale, group_scores] = *given;
   const int64_t E = logits.size(1);
   TORCH_CHECK_VALUE(groups >= 1 && groups <= tb::kMaxExpertGroups && E % groups == 0, what, ": ", E, " experts in ", groups,
                     " equal groups (at most ", tb::kMaxExpertGroups, ")");
   TORCH_CHECK_VALUE(top_groups >= 1 && top_groups <= groups, what, ": ", top_groups, " of ", groups, " groups");
   TORCH_CHECK_VALUE(k <= top_groups * (E / groups), what, ": top_k of ", k, " among ", top_groups, " groups of ", E / groups, " experts");
   TORCH_CHECK_VALUE(std::isnormal((float)scale) && scale > 0, what, ": scale ", scale);
-  Scoring s{sigmoid, {}, groups, top_groups, normalize, scale};
+  TORCH_CHECK_VALUE(group_scores == 1 || group_scores == 2, what, ": the largest ", group_scores, " scores of a group (1 or 2 expected)");
+  Scoring s{sigmoid, {}, groups, top_groups, normalize, scale, group_scores};
   if (has(bias)) {
     TORCH_CHECK_TYPE(bias->scalar_type() == torch::kFloat32, what, ": a bias in fp32 expected, got ", bias->scalar_type());
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits.device(), what, ": a bias of ", E,

@@ -440,7 +440,7 @@ route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restri
 
 // ---- choice by scores, with a bias and groups of experts -----------------------------------------------
 // s = sigmoid(l) or softmax(l), rounded to fp32 from 64 bits; with a bias or groups the choice goes by c = s + bias, else by l.  A group's score is
-// the sum of its two largest c; the experts of the top_groups largest groups stay open (ties to the lowest index).  Weights of the choices made:
+// the sum of its two largest c, or (group_scores 1) its largest; the experts of the top_groups largest groups stay open (ties to the lowest index).  Weights of the choices made:
 //   w_j = scale s_j / (normalize: sum over the chosen of s_i, else 1);  aux = E sum_e share_e mean_t P[t, e], P = s / sum over all of s
 // and with what = w / scale, d = 1 - s (sigmoid) or 1 (softmax):
 //   dl_j += d_j what_j (scale dw_j - (normalize ? inner : 0)), inner = sum_i what_i scale dw_i;  softmax, not normalized: dl_e -= s_e inner
@@ -454,7 +454,7 @@ struct ScoreArgs {
   const float* bias;       // nullptr: none
   int groups, top_groups, each;      // each: experts of a group
   int groups_log2;         // of the power of two that holds `groups`
-  int sigmoid, normalize;
+  int sigmoid, normalize, group_scores;
   float scale;
 };
 
@@ -611,7 +611,7 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
         second = max(max(second, g), min(first, f));
         first = max(first, f);
       }
-      const uint32_t total = second <= kKeyMinusInf ? first : to_key(from_key(first) + from_key(second));
+      const uint32_t total = how.group_scores == 1 || second <= kKeyMinusInf ? first : to_key(from_key(first) + from_key(second));
       int ahead = 0;
       for (int g = 0; g < how.groups; ++g) {
         const uint32_t other = __shfl_sync(mask, total, g * per, LANES);
@@ -829,7 +829,7 @@ int vals_for(int E) {
 
 bool score_fits(int E, int k, const RouteScore& how) {
   return how.groups >= 1 && how.groups <= kMaxExpertGroups && E % how.groups == 0 && how.top_groups >= 1 && how.top_groups <= how.groups &&
-         k <= how.top_groups * (E / how.groups);
+         (how.group_scores == 1 || how.group_scores == 2) && k <= how.top_groups * (E / how.groups);
 }
 
 // Threads of a token, logits of a thread and log2 of the groups' places: each group has the same power of two of threads.
@@ -879,7 +879,7 @@ int launch_scored(const T* logits, const RouteArgs& a, const RouteScore& how, in
   ScoreArgs s{};
   scored_shape(a.E, how, lanes, vals, s.groups_log2);
   s.bias = how.bias; s.groups = how.groups; s.top_groups = how.top_groups; s.each = a.E / how.groups;
-  s.sigmoid = how.sigmoid; s.normalize = how.normalize; s.scale = how.scale;
+  s.sigmoid = how.sigmoid; s.normalize = how.normalize; s.scale = how.scale; s.group_scores = how.group_scores;
   const int plan = plan_smem_ints(a.E), sums = kWarps * (a.E | 1);
   const int smem = 4 * (chunks == 1 ? 2 * a.E + a.T * a.k + (sums > plan ? sums : plan) : 2 * a.E + sums);
 #define CASE(L, V)                                                                                                                 \

@@ -5,7 +5,7 @@ so that the expert-parallel layer (``parallel/expert_parallel.py``) has a model 
 keeps the dense model's attention and norms and swaps the MLP for ``MoELayer``.  The blocks run the PyTorch path
 (``impl`` is fixed to "torch"); ``experts: "grouped"`` runs the feed-forwards on the sm_100a operators of ``ops/moe.py``
 instead of batched library products over padded buffers, and ``act_bits: 8`` keeps their gate and up in 8 bits between the
-passes.  ``router`` ({"score", "groups", "top_groups", "normalize", "scale", "bias_rate"}) chooses experts by scores, with a bias that
+passes.  ``router`` ({"score", "groups", "top_groups", "group_scores", "normalize", "scale", "bias_rate"}) chooses experts by scores, with a bias that
 the Trainer moves after every step; ``embedding: "sorted"`` looks tokens up with ``ops/embedding.py``, whose gradient sums a
 token's rows in a fixed order, and ``embed_scale`` multiplies the rows.
 

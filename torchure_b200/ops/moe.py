@@ -61,10 +61,11 @@ class Scoring(NamedTuple):
     top_groups: int = 1               # groups that stay open to a token
     normalize: bool = True            # weights over their sum
     scale: float = 1.0                # ... times this
+    group_scores: int = 2             # a group counts by its so many largest scores, 1 or 2
 
 
 def scoring(experts: int, top_k: int, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1, top_groups: int = 0,
-            normalize: bool = True, scale: float = 1.0) -> Scoring | None:
+            normalize: bool = True, scale: float = 1.0, group_scores: int = 2) -> Scoring | None:
     """The ``Scoring`` of these arguments for a router of so many experts, or None where they ask for the plain choice by logits."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f'route: scores are "softmax" or "sigmoid", not {score!r}')
@@ -78,22 +79,24 @@ def scoring(experts: int, top_k: int, score: str = "softmax", bias: torch.Tensor
         raise ValueError(f"route: top_k of {top_k} among {top_groups} groups of {experts // groups} experts")
     if not 0 < scale < float("inf"):
         raise ValueError(f"route: scale {scale}")
+    if group_scores not in (1, 2):
+        raise ValueError(f"route: the largest {group_scores} scores of a group (1 or 2 expected)")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (experts,)):
         raise ValueError(f"route: a bias of {experts} fp32 elements expected, got {bias.dtype} {tuple(bias.shape)}")
     if score == "softmax" and bias is None and groups == 1 and normalize and scale == 1.0:
         return None
-    return Scoring(score, bias, groups, top_groups, bool(normalize), float(scale))
+    return Scoring(score, bias, groups, top_groups, bool(normalize), float(scale), int(group_scores))
 
 
 _checked = scoring      # (where an argument has its name)
 
 
 def _native(how: Scoring | None):
-    return None if how is None else (how.score == "sigmoid", how.bias, how.groups, how.top_groups, how.normalize, how.scale)
+    return None if how is None else (how.score == "sigmoid", how.bias, how.groups, how.top_groups, how.normalize, how.scale, how.group_scores)
 
 
 def route(logits: torch.Tensor, top_k: int, capacity: int = 0, *, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
-          top_groups: int = 0, normalize: bool = True, scale: float = 1.0) -> Routing:
+          top_groups: int = 0, normalize: bool = True, scale: float = 1.0, group_scores: int = 2) -> Routing:
     """The ``top_k`` experts of every token by its logits [T, E] (fp32 or bf16, others in fp32; at most 384 experts, 16 choices).
 
     Ties go to the lowest index.  A weight is the softmax over the token's choices (the probabilities renormalised over them).  An
@@ -102,14 +105,16 @@ def route(logits: torch.Tensor, top_k: int, capacity: int = 0, *, score: str = "
     E * sum_e (share of the choices, before the capacity, that went to e) * (mean probability of e).
 
     ``score`` "sigmoid": an expert's score s is the sigmoid of its logit, not its softmax.  ``bias`` (fp32 [E]) is added to the scores for
-    the choice alone, see ``balance_bias_``.  ``groups``: the experts lie in so many equal groups, of which the ``top_groups`` whose two
-    largest (biased) scores have the largest sum are open to a token.  With a bias or groups the choice goes by biased scores (each score
+    the choice alone, see ``balance_bias_``.  ``groups``: the experts lie in so many equal groups, at most 32, of which the ``top_groups``
+    whose two largest (biased) scores have the largest sum are open to a token; with ``group_scores`` 1 those whose largest score is largest, the
+    usual rule of routers without a bias.  With a bias or groups the choice goes by biased scores (each score
     rounded to fp32 once, so that it is the same on every machine), else by the logits.  ``normalize`` False: weights are the scores
     themselves, not divided by their sum over the choices; ``scale`` multiplies them.  The load-balancing term's probabilities are the
     scores over their sum.  A bias of -inf closes its expert to the choice."""
     how = None
-    if not (score == "softmax" and bias is None and groups == 1 and top_groups == 0 and normalize and scale == 1.0) and logits.dim() == 2:
-        how = scoring(logits.shape[1], top_k, score, bias, groups, top_groups, normalize, scale)
+    if not (score == "softmax" and bias is None and groups == 1 and top_groups == 0 and normalize and scale == 1.0
+            and group_scores == 2) and logits.dim() == 2:
+        how = scoring(logits.shape[1], top_k, score, bias, groups, top_groups, normalize, scale, group_scores)
     if not _plain(logits):
         return Routing(*_C().moe_route(logits, top_k, capacity, _native(how), debug.enabled()))
     if logits.dim() != 2 or not logits.is_floating_point():

@@ -202,9 +202,10 @@ def _plan_rows(experts, made, E, capacity):
     return slots.view(T, k).int(), offsets.int(), rows.int(), counts
 
 
-def route_scored(logits, k, capacity=0, score="softmax", bias=None, groups=1, top_groups=1, normalize=True, scale=1.0):
+def route_scored(logits, k, capacity=0, score="softmax", bias=None, groups=1, top_groups=1, normalize=True, scale=1.0, group_scores=2):
     """``route`` by scores: s = sigmoid or softmax of the logits, rounded to fp32 from 64 bits for the choice; with a bias or groups the choice goes
-    by s + bias inside the ``top_groups`` groups whose two largest have the largest sums, else by the logits."""
+    by s + bias inside the ``top_groups`` groups whose two largest have the largest sums (``group_scores`` 1: whose largest is largest), else by the
+    logits."""
     x = logits if logits.dtype == torch.float64 else logits.float()
     T, E = x.shape
     lowest = torch.full((), float("-inf"), device=x.device)
@@ -220,7 +221,8 @@ def route_scored(logits, k, capacity=0, score="softmax", bias=None, groups=1, to
         key = torch.where(is_open, s if bias is None else s + bias.detach(), lowest)
     if groups > 1:
         two = key.view(T, groups, E // groups).sort(-1, descending=True).values[..., :2]
-        total = torch.where((two == lowest)[..., 1:].any(-1) | (two.shape[-1] == 1), two[..., 0], two.sum(-1))
+        one = group_scores == 1 or two.shape[-1] == 1
+        total = two[..., 0] if one else torch.where(two[..., 1] == lowest, two[..., 0], two.sum(-1))
         best = torch.sort(total, dim=-1, descending=True, stable=True).indices[:, :top_groups]
         stays = torch.zeros(T, groups, dtype=torch.bool, device=x.device).scatter_(1, best, True)
         key = torch.where(stays.repeat_interleave(E // groups, 1), key, lowest)

@@ -13,7 +13,7 @@ shuffle is the even-split ``all_to_all``.  Here:
   grouped by expert instead of batched library products, with ``act_bits=8`` gate and up kept in 8 bits for the backward pass.  The
   capacity drops the same choices (``capacity_factor`` 0: none are dropped).  Spread over a mesh axis the exchange keeps its padded
   buffers (with ``capacity_factor`` 0 a row for every token of the rank) and the grouped products run on what arrives.
-* ``router`` ({"score", "groups", "top_groups", "normalize", "scale", "bias_rate"}) chooses experts by scores (``ops/moe.py::route``).
+* ``router`` ({"score", "groups", "top_groups", "group_scores", "normalize", "scale", "bias_rate"}) chooses experts by scores (``ops/moe.py::route``).
   With a ``bias_rate`` every expert has a bias for the choice, a buffer: ``balance`` moves it by that much against the choices
   that training passes have counted since the last call.
 """
@@ -59,7 +59,7 @@ class MoELayer(nn.Module):
         self.bias_rate = float(how.pop("bias_rate", 0.0))
         if not 0.0 <= self.bias_rate < float("inf"):
             raise ValueError(f"MoELayer: bias_rate {self.bias_rate}")
-        if unknown := set(how) - {"score", "groups", "top_groups", "normalize", "scale"}:
+        if unknown := set(how) - {"score", "groups", "top_groups", "group_scores", "normalize", "scale"}:
             raise ValueError(f"MoELayer: unknown router keys {sorted(unknown)}")
         self.scoring = moe.scoring(num_experts, top_k, bias=torch.zeros(num_experts) if self.bias_rate else None, **how)
         if self.bias_rate:
