@@ -588,3 +588,38 @@ def test_negative_zeros(device):
     want[5:100] = want[200:250] = 128
     want[0] = want[128] = want[256] = 127
     assert torch.equal(s["ms"][0].cpu(), want)
+
+
+def test_what_small_elements_of_a_block_move():
+    """400 steps with a constant gradient, eps 0: all elements of a 32-bit step would move alike.  A second moment above zero keeps its first step, 2^-34.9
+    of the block's largest, whose root is 2^-17.45: elements down to there move as the largest do, those below are damped in proportion, to
+    under a half at the first moment's first step, 2^-18.9.  A mean over 127 elements; single ones scatter by the rounding of both moments."""
+    powers = [8, 14, 16, 17, 17.45, 18, 18.9, 20]
+    g = torch.stack([torch.full((128,), 2.0 ** -p) for p in powers])
+    g[:, 0] = 1.0
+    p = torch.zeros_like(g)
+    m, v = torch.zeros_like(g, dtype=torch.uint8), torch.zeros_like(g, dtype=torch.uint8)
+    ms, vs = torch.zeros(len(powers)), torch.zeros(len(powers))
+    for t in range(1, 401):
+        oracle.adamw8([p], [g], [m], [ms], [v], [vs], [None], 1e-3, 0.9, 0.95, 0.0, 0.0, t)
+    way = -p
+    assert torch.allclose(way[:, 0], torch.tensor(0.4), rtol=1e-3)
+    moved = dict(zip(powers, way[:, 1:].mean(1).tolist()))
+    for power in powers:
+        if power <= 17.45:
+            assert 0.95 * 0.4 <= moved[power] <= 1.05 * 0.4, (power, moved)      # (an eighth of a code, averaged over steps and elements)
+        else:
+            floor = 2.0 ** (17.4535 - power)                                     # root of the first step over the element's own
+            assert 0.95 * floor * 0.4 <= moved[power] <= 1.1 * floor * 0.4, (power, moved)
+
+
+def test_how_far_a_first_moment_is_off():
+    """One step of its code at most, (|x| + FIRST scale) / 8: an eighth of large values, half of a value at 2^-18, all of one at the first step."""
+    for power, most in ((4, 1 / 8), (12, 1 / 8), (15, 1 / 7), (16, 1 / 6), (17, 1 / 4), (18, 1 / 2), (18.9, 1.0)):
+        x = torch.full((128,), 2.0 ** -power)
+        x[0] = 1.0
+        bound = (x[1] + FIRST[True] / TOP[True]) / 8
+        for r in range(0, 65536, 257):
+            kept = oracle.state8_decode(*oracle.state8_encode(x, torch.full((128,), r), True), True)
+            off = float((kept[1] - x[1]).abs())
+            assert off <= float(bound) + 2.0 ** -20 * float(x[1]) and off <= most * float(x[1]) * (1 + 2.0 ** -10)

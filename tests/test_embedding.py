@@ -286,3 +286,56 @@ def test_rows_of_16_bits_that_end_in_the_middle_of_a_word(T, D, gap):
     out = embedding(ids.cuda(), there.requires_grad_(), scale)
     dtable, = torch.autograd.grad(out, there, dthere)
     check(ids, table, dout, out, dtable, scale)
+
+
+def check_sparse(ids, table, dout, dtable, scale, padding):
+    """As ``check`` for tables too large to widen: the rows that have tokens, in 64 bits, and zeros everywhere else."""
+    keep = (ids >= 0) & (ids < table.shape[0]) & (ids != padding)
+    rows, place = torch.unique(ids[keep], return_inverse=True)
+    terms = dout[keep].double()
+    total = torch.zeros(len(rows), dout.shape[1], dtype=torch.float64, device=ids.device).index_add_(0, place, terms) * scale
+    size = torch.zeros_like(total).index_add_(0, place, terms.abs()) * abs(scale)
+    n = torch.bincount(place, minlength=len(rows))[:, None].double()
+    got = dtable[rows]
+    bound = size * n * 2.0 ** -24 + total.abs() * (HALF[dtable.dtype] + 2.0 ** -23) + 1e-40
+    assert ((got.double() - total).abs() <= bound).all()
+    assert int(torch.count_nonzero(dtable)) == int(torch.count_nonzero(got))
+
+
+# T, V, D, table: one CTA sorts up to 8192 tokens with its lists in shared memory, and up to 16384 with them in scratch memory where the gradient has 18000
+# bytes a token or more; two, three or four digits, so that the lists end in the same place after an even and an odd number of passes.
+SORTS = [
+    (8192, 40000, 64, torch.float32, True),
+    (8192, 300000, 64, torch.float32, True),
+    (8193, 40000, 921, torch.float32, False),          # 147.36 MB, 18000 a token are 147.47
+    (8193, 40000, 924, torch.float32, True),
+    (8193, 40000, 1845, torch.bfloat16, True),
+    (16384, 40000, 1844, torch.float32, True),
+    (16384, 300000, 248, torch.float32, True),
+    (12345, 300000, 186, torch.float32, True),
+    (16384, 140000000, 2, torch.bfloat16, True),
+    (16384, 300000, 244, torch.float32, False),
+    (16385, 40000, 1900, torch.float32, False),
+    (16385, 300000, 256, torch.float32, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T, V, D, table_type, whole", SORTS)
+@pytest.mark.parametrize("hot", [0.0, 0.4])
+def test_sorts_at_the_borders_of_their_rule(T, V, D, table_type, whole, hot):
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    ids = torch.randint(0, V, (T,), device="cuda", generator=g)
+    skewed = (V * torch.rand(T, device="cuda", generator=g, dtype=torch.float64) ** 8).long()       # a few ids many times
+    ids = torch.where(torch.rand(T, device="cuda", generator=g) < hot, skewed, ids)
+    ids[::97], ids[5::301], ids[7::1000] = V - 1, 3, V // 2
+    ids[11::500], ids[13::700] = -1, V                                                             # outside: no gradient
+    w = torch.zeros(V, D, dtype=table_type, device="cuda").requires_grad_()
+    dout = torch.randn(T, D, device="cuda", generator=g).to(table_type)
+    before = ops.launches()
+    dtable, = torch.autograd.grad(embedding(ids, w, 0.5, 3), w, dout)
+    digits = -(-V.bit_length() // 9)
+    assert ops.launches() - before == 1 + (1 if whole else 2 * digits) + 2
+    check_sparse(ids, w, dout, dtable, 0.5, 3)
+    again, = torch.autograd.grad(embedding(ids.int(), w, 0.5, 3), w, dout)
+    assert torch.equal(again, dtable)

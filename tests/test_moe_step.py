@@ -319,3 +319,48 @@ def test_layer_whose_groups_count_by_their_largest_score():
     assert not torch.equal(mine.counts, moe.route(logits, 2, **dict(router, group_scores=2)).counts)
     with pytest.raises(ValueError):
         MoELayer(16, 32, num_experts=8, top_k=2, router=dict(router, group_scores=3))
+
+
+@pytest.mark.gpu
+def test_replayed_steps_of_the_dense_trainer_move_as_eager_ones(tmp_path, monkeypatch):
+    """The dense model on the kernel engine with 8-bit moments, its step captured, against a run without the graph, measured by the way that the weights
+    go.  Gradients of the two runs differ in the order of fp32 sums, some 2^-20 of a tensor's norm, so that an element's update, m over the root of
+    v, is another only where its gradient is that small beside the rest, or where a code falls to the other side, by an eighth, for as rare an
+    element: far less than a sixteenth of the way.  A step that a replay leaves out, or takes twice, is a sixth of it."""
+    monkeypatch.setenv("TORCHURE_B200_HOME", str(tmp_path))
+    monkeypatch.setenv("MASTER_ADDR", "127.0.0.1")
+    import torch.distributed as dist
+
+    from tests.dist_utils import free_port
+    from tests.tiny import parity_config
+    from torchure_b200.train.trainer import Trainer
+
+    monkeypatch.setenv("MASTER_PORT", str(free_port()))
+    if not dist.is_initialized():
+        dist.init_process_group("nccl", rank=0, world_size=1)
+    try:
+        runs = []
+        for graph in (False, True):
+            cfg = parity_config(world=1, steps=8, accumulation=1)
+            cfg["model"]["config"].update(num_layers=2, num_heads=4, num_kv_heads=2, emb_dim=256, head_dim=128, vocab_size=1024, ffn_dim=512)
+            cfg["optimizer"]["config"].update(fused=True, state_bits=8)
+            cfg.update(cuda_graph=graph, cuda_graph_warmup=2)
+            tr = Trainer(cfg, 0, 0, 1, benchmark=True)
+            places = [[p.detach().clone() for p in tr.model.parameters()]]
+            losses = []
+            for _ in range(6):
+                losses += [h["loss"] for h in tr.train_n_step_test(1)]
+                places.append([p.detach().clone() for p in tr.model.parameters()])
+            tr.check_device_errors()
+            assert (tr._graph is not None) == graph
+            runs.append((places, losses))
+        (eager, le), (replayed, lr) = runs
+        assert all(torch.equal(p, q) for p, q in zip(eager[0], replayed[0]))
+        for t in range(1, 7):
+            for start, was, is_, other in zip(eager[0], replayed[t - 1], replayed[t], eager[t]):
+                assert not torch.equal(was, is_), t
+                assert float((is_ - other).norm()) <= float((other - start).norm()) / 16, t
+        # losses of weights that are as near, in bf16 products: a few units of 2^-9 of a logit of order one
+        assert all(abs(x - y) <= 2.0 ** -8 for x, y in zip(le, lr)), (le, lr)
+    finally:
+        dist.destroy_process_group()
