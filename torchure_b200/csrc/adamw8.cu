@@ -4,10 +4,13 @@
 // y = x TOP / a + FIRST and held as y's fp32 pattern cut to 3 bits of mantissa, counted from FIRST's pattern:
 //   code = ((bits(y) + (r << 4)) >> 20) - (bits(FIRST) >> 20),   x kept = (value(code) - FIRST) a / TOP
 // (even steps next to zero, steps of an eighth further up).  First moment: a sign bit and FIRST = 2^-15, 127 steps down to a 2^-19; second
-// moment: FIRST = 2^-31, 255 steps down to a 2^-35, so that its root covers what the first moment covers.  r are 16 random bits: a value goes to
-// one of its two neighbours with the probability that makes the mean its own.  To the nearest, a second moment that changes by 1 - beta2 of
+// moment: FIRST = 2^-31, 255 steps down to a 2^-35.  Either is off by a step of its code at most, (|x| + FIRST a / TOP) / 8: an eighth of large
+// values, half of a first moment at a 2^-18.  r are 16 random bits: a value goes to one of its two neighbours with the probability that makes the
+// mean its own.  To the nearest, a second moment that changes by 1 - beta2 of
 // itself a step, less than half a step of the code, would stay where it is for good.  A second moment above zero keeps at least the first step:
-// no update divides by eps alone where the gradients have been small beside the block's.
+// no update divides by eps alone where the gradients have been small beside the block's.  That step's root is a 2^-17.45 of the second moments' a:
+// elements with gradients down to 2^-17.45 of the block's largest move as in 32 bits, those below are damped in proportion (0.69 of the way
+// at 2^-18, 0.38 at 2^-18.9).
 // A block that holds something that is not finite reads back as NaN, one whose largest magnitude is under 2^-100 as zeros.
 //
 // Random bits: h(i) = mix(key ^ low 32 bits of i), key from (seed, step, the tensor's number, high bits of i), mix two rounds of xorshift and multiplication

@@ -8,9 +8,9 @@
 // in scratch memory, and a last kernel adds up the parts of such runs: however often one token occurs, its rows are read by many CTAs.
 // The table's gradient is mostly rows of no token: they are zeroed by CTAs of the sorting kernels, whose own work fills few SMs.
 //
-// Bound by memory: V D values of the gradient to write, T D to read.  8192 tokens, a table of 151936 x 1024 in fp32: lookup 10.3 us (6.5 TB/s), sort
-// and zeros 86 (7.2 TB/s of zeros), sums 12.7, runs over chunks 6.3; the whole pass 120, of which the bytes take 110 at copy bandwidth.  65521 tokens of
-// 1003 columns in bf16, 30 % padding: 45, 30, 39, 12.  Few tokens: a chain of kernels of 3 - 5 us.
+// Bound by memory: V D values of the gradient to write, T D to read.  8192 tokens, a table of 151936 x 1024 in fp32: lookup 10.2 us (6.6 TB/s), sort
+// and zeros 86 (7.2 TB/s of zeros), sums 12.7, runs over chunks 6.2; the whole pass 114, of which the bytes take 110 at copy bandwidth.  65521 tokens of
+// 1003 columns in bf16, 30 % padding: 43, 28, 39, 12.  Few tokens: a chain of kernels of 3 - 5 us.
 #include "common.cuh"
 #include "embed_api.h"
 

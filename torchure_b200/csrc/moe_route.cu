@@ -446,10 +446,13 @@ route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restri
 //   dl_j += d_j what_j (scale dw_j - (normalize ? inner : 0)), inner = sum_i what_i scale dw_i;  softmax, not normalized: dl_e -= s_e inner
 //   dl_e += daux E / T d_e P_e (share_e - sum_i share_i P_i)
 // Scores 1e-7 apart decide which expert a token goes to and with it the order of all rows behind; computed in 32 bits they would depend on the
-// machine's exp, rounded once from 64 they do not.
+// machine's exp.  Rounded once from 64 they do so only within 2^-46 of the middle between two fp32 numbers: about one score in 2^22 may be the
+// next number on another machine.
 //
-// Bound by instructions: a score in 64 bits takes 33 of them, a choice 25, and every token a warp.  8192 tokens x 256 experts in 8 groups, 8 choices:
-// 25 us, 9 for the rows, 9 for the gradient; 32768 x 128, 8 choices (8.4 MB of logits, 1.3 us): 32, 9 and 19; one token 7.6.
+// Bound by instructions and latency, not by bytes (a score in 64 bits takes 33 instructions, a choice 25, and every token a warp).  32768 tokens x 128
+// experts, 8 choices (8.4 MB of logits, 1.3 us): 32 us at 80 % of the issue slots, 780 instructions a token; 9 for the rows, 19 for the gradient at 57 %.
+// 8192 x 256 in 8 groups, 8 choices: 25 us, 1.7 k instructions a token at 55 - 61 %: half of it issue, the rest waits for the token before (32 warps an
+// SM, two rounds of tokens on 128 of them); 9 for the rows, 9 for the gradient (55 %).  One token 7.6.
 struct ScoreArgs {
   const float* bias;       // nullptr: none
   int groups, top_groups, each;      // each: experts of a group

@@ -108,7 +108,7 @@ def route(logits: torch.Tensor, top_k: int, capacity: int = 0, *, score: str = "
     the choice alone, see ``balance_bias_``.  ``groups``: the experts lie in so many equal groups, at most 32, of which the ``top_groups``
     whose two largest (biased) scores have the largest sum are open to a token; with ``group_scores`` 1 those whose largest score is largest, the
     usual rule of routers without a bias.  With a bias or groups the choice goes by biased scores (each score
-    rounded to fp32 once, so that it is the same on every machine), else by the logits.  ``normalize`` False: weights are the scores
+    rounded to fp32 once from 64 bits: a CPU and a GPU differ in about one of 2^22, by one unit), else by the logits.  ``normalize`` False: weights are the scores
     themselves, not divided by their sum over the choices; ``scale`` multiplies them.  The load-balancing term's probabilities are the
     scores over their sum.  A bias of -inf closes its expert to the choice."""
     how = None
