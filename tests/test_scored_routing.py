@@ -450,3 +450,27 @@ def test_expert_mlp_with_group_scores(T):
     want, _ = oracle.expert_mlp(*[t.double() for t in (x, logits, wgu, wd)], k, scoring=how)
     assert norm_off(out, want) < 8 * RMS
     assert torch.equal(counts, moe.route(logits, k, score="softmax", groups=4, top_groups=2, normalize=False, group_scores=1).counts)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("how", [dict(), dict(groups=2, top_groups=1), dict(groups=6, top_groups=3), dict(groups=3, top_groups=2, group_scores=1)])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_rows_that_are_not_numbers(device, score, how, biased, normalize):
+    """A NaN is no number to choose by, the largest there is: the lowest index has it first.  A term that such a row is part of is NaN, next to rows without experts
+    too, and so are its weights; other rows are as without it."""
+    inf, nan = float("inf"), float("nan")
+    good = torch.tensor([[0.5, 1.0, 0.0, 2.0, 0.25, -1.0], [-inf] * 6])
+    bias = torch.linspace(-0.1, 0.1, 6).to(device) if biased else None
+    want = moe.route(good.to(device), 2, score=score, bias=bias, normalize=normalize, scale=2.0, **how)
+    assert torch.isfinite(want.aux_loss)
+    for row, first in (([nan] * 6, [0, 1]), ([-inf, -inf, nan, nan, -inf, -inf], [2, 3]), ([-inf, nan, nan, nan, nan, nan], None), ([nan, 0.0, 1.0, 2.0, 3.0, nan], None)):
+        x = torch.cat([good, torch.tensor([row])]).to(device).requires_grad_()
+        r = moe.route(x, 2, score=score, bias=bias, normalize=normalize, scale=2.0, **how)
+        plain = moe.route(x.detach().cpu(), 2, score=score, bias=None if bias is None else bias.cpu(), normalize=normalize, scale=2.0, **how)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(r[2:], plain[2:]))
+        assert first is None or how or r.experts[2].tolist() == first      # (groups: theirs have a say)
+        assert torch.equal(r.weights[:2].detach(), want.weights) and torch.isnan(r.weights[2]).any() and torch.isnan(r.aux_loss)
+        grad, = torch.autograd.grad((r.weights[:2].sum(), r.aux_loss), (x,), (torch.ones((), device=device), torch.zeros((), device=device)))
+        assert torch.isfinite(grad[:2]).all() or device == "cpu"

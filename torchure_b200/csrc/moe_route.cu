@@ -588,11 +588,12 @@ route_scored_kernel(const T* __restrict__ logits, RouteArgs a, ScoreArgs how, in
 #pragma unroll
       for (int v = 0; v < VALS; ++v) {
         const float below = top - x[v];
-        e[v] = none ? 0.0 : below != below ? static_cast<double>(below) : exp_minus(below);
+        // (top passes NaN by: a row of -inf and NaN alone is not one without experts)
+        e[v] = none ? (x[v] != x[v] ? static_cast<double>(x[v]) : 0.0) : below != below ? static_cast<double>(below) : exp_minus(below);
         sum += e[v];
       }
       sum = group_sum64<LANES>(sum, mask);
-      const double r = none ? 0.0 : 1.0 / sum;
+      const double r = none ? sum : 1.0 / sum;      // (none: 0, or NaN)
 #pragma unroll
       for (int v = 0; v < VALS; ++v) s[v] = static_cast<float>(e[v] * r);
     }
